@@ -402,4 +402,60 @@ inline void gemm_mx_w4a8(const DevicePackedWm& w, const DeviceActMx8& x, __half*
   detail::raise(w4_gemm_mx_w4a8(&vw, &vx, detail::h(c), stream));
 }
 
+// ---- serving over a paged FP8 cache (additive; no reference counterpart) ------------
+// H pools of npages pages of `page` rows of D E4M3 bytes, one FP16 scale per page and head.
+struct DeviceF8Pages {
+  int H, D, page, npages;
+  const uint8_t* q_k;
+  const __half* s_k;
+  const uint8_t* q_v;
+  const __half* s_v;
+};
+// A batch of sequences over such a cache; the arrays are device memory (w4_abi.h has the
+// meaning of each).
+struct DevicePagedBatch {
+  int nseq, tokens, max_q, max_len, bt_stride;
+  const int* bt;
+  const int* lens;
+  const int* cu_q;
+};
+namespace detail {
+inline w4_f8_pages_view abi(const DeviceF8Pages& p) {
+  return w4_f8_pages_view{p.H, p.D, p.page, p.npages, p.q_k, h(p.s_k), p.q_v, h(p.s_v)};
+}
+inline w4_paged_batch abi(const DevicePagedBatch& b) {
+  return w4_paged_batch{b.nseq, b.tokens, b.max_q, b.max_len, b.bt_stride, b.bt, b.lens, b.cu_q};
+}
+}  // namespace detail
+inline void paged_tables(const DevicePagedBatch& batch, int page, int npages, const int* cached,
+                         const int* added, const int* free_pages, const int* free_range, int* slots,
+                         int* positions, int* result, hipStream_t stream = 0) {
+  const auto b = detail::abi(batch);
+  detail::raise(w4_paged_tables(&b, page, npages, cached, added, free_pages, free_range, slots,
+                                positions, result, stream));
+}
+inline void quantize_f8_pages_async(const DeviceF8Pages& p, const __half* k, const __half* v,
+                                    int row_stride, const int* slots, int tokens, int* status,
+                                    hipStream_t stream = 0) {
+  const auto vw = detail::abi(p);
+  detail::raise(w4_quantize_f8_pages(&vw, detail::h(k), detail::h(v), row_stride, slots, tokens,
+                                     status, stream));
+}
+inline size_t attention_f8_pages_workspace(const DeviceF8Pages& p, const DevicePagedBatch& batch,
+                                           int group) {
+  const auto vw = detail::abi(p);
+  const auto b = detail::abi(batch);
+  size_t bytes = 0;
+  detail::raise(w4_attention_f8_pages_workspace(&vw, &b, group, &bytes));
+  return bytes;
+}
+inline void attention_f8_pages(const DeviceF8Pages& p, const DevicePagedBatch& batch, int group,
+                               bool causal, const __half* q, int q_stride, __half* out,
+                               void* workspace, size_t workspace_bytes, hipStream_t stream = 0) {
+  const auto vw = detail::abi(p);
+  const auto b = detail::abi(batch);
+  detail::raise(w4_attention_f8_pages(&vw, &b, group, causal, detail::h(q), q_stride,
+                                      detail::h(out), workspace, workspace_bytes, stream));
+}
+
 }  // namespace w4::gpu

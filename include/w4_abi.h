@@ -74,6 +74,34 @@ typedef struct w4_act_mx8_view {
   const uint8_t* scales; /* M * B E8M0 bytes                               */
 } w4_act_mx8_view;
 
+/* Paged FP8 cache, device view: H pools (one per KV head) of npages pages of `page` rows of D
+ * E4M3 bytes, q[H][npages][page][D], and one FP16 scale per page and head, s[H][npages].  The
+ * values are E4M3 (OCP: 0x7F and 0xFF are NaN, which w4_quantize_f8_pages never writes) times the
+ * page's scale.  No counterpart in the reference. */
+typedef struct w4_f8_pages_view {
+  int H, D, page, npages;
+  const uint8_t* q_k;
+  const w4_half* s_k;
+  const uint8_t* q_v;
+  const w4_half* s_v;
+} w4_f8_pages_view;
+
+/* A batch of sequences over such a cache (no counterpart in the reference).  All arrays are
+ * device memory: sizes of a step may change under a captured graph. */
+typedef struct w4_paged_batch {
+  int nseq;       /* sequences                                                          */
+  int tokens;     /* places for packed tokens (queries, slots); those behind the last
+                     sequence's are padding                                             */
+  int max_q;      /* no sequence has more new tokens than this                          */
+  int max_len;    /* no sequence has more tokens than this                              */
+  int bt_stride;  /* entries of a sequence's block table                                */
+  const int* bt;  /* [nseq][bt_stride] pages in order; an entry outside [0, npages)
+                     names no page                                                      */
+  const int* lens; /* [nseq] tokens of each sequence, the new ones among them           */
+  const int* cu_q; /* [nseq + 1] offsets of the sequences among the packed tokens; NULL:
+                      one token each (tokens == nseq, max_q == 1)                       */
+} w4_paged_batch;
+
 const char* w4_last_error(void);
 
 /* M at or above this goes to the matrix-core kernel in w4_gemm / w4_gemm_mx.
@@ -255,6 +283,59 @@ int w4_gemm_mx_w4a8(const w4_packed_mx_view* w, const w4_act_mx8_view* x,
  * nonzero for MXFP8 activations; arrays aligned to 16 bytes.  *plan: 0 no tiles; 1 - 4 eight-wave tiles
  * of 128 columns x 32 times as many activation rows; 8 tiles of 256 x 128. */
 int w4_gemm_mx_plan_for(int x8, int M, int N, int K, int* plan);
+
+/* ---- serving over a paged FP8 cache (no counterpart in the reference) ----------
+ * A step: w4_paged_tables plans where the new tokens go, w4_quantize_f8_pages writes
+ * them (once per layer), w4_attention_f8_pages attends (once per layer).  None of them
+ * reads anything back to the host, allocates or synchronises: a step can be captured. */
+
+/* Block tables and slots from request lengths.  `cached` tokens of each sequence are in
+ * the cache, whose pages the table batch->bt names; `added` more come.  Pages for them are
+ * taken in order from free_pages[free_range[0] .. free_range[1]).  Writes batch->bt (the
+ * new entries only), batch->lens (cached + added), batch->cu_q (offsets by `added`,
+ * required here) and, for each of batch->tokens places, its slot (row of its head's pool,
+ * page id * page + place; -1: none) and its position in its sequence (-1: none);
+ * result[0]: pages taken, result[1]: bit 0 the free pages ran out, bit 1 a length below
+ * zero or past its table, bit 2 more tokens than places.  A sequence that runs into one
+ * of these gets no page: its tokens have no slot, its length stays max(cached, 0), and
+ * its packed tokens keep their places.  A token whose page's entry is no page of the pool
+ * has no slot either.  max_q and max_len are not looked at; `cached` must not be the array
+ * lens.  slots and positions may be NULL when tokens == 0. */
+int w4_paged_tables(const w4_paged_batch* batch, int page, int npages, const int* cached,
+                    const int* added, const int* free_pages, const int* free_range,
+                    int* slots, int* positions, int* result, w4_stream stream);
+
+/* Writes new tokens into the cache: k, v are FP16, token t's rows of H * D elements at
+ * t * row_stride (0: H * D).  Token t goes to row slots[t] of each head's pool; negative
+ * slots and slots past the pool are skipped.  Tokens of one page stand side by side with
+ * ascending slots, as w4_paged_tables gives them, and no page appears twice.
+ *   scale(a) = the smallest half that is at least a / 448, a: the largest finite magnitude
+ *   a page begun in this call (its first new token is its row 0): s = scale(a)
+ *   an older page: s = s_old * 2^k, the smallest k >= 0 with s >= scale(a) (scale(a) where
+ *   s_old is 0); where k > 0 its older rows are rounded again to code * 2^-k, which
+ *   changes subnormal codes only
+ *   code = x / s rounded to nearest even, 0 where s is 0, +-448 for infinities, 0 for NaN
+ * (status, bit 0: there was one of those; the call ORs into the word and never clears it). */
+int w4_quantize_f8_pages(const w4_f8_pages_view* view, const w4_half* k, const w4_half* v,
+                         int row_stride, const int* slots, int tokens, int* status,
+                         w4_stream stream);
+
+/* Attention of packed queries over the pages.  q: token t's H * group heads of D elements
+ * at t * q_stride (0: H * group * D), `group` query heads per KV head side by side; out:
+ * [tokens][H * group][D].  A sequence's n = cu_q[s + 1] - cu_q[s] queries are its last n
+ * tokens: with `causal` the i-th sees positions up to lens[s] - n + i, without it all
+ * lens[s].  Positions whose table entry is no page of the pool are not seen (pages that
+ * were given back).  A query that sees nothing gives zeros; rows of `out` behind the last
+ * sequence's are left as they are.  Scores are scaled by 1 / sqrt(D).
+ * workspace: device memory of w4_attention_f8_pages_workspace() bytes, 16-byte aligned
+ * (NULL when that is 0); cleared once by the caller before its first use, every call
+ * leaves it ready for the next.  Calls that overlap (streams, graphs) need one each. */
+int w4_attention_f8_pages(const w4_f8_pages_view* view, const w4_paged_batch* batch, int group,
+                          int causal, const w4_half* q, int q_stride, w4_half* out,
+                          void* workspace, size_t workspace_bytes, w4_stream stream);
+/* Plain arithmetic: needs no GPU, reads no device memory. */
+int w4_attention_f8_pages_workspace(const w4_f8_pages_view* view, const w4_paged_batch* batch,
+                                    int group, size_t* bytes);
 
 #ifdef __cplusplus
 }

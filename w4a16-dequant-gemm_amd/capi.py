@@ -48,6 +48,16 @@ class KVF8View(C.Structure):
                 ("q_k", vp), ("s_k", vp), ("q_v", vp), ("s_v", vp)]
 
 
+class F8PagesView(C.Structure):
+    _fields_ = [("H", C.c_int), ("D", C.c_int), ("page", C.c_int), ("npages", C.c_int), ("q_k", vp), ("s_k", vp),
+                ("q_v", vp), ("s_v", vp)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("nseq", C.c_int), ("tokens", C.c_int), ("max_q", C.c_int), ("max_len", C.c_int), ("bt_stride", C.c_int),
+                ("bt", vp), ("lens", vp), ("cu_q", vp)]
+
+
 # every symbol include/w4_abi.h declares, with its argument types
 SIGNATURES = {
     "w4_last_error": ([], C.c_char_p),
@@ -86,6 +96,12 @@ SIGNATURES = {
     "w4_gemm_mx_plan_for": ([C.c_int] * 4 + [C.POINTER(C.c_int)], C.c_int),
     "w4_quantize_cache": ([C.POINTER(KVView), vp, vp, C.c_int, vp, vp], C.c_int),
     "w4_quantize_cache_f8": ([C.POINTER(KVF8View), vp, vp, C.c_int, vp, vp], C.c_int),
+    "w4_paged_tables": ([C.POINTER(PagedBatch), C.c_int, C.c_int] + [vp] * 8, C.c_int),
+    "w4_quantize_f8_pages": ([C.POINTER(F8PagesView), vp, vp, C.c_int, vp, C.c_int, vp, vp], C.c_int),
+    "w4_attention_f8_pages": ([C.POINTER(F8PagesView), C.POINTER(PagedBatch), C.c_int, C.c_int, vp, C.c_int, vp, vp,
+                               C.c_size_t, vp], C.c_int),
+    "w4_attention_f8_pages_workspace": ([C.POINTER(F8PagesView), C.POINTER(PagedBatch), C.c_int,
+                                         C.POINTER(C.c_size_t)], C.c_int),
 }
 
 _lib = None
@@ -130,6 +146,9 @@ _NATIVE = {
     "quantize_cache_f8": ("w4_quantize_cache_f8", "view k v src_f16 status stream"),
     "gemm_mx_w4a4": ("w4_gemm_mx_w4a4", None),
     "gemm_mx_w4a8": ("w4_gemm_mx_w4a8", None),
+    "paged_tables": ("w4_paged_tables", None),
+    "quantize_f8_pages": ("w4_quantize_f8_pages", None),
+    "attention_f8_pages": ("w4_attention_f8_pages", None),
 }
 
 
@@ -326,3 +345,35 @@ def gemm_mx_plan_for(x8, M, N, K):
     plan = C.c_int()
     check(load().w4_gemm_mx_plan_for(int(x8), M, N, K, C.byref(plan)))
     return plan.value
+
+
+# Serving over a paged FP8 cache: plan the pages of the new tokens, write them, attend.
+def f8_pages_view(H, D, page, npages, q_k, s_k, q_v, s_v):
+    return F8PagesView(H, D, page, npages, q_k or None, s_k or None, q_v or None, s_v or None)
+
+
+def paged_batch(nseq, tokens, max_q, max_len, bt, bt_stride, lens, cu_q=0):
+    return PagedBatch(nseq, tokens, max_q, max_len, bt_stride, bt or None, lens or None, cu_q or None)
+
+
+def paged_tables(batch, page, npages, cached, added, free_pages, free_range, slots, positions, result, stream=0):
+    """Block tables, lengths, offsets, slots and positions of a step; result: pages taken, status bits."""
+    check(load().w4_paged_tables(C.byref(batch), page, npages, _n(cached), _n(added), _n(free_pages), _n(free_range),
+                                 _n(slots), _n(positions), _n(result), _n(stream)))
+
+
+def quantize_f8_pages(view, k, v, row_stride, slots, tokens, status, stream=0):
+    """FP16 rows of new tokens into their slots; ORs bit 0 into `status` for non-finite input, never clears it."""
+    check(load().w4_quantize_f8_pages(C.byref(view), _n(k), _n(v), row_stride, _n(slots), tokens, _n(status), _n(stream)))
+
+
+def attention_f8_pages_workspace(view, batch, group):
+    """Bytes of device memory that attention_f8_pages needs, cleared once before its first call."""
+    n = C.c_size_t()
+    check(load().w4_attention_f8_pages_workspace(C.byref(view), C.byref(batch), group, C.byref(n)))
+    return n.value
+
+
+def attention_f8_pages(view, batch, group, causal, q, q_stride, out, workspace=0, workspace_bytes=0, stream=0):
+    check(load().w4_attention_f8_pages(C.byref(view), C.byref(batch), group, int(causal), _n(q), q_stride, _n(out),
+                                       _n(workspace), workspace_bytes, _n(stream)))

@@ -619,6 +619,105 @@ int w4_quantize_cache_f8(const w4_kv_f8_view* out, const void* k, const void* v,
                                         out->gs, status, (hipStream_t)stream));
 }
 
+// ---- serving over a paged FP8 cache -------------------------------------------------
+
+static int check_pages(const w4_f8_pages_view* p, const char* who) {
+  static thread_local char buf[96];
+#define PG(cond, text)                                \
+  do {                                                \
+    if (!(cond)) {                                    \
+      snprintf(buf, sizeof buf, "%s: %s", who, text); \
+      return invalid(buf);                            \
+    }                                                 \
+  } while (0)
+  PG(p != nullptr, "null view");
+  PG(p->H >= 1 && p->D >= 1, "bad dims");
+  PG(p->H <= 65535, "too many heads");
+  PG(p->D <= 512, "D exceeds the 512-element bound");
+  PG(p->D % 4 == 0, "D must be a multiple of 4");
+  PG(p->page >= 1 && p->npages >= 1 && (long long)p->npages * p->page < (1LL << 31), "bad page geometry");
+  PG(p->q_k && p->s_k && p->q_v && p->s_v, "null pointer");
+  PG((((uintptr_t)p->q_k | (uintptr_t)p->q_v) & 3) == 0, "cache bases 4-byte aligned");
+#undef PG
+  return W4_OK;
+}
+
+int w4_paged_tables(const w4_paged_batch* b, int page, int npages, const int* cached, const int* added,
+                    const int* free_pages, const int* free_range, int* slots, int* positions, int* result,
+                    w4_stream stream) {
+  REQUIRE(b != nullptr, "paged tables: null batch");
+  REQUIRE(b->nseq >= 1 && b->tokens >= 0 && b->bt_stride >= 1, "paged tables: bad dims");
+  REQUIRE(page >= 1 && npages >= 1 && (long long)npages * page < (1LL << 31), "paged tables: bad page geometry");
+  REQUIRE(b->bt && b->lens && b->cu_q && cached && added && free_pages && free_range && result,
+          "paged tables: null pointer");
+  REQUIRE(b->tokens == 0 || (slots && positions), "paged tables: null slots or positions");
+  REQUIRE(cached != b->lens && added != b->lens, "paged tables: lens is an output, not the cached or added lengths");
+  const w4k::PagedTables a{b->nseq, page, npages, b->bt_stride, b->tokens, (int*)b->bt, cached, added, free_pages,
+                           free_range, (int*)b->lens, (int*)b->cu_q, slots, positions, result};
+  return done("paged_tables", w4k::launch_paged_tables(a, (hipStream_t)stream));
+}
+
+int w4_quantize_f8_pages(const w4_f8_pages_view* p, const w4_half* k, const w4_half* v, int row_stride,
+                         const int* slots, int tokens, int* status, w4_stream stream) {
+  if (int rc = check_pages(p, "quantize_f8_pages")) return rc;
+  REQUIRE(tokens >= 0, "quantize_f8_pages: bad dims");
+  REQUIRE(k && v && status && (slots || tokens == 0), "quantize_f8_pages: null io pointer");
+  REQUIRE(row_stride == 0 || row_stride >= (long long)p->H * p->D, "quantize_f8_pages: row_stride is shorter than a row");
+  REQUIRE((long long)tokens * 2 * p->H < (1LL << 30), "quantize_f8_pages: too many rows");
+  if (tokens == 0) return W4_OK;
+  const long long stride = row_stride ? row_stride : (long long)p->H * p->D;
+  return done("quantize_f8_pages",
+              w4k::launch_quantize_f8_pages(*p, k, v, stride, slots, tokens, status, (hipStream_t)stream));
+}
+
+static int pages_args(w4k::PagesArgs& a, const w4_f8_pages_view* p, const w4_paged_batch* b, int group) {
+  if (int rc = check_pages(p, "attention f8 pages")) return rc;
+  REQUIRE(b != nullptr, "attention f8 pages: null batch");
+  REQUIRE(b->nseq >= 1 && b->tokens >= 0 && b->max_q >= 1 && b->max_len >= 1 && b->bt_stride >= 1,
+          "attention f8 pages: bad dims");
+  REQUIRE(b->bt && b->lens, "attention f8 pages: null pointer");
+  REQUIRE(b->cu_q || (b->tokens == b->nseq && b->max_q == 1), "attention f8 pages: several tokens per sequence need cu_q");
+  REQUIRE(group >= 1 && group <= 64, "attention f8 pages: bad query group");
+  REQUIRE((long long)b->nseq * p->H < (1LL << 31) && (long long)b->tokens * p->H * group < (1LL << 31),
+          "attention f8 pages: too many rows");
+  a = w4k::PagesArgs{};
+  a.H = p->H; a.D = p->D; a.page = p->page; a.npages = p->npages;
+  a.q_k = p->q_k; a.s_k = p->s_k; a.q_v = p->q_v; a.s_v = p->s_v;
+  a.nseq = b->nseq; a.tokens = b->tokens; a.max_q = b->max_q; a.stride = b->bt_stride;
+  // (no position past a table is looked at)
+  const long long in_table = (long long)b->bt_stride * p->page;
+  a.max_len = in_table < b->max_len ? (int)in_table : b->max_len;
+  a.bt = b->bt; a.lens = b->lens; a.cu = b->cu_q;
+  a.group = group;
+  return W4_OK;
+}
+
+int w4_attention_f8_pages_workspace(const w4_f8_pages_view* p, const w4_paged_batch* b, int group, size_t* bytes) {
+  w4k::PagesArgs a;
+  if (int rc = pages_args(a, p, b, group)) return rc;
+  REQUIRE(bytes != nullptr, "attention f8 pages: null pointer");
+  *bytes = w4k::pages_attention_space(a);
+  return W4_OK;
+}
+
+int w4_attention_f8_pages(const w4_f8_pages_view* p, const w4_paged_batch* b, int group, int causal, const w4_half* q,
+                          int q_stride, w4_half* out, void* workspace, size_t workspace_bytes, w4_stream stream) {
+  w4k::PagesArgs a;
+  if (int rc = pages_args(a, p, b, group)) return rc;
+  REQUIRE(q && out, "attention f8 pages: null io pointer");
+  REQUIRE(causal == 0 || causal == 1, "attention f8 pages: causal is 0 or 1");
+  const long long row = (long long)p->H * group * p->D;
+  REQUIRE(q_stride == 0 || q_stride >= row, "attention f8 pages: q_stride is shorter than a token");
+  const size_t need = w4k::pages_attention_space(a);
+  REQUIRE(workspace_bytes >= need && (workspace || !need), "attention f8 pages: workspace too small");
+  REQUIRE(((uintptr_t)workspace & 15) == 0, "attention f8 pages: workspace 16-byte aligned");
+  if (b->tokens == 0) return W4_OK;
+  a.causal = causal;
+  a.q = q; a.q_stride = q_stride ? q_stride : row; a.out = out;
+  a.space = (char*)workspace;
+  return done("attention_f8_pages", w4k::launch_pages_attention(a, (hipStream_t)stream));
+}
+
 }  // extern "C"
 
 // ---- two-pass baseline -------------------------------------------------------------

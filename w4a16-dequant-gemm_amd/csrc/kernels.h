@@ -186,4 +186,36 @@ int mx_plan(bool x8, int M, int N, int K);
 hipError_t launch_quantize_mx8(const void* src, int src_f16, long long rows, int K, uint8_t* q,
                                uint8_t* scales, int* status, hipStream_t s);
 
+// ---- serving over a paged FP8 cache ----------------------------------------------------
+// paged_tables.hip
+struct PagedTables {
+  int nseq, page, npages, stride, tokens;
+  int* bt;
+  const int *cached, *added, *free_pages, *free_range;
+  int *lens, *cu, *slots, *positions, *result;
+};
+hipError_t launch_paged_tables(const PagedTables& a, hipStream_t s);
+
+// quantize_pages.hip
+hipError_t launch_quantize_f8_pages(const w4_f8_pages_view& p, const w4_half* k, const w4_half* v, long long row_stride,
+                                    const int* slots, int tokens, int* status, hipStream_t s);
+
+// pages_attention.hip
+struct PagesArgs {
+  int H, D, page, npages;
+  const uint8_t* q_k;
+  const w4_half* s_k;
+  const uint8_t* q_v;
+  const w4_half* s_v;
+  int nseq, tokens, max_q, max_len, stride;
+  const int *bt, *lens, *cu;
+  int group, causal;
+  const w4_half* q;
+  long long q_stride;
+  w4_half* out;
+  char* space;
+};
+size_t pages_attention_space(const PagesArgs& a);
+hipError_t launch_pages_attention(const PagesArgs& a, hipStream_t s);
+
 }  // namespace w4k

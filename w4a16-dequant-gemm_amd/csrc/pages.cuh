@@ -1,0 +1,72 @@
+// What the kernels of paged FP8 attention share: which rows a sequence has, where a position lies, and
+// how the parts of a row that several workgroups formed are joined.
+//
+// A row is one query token and head.  For position t on page p with scales sk, sv and a row's raw dot product s of
+// codes, its score in units of log2 is x = s sk c, c = log2(e) / sqrt(D), and its weight on the raw V codes is
+// 2^x sv.  Sums are kept relative to M, the running maximum of x + log2(sv): the weights that enter the matrix
+// product in FP16 then stay at most 1 whatever the scales are, and the denominators, 2^(x - M), stay in FP32.
+// (Relative to the maximum of x alone, weights of pages whose V scale is small would fall below FP16's range.)
+#pragma once
+
+#include "dq.cuh"
+#include "kernels.h"
+
+namespace w4k {
+
+constexpr float PG_LOG2_FLOOR = -24.0f;  // of a page's V scale: below the smallest half (a scale of 0 weighs nothing)
+
+struct PagesPlan {
+  int split_len, nsplit;  // positions per split, splits of the longest sequence
+};
+
+struct Pages : PagesArgs {
+  uint32_t magic;  // page_of()
+  int shift;
+  PagesPlan plan;
+  float* part;  // [row][split][D + 2]: M, denominator, O
+};
+
+// t / page for 0 <= t < 2^31
+__device__ __forceinline__ int page_of(const Pages& a, int t) { return (int)(__umulhi(2u * (uint32_t)t, a.magic) >> a.shift); }
+inline void set_page(Pages& a) {
+  a.shift = 0;
+  while ((1ll << a.shift) < a.page) ++a.shift;
+  a.magic = (uint32_t)((1ull << (31 + a.shift)) / (uint32_t)a.page + 1);
+}
+
+// Sequence that holds packed token `tok`; -1: none.
+__device__ __forceinline__ int sequence_of(const Pages& a, int tok) {
+  if (!a.cu) return tok < a.nseq ? tok : -1;
+  int lo = 0, hi = a.nseq;  // cu[lo] <= tok < cu[hi]
+  if (tok < a.cu[0] || tok >= a.cu[a.nseq]) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu[mid] <= tok) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A sequence's queries and positions.  What lies outside the packed tokens, the tables or the bounds of the
+// call is left out.
+struct Seq {
+  int q0, n, len, shown;  // first packed token, tokens, positions; the first token sees shown positions, each next one more
+};
+__device__ __forceinline__ Seq sequence(const Pages& a, int s) {
+  Seq q;
+  q.q0 = a.cu ? a.cu[s] : s;
+  const int end = a.cu ? a.cu[s + 1] : s + 1;
+  q.n = q.q0 < 0 ? 0 : min(min(end, a.tokens) - q.q0, a.max_q);
+  const int len = a.lens[s];
+  q.len = max(0, min(len, a.max_len));
+  q.shown = a.causal ? len - (end - q.q0) + 1 : q.len;
+  return q;
+}
+
+__device__ __forceinline__ float f8_to_float(uint32_t b) {
+  const float m = __builtin_bit_cast(float, (b & 0x7Fu) << 20) * 0x1p120f;
+  const float v = (b & 0x7Fu) == 0x7Fu ? __builtin_nanf("") : m;
+  return b & 0x80u ? -v : v;
+}
+
+}  // namespace w4k

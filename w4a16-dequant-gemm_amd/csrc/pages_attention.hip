@@ -1,0 +1,152 @@
+// Attention of packed queries over a paged FP8 cache: plan, general kernel, and the join of split rows.
+#include "pages.cuh"
+
+namespace w4k {
+namespace {
+
+// ---- any head dimension, page size and alignment -----------------------------------------------
+// One workgroup per row and split, tiles of 256 positions: a thread forms one position's score, then owns four
+// columns of O for every (256 / (D / 4))-th position of the tile.
+__global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
+  __shared__ float qs[512], red[4], weight[256], o4[256][4];
+  __shared__ long long at[256];  // offset of a position's row in the codes; -1: not seen
+  const int tid = threadIdx.x, D = a.D, heads = a.H * a.group;
+  const int tok = (int)(blockIdx.x / heads), head = (int)(blockIdx.x % heads), h = head / a.group;
+  const int s = sequence_of(a, tok);
+  if (s < 0) return;
+  const Seq q = sequence(a, s);
+  const int i = tok - q.q0;
+  if (i >= q.n) return;
+  const int end = min(q.len, a.causal ? q.shown + i : q.len);  // positions that the row sees
+  const int ns = max(1, (q.len + a.plan.split_len - 1) / a.plan.split_len);
+  const int split = blockIdx.y;
+  if (split >= ns) return;
+  const int s0 = split * a.plan.split_len, s1 = min(end, s0 + a.plan.split_len);
+  const float c = 1.44269504088896340736f / sqrtf((float)D);
+  const uint8_t* const kp = a.q_k + (long long)h * a.npages * a.page * D;
+  const uint8_t* const vp = a.q_v + (long long)h * a.npages * a.page * D;
+  for (int d = tid; d < D; d += 256) qs[d] = half_bits_to_float(a.q[(long long)tok * a.q_stride + (long long)head * D + d]);
+  const int cols = D / 4, groups = 256 / cols, g = tid / cols, col = tid - g * cols;
+  float M = -INFINITY, l = 0.0f, o[4] = {};
+  __syncthreads();
+  for (int t0 = s0; t0 < s1; t0 += 256) {
+    const int t = t0 + tid;
+    float x = -INFINITY, y = -INFINITY, sv = 0.0f;
+    long long off = -1;
+    if (t < s1) {
+      const int j = page_of(a, t);
+      const int id = a.bt[(long long)s * a.stride + j];
+      if (id >= 0 && id < a.npages) {
+        off = ((long long)id * a.page + (t - j * a.page)) * D;
+        const uint32_t* const row = (const uint32_t*)(kp + off);
+        float dot = 0.0f;
+        for (int d = 0; d < D; d += 4) {
+          const uint32_t w = row[d / 4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(qs[d + e], f8_to_float((w >> (8 * e)) & 0xFFu), dot);
+        }
+        sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
+        x = dot * (half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c);
+        y = x + fmaxf(__log2f(sv), PG_LOG2_FLOOR);
+      }
+    }
+    at[tid] = off;
+    float m = y;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    const float m_new = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), M);
+    const float use = m_new == -INFINITY ? 0.0f : m_new;
+    const float alpha = exp2f(M - use);
+    const float p = off >= 0 ? exp2f(x - use) : 0.0f;
+    weight[tid] = p * sv;
+    M = m_new;
+    l = l * alpha + p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= alpha;
+    __syncthreads();
+    if (g < groups) {
+      const int here = min(256, s1 - t0);
+      for (int k = g; k < here; k += groups)
+        if (at[k] >= 0) {
+          const uint32_t w = *(const uint32_t*)(vp + at[k] + 4 * col);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(weight[k], f8_to_float((w >> (8 * e)) & 0xFFu), o[e]);
+        }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+  if ((tid & 63) == 0) red[tid >> 6] = l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o4[tid][e] = o[e];
+  __syncthreads();
+  l = red[0] + red[1] + red[2] + red[3];
+  const long long row = (long long)tok * heads + head;
+  float* const part = a.part + (row * a.plan.nsplit + split) * (D + 2);
+  for (int d = tid; d < D; d += 256) {
+    float sum = 0.0f;
+    for (int k = 0; k < groups; ++k) sum += o4[k * cols + d / 4][d & 3];
+    if (ns > 1) part[2 + d] = sum;
+    else a.out[row * D + d] = __builtin_bit_cast(uint16_t, (_Float16)(l == 0.0f ? 0.0f : sum / l));
+  }
+  if (ns > 1 && tid == 0) part[0] = M, part[1] = l;
+}
+
+// ---- rows that several workgroups formed ----------------------------------------------------------
+__global__ __launch_bounds__(128) void pages_join_kernel(const Pages a) {
+  const int D = a.D, heads = a.H * a.group;
+  const int tok = (int)(blockIdx.x / heads), head = (int)(blockIdx.x % heads);
+  const int s = sequence_of(a, tok);
+  if (s < 0) return;
+  const Seq q = sequence(a, s);
+  const int ns = (q.len + a.plan.split_len - 1) / a.plan.split_len;
+  if (tok - q.q0 >= q.n || ns <= 1) return;
+  const long long row = (long long)tok * heads + head;
+  const float* const part = a.part + row * a.plan.nsplit * (D + 2);
+  float M = -INFINITY;
+  for (int k = 0; k < ns; ++k) M = fmaxf(M, part[(long long)k * (D + 2)]);
+  const float use = M == -INFINITY ? 0.0f : M;
+  float l = 0.0f;
+  for (int k = 0; k < ns; ++k) l += exp2f(part[(long long)k * (D + 2)] - use) * part[(long long)k * (D + 2) + 1];
+  for (int d = threadIdx.x; d < D; d += 128) {
+    float sum = 0.0f;
+    for (int k = 0; k < ns; ++k) sum += exp2f(part[(long long)k * (D + 2)] - use) * part[(long long)k * (D + 2) + 2 + d];
+    a.out[row * D + d] = __builtin_bit_cast(uint16_t, (_Float16)(l == 0.0f ? 0.0f : sum / l));
+  }
+}
+
+PagesPlan plan_of(const PagesArgs& a) {
+  // enough splits for four workgroups per compute unit, none shorter than a tile
+  const long long rows = (long long)a.tokens * a.H * a.group;
+  const int most = (a.max_len + 255) / 256;
+  long long n = rows > 0 ? 1024 / rows : 1;
+  n = n < 1 ? 1 : n > most ? most : n;
+  PagesPlan p;
+  p.split_len = (int)(((a.max_len + n - 1) / n + 255) / 256 * 256);
+  p.nsplit = (a.max_len + p.split_len - 1) / p.split_len;
+  return p;
+}
+
+}  // namespace
+
+size_t pages_attention_space(const PagesArgs& a) {
+  const PagesPlan p = plan_of(a);
+  return p.nsplit > 1 ? (size_t)a.tokens * a.H * a.group * p.nsplit * (a.D + 2) * sizeof(float) : 0;
+}
+
+hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
+  Pages a;
+  (PagesArgs&)a = args;
+  set_page(a);
+  a.plan = plan_of(args);
+  a.part = (float*)a.space;
+  const unsigned rows = (unsigned)((long long)a.tokens * a.H * a.group);
+  pages_general_kernel<<<dim3(rows, a.plan.nsplit), 256, 0, s>>>(a);
+  if (a.plan.nsplit > 1) pages_join_kernel<<<rows, 128, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace w4k

@@ -1,0 +1,209 @@
+// New tokens into a paged FP8 cache: FP16 rows to E4M3 under one FP16 scale per (page, head, side).
+//
+// A unit of L lanes owns one run -- the new tokens of one page, which stand side by side in the slot list --
+// of one head and side, so nothing is shared between units: it finds the run's length, the largest magnitude of
+// its rows (kept in registers: one pass over the data), the page's scale, and writes the codes.
+//   scale: the smallest half >= amax / 448, so nothing saturates; an older page's scale is only ever raised, by
+//   a power of two, which leaves the codes of its older rows what they were in value but for subnormals --
+//   raised to the new maximum itself, a page of n tokens would round its first rows up to n times.
+//   code: RNE(x / s).  Quotients of two halves are exact ties or 2^-17 away from one, so a quotient that is right
+//   to the last bit of an FP32 is enough; x * (1 / s) with one residual step is.
+// Bound: HBM for prompts (6 bytes per element and side); latency for a decode step.
+#include "dq.cuh"
+#include "kernels.h"
+
+namespace w4k {
+namespace {
+
+constexpr int QP_KEEP = 8;  // pieces of 8 elements that a lane keeps between the two steps
+
+struct QuantPages {
+  const w4_half *k, *v;
+  uint8_t *q_k, *q_v;
+  w4_half *s_k, *s_v;
+  const int* slots;
+  int* status;
+  long long row_stride;
+  int H, D, page, npages, tokens;
+  int chunk;  // tokens whose runs a unit looks for
+  uint32_t units;
+};
+
+__device__ __forceinline__ float half_up(float amax) {
+  const float want = amax / 448.0f;
+  const uint16_t h = __builtin_bit_cast(uint16_t, (_Float16)want);
+  const float f = half_bits_to_float(h);
+  return f * 448.0f < amax ? half_bits_to_float(h + 1) : f;  // (11 bits times 3: exact)
+}
+
+// Largest finite magnitude of eight halves, as FP32 bits' order-preserving integers; `odd`: one was not finite.
+__device__ __forceinline__ uint32_t finite_max(const u4& x, uint32_t m, bool& odd) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = x[i] & 0x7FFFu, hi = (x[i] >> 16) & 0x7FFFu;
+    if (lo >= 0x7C00u || hi >= 0x7C00u) {
+      odd = true;
+      if (lo < 0x7C00u) m = max(m, lo);
+      if (hi < 0x7C00u) m = max(m, hi);
+    } else {
+      m = max(m, max(lo, hi));
+    }
+  }
+  return m;
+}
+
+// Four codes of x / s; r = 1 / s, 0 where s is 0.
+__device__ __forceinline__ uint32_t encode4(const float* x, float s, float r) {
+  float q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[i] * r;
+    q[i] = copysignf(__builtin_fmaf(__builtin_fmaf(-a, s, x[i]), r, a), x[i]);  // (-0 stays what it is)
+    if (!(fabsf(x[i]) <= 65504.0f)) q[i] = x[i] != x[i] || r == 0.0f ? 0.0f : x[i];
+    q[i] = fminf(fmaxf(q[i], -448.0f), 448.0f);
+  }
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+}
+
+// Four codes times a power of two below 1; NaN codes keep their byte.
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float f) {
+  float x[4];
+  uint32_t nan = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t b = (w >> (8 * i)) & 0xFFu;
+    // bits 6..0 as exponent and significand are 2^-120 times the E4M3 value, subnormals included
+    const float mag = __builtin_bit_cast(float, (b & 0x7Fu) << 20) * 0x1p120f * f;
+    x[i] = b & 0x80u ? -mag : mag;
+    if ((b & 0x7Fu) == 0x7Fu) nan |= 0xFFu << (8 * i);
+  }
+  int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return ((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], p, true) & ~nan) | (w & nan);
+}
+
+// VEC: elements of a piece (8: 16-byte loads; 4: rows of any alignment).  L: lanes of a unit.
+template <int VEC, int L>
+__global__ __launch_bounds__(256) void quantize_pages_kernel(const QuantPages a) {
+  const uint32_t unit = (blockIdx.x * 256u + threadIdx.x) / L;
+  if (unit >= a.units) return;  // (a unit's lanes leave together)
+  const int lane = threadIdx.x & (L - 1);
+  const uint32_t sides = 2u * a.H;
+  const int c0 = (int)(unit / sides) * a.chunk, c1 = min(c0 + a.chunk, a.tokens);
+  const uint32_t hs = unit % sides;
+  const int h = (int)(hs >> 1);
+  const bool vside = hs & 1;
+  const w4_half* const src = (vside ? a.v : a.k) + (long long)h * a.D;
+  uint8_t* const pool = (vside ? a.q_v : a.q_k) + (long long)h * a.npages * a.page * a.D;
+  w4_half* const scales = (vside ? a.s_v : a.s_k) + (long long)h * a.npages;
+  const int rows = a.npages * a.page;
+  const int per_row = a.D / VEC;
+
+  int prev = c0 ? a.slots[c0 - 1] : -1;
+  for (int t = c0; t < c1;) {
+    const int slot = a.slots[t];
+    if (slot < 0 || slot >= rows) {
+      prev = -1;
+      ++t;
+      continue;
+    }
+    const int pg = slot / a.page, r0 = slot - pg * a.page;
+    if (prev >= 0 && prev + 1 == slot && r0) {  // inside a run that another unit, or an earlier step, has
+      prev = slot;
+      ++t;
+      continue;
+    }
+    // length of the run
+    const int room = min(a.page - r0, a.tokens - t);
+    int n = 1;
+    while (n < room) {
+      const int j = n + lane;
+      const bool more = j < room && a.slots[t + min(j, room - 1)] == slot + j;
+      const unsigned long long all = __builtin_amdgcn_ballot_w64(more);
+      const uint32_t base = (threadIdx.x & 63) & ~(L - 1);
+      const unsigned long long ours = L == 64 ? all : (all >> base) & ((1ull << (L & 63)) - 1);
+      const int got = L == 64 ? (ours == ~0ull ? 64 : __builtin_ctzll(~ours)) : __builtin_ctzll(~ours);
+      n += got;
+      if (got < L) break;
+    }
+    // ---- the largest magnitude
+    const int pieces = n * per_row;
+    u4 keep[QP_KEEP];
+    uint32_t top = 0;
+    bool odd = false;
+    auto load = [&](int e) -> u4 {
+      const int r = e / per_row, d = (e - r * per_row) * VEC;
+      const w4_half* const p = src + (long long)(t + r) * a.row_stride + d;
+      if constexpr (VEC == 8) {
+        return *(const u4*)p;
+      } else {
+        return u4{p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, 0u, 0u};
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < QP_KEEP; ++i) {
+      const int e = lane + i * L;
+      keep[i] = e < pieces ? load(e) : u4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int i = 0; i < QP_KEEP; ++i) top = finite_max(keep[i], top, odd);
+    for (int e = lane + QP_KEEP * L; e < pieces; e += L) top = finite_max(load(e), top, odd);
+#pragma unroll
+    for (int d = L / 2; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    if (odd) atomicOr(a.status, 1);
+    // ---- the page's scale
+    float s = half_up(half_bits_to_float(top)), lowered = 1.0f;
+    if (r0) {
+      const float old = half_bits_to_float(scales[pg]);
+      if (old > 0.0f) {
+        float now = old;
+        while (now < s) now *= 2.0f, lowered *= 0.5f;
+        s = now;
+      }
+    }
+    uint8_t* const at = pool + (long long)pg * a.page * a.D;
+    if (lowered < 1.0f) {  // older rows under the raised scale
+      const int words = r0 * (a.D / 4);
+      for (int e = lane; e < words; e += L) ((uint32_t*)at)[e] = recode4(((const uint32_t*)at)[e], lowered);
+    }
+    // ---- the codes
+    const float r = s > 0.0f ? 1.0f / s : 0.0f;
+    auto store = [&](int e, const u4& x) {
+      uint32_t w[2];
+#pragma unroll
+      for (int p = 0; p < VEC / 4; ++p) {
+        float f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = half_bits_to_float((x[2 * p + (i >> 1)] >> (16 * (i & 1))) & 0xFFFFu);
+        w[p] = encode4(f, s, r);
+      }
+      uint8_t* const dst = at + (long long)r0 * a.D + (long long)e * VEC;
+      if constexpr (VEC == 8) *(u2*)dst = u2{w[0], w[1]};
+      else *(uint32_t*)dst = w[0];
+    };
+#pragma unroll
+    for (int i = 0; i < QP_KEEP; ++i)
+      if (lane + i * L < pieces) store(lane + i * L, keep[i]);
+    for (int e = lane + QP_KEEP * L; e < pieces; e += L) store(e, load(e));
+    if (lane == 0) scales[pg] = __builtin_bit_cast(uint16_t, (_Float16)s);
+    prev = slot + n - 1;
+    t += n;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_quantize_f8_pages(const w4_f8_pages_view& p, const w4_half* k, const w4_half* v, long long row_stride,
+                                    const int* slots, int tokens, int* status, hipStream_t s) {
+  QuantPages a{k, v, (uint8_t*)p.q_k, (uint8_t*)p.q_v, (w4_half*)p.s_k, (w4_half*)p.s_v, slots, status, row_stride,
+               p.H, p.D, p.page, p.npages, tokens, 1, 0};
+  const bool wide = p.D % 8 == 0 && row_stride % 8 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0 &&
+                    (((uintptr_t)p.q_k | (uintptr_t)p.q_v) & 7) == 0;
+  const long long units = (long long)tokens * 2 * p.H;
+  a.units = (uint32_t)units;
+  if (wide) quantize_pages_kernel<8, 64><<<(unsigned)((units * 64 + 255) / 256), 256, 0, s>>>(a);
+  else quantize_pages_kernel<4, 64><<<(unsigned)((units * 64 + 255) / 256), 256, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+}  // namespace w4k
