@@ -19,12 +19,20 @@ struct PagesPlan {
   int split_len, nsplit;  // positions per split, splits of the longest sequence
 };
 
+// Sequences of up to few_rows rows per KV head are the kernel's for few rows, the others the one for many.
 struct Pages : PagesArgs {
   uint32_t magic;  // page_of()
   int shift;
-  PagesPlan plan;
-  float* part;  // [row][split][D + 2]: M, denominator, O
+  int few_rows;
+  PagesPlan few, many;
+  int slots;    // splits of a row that the workspace has room for
+  float* part;  // [row][slots][D + 2]: M, denominator, O
 };
+
+// pages_few.hip.  Most rows of a sequence and KV head that its kernel takes; 0: not this call's dimensions.
+int pages_few_most(const PagesArgs& a);
+PagesPlan pages_few_plan(const PagesArgs& a, int rows);
+hipError_t launch_pages_few(const Pages& a, hipStream_t s);
 
 // t / page for 0 <= t < 2^31
 __device__ __forceinline__ int page_of(const Pages& a, int t) { return (int)(__umulhi(2u * (uint32_t)t, a.magic) >> a.shift); }
@@ -61,6 +69,11 @@ __device__ __forceinline__ Seq sequence(const Pages& a, int s) {
   q.len = max(0, min(len, a.max_len));
   q.shown = a.causal ? len - (end - q.q0) + 1 : q.len;
   return q;
+}
+
+__device__ __forceinline__ int splits(const PagesPlan& p, int len) { return (len + p.split_len - 1) / p.split_len; }
+__device__ __forceinline__ float* part_of(const Pages& a, long long row, int split) {
+  return a.part + (row * a.slots + split) * (a.D + 2);
 }
 
 __device__ __forceinline__ float f8_to_float(uint32_t b) {

@@ -16,12 +16,12 @@ __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
   if (s < 0) return;
   const Seq q = sequence(a, s);
   const int i = tok - q.q0;
-  if (i >= q.n) return;
+  if (i >= q.n || q.n * a.group <= a.few_rows) return;
   const int end = min(q.len, a.causal ? q.shown + i : q.len);  // positions that the row sees
-  const int ns = max(1, (q.len + a.plan.split_len - 1) / a.plan.split_len);
+  const int ns = max(1, splits(a.many, q.len));
   const int split = blockIdx.y;
   if (split >= ns) return;
-  const int s0 = split * a.plan.split_len, s1 = min(end, s0 + a.plan.split_len);
+  const int s0 = split * a.many.split_len, s1 = min(end, s0 + a.many.split_len);
   const float c = 1.44269504088896340736f / sqrtf((float)D);
   const uint8_t* const kp = a.q_k + (long long)h * a.npages * a.page * D;
   const uint8_t* const vp = a.q_v + (long long)h * a.npages * a.page * D;
@@ -85,7 +85,7 @@ __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
   __syncthreads();
   l = red[0] + red[1] + red[2] + red[3];
   const long long row = (long long)tok * heads + head;
-  float* const part = a.part + (row * a.plan.nsplit + split) * (D + 2);
+  float* const part = part_of(a, row, split);
   for (int d = tid; d < D; d += 256) {
     float sum = 0.0f;
     for (int k = 0; k < groups; ++k) sum += o4[k * cols + d / 4][d & 3];
@@ -102,10 +102,10 @@ __global__ __launch_bounds__(128) void pages_join_kernel(const Pages a) {
   const int s = sequence_of(a, tok);
   if (s < 0) return;
   const Seq q = sequence(a, s);
-  const int ns = (q.len + a.plan.split_len - 1) / a.plan.split_len;
+  const int ns = splits(q.n * a.group <= a.few_rows ? a.few : a.many, q.len);
   if (tok - q.q0 >= q.n || ns <= 1) return;
   const long long row = (long long)tok * heads + head;
-  const float* const part = a.part + row * a.plan.nsplit * (D + 2);
+  const float* const part = part_of(a, row, 0);
   float M = -INFINITY;
   for (int k = 0; k < ns; ++k) M = fmaxf(M, part[(long long)k * (D + 2)]);
   const float use = M == -INFINITY ? 0.0f : M;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(128) void pages_join_kernel(const Pages a) {
   }
 }
 
-PagesPlan plan_of(const PagesArgs& a) {
+PagesPlan general_plan(const PagesArgs& a) {
   // enough splits for four workgroups per compute unit, none shorter than a tile
   const long long rows = (long long)a.tokens * a.H * a.group;
   const int most = (a.max_len + 255) / 256;
@@ -130,23 +130,47 @@ PagesPlan plan_of(const PagesArgs& a) {
   return p;
 }
 
+// Which kernels take the call's sequences, and how they split them.
+void plan(Pages& a) {
+  const int most = pages_few_most(a);
+  const long long rows = (long long)a.max_q * a.group;
+  a.few = a.many = PagesPlan{a.max_len, 1};
+  a.few_rows = 0;
+  if (rows <= most) a.few_rows = (int)rows;                               // every sequence
+  else if (a.group <= most && a.nseq > 1) a.few_rows = a.group;           // decoding ones next to prompts
+  if (a.few_rows) a.few_rows = (a.few_rows + 15) / 16 * 16;
+  if (a.few_rows) a.few = pages_few_plan(a, a.few_rows);
+  if (rows > a.few_rows) a.many = general_plan(a);
+  a.slots = a.few.nsplit > a.many.nsplit ? a.few.nsplit : a.many.nsplit;
+}
+
 }  // namespace
 
-size_t pages_attention_space(const PagesArgs& a) {
-  const PagesPlan p = plan_of(a);
-  return p.nsplit > 1 ? (size_t)a.tokens * a.H * a.group * p.nsplit * (a.D + 2) * sizeof(float) : 0;
+size_t pages_attention_space(const PagesArgs& args) {
+  Pages a;
+  (PagesArgs&)a = args;
+  plan(a);
+  return a.slots > 1 ? (size_t)a.tokens * a.H * a.group * a.slots * (a.D + 2) * sizeof(float) : 0;
 }
 
 hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   Pages a;
   (PagesArgs&)a = args;
   set_page(a);
-  a.plan = plan_of(args);
+  plan(a);
   a.part = (float*)a.space;
   const unsigned rows = (unsigned)((long long)a.tokens * a.H * a.group);
-  pages_general_kernel<<<dim3(rows, a.plan.nsplit), 256, 0, s>>>(a);
-  if (a.plan.nsplit > 1) pages_join_kernel<<<rows, 128, 0, s>>>(a);
-  return hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (a.few_rows) e = launch_pages_few(a, s);
+  if (e == hipSuccess && (long long)a.max_q * a.group > a.few_rows) {
+    pages_general_kernel<<<dim3(rows, a.many.nsplit), 256, 0, s>>>(a);
+    e = hipGetLastError();
+  }
+  if (e == hipSuccess && a.slots > 1) {
+    pages_join_kernel<<<rows, 128, 0, s>>>(a);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 }  // namespace w4k
