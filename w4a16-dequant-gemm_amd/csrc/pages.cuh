@@ -13,8 +13,6 @@
 
 namespace w4k {
 
-constexpr float PG_LOG2_FLOOR = -24.0f;  // of a page's V scale: below the smallest half (a scale of 0 weighs nothing)
-
 struct PagesPlan {
   int split_len, nsplit;  // positions per split, splits of the longest sequence
 };
@@ -33,6 +31,10 @@ struct Pages : PagesArgs {
 int pages_few_most(const PagesArgs& a);
 PagesPlan pages_few_plan(const PagesArgs& a, int rows);
 hipError_t launch_pages_few(const Pages& a, hipStream_t s);
+// pages_many.hip
+bool pages_many_applies(const PagesArgs& a);
+PagesPlan pages_many_plan(const PagesArgs& a);
+hipError_t launch_pages_many(const Pages& a, hipStream_t s);
 
 // t / page for 0 <= t < 2^31
 __device__ __forceinline__ int page_of(const Pages& a, int t) { return (int)(__umulhi(2u * (uint32_t)t, a.magic) >> a.shift); }
@@ -74,6 +76,47 @@ __device__ __forceinline__ Seq sequence(const Pages& a, int s) {
 __device__ __forceinline__ int splits(const PagesPlan& p, int len) { return (len + p.split_len - 1) / p.split_len; }
 __device__ __forceinline__ float* part_of(const Pages& a, long long row, int split) {
   return a.part + (row * a.slots + split) * (a.D + 2);
+}
+
+// A page of a split or a stretch of one, in LDS.  Where the V scale is 0 the kernels read zeros for the codes.
+struct PageEntry {
+  int row0;   // first row of the page in its head's pool; -1: no page of the pool
+  float skc;  // scale of K times c, not 0 (a masked score, -infinity, stays that when multiplied)
+  float lsv;  // log2 of the scale of V (at least -24: a half); PG_NO_SCALE where it is 0
+  float inv;  // 2^-lsv
+};
+constexpr float PG_NO_SCALE = -25.0f;
+__device__ __forceinline__ bool has_scale(const PageEntry& e) { return e.lsv > -24.5f; }
+__device__ __forceinline__ PageEntry page_entry(const Pages& a, int s, int h, int j, float c) {
+  const int id = a.bt[(long long)s * a.stride + j];
+  PageEntry e{-1, 1.0f, PG_NO_SCALE, 0x1p25f};
+  if (id >= 0 && id < a.npages) {
+    e.row0 = id * a.page;
+    e.skc = fmaxf(half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c, 1e-30f);
+    const float sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
+    if (sv > 0.0f) e.lsv = __log2f(sv), e.inv = 1.0f / sv;
+  }
+  return e;
+}
+
+// Eight E4M3 codes as halves (exact).
+__device__ __forceinline__ h8 codes_to_half(uint32_t lo, uint32_t hi) {
+  const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef int i2 __attribute__((ext_vector_type(2)));
+// 8 rows x 16 bytes read transposed by 16 lanes: lane i gives the address of half a row (row i / 2) and gets byte i of
+// the eight rows.
+__device__ __forceinline__ u2 read_transposed(const uint8_t* p) {
+  const i2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2*)p);
+  return u2{(uint32_t)w[0], (uint32_t)w[1]};
+}
+// 16 bytes a lane straight into LDS at `lds` + 16 * lane.
+__device__ __forceinline__ void load_to_lds(const uint8_t* from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(lds) : "memory", "m0");
 }
 
 __device__ __forceinline__ float f8_to_float(uint32_t b) {

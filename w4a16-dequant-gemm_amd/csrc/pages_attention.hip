@@ -47,7 +47,7 @@ __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
         }
         sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
         x = dot * (half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c);
-        y = x + fmaxf(__log2f(sv), PG_LOG2_FLOOR);
+        y = x + (sv > 0.0f ? __log2f(sv) : -25.0f);
       }
     }
     at[tid] = off;
@@ -140,7 +140,7 @@ void plan(Pages& a) {
   else if (a.group <= most && a.nseq > 1) a.few_rows = a.group;           // decoding ones next to prompts
   if (a.few_rows) a.few_rows = (a.few_rows + 15) / 16 * 16;
   if (a.few_rows) a.few = pages_few_plan(a, a.few_rows);
-  if (rows > a.few_rows) a.many = general_plan(a);
+  if (rows > a.few_rows) a.many = pages_many_applies(a) ? pages_many_plan(a) : general_plan(a);
   a.slots = a.few.nsplit > a.many.nsplit ? a.few.nsplit : a.many.nsplit;
 }
 
@@ -162,7 +162,10 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   const unsigned rows = (unsigned)((long long)a.tokens * a.H * a.group);
   hipError_t e = hipSuccess;
   if (a.few_rows) e = launch_pages_few(a, s);
-  if (e == hipSuccess && (long long)a.max_q * a.group > a.few_rows) {
+  const bool more = (long long)a.max_q * a.group > a.few_rows;
+  if (e == hipSuccess && more && pages_many_applies(a)) {
+    e = launch_pages_many(a, s);
+  } else if (e == hipSuccess && more) {
     pages_general_kernel<<<dim3(rows, a.many.nsplit), 256, 0, s>>>(a);
     e = hipGetLastError();
   }

@@ -10,8 +10,6 @@
 // K and V tiles reach LDS as whole rows by direct loads (16 bytes a lane, two slots per wave), with pieces swapped
 // by row so that neither read has bank conflicts.  Page ids and scales of the split lie in a table in LDS.
 // Bound: HBM, 2 D bytes per position and KV head.
-#include <type_traits>
-
 #include "pages.cuh"
 
 namespace w4k {
@@ -20,20 +18,6 @@ namespace {
 constexpr int PF_TILE = 32, PF_WAVES = 4, PF_RING = 2;
 constexpr int PF_STEP = PF_TILE * PF_WAVES;  // positions that a workgroup's waves take together
 constexpr int PF_TABLE = 512;                // pages of a split
-typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef int i2 __attribute__((ext_vector_type(2)));
-
-struct Entry {
-  int row0;        // first row of the page in its head's pool; -1: no page of the pool
-  float skc, sv;   // scale of K times c, scale of V
-  float lsv;       // log2 of the latter
-};
-
-__device__ __forceinline__ h8 codes_to_half(uint32_t lo, uint32_t hi) {
-  const h2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-  const h2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-  return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // PG4: pages of a multiple of 4 rows (four neighbouring positions have one page).
 template <int D, int NT, bool PG4>
@@ -44,7 +28,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   constexpr int LDW = D + 4;  // floats of a merge row: O[D], denominator, M
   static_assert(16 * LDW * 4 <= PF_RING * SLOT, "the merge rows take the ring's place");
   __shared__ __attribute__((aligned(16))) uint8_t ring[PF_WAVES][PF_RING * SLOT];
-  __shared__ Entry table[PF_TABLE];
+  __shared__ PageEntry table[PF_TABLE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, q4 = lane >> 4;
@@ -59,17 +43,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
 
   // ---- the split's pages
   const int j0 = page_of(a, s0), pages = s1 > s0 ? page_of(a, s1 - 1) - j0 + 1 : 0;
-  for (int i = tid; i < pages; i += PF_WAVES * 64) {
-    const int id = a.bt[(long long)s * a.stride + j0 + i];
-    Entry e{-1, 0.0f, 0.0f, 0.0f};
-    if (id >= 0 && id < a.npages) {
-      e.row0 = id * a.page;
-      e.skc = half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c;
-      e.sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
-      e.lsv = fmaxf(__log2f(e.sv), PG_LOG2_FLOOR);
-    }
-    table[i] = e;
-  }
+  for (int i = tid; i < pages; i += PF_WAVES * 64) table[i] = page_entry(a, s, h, j0 + i, c);
   // ---- queries: lane (row c16, q4) of MFMA m holds 8 elements from kcol(m)
   auto kcol = [&](int m) { return WIDE ? 16 * (4 * (m >> 1) + q4) + 8 * (m & 1) : 8 * (4 * m + q4); };
   h8 qop[NT][NC];
@@ -94,29 +68,24 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
     const int hi = (r >> 4) & 1;
     return P == 16 ? (r & 7) | hi << 3 : P == 8 ? ((r >> 1) & 3) | hi << 2 : P == 4 ? ((r >> 2) & 1) | hi << 1 : 0;
   };
-  auto dma16 = [](const uint8_t* from, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(lds) : "memory", "m0");
-  };
-  // Table entry of a position of the split.
-  auto entry = [&](int t) { return page_of(a, t) - j0; };
-
-  // Requests the tile at t0 into slot sl; returns which of its rows are there.
-  auto request = [&](int sl, int t0) -> uint32_t {
+  // Requests the tile at t0 into slot sl; returns which of its positions are there (low half), and which of their
+  // rows of V count (high half: there, under a scale that is not 0).
+  auto request = [&](int sl, int t0) -> uint64_t {
     const int t = t0 + (lane & 31);
     bool there = t < s1;
     const int j = there ? page_of(a, t) : j0;
-    const int row0 = table[j - j0].row0;
-    there = there && row0 >= 0;
-    const int row = there ? row0 + (t - j * a.page) : 0;  // (others read row 0 and drop it)
+    const PageEntry e = table[j - j0];
+    there = there && e.row0 >= 0;
+    const int row = there ? e.row0 + (t - j * a.page) : 0;  // (others read row 0 and drop it)
     const uint32_t at = lds_wave + sl * SLOT;
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       const int u = i * 64 + lane, r = u / P, piece = u % P;
       const long long off = (long long)__shfl(row, r, 64) * D;
-      dma16(kbase + off + 16 * (piece ^ kswz(r)), at + i * 1024);
-      dma16(vbase + off + 16 * (piece ^ vswz(r)), at + SIDE + i * 1024);
+      load_to_lds(kbase + off + 16 * (piece ^ kswz(r)), at + i * 1024);
+      load_to_lds(vbase + off + 16 * (piece ^ vswz(r)), at + SIDE + i * 1024);
     }
-    return (uint32_t)__builtin_amdgcn_ballot_w64(there);
+    return __builtin_amdgcn_ballot_w64(there && (lane < 32 || has_scale(e)));
   };
 
   f4 o[NT][NE];
@@ -130,21 +99,18 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
 
   const int vrow = (c16 >> 1) < 4 ? 4 * q4 + (c16 >> 1) : 16 + 4 * q4 + (c16 >> 1) - 4;
 
-  // WHOLE: every position of the tile is there and every row sees it.
-  auto compute = [&](int sl, int t0, uint32_t there, auto whole) {
-    constexpr bool WHOLE = decltype(whole)::value;
-    const uint8_t* const slot = ring[wave] + sl * SLOT;
+  auto compute = [&](uint8_t* slot, int t0, uint64_t rows_there) {
+    const uint32_t there = (uint32_t)rows_there, fine = (uint32_t)(rows_there >> 32);
     f4 sc[NT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int r = 16 * j + c16;
-      const uint8_t* const kr = slot + r * D;
+      const uint8_t* const kr = slot + 16 * j * D + c16 * D;
 #pragma unroll
       for (int t = 0; t < NT; ++t) sc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
       if constexpr (WIDE) {
 #pragma unroll
         for (int i = 0; i < P / 4; ++i) {
-          const u4 w = *(const u4*)(kr + 16 * ((4 * i + q4) ^ kswz(r)));
+          const u4 w = *(const u4*)(kr + 16 * ((4 * i + q4) ^ kswz(c16)));
           const h8 k0 = codes_to_half(w[0], w[1]), k1 = codes_to_half(w[2], w[3]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -162,38 +128,44 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         }
       }
     }
-    // the scales of the lane's eight positions
-    float skc[8], sv[8], lsv[8];
+    // register k = 4 j + i of a row's scores is position 16 j + 4 q4 + i
+    if (there != ~0u || t0 + PF_TILE > q.shown) {  // wave-uniform
+      const uint32_t mine = there >> (4 * q4);
 #pragma unroll
-    for (int k = 0; k < 8; k += PG4 ? 4 : 1) {
-      const int t = t0 + 16 * (k >> 2) + 4 * q4 + (k & 3);
-      const Entry e = table[WHOLE || t < s1 ? entry(t) : 0];
+      for (int t = 0; t < NT; ++t) {
+        const int left = sees[t] - t0 - 4 * q4;
 #pragma unroll
-      for (int i = 0; i < (PG4 ? 4 : 1); ++i) skc[k + i] = e.skc, sv[k + i] = e.sv, lsv[k + i] = e.lsv;
+        for (int k = 0; k < 8; ++k) {
+          const int at = 16 * (k >> 2) + (k & 3);
+          if (!((mine >> at) & 1) || at >= left) sc[t][k >> 2][k & 3] = -INFINITY;
+        }
+      }
+    }
+    if (fine != ~0u) {
+      // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place
+      if (lane < PF_TILE && !((fine >> lane) & 1))
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    }
+    const int last = (s1 - 1) - t0;  // (positions past the split have the last one's entry)
+    constexpr int SAME = PG4 ? 4 : 1;
+    float skc[8 / SAME], lsv[8 / SAME], inv[8 / SAME];
+#pragma unroll
+    for (int k = 0; k < 8; k += SAME) {
+      const PageEntry e = table[page_of(a, t0 + min(16 * (k >> 2) + 4 * q4 + (k & 3), last)) - j0];
+      skc[k / SAME] = e.skc, lsv[k / SAME] = e.lsv, inv[k / SAME] = e.inv;
     }
     h8 pop[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float top = -INFINITY;
-      bool see[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int at = 16 * (k >> 2) + 4 * q4 + (k & 3);
-        see[k] = WHOLE || (((there >> at) & 1) && t0 + at < sees[t]);
-      }
-      if constexpr (PG4 && WHOLE) {
+      for (int k = 0; k < 8; k += SAME) {
+        float m = sc[t][k >> 2][k & 3];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const f4 x = sc[t][j];
-          const float m4 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          top = fmaxf(top, __builtin_fmaf(m4, skc[4 * j], lsv[4 * j]));
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float y = __builtin_fmaf(sc[t][k >> 2][k & 3], skc[k], lsv[k]);
-          top = fmaxf(top, see[k] ? y : -INFINITY);
-        }
+        for (int i = 1; i < SAME; ++i) m = fmaxf(m, sc[t][k >> 2][(k & 3) + i]);
+        top = fmaxf(top, __builtin_fmaf(m, skc[k / SAME], lsv[k / SAME]));
       }
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -206,31 +178,24 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         l[t] *= alpha;
       }
       M[t] = m_new;
-      float w[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][k >> 2][k & 3], skc[k], -use));
-        w[k] = p * sv[k];
-        if (!WHOLE && !see[k]) p = w[k] = 0.0f;
-        l[t] += p;
-      }
+      for (int k = 0; k < 8; k += SAME) {
+        const float add = lsv[k / SAME] - use;
+        float sum = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) pop[t][k] = (_Float16)w[k];
-    }
-    // rows that are not there are anything, and 0 times that may be NaN
-    uint32_t mask[2] = {~0u, ~0u};
-    if constexpr (!WHOLE) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t b = there >> (16 * j + 4 * q4);
-        mask[j] = (b & 1 ? 0xFFu : 0u) | (b & 2 ? 0xFF00u : 0u) | (b & 4 ? 0xFF0000u : 0u) | (b & 8 ? 0xFF000000u : 0u);
+        for (int i = k; i < k + SAME; ++i) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i >> 2][i & 3], skc[k / SAME], add));
+          sum += w;
+          pop[t][i] = (_Float16)w;
+        }
+        l[t] = __builtin_fmaf(sum, inv[k / SAME], l[t]);
       }
     }
     const uint8_t* const vr = slot + SIDE + vrow * D + 8 * (c16 & 1);
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
-      const i2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i2*)(vr + 16 * (e ^ vswz(vrow))));
-      const h8 v = codes_to_half((uint32_t)w[0] & mask[0], (uint32_t)w[1] & mask[1]);
+      const u2 w = read_transposed(vr + 16 * (e ^ vswz(vrow)));
+      const h8 v = codes_to_half(w[0], w[1]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pop[t], o[t][e], 0, 0, 0);
     }
@@ -239,7 +204,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   // ---- tiles of this wave: s0 + 32 (wave + 4 it)
   const int nit = (s1 - s0 + PF_STEP - 1) / PF_STEP;
   auto tile_start = [&](int it) { return s0 + PF_TILE * (wave + PF_WAVES * it); };
-  uint32_t there[PF_RING];
+  uint64_t there[PF_RING];
 #pragma unroll
   for (int d = 0; d < PF_RING; ++d)
     if (d < nit) there[d] = request(d, tile_start(d));
@@ -251,8 +216,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         // tile `it` has landed; the ones after it may be in flight
         if (it + PF_RING <= nit) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((PF_RING - 1) * 2 * KI) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-        if (there[d] == ~0u && tile_start(it) + PF_TILE <= q.shown) compute(d, tile_start(it), there[d], std::true_type{});
-        else if (there[d]) compute(d, tile_start(it), there[d], std::false_type{});
+        if ((uint32_t)there[d]) compute(ring[wave] + d * SLOT, tile_start(it), there[d]);
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the slot has been read: refill it
         if (it + PF_RING < nit) there[d] = request(d, tile_start(it + PF_RING));
       }

@@ -1,0 +1,295 @@
+// Paged FP8 attention for many rows: prompts and chunks of them.
+//
+// A workgroup takes 128 rows of one (sequence, KV head) -- row = token * group + head, so the heads of a group
+// share what is read -- and the positions of a split; a wave has 32 rows as the columns of
+//   scores  S[t][row] = sum_d K[t][d] q[row][d]    v_mfma_f32_32x32x16_f16, A = 32 K rows, B = queries (in registers)
+//   output  O^T[d][row] += sum_t V[t][d] w[t][row]  A = 32 d of V transposed, B = the weights straight from the score registers:
+//           lane (row, half f) has positions 8 g + 4 f .. + 3 of the 32, and the transposed reads of V follow that
+// Tiles of 64 positions go through three slots of LDS: whole rows by direct loads, requested two tiles ahead, one
+// barrier per tile.  Codes are converted by each wave after it has read them: half the LDS traffic of
+// converted tiles, which would take as long as the matrix products.
+// Weights are formed as 2^(x + log2(sv) - M) at once; the denominator takes a page's sum times 1 / sv.
+// Bound: the vector ALUs (exponentials and what surrounds them) next to the matrix cores.
+#include "pages.cuh"
+
+namespace w4k {
+namespace {
+
+constexpr int PM_ROWS = 128, PM_TILE = 64, PM_WAVES = 4;
+constexpr int PM_SLOTS = 3;  // one is multiplied, one lands, one is requested
+constexpr int PM_TABLE = 512;  // pages that are looked up at a time
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+// PG: 16: pages of a multiple of 16 rows, 4: of 4, 1: any.
+template <int D, int PG>
+__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_kernel(const Pages a, const int tiles) {
+  constexpr int P = D / 16, NE = D / 32;  // pieces of a row, 32-element blocks of it
+  constexpr int SIDE = PM_TILE * D, SLOT = 2 * SIDE, LOADS = 2 * P / PM_WAVES;
+  __shared__ __attribute__((aligned(16))) uint8_t ring[PM_SLOTS][SLOT];
+  __shared__ PageEntry table[PM_TABLE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c32 = lane & 31, half = lane >> 5;
+  // heads first: the workgroups of one head's pages run on one XCD where there are eight heads; later tokens
+  // first: under a causal mask they have the most to do
+  const int h = blockIdx.x % a.H, rest = blockIdx.x / a.H;
+  const int s = rest % a.nseq, tile = tiles - 1 - rest / a.nseq, split = blockIdx.y;
+  const Seq q = sequence(a, s);
+  const int rows = q.n * a.group, heads = a.H * a.group, r0 = tile * PM_ROWS;
+  if (q.n <= 0 || rows <= a.few_rows || r0 >= rows) return;
+  const int ns = max(1, splits(a.many, q.len));
+  if (split >= ns) return;
+  const float c = 1.44269504088896340736f / sqrtf((float)D);
+  // positions that the workgroup's rows see, that the wave's rows see, that all of the wave's rows see
+  const int w0 = r0 + 32 * wave;
+  auto seen_by = [&](int row) { return a.causal ? min(q.len, q.shown + min(row, rows - 1) / a.group) : q.len; };
+  const int s0 = split * a.many.split_len, s1 = min(seen_by(r0 + PM_ROWS - 1), s0 + a.many.split_len);
+  const int wave_end = w0 < rows ? min(s1, seen_by(w0 + 31)) : 0, wave_all = seen_by(w0);
+  const int row = min(w0 + c32, rows - 1), tok = row / a.group;
+  const int sees = seen_by(row);
+  const long long at = (long long)(q.q0 + tok) * heads + h * a.group + (row - tok * a.group);
+
+  // ---- queries: step m of the lane's half holds 8 elements from 16 (2 (m / 2) + half) + 8 (m % 2)
+  h8 qop[P];
+  {
+    const w4_half* const qp = a.q + (long long)(q.q0 + tok) * a.q_stride + (long long)(h * a.group + (row - tok * a.group)) * D;
+#pragma unroll
+    for (int m = 0; m < P; ++m) __builtin_memcpy(&qop[m], qp + 16 * (2 * (m >> 1) + half) + 8 * (m & 1), 16);
+  }
+
+  const uint8_t* const kbase = a.q_k + (long long)h * a.npages * a.page * D;
+  const uint8_t* const vbase = a.q_v + (long long)h * a.npages * a.page * D;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)ring;
+  // pieces swapped by row: 16 K rows x one piece, and 8 V rows x two pieces, on different banks
+  auto kswz = [](int r) { return P == 16 ? r & 15 : P == 8 ? (r >> 1) & 7 : P == 4 ? (r >> 2) & 3 : 0; };
+  auto vswz = [](int r) {
+    const int hi = (r >> 3) & 1;
+    return P == 16 ? ((r & 3) | hi << 2) << 1 : P == 8 ? (((r >> 1) & 1) | hi << 1) << 1 : P == 4 ? hi << 1 : 0;
+  };
+
+  f16v o[NE];
+#pragma unroll
+  for (int e = 0; e < NE; ++e) o[e] = f16v{};
+  float M = -INFINITY, l = 0.0f;
+  int j0 = 0;  // first page of the table
+
+  // Requests the wave's share of the tile at t0 into slot sl; returns which of its positions are there, and which of
+  // their rows of V count (`fine`: there, under a scale that is not 0).
+  auto request = [&](int sl, int t0, uint64_t& fine) -> uint64_t {
+    const int t = t0 + lane;
+    bool there = t < s1;
+    const int j = there ? page_of(a, t) : j0;
+    const PageEntry e = table[j - j0];
+    there = there && e.row0 >= 0;
+    const int row = there ? e.row0 + (t - j * a.page) : 0;  // (others read row 0 and drop it)
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int n = wave * LOADS + i, u = (n % P) * 64 + lane, r = u / P, piece = u % P;
+      const long long off = (long long)__shfl(row, r, 64) * D;
+      const bool v = n >= P;
+      load_to_lds((v ? vbase : kbase) + off + 16 * (piece ^ (v ? vswz(r) : kswz(r))), lds0 + sl * SLOT + n * 1024);
+    }
+    fine = __builtin_amdgcn_ballot_w64(there && has_scale(e));
+    return __builtin_amdgcn_ballot_w64(there);
+  };
+
+  const int i16 = lane & 15, dhalf = (lane >> 4) & 1;
+  const int vrow = ((i16 >> 1) < 4 ? (i16 >> 1) : 4 + (i16 >> 1)) + 4 * half;  // of the 16 positions of a step
+
+  auto compute = [&](uint8_t* slot, int t0, uint64_t there, uint64_t fine) {
+    f16v sc[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      sc[b] = f16v{};
+#pragma unroll
+      for (int i = 0; i < P / 2; ++i) {
+        const u4 w = *(const u4*)(slot + 32 * b * D + c32 * D + 16 * ((2 * i + half) ^ kswz(c32)));
+        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[0], w[1]), qop[2 * i], sc[b], 0, 0, 0);
+        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[2], w[3]), qop[2 * i + 1], sc[b], 0, 0, 0);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // register k = 16 b + 4 g + i of the scores is position 32 b + 8 g + 4 half + i
+    auto position = [&](int k) { return 32 * (k >> 4) + 8 * ((k >> 2) & 3) + 4 * half + (k & 3); };
+    if (there != ~0ull || t0 + PM_TILE > wave_all) {  // wave-uniform
+      const uint64_t mine = there >> (4 * half);
+      const int left = sees - t0 - 4 * half;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int at = position(k) - 4 * half;
+        if (!((mine >> at) & 1) || at >= left) sc[k >> 4][k & 15] = -INFINITY;
+      }
+    }
+    if (fine != ~0ull) {
+      // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place (every wave
+      // writes the same ones, before its own reads)
+      if (!((fine >> lane) & 1))
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    }
+    const int last = (s1 - 1) - t0;  // (positions past the split have the last one's entry)
+    auto entry = [&](int k) {
+      const int at = PG == 16 ? position(k) - 4 * half : position(k);
+      return table[page_of(a, t0 + min(at, last)) - j0];
+    };
+    constexpr int SAME = PG == 1 ? 1 : PG == 4 ? 4 : 8;  // registers in a row with one page
+    float skc[32 / SAME], lsv[32 / SAME], inv[32 / SAME];
+    float top = -INFINITY;
+    if constexpr (SAME > 1) {
+#pragma unroll
+      for (int k = 0; k < 32; k += SAME) {
+        const PageEntry e = entry(k);
+        skc[k / SAME] = e.skc, lsv[k / SAME] = e.lsv, inv[k / SAME] = e.inv;
+        float m = sc[k >> 4][k & 15];
+#pragma unroll
+        for (int i = 1; i < SAME; ++i) m = fmaxf(m, sc[k >> 4][(k & 15) + i]);
+        top = fmaxf(top, __builtin_fmaf(m, e.skc, e.lsv));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const PageEntry e = entry(k);
+        const float y = __builtin_fmaf(sc[k >> 4][k & 15], e.skc, e.lsv);
+        sc[k >> 4][k & 15] = y;
+        top = fmaxf(top, y);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float m_new = fmaxf(M, top);
+    const float use = m_new == -INFINITY ? 0.0f : m_new;
+    if (__builtin_amdgcn_ballot_w64(m_new > M) != 0) {  // wave-uniform
+      const float alpha = __builtin_amdgcn_exp2f(M - use);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[e] *= alpha;
+      l *= alpha;
+    }
+    M = m_new;
+    h8 pop[4];
+#pragma unroll
+    for (int k0 = 0; k0 < 32; k0 += SAME) {
+      const float add = SAME > 1 ? lsv[k0 / SAME] - use : -use;
+      float sum = 0.0f;
+#pragma unroll
+      for (int k = k0; k < k0 + SAME; ++k) {
+        const float x = sc[k >> 4][k & 15];
+        const float w = __builtin_amdgcn_exp2f(SAME > 1 ? __builtin_fmaf(x, skc[k0 / SAME], add) : x + add);
+        sum += w;
+        pop[k >> 3][k & 7] = (_Float16)w;
+      }
+      l = __builtin_fmaf(sum, SAME > 1 ? inv[k0 / SAME] : entry(k0).inv, l);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {  // 16 positions
+      const uint8_t* const vr = slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        const u2 w = read_transposed(vr + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
+        o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[0], w[1]), pop[kk], o[e], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // ---- stretches of the split whose pages fit the table
+  const int stretch = (int)min((long long)(PM_TABLE - 2) * a.page / PM_TILE * PM_TILE, (long long)a.many.split_len);
+  for (int c0 = s0; c0 < s1; c0 += stretch) {
+    const int c1 = min(s1, c0 + stretch);
+    j0 = page_of(a, c0);
+    const int pages = page_of(a, c1 - 1) - j0 + 1;
+    if (c0 > s0) __syncthreads();  // the table and the slots are still being read
+    for (int i = tid; i < pages; i += PM_WAVES * 64) table[i] = page_entry(a, s, h, j0 + i, c);
+    __syncthreads();
+    const int nit = (c1 - c0 + PM_TILE - 1) / PM_TILE;
+    // (what is known of the tile at hand, and of the next one)
+    uint64_t there = 0, fine = 0, there1 = 0, fine1 = 0;
+    there = request(0, c0, fine);
+    if (1 < nit) there1 = request(1, c0 + PM_TILE, fine1);
+    int sl = 0;
+#pragma unroll 1
+    for (int it = 0; it < nit; ++it) {
+      const int t0 = c0 + PM_TILE * it;
+      // the wave's share of tile `it` has landed (the next tile's may be in flight), then everybody's, and nobody
+      // reads the slot before it any more
+      if (it + 1 < nit) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" : : : "memory");
+      uint64_t there2 = 0, fine2 = 0;
+      if (it + 2 < nit) there2 = request(sl == 0 ? 2 : sl - 1, t0 + 2 * PM_TILE, fine2);
+      if (t0 < wave_end && there) compute(ring[sl], t0, there, fine);
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      there = there1, fine = fine1, there1 = there2, fine1 = fine2;
+      sl = sl == 2 ? 0 : sl + 1;
+    }
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  if (w0 + c32 >= rows) return;
+  // element 32 e + 8 g + 4 half + i of the row is o[e][4 g + i]
+  if (ns == 1) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    w4_half* const dst = a.out + at * D + 4 * half;
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u2 v = u2{as_u32(h2{(_Float16)(o[e][4 * g] * inv), (_Float16)(o[e][4 * g + 1] * inv)}),
+                        as_u32(h2{(_Float16)(o[e][4 * g + 2] * inv), (_Float16)(o[e][4 * g + 3] * inv)})};
+        __builtin_memcpy(dst + 32 * e + 8 * g, &v, 8);
+      }
+  } else {
+    float* const dst = part_of(a, at, split);
+    if (half == 0) dst[0] = M, dst[1] = l;
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float* const p = dst + 2 + 32 * e + 8 * g + 4 * half;
+        *(float2*)p = float2{o[e][4 * g], o[e][4 * g + 1]};
+        *(float2*)(p + 2) = float2{o[e][4 * g + 2], o[e][4 * g + 3]};
+      }
+  }
+}
+
+template <int D>
+hipError_t go(const Pages& a, hipStream_t s) {
+  const int tiles = (int)(((long long)a.max_q * a.group + PM_ROWS - 1) / PM_ROWS);
+  const dim3 grid((unsigned)((long long)a.nseq * a.H * tiles), (unsigned)a.many.nsplit);
+  if (a.page % 16 == 0) pages_many_kernel<D, 16><<<grid, PM_WAVES * 64, 0, s>>>(a, tiles);
+  else if (a.page % 4 == 0) pages_many_kernel<D, 4><<<grid, PM_WAVES * 64, 0, s>>>(a, tiles);
+  else pages_many_kernel<D, 1><<<grid, PM_WAVES * 64, 0, s>>>(a, tiles);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+bool pages_many_applies(const PagesArgs& a) {
+  const long long tiles = ((long long)a.max_q * a.group + PM_ROWS - 1) / PM_ROWS;
+  return (a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && (((uintptr_t)a.q_k | (uintptr_t)a.q_v) & 15) == 0 &&
+         (long long)a.nseq * a.H * tiles < (1ll << 31);
+}
+
+PagesPlan pages_many_plan(const PagesArgs& a) {
+  // two workgroups per compute unit where the rows do not give them, no split shorter than 512 positions
+  const long long tiles = ((long long)a.tokens * a.group + PM_ROWS - 1) / PM_ROWS * a.H;
+  const int most = (a.max_len + 511) / 512;
+  long long n = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
+  n = n > most ? most : n < 1 ? 1 : n;
+  PagesPlan p;
+  p.split_len = (int)(((a.max_len + n - 1) / n + PM_TILE - 1) / PM_TILE * PM_TILE);
+  p.nsplit = (a.max_len + p.split_len - 1) / p.split_len;
+  return p;
+}
+
+hipError_t launch_pages_many(const Pages& a, hipStream_t s) {
+  switch (a.D) {
+    case 64: return go<64>(a, s);
+    case 96: return go<96>(a, s);
+    case 128: return go<128>(a, s);
+    default: return go<256>(a, s);
+  }
+}
+
+}  // namespace w4k
