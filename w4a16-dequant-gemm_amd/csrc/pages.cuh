@@ -13,14 +13,26 @@
 
 namespace w4k {
 
+// t / d for 0 <= t < 2^31 without a division
+struct Divider {
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ int operator()(int t) const { return (int)(__umulhi(2u * (uint32_t)t, magic) >> shift); }
+};
+inline Divider divider(int d) {
+  Divider v{0, 0};
+  while ((1ll << v.shift) < d) ++v.shift;
+  v.magic = (uint32_t)((1ull << (31 + v.shift)) / (uint32_t)d + 1);
+  return v;
+}
+
 struct PagesPlan {
   int split_len, nsplit;  // positions per split, splits of the longest sequence
 };
 
 // Sequences of up to few_rows rows per KV head are the kernel's for few rows, the others the one for many.
 struct Pages : PagesArgs {
-  uint32_t magic;  // page_of()
-  int shift;
+  Divider by_page;
   int few_rows;
   PagesPlan few, many;
   int slots;    // splits of a row that the workspace has room for
@@ -36,13 +48,7 @@ bool pages_many_applies(const PagesArgs& a);
 PagesPlan pages_many_plan(const PagesArgs& a);
 hipError_t launch_pages_many(const Pages& a, hipStream_t s);
 
-// t / page for 0 <= t < 2^31
-__device__ __forceinline__ int page_of(const Pages& a, int t) { return (int)(__umulhi(2u * (uint32_t)t, a.magic) >> a.shift); }
-inline void set_page(Pages& a) {
-  a.shift = 0;
-  while ((1ll << a.shift) < a.page) ++a.shift;
-  a.magic = (uint32_t)((1ull << (31 + a.shift)) / (uint32_t)a.page + 1);
-}
+__device__ __forceinline__ int page_of(const Pages& a, int t) { return a.by_page(t); }
 
 // Sequence that holds packed token `tok`; -1: none.
 __device__ __forceinline__ int sequence_of(const Pages& a, int tok) {

@@ -156,7 +156,7 @@ size_t pages_attention_space(const PagesArgs& args) {
 hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   Pages a;
   (PagesArgs&)a = args;
-  set_page(a);
+  a.by_page = divider(a.page);
   plan(a);
   a.part = (float*)a.space;
   const unsigned rows = (unsigned)((long long)a.tokens * a.H * a.group);
