@@ -35,14 +35,22 @@ struct Pages : PagesArgs {
   Divider by_page;
   int few_rows;
   PagesPlan few, many;
-  int slots;    // splits of a row that the workspace has room for
-  float* part;  // [row][slots][D + 2]: M, denominator, O
+  int slots;        // splits of a row that the workspace has room for
+  float* part;      // [row][slots][D + 2]: M, denominator, O
+  uint32_t* count;  // arrivals, for the kernel for few rows; null: the join kernel has its rows
+  int count_shift;  // (sequence, KV head) units are 2^count_shift counters apart
 };
+// The workspace begins with a fixed room for counters: wherever another call's partial sums begin, no
+// call finds anything but zeros where it counts.  Counters are spread over it, because arrivals on one line wait for
+// each other.
+constexpr int PG_COUNTERS = 16384;
 
 // pages_few.hip.  Most rows of a sequence and KV head that its kernel takes; 0: not this call's dimensions.
 int pages_few_most(const PagesArgs& a);
 PagesPlan pages_few_plan(const PagesArgs& a, int rows);
 hipError_t launch_pages_few(const Pages& a, hipStream_t s);
+// Whether the last workgroup of every unit joins its splits itself.
+bool pages_few_joins(const PagesArgs& a, const PagesPlan& p, int rows);
 // pages_many.hip
 bool pages_many_applies(const PagesArgs& a);
 PagesPlan pages_many_plan(const PagesArgs& a);
@@ -80,6 +88,55 @@ __device__ __forceinline__ Seq sequence(const Pages& a, int s) {
 }
 
 __device__ __forceinline__ int splits(const PagesPlan& p, int len) { return (len + p.split_len - 1) / p.split_len; }
+// Partial sums pass between workgroups of one launch by stores and loads of agent scope, which go where every XCD sees
+// them (a fence instead would write the whole L2 of an XCD back).
+__device__ __forceinline__ void publish(float* p, float x, float y) {
+  const uint64_t v = __builtin_bit_cast(uint32_t, x) | ((uint64_t)__builtin_bit_cast(uint32_t, y) << 32);
+  __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 published(const float* p) {
+  const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return float2{__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32))};
+}
+// One wave joins the splits of a row into its output.
+template <int BATCH>
+__device__ __forceinline__ void join_row(const float* part, int ns, int D, w4_half* out) {
+  const int lane = threadIdx.x & 63, pitch = D + 2;
+  float M = -INFINITY, den = 0.0f;
+  for (int t0 = 0; t0 < ns; t0 += 64) {
+    const float2 ml = published(part + (long long)min(t0 + lane, ns - 1) * pitch);
+    float m = t0 + lane < ns ? ml.x : -INFINITY;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    m = fmaxf(M, m);
+    const float use = m == -INFINITY ? 0.0f : m;
+    float w = t0 + lane < ns ? __builtin_amdgcn_exp2f(ml.x - use) * ml.y : 0.0f;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) w += __shfl_xor(w, d, 64);
+    den = den * __builtin_amdgcn_exp2f(M - use) + w;
+    M = m;
+  }
+  const float use = M == -INFINITY ? 0.0f : M, inv = den == 0.0f ? 0.0f : 1.0f / den;
+  for (int d0 = 2 * lane; d0 < D; d0 += 128) {
+    float sum0 = 0.0f, sum1 = 0.0f;
+    for (int t0 = 0; t0 < ns; t0 += BATCH) {
+      float2 col[BATCH];
+      float m[BATCH];
+#pragma unroll
+      for (int t = 0; t < BATCH; ++t) {
+        const float* const p = part + (long long)min(t0 + t, ns - 1) * pitch;
+        col[t] = published(p + 2 + d0), m[t] = published(p).x;
+      }
+#pragma unroll
+      for (int t = 0; t < BATCH; ++t) {
+        const float w = t0 + t < ns ? __builtin_amdgcn_exp2f(m[t] - use) : 0.0f;
+        sum0 += w * col[t].x, sum1 += w * col[t].y;
+      }
+    }
+    const h2 v = h2{(_Float16)(sum0 * inv), (_Float16)(sum1 * inv)};
+    out[d0] = (uint16_t)as_u32(v), out[d0 + 1] = (uint16_t)(as_u32(v) >> 16);
+  }
+}
 __device__ __forceinline__ float* part_of(const Pages& a, long long row, int split) {
   return a.part + (row * a.slots + split) * (a.D + 2);
 }

@@ -96,26 +96,18 @@ __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
 }
 
 // ---- rows that several workgroups formed ----------------------------------------------------------
-__global__ __launch_bounds__(128) void pages_join_kernel(const Pages a) {
-  const int D = a.D, heads = a.H * a.group;
-  const int tok = (int)(blockIdx.x / heads), head = (int)(blockIdx.x % heads);
+__global__ __launch_bounds__(256) void pages_join_kernel(const Pages a) {
+  const int heads = a.H * a.group;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (long long)a.tokens * heads) return;
+  const int tok = (int)(row / heads);
   const int s = sequence_of(a, tok);
   if (s < 0) return;
   const Seq q = sequence(a, s);
-  const int ns = splits(q.n * a.group <= a.few_rows ? a.few : a.many, q.len);
-  if (tok - q.q0 >= q.n || ns <= 1) return;
-  const long long row = (long long)tok * heads + head;
-  const float* const part = part_of(a, row, 0);
-  float M = -INFINITY;
-  for (int k = 0; k < ns; ++k) M = fmaxf(M, part[(long long)k * (D + 2)]);
-  const float use = M == -INFINITY ? 0.0f : M;
-  float l = 0.0f;
-  for (int k = 0; k < ns; ++k) l += exp2f(part[(long long)k * (D + 2)] - use) * part[(long long)k * (D + 2) + 1];
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float sum = 0.0f;
-    for (int k = 0; k < ns; ++k) sum += exp2f(part[(long long)k * (D + 2)] - use) * part[(long long)k * (D + 2) + 2 + d];
-    a.out[row * D + d] = __builtin_bit_cast(uint16_t, (_Float16)(l == 0.0f ? 0.0f : sum / l));
-  }
+  const bool few = q.n * a.group <= a.few_rows;
+  if (tok - q.q0 >= q.n || (few && a.count)) return;
+  const int ns = splits(few ? a.few : a.many, q.len);
+  if (ns > 1) join_row<8>(part_of(a, row, 0), ns, a.D, a.out + row * a.D);
 }
 
 PagesPlan general_plan(const PagesArgs& a) {
@@ -142,6 +134,12 @@ void plan(Pages& a) {
   if (a.few_rows) a.few = pages_few_plan(a, a.few_rows);
   if (rows > a.few_rows) a.many = pages_many_applies(a) ? pages_many_plan(a) : general_plan(a);
   a.slots = a.few.nsplit > a.many.nsplit ? a.few.nsplit : a.many.nsplit;
+  a.count = nullptr;
+  if (a.few.nsplit > 1 && (long long)a.nseq * a.H <= PG_COUNTERS && pages_few_joins(a, a.few, a.few_rows)) {
+    a.count = (uint32_t*)a.space;
+    a.count_shift = 0;
+    while (((long long)a.nseq * a.H << (a.count_shift + 1)) <= PG_COUNTERS) ++a.count_shift;
+  }
 }
 
 }  // namespace
@@ -150,7 +148,8 @@ size_t pages_attention_space(const PagesArgs& args) {
   Pages a;
   (PagesArgs&)a = args;
   plan(a);
-  return a.slots > 1 ? (size_t)a.tokens * a.H * a.group * a.slots * (a.D + 2) * sizeof(float) : 0;
+  if (a.slots == 1) return 0;
+  return PG_COUNTERS * sizeof(uint32_t) + (size_t)a.tokens * a.H * a.group * a.slots * (a.D + 2) * sizeof(float);
 }
 
 hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
@@ -158,19 +157,19 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   (PagesArgs&)a = args;
   a.by_page = divider(a.page);
   plan(a);
-  a.part = (float*)a.space;
-  const unsigned rows = (unsigned)((long long)a.tokens * a.H * a.group);
+  a.part = (float*)(a.space + PG_COUNTERS * sizeof(uint32_t));
+  const long long rows = (long long)a.tokens * a.H * a.group;
+  const bool more = (long long)a.max_q * a.group > a.few_rows;
   hipError_t e = hipSuccess;
   if (a.few_rows) e = launch_pages_few(a, s);
-  const bool more = (long long)a.max_q * a.group > a.few_rows;
   if (e == hipSuccess && more && pages_many_applies(a)) {
     e = launch_pages_many(a, s);
   } else if (e == hipSuccess && more) {
-    pages_general_kernel<<<dim3(rows, a.many.nsplit), 256, 0, s>>>(a);
+    pages_general_kernel<<<dim3((unsigned)rows, a.many.nsplit), 256, 0, s>>>(a);
     e = hipGetLastError();
   }
-  if (e == hipSuccess && a.slots > 1) {
-    pages_join_kernel<<<rows, 128, 0, s>>>(a);
+  if (e == hipSuccess && ((a.few.nsplit > 1 && !a.count) || a.many.nsplit > 1)) {
+    pages_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
     e = hipGetLastError();
   }
   return e;

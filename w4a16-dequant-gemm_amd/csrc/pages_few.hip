@@ -256,11 +256,28 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         dst[0] = (uint16_t)as_u32(v), dst[1] = (uint16_t)(as_u32(v) >> 16);
       } else {
         float* const dst = part_of(a, at, split);
-        dst[2 + d] = sum0, dst[3 + d] = sum1;
-        if (d == 0) dst[0] = top, dst[1] = den4;
+        publish(dst + 2 + d, sum0, sum1);
+        if (d == 0) publish(dst, top, den4);
       }
     }
     if (t + 1 < NT) __syncthreads();
+  }
+  if (ns == 1 || !a.count) return;
+
+  // The unit's workgroup that finishes last joins its splits.  Each counts itself once its partial sums have been
+  // written (the stores have come back); the counter wraps to 0 with the last one.
+  __shared__ uint32_t arrived;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0)
+    arrived = __builtin_amdgcn_atomic_inc32(&a.count[(long long)blockIdx.x << a.count_shift], (uint32_t)(ns - 1), __ATOMIC_RELAXED,
+                                            "agent");
+  __syncthreads();
+  if (arrived != (uint32_t)(ns - 1)) return;
+  for (int r = wave; r < rows; r += PF_WAVES) {
+    const int tok = r / a.group;
+    const long long at = (long long)(q.q0 + tok) * heads + h * a.group + (r - tok * a.group);
+    join_row<16>(part_of(a, at, 0), ns, D, a.out + at * D);
   }
 }
 
@@ -301,6 +318,12 @@ PagesPlan pages_few_plan(const PagesArgs& a, int rows) {
   p.split_len = (int)len;
   p.nsplit = (int)((a.max_len + len - 1) / len);
   return p;
+}
+
+// One workgroup reads all partial sums of a unit: with many of them a launch of its own is ahead.
+bool pages_few_joins(const PagesArgs& a, const PagesPlan& p, int rows) {
+  const long long most = (long long)a.max_q * a.group;
+  return (most < rows ? most : rows) * p.nsplit <= 160;
 }
 
 hipError_t launch_pages_few(const Pages& a, hipStream_t s) {

@@ -20,9 +20,15 @@ constexpr int PM_SLOTS = 3;  // one is multiplied, one lands, one is requested
 constexpr int PM_TABLE = 512;  // pages that are looked up at a time
 typedef float f16v __attribute__((ext_vector_type(16)));
 
+// Tiles of rows that a sequence has here.
+__device__ __forceinline__ int tiles_of(const Pages& a, int s) {
+  const int rows = sequence(a, s).n * a.group;
+  return rows <= a.few_rows ? 0 : (rows + PM_ROWS - 1) / PM_ROWS;
+}
+
 // PG: 16: pages of a multiple of 16 rows, 4: of 4, 1: any.
 template <int D, int PG>
-__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_kernel(const Pages a, const int tiles) {
+__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_kernel(const Pages a) {
   constexpr int P = D / 16, NE = D / 32;  // pieces of a row, 32-element blocks of it
   constexpr int SIDE = PM_TILE * D, SLOT = 2 * SIDE, LOADS = 2 * P / PM_WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t ring[PM_SLOTS][SLOT];
@@ -30,13 +36,33 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, half = lane >> 5;
-  // heads first: the workgroups of one head's pages run on one XCD where there are eight heads; later tokens
-  // first: under a causal mask they have the most to do
-  const int h = blockIdx.x % a.H, rest = blockIdx.x / a.H;
-  const int s = rest % a.nseq, tile = tiles - 1 - rest / a.nseq, split = blockIdx.y;
+  // heads first: the workgroups of one head's pages run on one XCD where there are eight heads
+  const int h = blockIdx.x % a.H, split = blockIdx.y;
+  // ---- which tile of which sequence: 64 sequences at a time, the lanes sum up their tiles
+  int s = 0, left = blockIdx.x / a.H, count = 0;
+  for (int base = 0;; base += 64) {
+    if (base >= a.nseq) return;
+    count = base + lane < a.nseq ? tiles_of(a, base + lane) : 0;
+    int sum = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += y;
+    }
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sum > left);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      left -= __shfl(sum - count, at, 64);
+      count = __shfl(count, at, 64);
+      s = __builtin_amdgcn_readfirstlane(base + at);
+      break;
+    }
+    left -= __shfl(sum, 63, 64);
+  }
+  // later tokens first: under a causal mask they have the most to do
+  const int tile = __builtin_amdgcn_readfirstlane(count - 1 - left);
   const Seq q = sequence(a, s);
   const int rows = q.n * a.group, heads = a.H * a.group, r0 = tile * PM_ROWS;
-  if (q.n <= 0 || rows <= a.few_rows || r0 >= rows) return;
   const int ns = max(1, splits(a.many, q.len));
   if (split >= ns) return;
   const float c = 1.44269504088896340736f / sqrtf((float)D);
@@ -253,22 +279,27 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   }
 }
 
+// Most tiles of a call's sequences: whole ones, and one that is not for each sequence that has more than few_rows.
+long long most_tiles(const PagesArgs& a, int few_rows) {
+  const long long rows = (long long)a.tokens * a.group, seqs = rows / (few_rows + 1);
+  const long long each = ((long long)a.max_q * a.group + PM_ROWS - 1) / PM_ROWS;
+  const long long packed = rows / PM_ROWS + (seqs < a.nseq ? seqs : a.nseq);
+  return packed < each * a.nseq ? packed : each * a.nseq;
+}
+
 template <int D>
 hipError_t go(const Pages& a, hipStream_t s) {
-  const int tiles = (int)(((long long)a.max_q * a.group + PM_ROWS - 1) / PM_ROWS);
-  const dim3 grid((unsigned)((long long)a.nseq * a.H * tiles), (unsigned)a.many.nsplit);
-  if (a.page % 16 == 0) pages_many_kernel<D, 16><<<grid, PM_WAVES * 64, 0, s>>>(a, tiles);
-  else if (a.page % 4 == 0) pages_many_kernel<D, 4><<<grid, PM_WAVES * 64, 0, s>>>(a, tiles);
-  else pages_many_kernel<D, 1><<<grid, PM_WAVES * 64, 0, s>>>(a, tiles);
+  const dim3 grid((unsigned)(most_tiles(a, a.few_rows) * a.H), (unsigned)a.many.nsplit);
+  if (a.page % 16 == 0) pages_many_kernel<D, 16><<<grid, PM_WAVES * 64, 0, s>>>(a);
+  else if (a.page % 4 == 0) pages_many_kernel<D, 4><<<grid, PM_WAVES * 64, 0, s>>>(a);
+  else pages_many_kernel<D, 1><<<grid, PM_WAVES * 64, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
 bool pages_many_applies(const PagesArgs& a) {
-  const long long tiles = ((long long)a.max_q * a.group + PM_ROWS - 1) / PM_ROWS;
-  return (a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && (((uintptr_t)a.q_k | (uintptr_t)a.q_v) & 15) == 0 &&
-         (long long)a.nseq * a.H * tiles < (1ll << 31);
+  return (a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && (((uintptr_t)a.q_k | (uintptr_t)a.q_v) & 15) == 0;
 }
 
 PagesPlan pages_many_plan(const PagesArgs& a) {
