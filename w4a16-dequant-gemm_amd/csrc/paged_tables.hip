@@ -38,25 +38,11 @@ __device__ __forceinline__ Wish wish_of(const Tables& t, int c, int a, uint32_t 
   return w;
 }
 
-// Inclusive prefix sum over a wave by lane moves inside the vector ALU.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t moved(uint32_t x) {
-  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true);
-}
-__device__ __forceinline__ uint32_t wave_sums(uint32_t x) {
-  x = plus(x, moved<0x111, 0xF>(x));  // the lane 1, 2, 4, 8 before, in rows of 16
-  x = plus(x, moved<0x112, 0xF>(x));
-  x = plus(x, moved<0x114, 0xF>(x));
-  x = plus(x, moved<0x118, 0xF>(x));
-  x = plus(x, moved<0x142, 0xA>(x));  // lane 15 of rows 0 and 2 into rows 1 and 3
-  x = plus(x, moved<0x143, 0xC>(x));  // lane 31 into rows 2 and 3
-  return x;
-}
 // Exclusive prefix sum over the workgroup; `total` of all.  sums: one entry per wave, not used again before a barrier.
 template <int T>
 __device__ __forceinline__ uint32_t exclusive_sum(uint32_t v, uint32_t* sums, uint32_t& total) {
   const int wave = threadIdx.x >> 6;
-  const uint32_t x = wave_sums(v);
+  const uint32_t x = (uint32_t)wave_scan((int)v, 0, [](int a, int b) { return (int)plus((uint32_t)a, (uint32_t)b); });
   if ((threadIdx.x & 63) == 63) sums[wave] = x;
   __syncthreads();
   uint32_t before = 0;

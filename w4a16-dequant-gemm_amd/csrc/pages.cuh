@@ -26,19 +26,62 @@ inline Divider divider(int d) {
   return v;
 }
 
+// Sums and maxima over a wave by lane moves inside the vector ALU (an exchange through LDS takes a hundred cycles a
+// step): inclusive from lane 0 on, so lane 63 has them all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int x, int none) {
+  return __builtin_amdgcn_update_dpp(none, x, CTRL, ROWS, 0xF, false);
+}
+template <typename F>
+__device__ __forceinline__ int wave_scan(int x, int none, F f) {
+  x = f(x, moved<0x111, 0xF>(x, none));  // the lane 1, 2, 4, 8 before, in rows of 16
+  x = f(x, moved<0x112, 0xF>(x, none));
+  x = f(x, moved<0x114, 0xF>(x, none));
+  x = f(x, moved<0x118, 0xF>(x, none));
+  x = f(x, moved<0x142, 0xA>(x, none));  // lane 15 of rows 0 and 2 into rows 1 and 3
+  x = f(x, moved<0x143, 0xC>(x, none));  // lane 31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ int wave_prefix(int x) {
+  return wave_scan(x, 0, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); }
+__device__ __forceinline__ int wave_most(int x) {  // of values that are not negative
+  return __builtin_amdgcn_readlane(wave_scan(x, 0, [](int a, int b) { return max(a, b); }), 63);
+}
+// The larger of a value and the one 32 (16) lanes away.
+__device__ __forceinline__ float max_over_32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float max_over_16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
 struct PagesPlan {
   int split_len, nsplit;  // positions per split, splits of the longest sequence
+};
+
+// How the kernel for few rows spreads its work.  Lengths are known on the device alone: its workgroups
+// find their splits from them (pages_few.hip).
+struct FewPlan {
+  int grid;        // workgroups
+  int step_least;  // a split has 128 times this positions at least
+  int alone;       // 1: no unit (sequence and KV head) is split
+  int rows;        // rows of a unit that the workspace has room for
 };
 
 // Sequences of up to few_rows rows per KV head are the kernel's for few rows, the others the one for many.
 struct Pages : PagesArgs {
   Divider by_page;
   int few_rows;
-  PagesPlan few, many;
-  int slots;        // splits of a row that the workspace has room for
-  float* part;      // [row][slots][D + 2]: M, denominator, O
-  uint32_t* count;  // arrivals, for the kernel for few rows; null: the join kernel has its rows
-  int count_shift;  // (sequence, KV head) units are 2^count_shift counters apart
+  FewPlan few;
+  PagesPlan many;
+  uint32_t* count;  // few rows: arrivals of a unit, at its first workgroup's number << count_shift
+  int count_shift;
+  float* few_part;  // [workgroup][row][D + 2]: M, denominator, O
+  float* part;      // many rows: [row][split][D + 2]
 };
 // The workspace begins with a fixed room for counters: wherever another call's partial sums begin, no
 // call finds anything but zeros where it counts.  Counters are spread over it, because arrivals on one line wait for
@@ -47,10 +90,8 @@ constexpr int PG_COUNTERS = 16384;
 
 // pages_few.hip.  Most rows of a sequence and KV head that its kernel takes; 0: not this call's dimensions.
 int pages_few_most(const PagesArgs& a);
-PagesPlan pages_few_plan(const PagesArgs& a, int rows);
+FewPlan pages_few_plan(const PagesArgs& a, int rows);
 hipError_t launch_pages_few(const Pages& a, hipStream_t s);
-// Whether the last workgroup of every unit joins its splits itself.
-bool pages_few_joins(const PagesArgs& a, const PagesPlan& p, int rows);
 // pages_many.hip
 bool pages_many_applies(const PagesArgs& a);
 PagesPlan pages_many_plan(const PagesArgs& a);
@@ -76,15 +117,27 @@ __device__ __forceinline__ int sequence_of(const Pages& a, int tok) {
 struct Seq {
   int q0, n, len, shown;  // first packed token, tokens, positions; the first token sees shown positions, each next one more
 };
-__device__ __forceinline__ Seq sequence(const Pages& a, int s) {
+__device__ __forceinline__ Seq sequence_from(const Pages& a, int q0, int end, int len) {
   Seq q;
-  q.q0 = a.cu ? a.cu[s] : s;
-  const int end = a.cu ? a.cu[s + 1] : s + 1;
-  q.n = q.q0 < 0 ? 0 : min(min(end, a.tokens) - q.q0, a.max_q);
-  const int len = a.lens[s];
+  q.q0 = q0;
+  q.n = q0 < 0 ? 0 : min(min(end, a.tokens) - q0, a.max_q);
   q.len = max(0, min(len, a.max_len));
-  q.shown = a.causal ? len - (end - q.q0) + 1 : q.len;
+  q.shown = a.causal ? len - (end - q0) + 1 : q.len;
   return q;
+}
+// (Three loads together: each of them under the condition that needs it is a trip to the cache of its own, which is
+// what the empty statement and the lane reads prevent.)
+__device__ __forceinline__ Seq sequence(const Pages& a, int s) {  // s: the same in all lanes
+  const int* const cu = a.cu ? a.cu + s : a.lens + s;
+  const int q0 = __builtin_amdgcn_readfirstlane(cu[0]), end = __builtin_amdgcn_readfirstlane(cu[a.cu ? 1 : 0]);
+  const int len = __builtin_amdgcn_readfirstlane(a.lens[s]);
+  return sequence_from(a, a.cu ? q0 : s, a.cu ? end : s + 1, len);
+}
+__device__ __forceinline__ Seq sequence_of_lane(const Pages& a, int s) {
+  const int* const cu = a.cu ? a.cu : a.lens;
+  int q0 = cu[s], end = cu[s + (a.cu ? 1 : 0)], len = a.lens[s];
+  asm volatile("" : "+v"(q0), "+v"(end), "+v"(len));
+  return sequence_from(a, a.cu ? q0 : s, a.cu ? end : s + 1, len);
 }
 
 __device__ __forceinline__ int splits(const PagesPlan& p, int len) { return (len + p.split_len - 1) / p.split_len; }
@@ -98,47 +151,49 @@ __device__ __forceinline__ float2 published(const float* p) {
   const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   return float2{__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32))};
 }
-// One wave joins the splits of a row into its output.
-template <int BATCH>
-__device__ __forceinline__ void join_row(const float* part, int ns, int D, w4_half* out) {
-  const int lane = threadIdx.x & 63, pitch = D + 2;
-  float M = -INFINITY, den = 0.0f;
-  for (int t0 = 0; t0 < ns; t0 += 64) {
-    const float2 ml = published(part + (long long)min(t0 + lane, ns - 1) * pitch);
-    float m = t0 + lane < ns ? ml.x : -INFINITY;
+// One wave joins the splits of N rows into their outputs: every lane has its columns, and all loads of BATCH splits are in
+// flight at once.
+template <int N, int BATCH>
+__device__ __forceinline__ void join_rows(const float* const (&part)[N], long long pitch, int ns, int D,
+                                          w4_half* const (&out)[N]) {
+  for (int d0 = 2 * (threadIdx.x & 63); d0 < D; d0 += 128) {
+    float M[N], den[N], sum0[N], sum1[N];
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    m = fmaxf(M, m);
-    const float use = m == -INFINITY ? 0.0f : m;
-    float w = t0 + lane < ns ? __builtin_amdgcn_exp2f(ml.x - use) * ml.y : 0.0f;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) w += __shfl_xor(w, d, 64);
-    den = den * __builtin_amdgcn_exp2f(M - use) + w;
-    M = m;
-  }
-  const float use = M == -INFINITY ? 0.0f : M, inv = den == 0.0f ? 0.0f : 1.0f / den;
-  for (int d0 = 2 * lane; d0 < D; d0 += 128) {
-    float sum0 = 0.0f, sum1 = 0.0f;
+    for (int r = 0; r < N; ++r) M[r] = -INFINITY, den[r] = sum0[r] = sum1[r] = 0.0f;
     for (int t0 = 0; t0 < ns; t0 += BATCH) {
-      float2 col[BATCH];
-      float m[BATCH];
+      float2 ml[N][BATCH], col[N][BATCH];
 #pragma unroll
-      for (int t = 0; t < BATCH; ++t) {
-        const float* const p = part + (long long)min(t0 + t, ns - 1) * pitch;
-        col[t] = published(p + 2 + d0), m[t] = published(p).x;
-      }
+      for (int t = 0; t < BATCH; ++t)
 #pragma unroll
-      for (int t = 0; t < BATCH; ++t) {
-        const float w = t0 + t < ns ? __builtin_amdgcn_exp2f(m[t] - use) : 0.0f;
-        sum0 += w * col[t].x, sum1 += w * col[t].y;
+        for (int r = 0; r < N; ++r) {
+          const float* const p = part[r] + min(t0 + t, ns - 1) * pitch;
+          ml[r][t] = published(p), col[r][t] = published(p + 2 + d0);
+        }
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        float m = M[r];
+#pragma unroll
+        for (int t = 0; t < BATCH; ++t) m = fmaxf(m, ml[r][t].x);  // (the last split again where there are no more)
+        const float use = m == -INFINITY ? 0.0f : m, alpha = __builtin_amdgcn_exp2f(M[r] - use);
+        M[r] = m;
+        den[r] *= alpha, sum0[r] *= alpha, sum1[r] *= alpha;
+#pragma unroll
+        for (int t = 0; t < BATCH; ++t) {
+          const float w = t0 + t < ns ? __builtin_amdgcn_exp2f(ml[r][t].x - use) : 0.0f;
+          den[r] += w * ml[r][t].y, sum0[r] += w * col[r][t].x, sum1[r] += w * col[r][t].y;
+        }
       }
     }
-    const h2 v = h2{(_Float16)(sum0 * inv), (_Float16)(sum1 * inv)};
-    out[d0] = (uint16_t)as_u32(v), out[d0 + 1] = (uint16_t)(as_u32(v) >> 16);
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+      const float inv = den[r] == 0.0f ? 0.0f : 1.0f / den[r];
+      const h2 v = h2{(_Float16)(sum0[r] * inv), (_Float16)(sum1[r] * inv)};
+      out[r][d0] = (uint16_t)as_u32(v), out[r][d0 + 1] = (uint16_t)(as_u32(v) >> 16);
+    }
   }
 }
 __device__ __forceinline__ float* part_of(const Pages& a, long long row, int split) {
-  return a.part + (row * a.slots + split) * (a.D + 2);
+  return a.part + (row * a.many.nsplit + split) * (a.D + 2);
 }
 
 // A page of a split or a stretch of one, in LDS.  Where the V scale is 0 the kernels read zeros for the codes.
@@ -150,14 +205,17 @@ struct PageEntry {
 };
 constexpr float PG_NO_SCALE = -25.0f;
 __device__ __forceinline__ bool has_scale(const PageEntry& e) { return e.lsv > -24.5f; }
+__device__ __forceinline__ void set_scales(PageEntry& e, float sk, float sv, float c) {
+  e.skc = fmaxf(sk * c, 1e-30f);
+  if (sv > 0.0f) e.lsv = __log2f(sv), e.inv = 1.0f / sv;
+}
 __device__ __forceinline__ PageEntry page_entry(const Pages& a, int s, int h, int j, float c) {
   const int id = a.bt[(long long)s * a.stride + j];
   PageEntry e{-1, 1.0f, PG_NO_SCALE, 0x1p25f};
   if (id >= 0 && id < a.npages) {
     e.row0 = id * a.page;
-    e.skc = fmaxf(half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c, 1e-30f);
-    const float sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
-    if (sv > 0.0f) e.lsv = __log2f(sv), e.inv = 1.0f / sv;
+    const long long at = (long long)h * a.npages + id;
+    set_scales(e, half_bits_to_float(a.s_k[at]), half_bits_to_float(a.s_v[at]), c);
   }
   return e;
 }

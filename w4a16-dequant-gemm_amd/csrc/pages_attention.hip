@@ -104,10 +104,9 @@ __global__ __launch_bounds__(256) void pages_join_kernel(const Pages a) {
   const int s = sequence_of(a, tok);
   if (s < 0) return;
   const Seq q = sequence(a, s);
-  const bool few = q.n * a.group <= a.few_rows;
-  if (tok - q.q0 >= q.n || (few && a.count)) return;
-  const int ns = splits(few ? a.few : a.many, q.len);
-  if (ns > 1) join_row<8>(part_of(a, row, 0), ns, a.D, a.out + row * a.D);
+  if (tok - q.q0 >= q.n || q.n * a.group <= a.few_rows) return;
+  const int ns = splits(a.many, q.len);
+  if (ns > 1) join_rows<1, 16>({part_of(a, row, 0)}, a.D + 2, ns, a.D, {a.out + row * a.D});
 }
 
 PagesPlan general_plan(const PagesArgs& a) {
@@ -122,24 +121,30 @@ PagesPlan general_plan(const PagesArgs& a) {
   return p;
 }
 
-// Which kernels take the call's sequences, and how they split them.
-void plan(Pages& a) {
+// Which kernels take the call's sequences, how they split them, and where the workspace's parts lie.
+size_t plan(Pages& a) {
   const int most = pages_few_most(a);
   const long long rows = (long long)a.max_q * a.group;
-  a.few = a.many = PagesPlan{a.max_len, 1};
+  a.few = FewPlan{};
+  a.many = PagesPlan{a.max_len, 1};
   a.few_rows = 0;
-  if (rows <= most) a.few_rows = (int)rows;                               // every sequence
-  else if (a.group <= most && a.nseq > 1) a.few_rows = a.group;           // decoding ones next to prompts
+  if (rows <= most) a.few_rows = (int)rows;                      // every sequence
+  else if (a.group <= most && a.nseq > 1) a.few_rows = a.group;  // decoding ones next to prompts
   if (a.few_rows) a.few_rows = (a.few_rows + 15) / 16 * 16;
-  if (a.few_rows) a.few = pages_few_plan(a, a.few_rows);
+  if (a.few_rows) a.few = pages_few_plan(a, rows < a.few_rows ? (int)rows : a.few_rows);
   if (rows > a.few_rows) a.many = pages_many_applies(a) ? pages_many_plan(a) : general_plan(a);
-  a.slots = a.few.nsplit > a.many.nsplit ? a.few.nsplit : a.many.nsplit;
+  size_t floats = 0;
   a.count = nullptr;
-  if (a.few.nsplit > 1 && (long long)a.nseq * a.H <= PG_COUNTERS && pages_few_joins(a, a.few, a.few_rows)) {
+  if (a.few_rows && !a.few.alone) {
     a.count = (uint32_t*)a.space;
     a.count_shift = 0;
-    while (((long long)a.nseq * a.H << (a.count_shift + 1)) <= PG_COUNTERS) ++a.count_shift;
+    while ((long long)a.few.grid << (a.count_shift + 1) <= PG_COUNTERS) ++a.count_shift;
+    a.few_part = (float*)a.space + PG_COUNTERS;
+    floats = (size_t)a.few.grid * a.few.rows * (a.D + 2);
   }
+  a.part = (float*)a.space + PG_COUNTERS + floats;
+  if (a.many.nsplit > 1) floats += (size_t)a.tokens * a.H * a.group * a.many.nsplit * (a.D + 2);
+  return floats ? (PG_COUNTERS + floats) * sizeof(float) : 0;
 }
 
 }  // namespace
@@ -147,9 +152,7 @@ void plan(Pages& a) {
 size_t pages_attention_space(const PagesArgs& args) {
   Pages a;
   (PagesArgs&)a = args;
-  plan(a);
-  if (a.slots == 1) return 0;
-  return PG_COUNTERS * sizeof(uint32_t) + (size_t)a.tokens * a.H * a.group * a.slots * (a.D + 2) * sizeof(float);
+  return plan(a);
 }
 
 hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
@@ -157,7 +160,6 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   (PagesArgs&)a = args;
   a.by_page = divider(a.page);
   plan(a);
-  a.part = (float*)(a.space + PG_COUNTERS * sizeof(uint32_t));
   const long long rows = (long long)a.tokens * a.H * a.group;
   const bool more = (long long)a.max_q * a.group > a.few_rows;
   hipError_t e = hipSuccess;
@@ -168,7 +170,7 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
     pages_general_kernel<<<dim3((unsigned)rows, a.many.nsplit), 256, 0, s>>>(a);
     e = hipGetLastError();
   }
-  if (e == hipSuccess && ((a.few.nsplit > 1 && !a.count) || a.many.nsplit > 1)) {
+  if (e == hipSuccess && a.many.nsplit > 1) {
     pages_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
     e = hipGetLastError();
   }

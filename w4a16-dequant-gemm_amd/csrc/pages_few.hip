@@ -10,6 +10,8 @@
 // K and V tiles reach LDS as whole rows by direct loads (16 bytes a lane, two slots per wave), with pieces swapped
 // by row so that neither read has bank conflicts.  Page ids and scales of the split lie in a table in LDS.
 // Bound: HBM, 2 D bytes per position and KV head.
+#include <type_traits>
+
 #include "pages.cuh"
 
 namespace w4k {
@@ -17,7 +19,75 @@ namespace {
 
 constexpr int PF_TILE = 32, PF_WAVES = 4, PF_RING = 2;
 constexpr int PF_STEP = PF_TILE * PF_WAVES;  // positions that a workgroup's waves take together
-constexpr int PF_TABLE = 512;                // pages of a split
+constexpr int PF_TABLE = 512;                // pages that are looked up at a time
+constexpr int PF_JOIN = 384;                 // most partial sums (rows times splits) that one workgroup joins
+
+// A workgroup's share: a split of a sequence for one KV head.
+struct Share {
+  int s, h, split, ns, len;  // ns splits of len positions each; s < 0: none
+  int first;                 // the unit's first workgroup
+};
+
+// What a sequence has to read, in steps of 128 positions; 0: it is not this kernel's.
+__device__ __forceinline__ int steps_of(const Pages& a, int s) {
+  const Seq q = sequence_of_lane(a, min(s, a.nseq - 1));
+  return s >= a.nseq || q.n <= 0 || q.n * a.group > a.few_rows ? 0 : max(1, (q.len + PF_STEP - 1) / PF_STEP);
+}
+
+// ceil(u / k) for u below 2^24 and r = 1 / k to the last bits: the quotient is right, or one off
+__device__ __forceinline__ int over(int u, int k, float r) {
+  const int n = (int)((float)u * r), left = u - n * k;
+  return n + (left > 0 ? 1 : left <= -k ? -1 : 0);
+}
+__device__ __forceinline__ int over(int u, int k) { return over(u, k, __builtin_amdgcn_rcpf((float)k)); }
+
+// Splits of k steps, the same k for all, as short as the grid allows: with U steps in all sequences and A sequences,
+// H (U / k + A) workgroups are always enough, and H U / k have to be; in between four k are tried.  So one
+// long sequence among short ones is spread over the card, and equal ones are cut into one round of
+// workgroups.  NB: 64 sequences a register.
+template <int NB>
+__device__ __forceinline__ Share find_share(const Pages& a) {
+  const int lane = threadIdx.x & 63;
+  int u[NB], U = 0, A = 0, longest = 0;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) u[b] = steps_of(a, 64 * b + lane);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) U += u[b], A += u[b] > 0, longest = max(longest, u[b]);
+  U = wave_total(U), A = wave_total(A), longest = wave_most(longest);
+  // (a unit's last workgroup joins its rows' splits: no more than PF_JOIN of them)
+  const int least = max(a.few.step_least, (int)(((long long)longest * a.few.rows + PF_JOIN - 1) / PF_JOIN));
+  const int work = U * a.H, free = a.few.grid - A * a.H;
+  const int lo = max(least, (int)((float)work / (float)a.few.grid)), hi = max(least, (int)((float)work / (float)free) + 1);
+  int k = hi;
+#pragma unroll
+  for (int c = 3; c >= 0; --c) {
+    const int t = lo + (hi - lo) / 4 * c;
+    const float r = __builtin_amdgcn_rcpf((float)t);
+    int n = 0;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) n += over(u[b], t, r);
+    if (wave_total(n) * a.H <= a.few.grid) k = t;
+  }
+  Share x{-1, 0, 0, 0, k * PF_STEP, 0};
+  int left = blockIdx.x;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int n = over(u[b], k);
+    const int sum = wave_prefix(n * a.H);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(sum > left);
+    if (x.s < 0 && past) {
+      const int at = __builtin_ctzll(past);
+      x.s = __builtin_amdgcn_readfirstlane(64 * b + at);
+      x.ns = __builtin_amdgcn_readlane(n, at);
+      const int in = __builtin_amdgcn_readfirstlane(left) - (__builtin_amdgcn_readlane(sum, at) - x.ns * a.H);
+      x.h = over(in + 1, x.ns) - 1;
+      x.split = in - x.h * x.ns;
+    }
+    left -= __builtin_amdgcn_readlane(sum, 63);
+  }
+  x.first = blockIdx.x - x.split;
+  return x;
+}
 
 // PG4: pages of a multiple of 4 rows (four neighbouring positions have one page).
 template <int D, int NT, bool PG4>
@@ -29,21 +99,38 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   static_assert(16 * LDW * 4 <= PF_RING * SLOT, "the merge rows take the ring's place");
   __shared__ __attribute__((aligned(16))) uint8_t ring[PF_WAVES][PF_RING * SLOT];
   __shared__ PageEntry table[PF_TABLE];
+  __shared__ int scaleless;  // a page of the split has a V scale of 0
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, q4 = lane >> 4;
-  const int s = blockIdx.x / a.H, h = blockIdx.x - s * a.H, split = blockIdx.y;
+  Share x;
+  if (a.few.alone) {
+    x = Share{(int)(blockIdx.x / a.H), (int)(blockIdx.x % a.H), 0, 1, a.max_len, (int)blockIdx.x};
+  } else {
+    x = a.nseq <= 64 ? find_share<1>(a) : find_share<4>(a);
+    if (x.s < 0) return;
+  }
+  x.s = __builtin_amdgcn_readfirstlane(x.s), x.h = __builtin_amdgcn_readfirstlane(x.h);
+  x.split = __builtin_amdgcn_readfirstlane(x.split), x.ns = __builtin_amdgcn_readfirstlane(x.ns);
+  x.len = __builtin_amdgcn_readfirstlane(x.len), x.first = __builtin_amdgcn_readfirstlane(x.first);
+  const int s = x.s, h = x.h, ns = x.ns, s0 = x.split * x.len;
+  // ---- the first pages of the split, asked for next to what the sequence is
+  const int stretch = (int)min((long long)(PF_TABLE - 2) * a.page / PF_STEP * PF_STEP, (long long)x.len);
+  constexpr int EACH = PF_TABLE / (PF_WAVES * 64);
+  int id[EACH];
+  auto look_up = [&](int j0, int pages) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      id[k] = a.bt[(long long)s * a.stride + j0 + min(tid + k * PF_WAVES * 64, pages - 1)];
+    }
+  };
+  look_up(page_of(a, s0), page_of(a, min(a.max_len, s0 + stretch) - 1) - page_of(a, s0) + 1);
   const Seq q = sequence(a, s);
   const int rows = q.n * a.group, heads = a.H * a.group;
   if (q.n <= 0 || rows > a.few_rows) return;
-  const int ns = max(1, splits(a.few, q.len));
-  if (split >= ns) return;
-  const int s0 = split * a.few.split_len, s1 = min(q.len, s0 + a.few.split_len);
+  const int s1 = min(q.len, s0 + x.len);
   const float c = 1.44269504088896340736f / sqrtf((float)D);
 
-  // ---- the split's pages
-  const int j0 = page_of(a, s0), pages = s1 > s0 ? page_of(a, s1 - 1) - j0 + 1 : 0;
-  for (int i = tid; i < pages; i += PF_WAVES * 64) table[i] = page_entry(a, s, h, j0 + i, c);
   // ---- queries: lane (row c16, q4) of MFMA m holds 8 elements from kcol(m)
   auto kcol = [&](int m) { return WIDE ? 16 * (4 * (m >> 1) + q4) + 8 * (m & 1) : 8 * (4 * m + q4); };
   h8 qop[NT][NC];
@@ -56,7 +143,6 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
     for (int m = 0; m < NC; ++m) __builtin_memcpy(&qop[t][m], qp + kcol(m), 16);
     sees[t] = a.causal ? q.shown + tok : q.len;
   }
-  __syncthreads();
 
   const uint8_t* const kbase = a.q_k + (long long)h * a.npages * a.page * D;
   const uint8_t* const vbase = a.q_v + (long long)h * a.npages * a.page * D;
@@ -68,15 +154,15 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
     const int hi = (r >> 4) & 1;
     return P == 16 ? (r & 7) | hi << 3 : P == 8 ? ((r >> 1) & 3) | hi << 2 : P == 4 ? ((r >> 2) & 1) | hi << 1 : 0;
   };
-  // Requests the tile at t0 into slot sl; returns which of its positions are there (low half), and which of their
-  // rows of V count (high half: there, under a scale that is not 0).
-  auto request = [&](int sl, int t0) -> uint64_t {
+  int j0 = 0;  // first page of the table
+  // Requests the tile at t0 into slot sl; returns which of its positions are there.
+  auto request = [&](int sl, int t0) -> uint32_t {
     const int t = t0 + (lane & 31);
     bool there = t < s1;
     const int j = there ? page_of(a, t) : j0;
-    const PageEntry e = table[j - j0];
-    there = there && e.row0 >= 0;
-    const int row = there ? e.row0 + (t - j * a.page) : 0;  // (others read row 0 and drop it)
+    const int row0 = table[j - j0].row0;
+    there = there && row0 >= 0;
+    const int row = there ? row0 + (t - j * a.page) : 0;  // (others read row 0 and drop it)
     const uint32_t at = lds_wave + sl * SLOT;
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
@@ -85,7 +171,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
       load_to_lds(kbase + off + 16 * (piece ^ kswz(r)), at + i * 1024);
       load_to_lds(vbase + off + 16 * (piece ^ vswz(r)), at + SIDE + i * 1024);
     }
-    return __builtin_amdgcn_ballot_w64(there && (lane < 32 || has_scale(e)));
+    return (uint32_t)__builtin_amdgcn_ballot_w64(there);
   };
 
   f4 o[NT][NE];
@@ -97,10 +183,10 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
     for (int e = 0; e < NE; ++e) o[t][e] = f4{0.f, 0.f, 0.f, 0.f};
   }
 
+  bool no_scales = false;
   const int vrow = (c16 >> 1) < 4 ? 4 * q4 + (c16 >> 1) : 16 + 4 * q4 + (c16 >> 1) - 4;
 
-  auto compute = [&](uint8_t* slot, int t0, uint64_t rows_there) {
-    const uint32_t there = (uint32_t)rows_there, fine = (uint32_t)(rows_there >> 32);
+  auto compute = [&](uint8_t* slot, int t0, uint32_t there) {
     f4 sc[NT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -141,9 +227,11 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         }
       }
     }
-    if (fine != ~0u) {
-      // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place
-      if (lane < PF_TILE && !((fine >> lane) & 1))
+    if (there != ~0u || no_scales) {
+      // rows of V that are not there may hold anything, and 0 times that may be NaN: zeros in their place, and in that
+      // of rows under a scale of 0
+      const int t = min(t0 + (lane & 31), s1 - 1);
+      if (lane < PF_TILE && (!((there >> lane) & 1) || !has_scale(table[page_of(a, t) - j0])))
 #pragma unroll 1
         for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
@@ -167,8 +255,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         for (int i = 1; i < SAME; ++i) m = fmaxf(m, sc[t][k >> 2][(k & 3) + i]);
         top = fmaxf(top, __builtin_fmaf(m, skc[k / SAME], lsv[k / SAME]));
       }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      top = max_over_32(max_over_16(top));
       const float m_new = fmaxf(M[t], top);
       const float use = m_new == -INFINITY ? 0.0f : m_new;
       if (__builtin_amdgcn_ballot_w64(m_new > M[t]) != 0) {  // wave-uniform
@@ -201,24 +288,58 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
     }
   };
 
-  // ---- tiles of this wave: s0 + 32 (wave + 4 it)
-  const int nit = (s1 - s0 + PF_STEP - 1) / PF_STEP;
-  auto tile_start = [&](int it) { return s0 + PF_TILE * (wave + PF_WAVES * it); };
-  uint64_t there[PF_RING];
+  // ---- stretches of the split whose pages fit the table; in each, the wave's tiles: c0 + 32 (wave + 4 it)
+  for (int c0 = s0; c0 < s1; c0 += stretch) {
+    const int c1 = min(s1, c0 + stretch);
+    j0 = page_of(a, c0);
+    const int pages = page_of(a, c1 - 1) - j0 + 1;
+    if (c0 > s0) {
+      __syncthreads();  // the table is still being read
+      look_up(j0, pages);
+    }
+    // (what the first tile waits for is a table entry; the scales come with the tile, and are loaded as halves and
+    // without a branch so that nothing waits for them here)
+    _Float16 sk[EACH], sv[EACH];
+    if (tid == 0) scaleless = 0;
 #pragma unroll
-  for (int d = 0; d < PF_RING; ++d)
-    if (d < nit) there[d] = request(d, tile_start(d));
-  for (int it0 = 0; it0 < nit; it0 += PF_RING) {
+    for (int k = 0; k < EACH; ++k) {
+      const int i = tid + k * PF_WAVES * 64;
+      if (id[k] < 0 || id[k] >= a.npages) id[k] = -1;
+      const long long at = (long long)h * a.npages + max(id[k], 0);
+      sk[k] = ((const _Float16*)a.s_k)[at], sv[k] = ((const _Float16*)a.s_v)[at];
+      if (i < pages) table[i].row0 = id[k] < 0 ? -1 : id[k] * a.page;
+    }
+    __syncthreads();
+    const int nit = (c1 - c0 + PF_STEP - 1) / PF_STEP;
+    auto tile_start = [&](int it) { return c0 + PF_TILE * (wave + PF_WAVES * it); };
+    uint32_t there[PF_RING];
 #pragma unroll
-    for (int d = 0; d < PF_RING; ++d) {
-      const int it = it0 + d;
-      if (it < nit) {
-        // tile `it` has landed; the ones after it may be in flight
-        if (it + PF_RING <= nit) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((PF_RING - 1) * 2 * KI) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-        if ((uint32_t)there[d]) compute(ring[wave] + d * SLOT, tile_start(it), there[d]);
-        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the slot has been read: refill it
-        if (it + PF_RING < nit) there[d] = request(d, tile_start(it + PF_RING));
+    for (int d = 0; d < PF_RING; ++d)
+      if (d < nit) there[d] = request(d, tile_start(d));
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int i = tid + k * PF_WAVES * 64;
+      if (i < pages) {
+        PageEntry e{id[k] < 0 ? -1 : id[k] * a.page, 1.0f, PG_NO_SCALE, 0x1p25f};
+        if (id[k] >= 0) set_scales(e, (float)sk[k], (float)sv[k], c);
+        if (!has_scale(e)) scaleless = 1;
+        table[i] = e;
+      }
+    }
+    __syncthreads();
+    no_scales = scaleless != 0;
+    for (int it0 = 0; it0 < nit; it0 += PF_RING) {
+#pragma unroll
+      for (int d = 0; d < PF_RING; ++d) {
+        const int it = it0 + d;
+        if (it < nit) {
+          // tile `it` has landed; the ones after it may be in flight
+          if (it + PF_RING <= nit) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((PF_RING - 1) * 2 * KI) : "memory");
+          else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+          if (there[d]) compute(ring[wave] + d * SLOT, tile_start(it), there[d]);
+          asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");  // the slot has been read: refill it
+          if (it + PF_RING < nit) there[d] = request(d, tile_start(it + PF_RING));
+        }
       }
     }
   }
@@ -255,14 +376,14 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         w4_half* const dst = a.out + at * D + d;
         dst[0] = (uint16_t)as_u32(v), dst[1] = (uint16_t)(as_u32(v) >> 16);
       } else {
-        float* const dst = part_of(a, at, split);
+        float* const dst = a.few_part + ((long long)blockIdx.x * a.few.rows + row) * (D + 2);
         publish(dst + 2 + d, sum0, sum1);
         if (d == 0) publish(dst, top, den4);
       }
     }
     if (t + 1 < NT) __syncthreads();
   }
-  if (ns == 1 || !a.count) return;
+  if (ns == 1) return;
 
   // The unit's workgroup that finishes last joins its splits.  Each counts itself once its partial sums have been
   // written (the stores have come back); the counter wraps to 0 with the last one.
@@ -270,20 +391,33 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0)
-    arrived = __builtin_amdgcn_atomic_inc32(&a.count[(long long)blockIdx.x << a.count_shift], (uint32_t)(ns - 1), __ATOMIC_RELAXED,
+    arrived = __builtin_amdgcn_atomic_inc32(&a.count[x.first << a.count_shift], (uint32_t)(ns - 1), __ATOMIC_RELAXED,
                                             "agent");
   __syncthreads();
   if (arrived != (uint32_t)(ns - 1)) return;
-  for (int r = wave; r < rows; r += PF_WAVES) {
-    const int tok = r / a.group;
-    const long long at = (long long)(q.q0 + tok) * heads + h * a.group + (r - tok * a.group);
-    join_row<16>(part_of(a, at, 0), ns, D, a.out + at * D);
-  }
+  const long long pitch = (long long)a.few.rows * (D + 2);
+  auto join = [&](auto rows_at_a_time, auto batch) {  // (of a wave; the first again where there are no more)
+    constexpr int N = decltype(rows_at_a_time)::value;
+    for (int r0 = wave; r0 < rows; r0 += N * PF_WAVES) {
+      const float* from[N];
+      w4_half* to[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = r0 + i * PF_WAVES < rows ? r0 + i * PF_WAVES : r0, tok = r / a.group;
+        from[i] = a.few_part + x.first * pitch + r * (D + 2);
+        to[i] = a.out + ((long long)(q.q0 + tok) * heads + h * a.group + (r - tok * a.group)) * D;
+      }
+      join_rows<N, decltype(batch)::value>(from, pitch, ns, D, to);
+    }
+  };
+  if (rows <= PF_WAVES) join(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+  else if (rows <= 2 * PF_WAVES || ns > 8) join(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
+  else join(std::integral_constant<int, 5>{}, std::integral_constant<int, 4>{});
 }
 
 template <int D>
 hipError_t go(const Pages& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.nseq * a.H, (unsigned)a.few.nsplit);
+  const unsigned grid = (unsigned)a.few.grid;
   const bool pg4 = a.page % 4 == 0;
 #define GO(NT)                                                          \
   do {                                                                  \
@@ -305,25 +439,19 @@ int pages_few_most(const PagesArgs& a) {
   return a.D == 256 ? 32 : 64;  // (registers: the sums of 64 rows x 256 elements take all of them)
 }
 
-PagesPlan pages_few_plan(const PagesArgs& a, int rows) {
-  (void)rows;
+FewPlan pages_few_plan(const PagesArgs& a, int rows) {
+  // What runs at a time: two workgroups per compute unit, one where LDS (D = 256) or registers (64 rows) leave no more.
+  const int places = a.D == 256 || rows > 32 ? 256 : 512;
   const long long units = (long long)a.nseq * a.H;
-  long long n = (1024 + units - 1) / units;
-  const long long most = a.max_len <= 512 ? 1 : (a.max_len + 255) / 256;
-  n = n < 1 ? 1 : n > most ? most : n;
-  long long len = ((a.max_len + n - 1) / n + PF_STEP - 1) / PF_STEP * PF_STEP;
-  const long long room = (long long)(PF_TABLE - 2) * a.page / PF_STEP * PF_STEP;  // (a split may begin inside a page)
-  if (len > room) len = room;
-  PagesPlan p;
-  p.split_len = (int)len;
-  p.nsplit = (int)((a.max_len + len - 1) / len);
+  FewPlan p{};
+  p.rows = rows;
+  // Caches of up to 512 positions take less time than a split costs (partial sums, arrival, join: 3 us); many units fill
+  // the card without, and beyond 256 sequences a workgroup does not look for its share.
+  p.alone = a.max_len <= 512 || a.nseq > 256 || units >= 8 * places ||
+            units * ((a.max_len + PF_STEP - 1) / PF_STEP) >= (1ll << 31);  // (counts are 32-bit)
+  p.grid = (int)(p.alone ? units : units <= places * 3 / 4 ? places : units + places);
+  p.step_least = 2;
   return p;
-}
-
-// One workgroup reads all partial sums of a unit: with many of them a launch of its own is ahead.
-bool pages_few_joins(const PagesArgs& a, const PagesPlan& p, int rows) {
-  const long long most = (long long)a.max_q * a.group;
-  return (most < rows ? most : rows) * p.nsplit <= 160;
 }
 
 hipError_t launch_pages_few(const Pages& a, hipStream_t s) {

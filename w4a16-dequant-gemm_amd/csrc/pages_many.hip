@@ -22,7 +22,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 // Tiles of rows that a sequence has here.
 __device__ __forceinline__ int tiles_of(const Pages& a, int s) {
-  const int rows = sequence(a, s).n * a.group;
+  const int rows = sequence_of_lane(a, s).n * a.group;
   return rows <= a.few_rows ? 0 : (rows + PM_ROWS - 1) / PM_ROWS;
 }
 
@@ -42,22 +42,18 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   int s = 0, left = blockIdx.x / a.H, count = 0;
   for (int base = 0;; base += 64) {
     if (base >= a.nseq) return;
-    count = base + lane < a.nseq ? tiles_of(a, base + lane) : 0;
-    int sum = count;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += y;
-    }
+    count = tiles_of(a, min(base + lane, a.nseq - 1));
+    if (base + lane >= a.nseq) count = 0;
+    const int sum = wave_prefix(count);
     const uint64_t past = __builtin_amdgcn_ballot_w64(sum > left);
     if (past) {
       const int at = __builtin_ctzll(past);
-      left -= __shfl(sum - count, at, 64);
-      count = __shfl(count, at, 64);
+      left -= __builtin_amdgcn_readlane(sum - count, at);
+      count = __builtin_amdgcn_readlane(count, at);
       s = __builtin_amdgcn_readfirstlane(base + at);
       break;
     }
-    left -= __shfl(sum, 63, 64);
+    left -= __builtin_amdgcn_readlane(sum, 63);
   }
   // later tokens first: under a causal mask they have the most to do
   const int tile = __builtin_amdgcn_readfirstlane(count - 1 - left);
@@ -181,7 +177,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
         top = fmaxf(top, y);
       }
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = max_over_32(top);
     const float m_new = fmaxf(M, top);
     const float use = m_new == -INFINITY ? 0.0f : m_new;
     if (__builtin_amdgcn_ballot_w64(m_new > M) != 0) {  // wave-uniform
