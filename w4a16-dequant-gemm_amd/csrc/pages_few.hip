@@ -90,7 +90,8 @@ __device__ __forceinline__ Share find_share(const Pages& a) {
 }
 
 // PG4: pages of a multiple of 4 rows (four neighbouring positions have one page).
-template <int D, int NT, bool PG4>
+// NB: how many times 64 sequences find_share() looks at; 0: no unit is split.
+template <int D, int NT, bool PG4, int NB>
 __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a) {
   constexpr int P = D / 16, NC = D / 32, NE = D / 16;  // 16-byte pieces of a row, MFMAs of a score, of an output
   constexpr bool WIDE = P % 4 == 0;                    // K operands by 16-byte reads
@@ -104,10 +105,10 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, q4 = lane >> 4;
   Share x;
-  if (a.few.alone) {
+  if constexpr (NB == 0) {
     x = Share{(int)(blockIdx.x / a.H), (int)(blockIdx.x % a.H), 0, 1, a.max_len, (int)blockIdx.x};
   } else {
-    x = a.nseq <= 64 ? find_share<1>(a) : find_share<4>(a);
+    x = find_share<NB>(a);
     if (x.s < 0) return;
   }
   x.s = __builtin_amdgcn_readfirstlane(x.s), x.h = __builtin_amdgcn_readfirstlane(x.h);
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
     }
     if (t + 1 < NT) __syncthreads();
   }
-  if (ns == 1) return;
+  if (NB == 0 || ns == 1) return;
 
   // The unit's workgroup that finishes last joins its splits.  Each counts itself once its partial sums have been
   // written (the stores have come back); the counter wraps to 0 with the last one.
@@ -415,19 +416,23 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   else join(std::integral_constant<int, 5>{}, std::integral_constant<int, 4>{});
 }
 
+template <int D, int NT, bool PG4>
+void go_share(const Pages& a, hipStream_t s) {
+  const unsigned grid = (unsigned)a.few.grid;
+  if (a.few.alone) pages_few_kernel<D, NT, PG4, 0><<<grid, 256, 0, s>>>(a);
+  else if (a.nseq <= 64) pages_few_kernel<D, NT, PG4, 1><<<grid, 256, 0, s>>>(a);
+  else pages_few_kernel<D, NT, PG4, 4><<<grid, 256, 0, s>>>(a);
+}
+template <int D, int NT>
+void go_page(const Pages& a, hipStream_t s) {
+  if (a.page % 4 == 0) go_share<D, NT, true>(a, s);
+  else go_share<D, NT, false>(a, s);
+}
 template <int D>
 hipError_t go(const Pages& a, hipStream_t s) {
-  const unsigned grid = (unsigned)a.few.grid;
-  const bool pg4 = a.page % 4 == 0;
-#define GO(NT)                                                          \
-  do {                                                                  \
-    if (pg4) pages_few_kernel<D, NT, true><<<grid, 256, 0, s>>>(a);     \
-    else pages_few_kernel<D, NT, false><<<grid, 256, 0, s>>>(a);        \
-  } while (0)
-  if (a.few_rows <= 16) GO(1);
-  else if (a.few_rows <= 32) GO(2);
-  else if constexpr (D <= 128) GO(4);
-#undef GO
+  if (a.few_rows <= 16) go_page<D, 1>(a, s);
+  else if (a.few_rows <= 32) go_page<D, 2>(a, s);
+  else if constexpr (D <= 128) go_page<D, 4>(a, s);
   return hipGetLastError();
 }
 
