@@ -203,6 +203,7 @@ struct PageEntry {
   float lsv;  // log2 of the scale of V (at least -24: a half); PG_NO_SCALE where it is 0
   float inv;  // 2^-lsv
 };
+constexpr float PG_SLACK = 8.0f;  // sums are rescaled only when the maximum has risen by this (weights stay below 2^9)
 constexpr float PG_NO_SCALE = -25.0f;
 __device__ __forceinline__ bool has_scale(const PageEntry& e) { return e.lsv > -24.5f; }
 __device__ __forceinline__ void set_scales(PageEntry& e, float sk, float sv, float c) {
@@ -238,6 +239,10 @@ __device__ __forceinline__ u2 read_transposed(const uint8_t* p) {
 // 16 bytes a lane straight into LDS at `lds` + 16 * lane.
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(lds) : "memory", "m0");
+}
+
+__device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 
 __device__ __forceinline__ float f8_to_float(uint32_t b) {

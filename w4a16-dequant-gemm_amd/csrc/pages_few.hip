@@ -257,15 +257,15 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         top = fmaxf(top, __builtin_fmaf(m, skc[k / SAME], lsv[k / SAME]));
       }
       top = max_over_32(max_over_16(top));
-      const float m_new = fmaxf(M[t], top);
-      const float use = m_new == -INFINITY ? 0.0f : m_new;
-      if (__builtin_amdgcn_ballot_w64(m_new > M[t]) != 0) {  // wave-uniform
-        const float alpha = __builtin_amdgcn_exp2f(M[t] - use);
+      if (__builtin_amdgcn_ballot_w64(top > M[t] + PG_SLACK) != 0) {  // wave-uniform
+        const float m_new = fmaxf(M[t], top);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M[t] - m_new);
 #pragma unroll
         for (int e = 0; e < NE; ++e) o[t][e] *= alpha;
         l[t] *= alpha;
+        M[t] = m_new;
       }
-      M[t] = m_new;
+      const float use = M[t] == -INFINITY ? 0.0f : M[t];
 #pragma unroll
       for (int k = 0; k < 8; k += SAME) {
         const float add = lsv[k / SAME] - use;

@@ -33,6 +33,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   constexpr int SIDE = PM_TILE * D, SLOT = 2 * SIDE, LOADS = 2 * P / PM_WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t ring[PM_SLOTS][SLOT];
   __shared__ PageEntry table[PM_TABLE];
+  __shared__ int odd;  // a page of the table is none of the pool, or has a V scale of 0
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c32 = lane & 31, half = lane >> 5;
@@ -94,10 +95,32 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   for (int e = 0; e < NE; ++e) o[e] = f16v{};
   float M = -INFINITY, l = 0.0f;
   int j0 = 0;  // first page of the table
+  bool odd_pages = false;
+  uint32_t lane_off[LOADS];  // of the wave's loads: a lane's bytes past the first row
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int n = wave * LOADS + i, u = (n % P) * 64 + lane, r = u / P;
+    lane_off[i] = (r - (n % P) * (64 / P)) * D + 16 * ((u % P) ^ (n >= P ? vswz(r) : kswz(r)));
+  }
 
   // Requests the wave's share of the tile at t0 into slot sl; returns which of its positions are there, and which of
   // their rows of V count (`fine`: there, under a scale that is not 0).
   auto request = [&](int sl, int t0, uint64_t& fine) -> uint64_t {
+    if constexpr (PG == 16 && 64 % P == 0) {
+      // Whole tiles of pages of whole 16s: the rows of a load lie side by side on one page, so its place is a scalar and
+      // a lane adds what it always adds.
+      if (t0 + PM_TILE <= s1 && !odd_pages) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int n = wave * LOADS + i, r = (n % P) * (64 / P), t = t0 + (r & ~15), j = page_of(a, t);
+          const int row = __builtin_amdgcn_readfirstlane(table[j - j0].row0) + (t - j * a.page) + (r & 15);
+          const bool v = n >= P;
+          load_to_lds((v ? vbase : kbase) + (long long)row * D, lane_off[i], lds0 + sl * SLOT + n * 1024);
+        }
+        fine = ~0ull;
+        return ~0ull;
+      }
+    }
     const int t = t0 + lane;
     bool there = t < s1;
     const int j = there ? page_of(a, t) : j0;
@@ -119,18 +142,46 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   const int vrow = ((i16 >> 1) < 4 ? (i16 >> 1) : 4 + (i16 >> 1)) + 4 * half;  // of the 16 positions of a step
 
   auto compute = [&](uint8_t* slot, int t0, uint64_t there, uint64_t fine) {
+    // Reads of LDS stand together ahead of what uses them, so that one latency is waited for and not one per
+    // matrix product: all of a tile's K (D = 256: a half), and its V before the softmax.
     f16v sc[2];
+    constexpr int KG = P <= 8 ? P / 2 : 4;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      sc[b] = f16v{};
+    for (int b = 0; b < 2; ++b) sc[b] = f16v{};
 #pragma unroll
-      for (int i = 0; i < P / 2; ++i) {
-        const u4 w = *(const u4*)(slot + 32 * b * D + c32 * D + 16 * ((2 * i + half) ^ kswz(c32)));
-        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[0], w[1]), qop[2 * i], sc[b], 0, 0, 0);
-        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[2], w[3]), qop[2 * i + 1], sc[b], 0, 0, 0);
-        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int g = 0; g < P / 2; g += KG) {
+      u4 w[2][KG];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < KG; ++i) w[b][i] = *(const u4*)(slot + 32 * b * D + c32 * D + 16 * ((2 * (g + i) + half) ^ kswz(c32)));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < KG; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[b][i][0], w[b][i][1]), qop[2 * (g + i)], sc[b], 0, 0, 0);
+          sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[b][i][2], w[b][i][3]), qop[2 * (g + i) + 1], sc[b], 0, 0, 0);
+        }
     }
+    if (fine != ~0ull) {
+      // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place (every wave
+      // writes the same ones, before its own reads)
+      if (!((fine >> lane) & 1))
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
+      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    }
+    constexpr int VG = NE > 4 ? 0 : PG == 1 && NE == 4 ? 1 : 4;  // steps of 16 positions whose V is read ahead
+    u2 vraw[VG ? VG : 1][NE];
+    auto read_v = [&](int kk, int e) {
+      return read_transposed(slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1) + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
+    };
+#pragma unroll
+    for (int kk = 0; kk < VG; ++kk)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) vraw[kk][e] = read_v(kk, e);
+    __builtin_amdgcn_sched_barrier(0);
     // register k = 16 b + 4 g + i of the scores is position 32 b + 8 g + 4 half + i
     auto position = [&](int k) { return 32 * (k >> 4) + 8 * ((k >> 2) & 3) + 4 * half + (k & 3); };
     if (there != ~0ull || t0 + PM_TILE > wave_all) {  // wave-uniform
@@ -141,14 +192,6 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
         const int at = position(k) - 4 * half;
         if (!((mine >> at) & 1) || at >= left) sc[k >> 4][k & 15] = -INFINITY;
       }
-    }
-    if (fine != ~0ull) {
-      // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place (every wave
-      // writes the same ones, before its own reads)
-      if (!((fine >> lane) & 1))
-#pragma unroll 1
-        for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
     const int last = (s1 - 1) - t0;  // (positions past the split have the last one's entry)
     auto entry = [&](int k) {
@@ -178,15 +221,15 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
       }
     }
     top = max_over_32(top);
-    const float m_new = fmaxf(M, top);
-    const float use = m_new == -INFINITY ? 0.0f : m_new;
-    if (__builtin_amdgcn_ballot_w64(m_new > M) != 0) {  // wave-uniform
-      const float alpha = __builtin_amdgcn_exp2f(M - use);
+    if (__builtin_amdgcn_ballot_w64(top > M + PG_SLACK) != 0) {  // wave-uniform
+      const float m_new = fmaxf(M, top);
+      const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - m_new);
 #pragma unroll
       for (int e = 0; e < NE; ++e) o[e] *= alpha;
       l *= alpha;
+      M = m_new;
     }
-    M = m_new;
+    const float use = M == -INFINITY ? 0.0f : M;
     h8 pop[4];
 #pragma unroll
     for (int k0 = 0; k0 < 32; k0 += SAME) {
@@ -196,7 +239,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
       for (int k = k0; k < k0 + SAME; ++k) {
         const float x = sc[k >> 4][k & 15];
         const float w = __builtin_amdgcn_exp2f(SAME > 1 ? __builtin_fmaf(x, skc[k0 / SAME], add) : x + add);
-        sum += w;
+        sum += w;  // (as it is in FP32: under a small scale of V the halves lose what the denominator needs)
         pop[k >> 3][k & 7] = (_Float16)w;
       }
       l = __builtin_fmaf(sum, SAME > 1 ? inv[k0 / SAME] : entry(k0).inv, l);
@@ -204,13 +247,12 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {  // 16 positions
-      const uint8_t* const vr = slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1);
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        const u2 w = read_transposed(vr + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
+        const u2 w = kk < VG ? vraw[kk < VG ? kk : 0][e] : read_v(kk, e);
         o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[0], w[1]), pop[kk], o[e], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (kk >= VG) __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -220,9 +262,16 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
     const int c1 = min(s1, c0 + stretch);
     j0 = page_of(a, c0);
     const int pages = page_of(a, c1 - 1) - j0 + 1;
-    if (c0 > s0) __syncthreads();  // the table and the slots are still being read
-    for (int i = tid; i < pages; i += PM_WAVES * 64) table[i] = page_entry(a, s, h, j0 + i, c);
+    __syncthreads();  // (the table and the slots of the stretch before are still being read)
+    if (tid == 0) odd = 0;
     __syncthreads();
+    for (int i = tid; i < pages; i += PM_WAVES * 64) {
+      const PageEntry e = page_entry(a, s, h, j0 + i, c);
+      table[i] = e;
+      if (e.row0 < 0 || !has_scale(e)) odd = 1;
+    }
+    __syncthreads();
+    odd_pages = __builtin_amdgcn_readfirstlane(odd) != 0;
     const int nit = (c1 - c0 + PM_TILE - 1) / PM_TILE;
     // (what is known of the tile at hand, and of the next one)
     uint64_t there = 0, fine = 0, there1 = 0, fine1 = 0;
