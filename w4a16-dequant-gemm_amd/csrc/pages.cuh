@@ -152,8 +152,8 @@ __device__ __forceinline__ float2 published(const float* p) {
   return float2{__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32))};
 }
 // One wave joins the splits of N rows into their outputs: every lane has its columns, and all loads of BATCH splits are in
-// flight at once.
-template <int N, int BATCH>
+// flight at once.  SAME: the sums come from workgroups of the same launch.
+template <int N, int BATCH, bool SAME>
 __device__ __forceinline__ void join_rows(const float* const (&part)[N], long long pitch, int ns, int D,
                                           w4_half* const (&out)[N]) {
   for (int d0 = 2 * (threadIdx.x & 63); d0 < D; d0 += 128) {
@@ -167,7 +167,8 @@ __device__ __forceinline__ void join_rows(const float* const (&part)[N], long lo
 #pragma unroll
         for (int r = 0; r < N; ++r) {
           const float* const p = part[r] + min(t0 + t, ns - 1) * pitch;
-          ml[r][t] = published(p), col[r][t] = published(p + 2 + d0);
+          ml[r][t] = SAME ? published(p) : *(const float2*)p;
+          col[r][t] = SAME ? published(p + 2 + d0) : *(const float2*)(p + 2 + d0);
         }
 #pragma unroll
       for (int r = 0; r < N; ++r) {

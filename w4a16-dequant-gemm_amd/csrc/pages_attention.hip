@@ -96,17 +96,27 @@ __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
 }
 
 // ---- rows that several workgroups formed ----------------------------------------------------------
-__global__ __launch_bounds__(256) void pages_join_kernel(const Pages a) {
+// A wave joins four heads of a token: what is read is twice what the output is times the splits, and all of it is asked
+// for at once (four splits of four rows).
+constexpr int PJ_ROWS = 4;
+__global__ __launch_bounds__(256) void pages_join_kernel(const Pages a, const int blocks) {
   const int heads = a.H * a.group;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (long long)a.tokens * heads) return;
-  const int tok = (int)(row / heads);
+  const int tok = (int)(blockIdx.x / blocks);
+  const int head = ((int)(blockIdx.x % blocks) * 4 + (threadIdx.x >> 6)) * PJ_ROWS;
   const int s = sequence_of(a, tok);
-  if (s < 0) return;
-  const Seq q = sequence(a, s);
+  if (s < 0 || head >= heads) return;
+  const Seq q = sequence(a, __builtin_amdgcn_readfirstlane(s));
   if (tok - q.q0 >= q.n || q.n * a.group <= a.few_rows) return;
   const int ns = splits(a.many, q.len);
-  if (ns > 1) join_rows<1, 16>({part_of(a, row, 0)}, a.D + 2, ns, a.D, {a.out + row * a.D});
+  if (ns <= 1) return;
+  const float* from[PJ_ROWS];
+  w4_half* to[PJ_ROWS];
+#pragma unroll
+  for (int i = 0; i < PJ_ROWS; ++i) {  // (the last head again where there are no more)
+    const long long row = (long long)tok * heads + min(head + i, heads - 1);
+    from[i] = part_of(a, row, 0), to[i] = a.out + row * a.D;
+  }
+  join_rows<PJ_ROWS, 4, false>(from, a.D + 2, ns, a.D, to);
 }
 
 PagesPlan general_plan(const PagesArgs& a) {
@@ -171,7 +181,8 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
     e = hipGetLastError();
   }
   if (e == hipSuccess && a.many.nsplit > 1) {
-    pages_join_kernel<<<(unsigned)((rows + 3) / 4), 256, 0, s>>>(a);
+    const int blocks = (a.H * a.group + 4 * PJ_ROWS - 1) / (4 * PJ_ROWS);
+    pages_join_kernel<<<(unsigned)a.tokens * blocks, 256, 0, s>>>(a, blocks);
     e = hipGetLastError();
   }
   return e;

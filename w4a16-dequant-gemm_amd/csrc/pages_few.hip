@@ -408,7 +408,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         from[i] = a.few_part + x.first * pitch + r * (D + 2);
         to[i] = a.out + ((long long)(q.q0 + tok) * heads + h * a.group + (r - tok * a.group)) * D;
       }
-      join_rows<N, decltype(batch)::value>(from, pitch, ns, D, to);
+      join_rows<N, decltype(batch)::value, true>(from, pitch, ns, D, to);
     }
   };
   if (rows <= PF_WAVES) join(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});

@@ -28,7 +28,7 @@ __device__ __forceinline__ int tiles_of(const Pages& a, int s) {
 
 // PG: 16: pages of a multiple of 16 rows, 4: of 4, 1: any.
 template <int D, int PG>
-__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_kernel(const Pages a) {
+__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pages_many_kernel(const Pages a) {
   constexpr int P = D / 16, NE = D / 32;  // pieces of a row, 32-element blocks of it
   constexpr int SIDE = PM_TILE * D, SLOT = 2 * SIDE, LOADS = 2 * P / PM_WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t ring[PM_SLOTS][SLOT];
@@ -110,12 +110,17 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
       // Whole tiles of pages of whole 16s: the rows of a load lie side by side on one page, so its place is a scalar and
       // a lane adds what it always adds.
       if (t0 + PM_TILE <= s1 && !odd_pages) {
+        int first[LOADS];
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
           const int n = wave * LOADS + i, r = (n % P) * (64 / P), t = t0 + (r & ~15), j = page_of(a, t);
-          const int row = __builtin_amdgcn_readfirstlane(table[j - j0].row0) + (t - j * a.page) + (r & 15);
-          const bool v = n >= P;
-          load_to_lds((v ? vbase : kbase) + (long long)row * D, lane_off[i], lds0 + sl * SLOT + n * 1024);
+          first[i] = table[j - j0].row0 + (t - j * a.page) + (r & 15);
+        }
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+          const int n = wave * LOADS + i;
+          load_to_lds((n >= P ? vbase : kbase) + (long long)__builtin_amdgcn_readfirstlane(first[i]) * D, lane_off[i],
+                      lds0 + sl * SLOT + n * 1024);
         }
         fine = ~0ull;
         return ~0ull;
@@ -141,10 +146,13 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   const int i16 = lane & 15, dhalf = (lane >> 4) & 1;
   const int vrow = ((i16 >> 1) < 4 ? (i16 >> 1) : 4 + (i16 >> 1)) + 4 * half;  // of the 16 positions of a step
 
-  auto compute = [&](uint8_t* slot, int t0, uint64_t there, uint64_t fine) {
-    // Reads of LDS stand together ahead of what uses them, so that one latency is waited for and not one per
-    // matrix product: all of a tile's K (D = 256: a half), and its V before the softmax.
-    f16v sc[2];
+  // A tile's three steps.  Reads of LDS stand together ahead of what uses them, so that one latency is waited for and
+  // not one per matrix product: all of a tile's K (D = 256: a half), and its V before the softmax.
+  f16v sc[2];
+  constexpr int VG = NE > 4 ? 0 : 4;  // steps of 16 positions whose V is read ahead
+  u2 vraw[VG ? VG : 1][NE];
+  h8 pop[4];
+  auto scores = [&](const uint8_t* slot) {
     constexpr int KG = P <= 8 ? P / 2 : 4;
 #pragma unroll
     for (int b = 0; b < 2; ++b) sc[b] = f16v{};
@@ -164,6 +172,28 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
           sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[b][i][2], w[b][i][3]), qop[2 * (g + i) + 1], sc[b], 0, 0, 0);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto read_v = [&](const uint8_t* slot, int kk, int e) {
+    return read_transposed(slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1) + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
+  };
+  constexpr int SAME = PG == 1 ? 1 : PG == 4 ? 4 : 8;  // of a lane's scores: registers in a row with one page
+  float skc[32 / SAME], lsv[32 / SAME], inv[32 / SAME];
+  // register k = 16 b + 4 g + i of the scores is position 32 b + 8 g + 4 half + i
+  auto position = [&](int k) { return 32 * (k >> 4) + 8 * ((k >> 2) & 3) + 4 * half + (k & 3); };
+  auto entry = [&](int t0, int k) {  // (positions past the split have the last one's)
+    const int at = PG == 16 ? position(k) - 4 * half : position(k);
+    return table[page_of(a, min(t0 + at, s1 - 1)) - j0];
+  };
+  auto read_scales = [&](int t0) {
+    if constexpr (SAME > 1)
+#pragma unroll
+      for (int k = 0; k < 32; k += SAME) {
+        const PageEntry e = entry(t0, k);
+        skc[k / SAME] = e.skc, lsv[k / SAME] = e.lsv, inv[k / SAME] = e.inv;
+      }
+  };
+  auto weights = [&](uint8_t* slot, int t0, uint64_t there, uint64_t fine) {
     if (fine != ~0ull) {
       // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place (every wave
       // writes the same ones, before its own reads)
@@ -172,18 +202,11 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
         for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
-    constexpr int VG = NE > 4 ? 0 : PG == 1 && NE == 4 ? 1 : 4;  // steps of 16 positions whose V is read ahead
-    u2 vraw[VG ? VG : 1][NE];
-    auto read_v = [&](int kk, int e) {
-      return read_transposed(slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1) + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
-    };
 #pragma unroll
     for (int kk = 0; kk < VG; ++kk)
 #pragma unroll
-      for (int e = 0; e < NE; ++e) vraw[kk][e] = read_v(kk, e);
+      for (int e = 0; e < NE; ++e) vraw[kk][e] = read_v(slot, kk, e);
     __builtin_amdgcn_sched_barrier(0);
-    // register k = 16 b + 4 g + i of the scores is position 32 b + 8 g + 4 half + i
-    auto position = [&](int k) { return 32 * (k >> 4) + 8 * ((k >> 2) & 3) + 4 * half + (k & 3); };
     if (there != ~0ull || t0 + PM_TILE > wave_all) {  // wave-uniform
       const uint64_t mine = there >> (4 * half);
       const int left = sees - t0 - 4 * half;
@@ -193,28 +216,19 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
         if (!((mine >> at) & 1) || at >= left) sc[k >> 4][k & 15] = -INFINITY;
       }
     }
-    const int last = (s1 - 1) - t0;  // (positions past the split have the last one's entry)
-    auto entry = [&](int k) {
-      const int at = PG == 16 ? position(k) - 4 * half : position(k);
-      return table[page_of(a, t0 + min(at, last)) - j0];
-    };
-    constexpr int SAME = PG == 1 ? 1 : PG == 4 ? 4 : 8;  // registers in a row with one page
-    float skc[32 / SAME], lsv[32 / SAME], inv[32 / SAME];
     float top = -INFINITY;
     if constexpr (SAME > 1) {
 #pragma unroll
       for (int k = 0; k < 32; k += SAME) {
-        const PageEntry e = entry(k);
-        skc[k / SAME] = e.skc, lsv[k / SAME] = e.lsv, inv[k / SAME] = e.inv;
         float m = sc[k >> 4][k & 15];
 #pragma unroll
         for (int i = 1; i < SAME; ++i) m = fmaxf(m, sc[k >> 4][(k & 15) + i]);
-        top = fmaxf(top, __builtin_fmaf(m, e.skc, e.lsv));
+        top = fmaxf(top, __builtin_fmaf(m, skc[k / SAME], lsv[k / SAME]));
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
-        const PageEntry e = entry(k);
+        const PageEntry e = entry(t0, k);
         const float y = __builtin_fmaf(sc[k >> 4][k & 15], e.skc, e.lsv);
         sc[k >> 4][k & 15] = y;
         top = fmaxf(top, y);
@@ -230,7 +244,6 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
       M = m_new;
     }
     const float use = M == -INFINITY ? 0.0f : M;
-    h8 pop[4];
 #pragma unroll
     for (int k0 = 0; k0 < 32; k0 += SAME) {
       const float add = SAME > 1 ? lsv[k0 / SAME] - use : -use;
@@ -242,18 +255,25 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
         sum += w;  // (as it is in FP32: under a small scale of V the halves lose what the denominator needs)
         pop[k >> 3][k & 7] = (_Float16)w;
       }
-      l = __builtin_fmaf(sum, SAME > 1 ? inv[k0 / SAME] : entry(k0).inv, l);
+      l = __builtin_fmaf(sum, SAME > 1 ? inv[k0 / SAME] : entry(t0, k0).inv, l);
     }
     __builtin_amdgcn_sched_barrier(0);
+  };
+  auto add_values = [&](const uint8_t* slot) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {  // 16 positions
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        const u2 w = kk < VG ? vraw[kk < VG ? kk : 0][e] : read_v(kk, e);
+        const u2 w = kk < VG ? vraw[kk < VG ? kk : 0][e] : read_v(slot, kk, e);
         o[e] = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_to_half(w[0], w[1]), pop[kk], o[e], 0, 0, 0);
       }
       if (kk >= VG) __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  auto barrier = []() {
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
   };
 
   // ---- stretches of the split whose pages fit the table
@@ -285,11 +305,15 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
       // reads the slot before it any more
       if (it + 1 < nit) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LOADS) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" : : : "memory");
+      barrier();
       uint64_t there2 = 0, fine2 = 0;
       if (it + 2 < nit) there2 = request(sl == 0 ? 2 : sl - 1, t0 + 2 * PM_TILE, fine2);
-      if (t0 < wave_end && there) compute(ring[sl], t0, there, fine);
+      if (t0 < wave_end && there) {
+        read_scales(t0);
+        scores(ring[sl]);
+        weights(ring[sl], t0, there, fine);
+        add_values(ring[sl]);
+      }
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
       there = there1, fine = fine1, there1 = there2, fine1 = fine2;
       sl = sl == 2 ? 0 : sl + 1;
@@ -348,8 +372,8 @@ bool pages_many_applies(const PagesArgs& a) {
 }
 
 PagesPlan pages_many_plan(const PagesArgs& a) {
-  // two workgroups per compute unit where the rows do not give them, no split shorter than 512 positions
-  const long long tiles = ((long long)a.tokens * a.group + PM_ROWS - 1) / PM_ROWS * a.H;
+  // two workgroups of 128 rows per compute unit where the rows do not give them, no split shorter than 512 positions
+  const long long tiles = ((long long)a.tokens * a.group + 127) / 128 * a.H;
   const int most = (a.max_len + 511) / 512;
   long long n = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
   n = n > most ? most : n < 1 ? 1 : n;
