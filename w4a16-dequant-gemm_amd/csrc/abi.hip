@@ -683,7 +683,9 @@ static int pages_args(w4k::PagesArgs& a, const w4_f8_pages_view* p, const w4_pag
   a = w4k::PagesArgs{};
   a.H = p->H; a.D = p->D; a.page = p->page; a.npages = p->npages;
   a.q_k = p->q_k; a.s_k = p->s_k; a.q_v = p->q_v; a.s_v = p->s_v;
-  a.nseq = b->nseq; a.tokens = b->tokens; a.max_q = b->max_q; a.stride = b->bt_stride;
+  a.nseq = b->nseq; a.tokens = b->tokens;
+  a.max_q = b->max_q < b->tokens || b->tokens == 0 ? b->max_q : b->tokens;
+  a.stride = b->bt_stride;
   // (no position past a table is looked at)
   const long long in_table = (long long)b->bt_stride * p->page;
   a.max_len = in_table < b->max_len ? (int)in_table : b->max_len;

@@ -68,7 +68,9 @@ struct PagesPlan {
 struct FewPlan {
   int grid;        // workgroups
   int step_least;  // a split has 128 times this positions at least
-  int alone;       // 1: no unit (sequence and KV head) is split
+  int alone;       // 1: no unit (a block of a sequence's rows of one KV head) is split
+  int block;       // rows of a block: 16 or 32
+  int blocks;      // most of a sequence
   int rows;        // rows of a unit that the workspace has room for
 };
 
@@ -88,12 +90,12 @@ struct Pages : PagesArgs {
 // each other.
 constexpr int PG_COUNTERS = 16384;
 
-// pages_few.hip.  Most rows of a sequence and KV head that its kernel takes; 0: not this call's dimensions.
-int pages_few_most(const PagesArgs& a);
-FewPlan pages_few_plan(const PagesArgs& a, int rows);
+// pages_few.hip.  Whether its kernel takes this call's dimensions, and how it spreads sequences of up to so many rows
+// per KV head.
+bool pages_few_applies(const PagesArgs& a);
+FewPlan pages_few_plan(const PagesArgs& a, long long rows);
 hipError_t launch_pages_few(const Pages& a, hipStream_t s);
 // pages_many.hip
-bool pages_many_applies(const PagesArgs& a);
 PagesPlan pages_many_plan(const PagesArgs& a);
 hipError_t launch_pages_many(const Pages& a, hipStream_t s);
 

@@ -131,18 +131,28 @@ PagesPlan general_plan(const PagesArgs& a) {
   return p;
 }
 
+constexpr double FEW_WORK = 7e8;
+
 // Which kernels take the call's sequences, how they split them, and where the workspace's parts lie.
 size_t plan(Pages& a) {
-  const int most = pages_few_most(a);
   const long long rows = (long long)a.max_q * a.group;
+  const bool fast = pages_few_applies(a);
   a.few = FewPlan{};
   a.many = PagesPlan{a.max_len, 1};
   a.few_rows = 0;
-  if (rows <= most) a.few_rows = (int)rows;                      // every sequence
-  else if (a.group <= most && a.nseq > 1) a.few_rows = a.group;  // decoding ones next to prompts
-  if (a.few_rows) a.few_rows = (a.few_rows + 15) / 16 * 16;
-  if (a.few_rows) a.few = pages_few_plan(a, rows < a.few_rows ? (int)rows : a.few_rows);
-  if (rows > a.few_rows) a.many = pages_many_applies(a) ? pages_many_plan(a) : general_plan(a);
+  // Decode and a few tokens per sequence are the kernel's for few rows.  So is everything up to FEW_WORK (what the
+  // scores of all rows come to at most): one launch that cuts rows into blocks of 32 and positions into splits takes 7 - 25 us
+  // there, the kernel for many rows, which waits for tile after tile, and its join 10 - 35 us (60 calls; above twice
+  // that many it is ahead by 1.3 - 2).
+  if (fast) a.few = pages_few_plan(a, rows);
+  const double work = (double)a.tokens * a.H * a.group * a.max_len * a.D;
+  if (fast && (rows <= 32 || a.max_q == 1 || (work <= FEW_WORK && !a.few.alone))) {
+    a.few_rows = (int)rows;
+  } else if (fast && a.group <= 32 && a.nseq > 1) {  // decoding sequences next to prompts
+    a.few_rows = (a.group + 15) / 16 * 16;
+    a.few = pages_few_plan(a, a.few_rows);
+  }
+  if (rows > a.few_rows) a.many = fast ? pages_many_plan(a) : general_plan(a);
   size_t floats = 0;
   a.count = nullptr;
   if (a.few_rows && !a.few.alone) {
@@ -171,10 +181,10 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   a.by_page = divider(a.page);
   plan(a);
   const long long rows = (long long)a.tokens * a.H * a.group;
-  const bool more = (long long)a.max_q * a.group > a.few_rows;
+  const bool more = (long long)a.max_q * a.group > a.few_rows, fast = pages_few_applies(a);
   hipError_t e = hipSuccess;
   if (a.few_rows) e = launch_pages_few(a, s);
-  if (e == hipSuccess && more && pages_many_applies(a)) {
+  if (e == hipSuccess && more && fast) {
     e = launch_pages_many(a, s);
   } else if (e == hipSuccess && more) {
     pages_general_kernel<<<dim3((unsigned)rows, a.many.nsplit), 256, 0, s>>>(a);

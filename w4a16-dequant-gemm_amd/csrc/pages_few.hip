@@ -22,17 +22,11 @@ constexpr int PF_STEP = PF_TILE * PF_WAVES;  // positions that a workgroup's wav
 constexpr int PF_TABLE = 512;                // pages that are looked up at a time
 constexpr int PF_JOIN = 384;                 // most partial sums (rows times splits) that one workgroup joins
 
-// A workgroup's share: a split of a sequence for one KV head.
+// A workgroup's share: a split of a sequence for one KV head and a block of rows.
 struct Share {
-  int s, h, split, ns, len;  // ns splits of len positions each; s < 0: none
-  int first;                 // the unit's first workgroup
+  int s, h, block, split, ns, len;  // ns splits of len positions each; s < 0: none
+  int first;                        // the unit's first workgroup
 };
-
-// What a sequence has to read, in steps of 128 positions; 0: it is not this kernel's.
-__device__ __forceinline__ int steps_of(const Pages& a, int s) {
-  const Seq q = sequence_of_lane(a, min(s, a.nseq - 1));
-  return s >= a.nseq || q.n <= 0 || q.n * a.group > a.few_rows ? 0 : max(1, (q.len + PF_STEP - 1) / PF_STEP);
-}
 
 // ceil(u / k) for u below 2^24 and r = 1 / k to the last bits: the quotient is right, or one off
 __device__ __forceinline__ int over(int u, int k, float r) {
@@ -41,22 +35,36 @@ __device__ __forceinline__ int over(int u, int k, float r) {
 }
 __device__ __forceinline__ int over(int u, int k) { return over(u, k, __builtin_amdgcn_rcpf((float)k)); }
 
-// Splits of k steps, the same k for all, as short as the grid allows: with U steps in all sequences and A sequences,
-// H (U / k + A) workgroups are always enough, and H U / k have to be; in between four k are tried.  So one
+// What a sequence has: positions in steps of 128, and blocks of rows; 0: it is not this kernel's.
+struct Wants {
+  int steps, blocks;
+};
+__device__ __forceinline__ Wants wants_of(const Pages& a, int s) {
+  const Seq q = sequence_of_lane(a, min(s, a.nseq - 1));
+  const int rows = q.n * a.group;
+  const bool none = s >= a.nseq || q.n <= 0 || rows > a.few_rows;
+  return Wants{none ? 0 : max(1, (q.len + PF_STEP - 1) / PF_STEP), none ? 0 : (rows + a.few.block - 1) / a.few.block};
+}
+
+// Splits of k steps, the same k for all, as short as the grid allows: with U steps in all units and A units,
+// U / k + A workgroups are always enough, and U / k have to be; in between four k are tried.  So one
 // long sequence among short ones is spread over the card, and equal ones are cut into one round of
 // workgroups.  NB: 64 sequences a register.
 template <int NB>
-__device__ __forceinline__ Share find_share(const Pages& a) {
+__device__ __forceinline__ Share find_share(const Pages& a, int wg) {
   const int lane = threadIdx.x & 63;
-  int u[NB], U = 0, A = 0, longest = 0;
+  int u[NB], units[NB], U = 0, A = 0, longest = 0;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) u[b] = steps_of(a, 64 * b + lane);
+  for (int b = 0; b < NB; ++b) {
+    const Wants w = wants_of(a, 64 * b + lane);
+    u[b] = w.steps, units[b] = w.blocks * a.H;
+  }
 #pragma unroll
-  for (int b = 0; b < NB; ++b) U += u[b], A += u[b] > 0, longest = max(longest, u[b]);
-  U = wave_total(U), A = wave_total(A), longest = wave_most(longest);
+  for (int b = 0; b < NB; ++b) U += u[b] * units[b], A += units[b], longest = max(longest, u[b]);
+  const int work = wave_total(U), free = a.few.grid - wave_total(A);
+  longest = wave_most(longest);
   // (a unit's last workgroup joins its rows' splits: no more than PF_JOIN of them)
   const int least = max(a.few.step_least, (int)(((long long)longest * a.few.rows + PF_JOIN - 1) / PF_JOIN));
-  const int work = U * a.H, free = a.few.grid - A * a.H;
   const int lo = max(least, (int)((float)work / (float)a.few.grid)), hi = max(least, (int)((float)work / (float)free) + 1);
   int k = hi;
 #pragma unroll
@@ -65,27 +73,28 @@ __device__ __forceinline__ Share find_share(const Pages& a) {
     const float r = __builtin_amdgcn_rcpf((float)t);
     int n = 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) n += over(u[b], t, r);
-    if (wave_total(n) * a.H <= a.few.grid) k = t;
+    for (int b = 0; b < NB; ++b) n += over(u[b], t, r) * units[b];
+    if (wave_total(n) <= a.few.grid) k = t;
   }
-  Share x{-1, 0, 0, 0, k * PF_STEP, 0};
-  int left = blockIdx.x;
+  Share x{-1, 0, 0, 0, 0, k * PF_STEP, 0};
+  int left = wg;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    const int n = over(u[b], k);
-    const int sum = wave_prefix(n * a.H);
+    const int n = over(u[b], k), sum = wave_prefix(n * units[b]);
     const uint64_t past = __builtin_amdgcn_ballot_w64(sum > left);
     if (x.s < 0 && past) {
       const int at = __builtin_ctzll(past);
       x.s = __builtin_amdgcn_readfirstlane(64 * b + at);
       x.ns = __builtin_amdgcn_readlane(n, at);
-      const int in = __builtin_amdgcn_readfirstlane(left) - (__builtin_amdgcn_readlane(sum, at) - x.ns * a.H);
-      x.h = over(in + 1, x.ns) - 1;
-      x.split = in - x.h * x.ns;
+      const int in = __builtin_amdgcn_readfirstlane(left) - __builtin_amdgcn_readlane(sum - n * units[b], at);
+      const int unit = over(in + 1, x.ns) - 1;
+      x.split = in - unit * x.ns;
+      x.block = unit / a.H;
+      x.h = unit - x.block * a.H;
     }
     left -= __builtin_amdgcn_readlane(sum, 63);
   }
-  x.first = blockIdx.x - x.split;
+  x.first = wg - x.split;
   return x;
 }
 
@@ -106,11 +115,13 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   const int c16 = lane & 15, q4 = lane >> 4;
   Share x;
   if constexpr (NB == 0) {
-    x = Share{(int)(blockIdx.x / a.H), (int)(blockIdx.x % a.H), 0, 1, a.max_len, (int)blockIdx.x};
+    const int unit = blockIdx.x / a.H;
+    x = Share{unit / a.few.blocks, (int)blockIdx.x - unit * a.H, unit % a.few.blocks, 0, 1, a.max_len, (int)blockIdx.x};
   } else {
-    x = find_share<NB>(a);
+    x = find_share<NB>(a, blockIdx.x);
     if (x.s < 0) return;
   }
+  x.block = __builtin_amdgcn_readfirstlane(x.block);
   x.s = __builtin_amdgcn_readfirstlane(x.s), x.h = __builtin_amdgcn_readfirstlane(x.h);
   x.split = __builtin_amdgcn_readfirstlane(x.split), x.ns = __builtin_amdgcn_readfirstlane(x.ns);
   x.len = __builtin_amdgcn_readfirstlane(x.len), x.first = __builtin_amdgcn_readfirstlane(x.first);
@@ -127,9 +138,12 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   };
   look_up(page_of(a, s0), page_of(a, min(a.max_len, s0 + stretch) - 1) - page_of(a, s0) + 1);
   const Seq q = sequence(a, s);
-  const int rows = q.n * a.group, heads = a.H * a.group;
-  if (q.n <= 0 || rows > a.few_rows) return;
-  const int s1 = min(q.len, s0 + x.len);
+  const int all = q.n * a.group, heads = a.H * a.group, r0 = x.block * a.few.block, rows = min(all - r0, a.few.block);
+  if (q.n <= 0 || rows <= 0 || all > a.few_rows) return;
+  // positions that the block's first row sees, and its last
+  const int shown = a.causal ? q.shown + r0 / a.group : q.len;
+  const int shown_last = a.causal ? q.shown + (r0 + rows - 1) / a.group : q.len;
+  const int s1 = min(min(q.len, shown_last), s0 + x.len);
   const float c = 1.44269504088896340736f / sqrtf((float)D);
 
   // ---- queries: lane (row c16, q4) of MFMA m holds 8 elements from kcol(m)
@@ -138,7 +152,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   int sees[NT];  // positions that the lane's row sees
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int row = min(16 * t + c16, rows - 1), tok = row / a.group, head = row - tok * a.group;
+    const int row = r0 + min(16 * t + c16, rows - 1), tok = row / a.group, head = row - tok * a.group;
     const w4_half* const qp = a.q + (long long)(q.q0 + tok) * a.q_stride + (long long)(h * a.group + head) * D;
 #pragma unroll
     for (int m = 0; m < NC; ++m) __builtin_memcpy(&qop[t][m], qp + kcol(m), 16);
@@ -216,7 +230,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
       }
     }
     // register k = 4 j + i of a row's scores is position 16 j + 4 q4 + i
-    if (there != ~0u || t0 + PF_TILE > q.shown) {  // wave-uniform
+    if (there != ~0u || t0 + PF_TILE > shown) {  // wave-uniform
       const uint32_t mine = there >> (4 * q4);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -369,7 +383,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         const float e = __builtin_amdgcn_exp2f(p[D + 1] - use);
         sum0 += e * p[d], sum1 += e * p[d + 1], den4 += e * p[D];
       }
-      const int row = 16 * t + r, tok = row / a.group, head = row - tok * a.group;
+      const int row = r0 + 16 * t + r, tok = row / a.group, head = row - tok * a.group;
       const long long at = (long long)(q.q0 + tok) * heads + h * a.group + head;
       if (ns == 1) {
         const float inv = den4 == 0.0f ? 0.0f : 1.0f / den4;
@@ -377,7 +391,7 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
         w4_half* const dst = a.out + at * D + d;
         dst[0] = (uint16_t)as_u32(v), dst[1] = (uint16_t)(as_u32(v) >> 16);
       } else {
-        float* const dst = a.few_part + ((long long)blockIdx.x * a.few.rows + row) * (D + 2);
+        float* const dst = a.few_part + ((long long)blockIdx.x * a.few.rows + 16 * t + r) * (D + 2);
         publish(dst + 2 + d, sum0, sum1);
         if (d == 0) publish(dst, top, den4);
       }
@@ -399,14 +413,14 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   const long long pitch = (long long)a.few.rows * (D + 2);
   auto join = [&](auto rows_at_a_time, auto batch) {  // (of a wave; the first again where there are no more)
     constexpr int N = decltype(rows_at_a_time)::value;
-    for (int r0 = wave; r0 < rows; r0 += N * PF_WAVES) {
+    for (int i0 = wave; i0 < rows; i0 += N * PF_WAVES) {
       const float* from[N];
       w4_half* to[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int r = r0 + i * PF_WAVES < rows ? r0 + i * PF_WAVES : r0, tok = r / a.group;
+        const int r = i0 + i * PF_WAVES < rows ? i0 + i * PF_WAVES : i0, row = r0 + r, tok = row / a.group;
         from[i] = a.few_part + x.first * pitch + r * (D + 2);
-        to[i] = a.out + ((long long)(q.q0 + tok) * heads + h * a.group + (r - tok * a.group)) * D;
+        to[i] = a.out + ((long long)(q.q0 + tok) * heads + h * a.group + (row - tok * a.group)) * D;
       }
       join_rows<N, decltype(batch)::value, true>(from, pitch, ns, D, to);
     }
@@ -430,32 +444,31 @@ void go_page(const Pages& a, hipStream_t s) {
 }
 template <int D>
 hipError_t go(const Pages& a, hipStream_t s) {
-  if (a.few_rows <= 16) go_page<D, 1>(a, s);
-  else if (a.few_rows <= 32) go_page<D, 2>(a, s);
-  else if constexpr (D <= 128) go_page<D, 4>(a, s);
+  if (a.few.block == 16) go_page<D, 1>(a, s);
+  else go_page<D, 2>(a, s);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int pages_few_most(const PagesArgs& a) {
-  if (a.D != 64 && a.D != 96 && a.D != 128 && a.D != 256) return 0;
-  if (((uintptr_t)a.q_k | (uintptr_t)a.q_v) & 15) return 0;
-  return a.D == 256 ? 32 : 64;  // (registers: the sums of 64 rows x 256 elements take all of them)
+bool pages_few_applies(const PagesArgs& a) {
+  return (a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && (((uintptr_t)a.q_k | (uintptr_t)a.q_v) & 15) == 0;
 }
 
-FewPlan pages_few_plan(const PagesArgs& a, int rows) {
-  // What runs at a time: two workgroups per compute unit, one where LDS (D = 256) or registers (64 rows) leave no more.
-  const int places = a.D == 256 || rows > 32 ? 256 : 512;
-  const long long units = (long long)a.nseq * a.H;
+FewPlan pages_few_plan(const PagesArgs& a, long long rows) {
+  // What runs at a time: two workgroups per compute unit, one where LDS leaves no more.
+  const int places = a.D == 256 ? 256 : 512;
   FewPlan p{};
-  p.rows = rows;
-  // Caches of up to 512 positions take less time than a split costs (partial sums, arrival, join: 3 us); many units fill
-  // the card without, and beyond 256 sequences a workgroup does not look for its share.
-  p.alone = a.max_len <= 512 || a.nseq > 256 || units >= 8 * places ||
+  p.block = rows <= 16 ? 16 : 32;
+  p.blocks = (int)((rows + p.block - 1) / p.block);
+  p.rows = rows < p.block ? (int)rows : p.block;
+  const long long units = (long long)a.nseq * a.H * p.blocks;
+  // Units are not split where many of them fill the card without it, and beyond 256 sequences a workgroup does not look for
+  // its share; nor up to 512 positions, which take less time than a split costs (partial sums, arrival, join: 3 us).
+  p.step_least = a.max_len <= 512 ? 4 : 2;
+  p.alone = (a.max_len <= 512 && p.blocks == 1) || a.nseq > 256 || units >= 8 * places ||
             units * ((a.max_len + PF_STEP - 1) / PF_STEP) >= (1ll << 31);  // (counts are 32-bit)
   p.grid = (int)(p.alone ? units : units <= places * 3 / 4 ? places : units + places);
-  p.step_least = 2;
   return p;
 }
 

@@ -26,13 +26,15 @@ __device__ __forceinline__ int tiles_of(const Pages& a, int s) {
   return rows <= a.few_rows ? 0 : (rows + PM_ROWS - 1) / PM_ROWS;
 }
 
-// PG: 16: pages of a multiple of 16 rows, 4: of 4, 1: any.
-template <int D, int PG>
-__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pages_many_kernel(const Pages a) {
+// P16: pages of a multiple of 16 rows: eight of a lane's scores in a row have one page, the same in all lanes.  Otherwise
+// the scales of a tile's positions are laid out one by one when it is requested.
+template <int D, bool P16>
+__global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_kernel(const Pages a) {
   constexpr int P = D / 16, NE = D / 32;  // pieces of a row, 32-element blocks of it
   constexpr int SIDE = PM_TILE * D, SLOT = 2 * SIDE, LOADS = 2 * P / PM_WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t ring[PM_SLOTS][SLOT];
   __shared__ PageEntry table[PM_TABLE];
+  __shared__ __attribute__((aligned(16))) float scale_of[P16 ? 1 : PM_SLOTS][3][PM_TILE];  // skc, lsv, inv of each position
   __shared__ int odd;  // a page of the table is none of the pool, or has a V scale of 0
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
   // Requests the wave's share of the tile at t0 into slot sl; returns which of its positions are there, and which of
   // their rows of V count (`fine`: there, under a scale that is not 0).
   auto request = [&](int sl, int t0, uint64_t& fine) -> uint64_t {
-    if constexpr (PG == 16 && 64 % P == 0) {
+    if constexpr (P16 && 64 % P == 0) {
       // Whole tiles of pages of whole 16s: the rows of a load lie side by side on one page, so its place is a scalar and
       // a lane adds what it always adds.
       if (t0 + PM_TILE <= s1 && !odd_pages) {
@@ -131,6 +133,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
     const int j = there ? page_of(a, t) : j0;
     const PageEntry e = table[j - j0];
     there = there && e.row0 >= 0;
+    if (!P16 && lane >> 4 == wave) scale_of[sl][0][lane] = e.skc, scale_of[sl][1][lane] = e.lsv, scale_of[sl][2][lane] = e.inv;
     const int row = there ? e.row0 + (t - j * a.page) : 0;  // (others read row 0 and drop it)
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -177,23 +180,20 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
   auto read_v = [&](const uint8_t* slot, int kk, int e) {
     return read_transposed(slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1) + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
   };
-  constexpr int SAME = PG == 1 ? 1 : PG == 4 ? 4 : 8;  // of a lane's scores: registers in a row with one page
-  float skc[32 / SAME], lsv[32 / SAME], inv[32 / SAME];
+  constexpr int SAME = 8;
+  float skc[4], lsv[4], inv[4];
   // register k = 16 b + 4 g + i of the scores is position 32 b + 8 g + 4 half + i
   auto position = [&](int k) { return 32 * (k >> 4) + 8 * ((k >> 2) & 3) + 4 * half + (k & 3); };
-  auto entry = [&](int t0, int k) {  // (positions past the split have the last one's)
-    const int at = PG == 16 ? position(k) - 4 * half : position(k);
-    return table[page_of(a, min(t0 + at, s1 - 1)) - j0];
-  };
   auto read_scales = [&](int t0) {
-    if constexpr (SAME > 1)
+    if constexpr (P16)
 #pragma unroll
-      for (int k = 0; k < 32; k += SAME) {
-        const PageEntry e = entry(t0, k);
+      for (int k = 0; k < 32; k += SAME) {  // (positions past the split have the last one's)
+        const PageEntry e = table[page_of(a, min(t0 + position(k) - 4 * half, s1 - 1)) - j0];
         skc[k / SAME] = e.skc, lsv[k / SAME] = e.lsv, inv[k / SAME] = e.inv;
       }
   };
-  auto weights = [&](uint8_t* slot, int t0, uint64_t there, uint64_t fine) {
+  auto weights = [&](int sl, int t0, uint64_t there, uint64_t fine) {
+    uint8_t* const slot = ring[sl];
     if (fine != ~0ull) {
       // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place (every wave
       // writes the same ones, before its own reads)
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
       }
     }
     float top = -INFINITY;
-    if constexpr (SAME > 1) {
+    if constexpr (P16) {
 #pragma unroll
       for (int k = 0; k < 32; k += SAME) {
         float m = sc[k >> 4][k & 15];
@@ -227,11 +227,14 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        const PageEntry e = entry(t0, k);
-        const float y = __builtin_fmaf(sc[k >> 4][k & 15], e.skc, e.lsv);
-        sc[k >> 4][k & 15] = y;
-        top = fmaxf(top, y);
+      for (int k = 0; k < 32; k += 4) {
+        const f4 z = *(const f4*)&scale_of[sl][0][position(k)], v = *(const f4*)&scale_of[sl][1][position(k)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = __builtin_fmaf(sc[k >> 4][(k & 15) + i], z[i], v[i]);
+          sc[k >> 4][(k & 15) + i] = y;
+          top = fmaxf(top, y);
+        }
       }
     }
     top = max_over_32(top);
@@ -244,18 +247,32 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
       M = m_new;
     }
     const float use = M == -INFINITY ? 0.0f : M;
+    // (denominators take the weights as they are in FP32: under a small scale of V the halves lose what they need)
+    if constexpr (P16) {
 #pragma unroll
-    for (int k0 = 0; k0 < 32; k0 += SAME) {
-      const float add = SAME > 1 ? lsv[k0 / SAME] - use : -use;
-      float sum = 0.0f;
+      for (int k0 = 0; k0 < 32; k0 += SAME) {
+        const float add = lsv[k0 / SAME] - use;
+        float sum = 0.0f;
 #pragma unroll
-      for (int k = k0; k < k0 + SAME; ++k) {
-        const float x = sc[k >> 4][k & 15];
-        const float w = __builtin_amdgcn_exp2f(SAME > 1 ? __builtin_fmaf(x, skc[k0 / SAME], add) : x + add);
-        sum += w;  // (as it is in FP32: under a small scale of V the halves lose what the denominator needs)
-        pop[k >> 3][k & 7] = (_Float16)w;
+        for (int k = k0; k < k0 + SAME; ++k) {
+          const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k >> 4][k & 15], skc[k0 / SAME], add));
+          sum += w;
+          pop[k >> 3][k & 7] = (_Float16)w;
+        }
+        l = __builtin_fmaf(sum, inv[k0 / SAME], l);
       }
-      l = __builtin_fmaf(sum, SAME > 1 ? inv[k0 / SAME] : entry(t0, k0).inv, l);
+    } else {
+#pragma unroll
+      for (int k0 = 0; k0 < 32; k0 += 4) {
+        const f4 z = *(const f4*)&scale_of[sl][2][position(k0)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = k0 + i;
+          const float w = __builtin_amdgcn_exp2f(sc[k >> 4][k & 15] - use);
+          l = __builtin_fmaf(w, z[i], l);
+          pop[k >> 3][k & 7] = (_Float16)w;
+        }
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
@@ -311,7 +328,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 && PG > 1 ? 2 : 1) void pag
       if (t0 < wave_end && there) {
         read_scales(t0);
         scores(ring[sl]);
-        weights(ring[sl], t0, there, fine);
+        weights(sl, t0, there, fine);
         add_values(ring[sl]);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
@@ -359,21 +376,16 @@ long long most_tiles(const PagesArgs& a, int few_rows) {
 template <int D>
 hipError_t go(const Pages& a, hipStream_t s) {
   const dim3 grid((unsigned)(most_tiles(a, a.few_rows) * a.H), (unsigned)a.many.nsplit);
-  if (a.page % 16 == 0) pages_many_kernel<D, 16><<<grid, PM_WAVES * 64, 0, s>>>(a);
-  else if (a.page % 4 == 0) pages_many_kernel<D, 4><<<grid, PM_WAVES * 64, 0, s>>>(a);
-  else pages_many_kernel<D, 1><<<grid, PM_WAVES * 64, 0, s>>>(a);
+  if (a.page % 16 == 0) pages_many_kernel<D, true><<<grid, PM_WAVES * 64, 0, s>>>(a);
+  else pages_many_kernel<D, false><<<grid, PM_WAVES * 64, 0, s>>>(a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-bool pages_many_applies(const PagesArgs& a) {
-  return (a.D == 64 || a.D == 96 || a.D == 128 || a.D == 256) && (((uintptr_t)a.q_k | (uintptr_t)a.q_v) & 15) == 0;
-}
-
 PagesPlan pages_many_plan(const PagesArgs& a) {
-  // two workgroups of 128 rows per compute unit where the rows do not give them, no split shorter than 512 positions
-  const long long tiles = ((long long)a.tokens * a.group + 127) / 128 * a.H;
+  // two workgroups per compute unit where the rows do not give them, no split shorter than 512 positions
+  const long long tiles = ((long long)a.tokens * a.group + PM_ROWS - 1) / PM_ROWS * a.H;
   const int most = (a.max_len + 511) / 512;
   long long n = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
   n = n > most ? most : n < 1 ? 1 : n;
