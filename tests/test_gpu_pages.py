@@ -405,6 +405,32 @@ def test_nan_of_one_query_stays_its_own(adds):
     assert np.array_equal(got[keep].view(np.uint16), clean.view(np.uint16).reshape(got.shape)[keep])
 
 
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 7, 24), (256, 2, 64), (96, 16, 16), (128, 8, 1), (40, 2, 5)])
+@pytest.mark.parametrize("lens, adds", [([40, 33, 5], [4, 1, 5]), ([50, 300], [45, 150]), ([3000, 70], [1500, 70])])
+def test_nan_codes_reach_only_the_rows_that_see_them(D, group, page, lens, adds):
+    """A cached NaN makes NaN of its column (of V) or row (of K) where a causal query sees it, and of nothing else."""
+    if D == 40 and lens[0] == 3000:
+        lens, adds = [600, 70], [300, 70]
+    a = Attn(D + group, lens, adds, 1, group, D, page)
+    rng = np.random.default_rng(7)
+    for s, (n, m) in enumerate(zip(lens, adds)):
+        for back in {1, 2, max(1, m // 2), max(1, m - 1)}:  # among the last m tokens
+            t = n - back
+            row = a.bt[s, t // page] * page + t % page
+            a.v[0].reshape(-1, D)[row, rng.integers(0, D, 2)] = [0x7F, 0xFF]
+        if s == 1:
+            row = a.bt[s, (n - 2) // page] * page + (n - 2) % page
+            a.k[0].reshape(-1, D)[row, 3] = 0x7F
+    a.d[1].copy_(to_dev(a.k[0]).view(a.d[1].shape)), a.d[3].copy_(to_dev(a.v[0]).view(a.d[3].shape))
+    got = host(a.run()).view(np.float16).reshape(a.before.shape).astype(np.float64)
+    want, tol = a.want()
+    nan = np.isnan(want)
+    assert nan.any() and not nan.all()
+    assert np.array_equal(np.isnan(got), nan), np.argwhere(np.isnan(got) != nan)[:4].tolist()
+    off = np.abs(got - want)[~nan]
+    assert (off <= tol[~nan]).all()
+
+
 # ---- use ---------------------------------------------------------------------------------
 
 

@@ -663,7 +663,7 @@ int w4_quantize_f8_pages(const w4_f8_pages_view* p, const w4_half* k, const w4_h
   REQUIRE(tokens >= 0, "quantize_f8_pages: bad dims");
   REQUIRE(k && v && status && (slots || tokens == 0), "quantize_f8_pages: null io pointer");
   REQUIRE(row_stride == 0 || row_stride >= (long long)p->H * p->D, "quantize_f8_pages: row_stride is shorter than a row");
-  REQUIRE((long long)tokens * 2 * p->H < (1LL << 30), "quantize_f8_pages: too many rows");
+  REQUIRE((long long)tokens * 2 * p->H < (1LL << 29), "quantize_f8_pages: too many rows");
   if (tokens == 0) return W4_OK;
   const long long stride = row_stride ? row_stride : (long long)p->H * p->D;
   return done("quantize_f8_pages",
@@ -678,7 +678,7 @@ static int pages_args(w4k::PagesArgs& a, const w4_f8_pages_view* p, const w4_pag
   REQUIRE(b->bt && b->lens, "attention f8 pages: null pointer");
   REQUIRE(b->cu_q || (b->tokens == b->nseq && b->max_q == 1), "attention f8 pages: several tokens per sequence need cu_q");
   REQUIRE(group >= 1 && group <= 64, "attention f8 pages: bad query group");
-  REQUIRE((long long)b->nseq * p->H < (1LL << 31) && (long long)b->tokens * p->H * group < (1LL << 31),
+  REQUIRE((long long)b->nseq * p->H < (1LL << 23) && (long long)b->tokens * p->H * group < (1LL << 28),
           "attention f8 pages: too many rows");
   a = w4k::PagesArgs{};
   a.H = p->H; a.D = p->D; a.page = p->page; a.npages = p->npages;

@@ -231,6 +231,14 @@ __device__ __forceinline__ h8 codes_to_half(uint32_t lo, uint32_t hi) {
   return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Causal rows of a tile that do not see all of it.  A weight of 0 does not keep a NaN code of V out of a matrix product, so
+// tiles that hold one (0x7F, 0xFF) go a second way: the codes without it, and a product of what is NaN with what a row sees.
+__device__ __forceinline__ uint32_t has_nan_code(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // 0xFF at each
+  const uint32_t x = has_nan_code(w) >> 7;
+  return (x << 8) - x;
+}
+
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef int i2 __attribute__((ext_vector_type(2)));
 // 8 rows x 16 bytes read transposed by 16 lanes: lane i gives the address of half a row (row i / 2) and gets byte i of

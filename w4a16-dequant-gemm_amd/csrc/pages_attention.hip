@@ -5,94 +5,97 @@ namespace w4k {
 namespace {
 
 // ---- any head dimension, page size and alignment -----------------------------------------------
-// One workgroup per row and split, tiles of 256 positions: a thread forms one position's score, then owns four
-// columns of O for every (256 / (D / 4))-th position of the tile.
+// A workgroup takes rows of one split in turn, tiles of 256 positions: a thread forms one position's score, then owns
+// four columns of O for every (256 / (D / 4))-th position of the tile.
 __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
   __shared__ float qs[512], red[4], weight[256], o4[256][4];
   __shared__ long long at[256];  // offset of a position's row in the codes; -1: not seen
   const int tid = threadIdx.x, D = a.D, heads = a.H * a.group;
-  const int tok = (int)(blockIdx.x / heads), head = (int)(blockIdx.x % heads), h = head / a.group;
-  const int s = sequence_of(a, tok);
-  if (s < 0) return;
-  const Seq q = sequence(a, s);
-  const int i = tok - q.q0;
-  if (i >= q.n || q.n * a.group <= a.few_rows) return;
-  const int end = min(q.len, a.causal ? q.shown + i : q.len);  // positions that the row sees
-  const int ns = max(1, splits(a.many, q.len));
-  const int split = blockIdx.y;
-  if (split >= ns) return;
-  const int s0 = split * a.many.split_len, s1 = min(end, s0 + a.many.split_len);
-  const float c = 1.44269504088896340736f / sqrtf((float)D);
-  const uint8_t* const kp = a.q_k + (long long)h * a.npages * a.page * D;
-  const uint8_t* const vp = a.q_v + (long long)h * a.npages * a.page * D;
-  for (int d = tid; d < D; d += 256) qs[d] = half_bits_to_float(a.q[(long long)tok * a.q_stride + (long long)head * D + d]);
-  const int cols = D / 4, groups = 256 / cols, g = tid / cols, col = tid - g * cols;
-  float M = -INFINITY, l = 0.0f, o[4] = {};
-  __syncthreads();
-  for (int t0 = s0; t0 < s1; t0 += 256) {
-    const int t = t0 + tid;
-    float x = -INFINITY, y = -INFINITY, sv = 0.0f;
-    long long off = -1;
-    if (t < s1) {
-      const int j = page_of(a, t);
-      const int id = a.bt[(long long)s * a.stride + j];
-      if (id >= 0 && id < a.npages) {
-        off = ((long long)id * a.page + (t - j * a.page)) * D;
-        const uint32_t* const row = (const uint32_t*)(kp + off);
-        float dot = 0.0f;
-        for (int d = 0; d < D; d += 4) {
-          const uint32_t w = row[d / 4];
+  const int all_rows = a.tokens * heads;
+  for (int row = blockIdx.x; row < all_rows; row += gridDim.x) {
+    __syncthreads();  // (the row before has been read)
+    const int tok = row / heads, head = row - tok * heads, h = head / a.group;
+    const int s = sequence_of(a, tok);
+    if (s < 0) continue;
+    const Seq q = sequence(a, s);
+    const int i = tok - q.q0;
+    if (i >= q.n || q.n * a.group <= a.few_rows) continue;
+    const int end = min(q.len, a.causal ? q.shown + i : q.len);  // positions that the row sees
+    const int ns = max(1, splits(a.many, q.len));
+    const int split = blockIdx.y;
+    if (split >= ns) continue;
+    const int s0 = split * a.many.split_len, s1 = min(end, s0 + a.many.split_len);
+    const float c = 1.44269504088896340736f / sqrtf((float)D);
+    const uint8_t* const kp = a.q_k + (long long)h * a.npages * a.page * D;
+    const uint8_t* const vp = a.q_v + (long long)h * a.npages * a.page * D;
+    for (int d = tid; d < D; d += 256) qs[d] = half_bits_to_float(a.q[(long long)tok * a.q_stride + (long long)head * D + d]);
+    const int cols = D / 4, groups = 256 / cols, g = tid / cols, col = tid - g * cols;
+    float M = -INFINITY, l = 0.0f, o[4] = {};
+    __syncthreads();
+    for (int t0 = s0; t0 < s1; t0 += 256) {
+      const int t = t0 + tid;
+      float x = -INFINITY, y = -INFINITY, sv = 0.0f;
+      long long off = -1;
+      if (t < s1) {
+        const int j = page_of(a, t);
+        const int id = a.bt[(long long)s * a.stride + j];
+        if (id >= 0 && id < a.npages) {
+          off = ((long long)id * a.page + (t - j * a.page)) * D;
+          const uint32_t* const row = (const uint32_t*)(kp + off);
+          float dot = 0.0f;
+          for (int d = 0; d < D; d += 4) {
+            const uint32_t w = row[d / 4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(qs[d + e], f8_to_float((w >> (8 * e)) & 0xFFu), dot);
+            for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(qs[d + e], f8_to_float((w >> (8 * e)) & 0xFFu), dot);
+          }
+          sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
+          x = dot * (half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c);
+          y = x + (sv > 0.0f ? __log2f(sv) : -25.0f);
         }
-        sv = half_bits_to_float(a.s_v[(long long)h * a.npages + id]);
-        x = dot * (half_bits_to_float(a.s_k[(long long)h * a.npages + id]) * c);
-        y = x + (sv > 0.0f ? __log2f(sv) : -25.0f);
       }
+      at[tid] = off;
+      float m = y;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+      if ((tid & 63) == 0) red[tid >> 6] = m;
+      __syncthreads();
+      const float m_new = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), M);
+      const float use = m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = exp2f(M - use);
+      const float p = off >= 0 ? exp2f(x - use) : 0.0f;
+      weight[tid] = p * sv;
+      M = m_new;
+      l = l * alpha + p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= alpha;
+      __syncthreads();
+      if (g < groups) {
+        const int here = min(256, s1 - t0);
+        for (int k = g; k < here; k += groups)
+          if (at[k] >= 0) {
+            const uint32_t w = *(const uint32_t*)(vp + at[k] + 4 * col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(weight[k], f8_to_float((w >> (8 * e)) & 0xFFu), o[e]);
+          }
+      }
+      __syncthreads();
     }
-    at[tid] = off;
-    float m = y;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    if ((tid & 63) == 0) red[tid >> 6] = m;
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    if ((tid & 63) == 0) red[tid >> 6] = l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o4[tid][e] = o[e];
     __syncthreads();
-    const float m_new = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), M);
-    const float use = m_new == -INFINITY ? 0.0f : m_new;
-    const float alpha = exp2f(M - use);
-    const float p = off >= 0 ? exp2f(x - use) : 0.0f;
-    weight[tid] = p * sv;
-    M = m_new;
-    l = l * alpha + p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] *= alpha;
-    __syncthreads();
-    if (g < groups) {
-      const int here = min(256, s1 - t0);
-      for (int k = g; k < here; k += groups)
-        if (at[k] >= 0) {
-          const uint32_t w = *(const uint32_t*)(vp + at[k] + 4 * col);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(weight[k], f8_to_float((w >> (8 * e)) & 0xFFu), o[e]);
-        }
+    l = red[0] + red[1] + red[2] + red[3];
+    float* const part = part_of(a, row, split);
+    for (int d = tid; d < D; d += 256) {
+      float sum = 0.0f;
+      for (int k = 0; k < groups; ++k) sum += o4[k * cols + d / 4][d & 3];
+      if (ns > 1) part[2 + d] = sum;
+      else a.out[(long long)row * D + d] = __builtin_bit_cast(uint16_t, (_Float16)(l == 0.0f ? 0.0f : sum / l));
     }
-    __syncthreads();
+    if (ns > 1 && tid == 0) part[0] = M, part[1] = l;
   }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
-  if ((tid & 63) == 0) red[tid >> 6] = l;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o4[tid][e] = o[e];
-  __syncthreads();
-  l = red[0] + red[1] + red[2] + red[3];
-  const long long row = (long long)tok * heads + head;
-  float* const part = part_of(a, row, split);
-  for (int d = tid; d < D; d += 256) {
-    float sum = 0.0f;
-    for (int k = 0; k < groups; ++k) sum += o4[k * cols + d / 4][d & 3];
-    if (ns > 1) part[2 + d] = sum;
-    else a.out[row * D + d] = __builtin_bit_cast(uint16_t, (_Float16)(l == 0.0f ? 0.0f : sum / l));
-  }
-  if (ns > 1 && tid == 0) part[0] = M, part[1] = l;
 }
 
 // ---- rows that several workgroups formed ----------------------------------------------------------
@@ -187,7 +190,7 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   if (e == hipSuccess && more && fast) {
     e = launch_pages_many(a, s);
   } else if (e == hipSuccess && more) {
-    pages_general_kernel<<<dim3((unsigned)rows, a.many.nsplit), 256, 0, s>>>(a);
+    pages_general_kernel<<<dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20), a.many.nsplit), 256, 0, s>>>(a);
     e = hipGetLastError();
   }
   if (e == hipSuccess && a.many.nsplit > 1) {

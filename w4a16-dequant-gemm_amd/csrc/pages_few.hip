@@ -202,6 +202,49 @@ __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a)
   const int vrow = (c16 >> 1) < 4 ? 4 * q4 + (c16 >> 1) : 16 + 4 * q4 + (c16 >> 1) - 4;
 
   auto compute = [&](uint8_t* slot, int t0, uint32_t there) {
+    if (t0 + PF_TILE > shown && shown_last > shown) {  // wave-uniform: some rows see what others do not
+      int own = lane, from = vrow;  // (unknown to the compiler, which keeps addresses of this way out of the loop's registers)
+      asm volatile("" : "+v"(own), "+v"(from));
+      u4* const v = (u4*)(slot + SIDE) + own;
+      uint32_t nan = 0;
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const u4 w = v[64 * i];
+        nan |= has_nan_code(w[0]) | has_nan_code(w[1]) | has_nan_code(w[2]) | has_nan_code(w[3]);
+      }
+      if (__builtin_amdgcn_ballot_w64(nan != 0) != 0) {
+        const uint32_t mine = there >> (4 * q4);
+        h8 seen[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int at = 16 * (k >> 2) + (k & 3);
+            seen[t][k] = ((mine >> at) & 1) && at < sees[t] - t0 - 4 * q4 ? (_Float16)1.0f : (_Float16)0.0f;
+          }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers are for the way that is taken)
+          const u2 w = read_transposed(slot + SIDE + from * D + 8 * (own & 1) + 16 * (e ^ vswz(from)));
+          const h8 ones = codes_to_half(nan_codes(w[0]) & 0x38383838u, nan_codes(w[1]) & 0x38383838u);  // 0x38: 1
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            f4 n = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, seen[t], f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n[i] = n[i] > 0.0f ? __builtin_nanf("") : 0.0f;
+            o[t][e] += n;
+          }
+        }
+#pragma unroll 1
+        for (int i = 0; i < KI; ++i) {
+          u4 w = v[64 * i];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] &= ~nan_codes(w[j]);
+          v[64 * i] = w;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      }
+    }
     f4 sc[NT][2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -467,7 +510,7 @@ FewPlan pages_few_plan(const PagesArgs& a, long long rows) {
   // its share; nor up to 512 positions, which take less time than a split costs (partial sums, arrival, join: 3 us).
   p.step_least = a.max_len <= 512 ? 4 : 2;
   p.alone = (a.max_len <= 512 && p.blocks == 1) || a.nseq > 256 || units >= 8 * places ||
-            units * ((a.max_len + PF_STEP - 1) / PF_STEP) >= (1ll << 31);  // (counts are 32-bit)
+            units * ((a.max_len + PF_STEP - 1) / PF_STEP) >= (1ll << 28);  // (quotients of floats: see over())
   p.grid = (int)(p.alone ? units : units <= places * 3 / 4 ? places : units + places);
   return p;
 }

@@ -70,6 +70,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
   auto seen_by = [&](int row) { return a.causal ? min(q.len, q.shown + min(row, rows - 1) / a.group) : q.len; };
   const int s0 = split * a.many.split_len, s1 = min(seen_by(r0 + PM_ROWS - 1), s0 + a.many.split_len);
   const int wave_end = w0 < rows ? min(s1, seen_by(w0 + 31)) : 0, wave_all = seen_by(w0);
+  const int all_see = seen_by(r0);
   const int row = min(w0 + c32, rows - 1), tok = row / a.group;
   const int sees = seen_by(row);
   const long long at = (long long)(q.q0 + tok) * heads + h * a.group + (row - tok * a.group);
@@ -146,13 +147,13 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
     return __builtin_amdgcn_ballot_w64(there);
   };
 
-  const int i16 = lane & 15, dhalf = (lane >> 4) & 1;
+  const int i16 = lane & 15;
   const int vrow = ((i16 >> 1) < 4 ? (i16 >> 1) : 4 + (i16 >> 1)) + 4 * half;  // of the 16 positions of a step
 
   // A tile's three steps.  Reads of LDS stand together ahead of what uses them, so that one latency is waited for and
   // not one per matrix product: all of a tile's K (D = 256: a half), and its V before the softmax.
   f16v sc[2];
-  constexpr int VG = NE > 4 ? 0 : 4;  // steps of 16 positions whose V is read ahead
+  constexpr int VG = NE > 4 ? 0 : NE < 4 || P16 ? 4 : 2;  // steps of 16 positions whose V is read ahead, as registers allow
   u2 vraw[VG ? VG : 1][NE];
   h8 pop[4];
   auto scores = [&](const uint8_t* slot) {
@@ -177,8 +178,11 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
     }
     __builtin_amdgcn_sched_barrier(0);
   };
+  auto v_of = [&](const uint8_t* slot, int kk, int e, int from, int l) {
+    return slot + SIDE + 16 * kk * D + from * D + 8 * (l & 1) + 16 * ((2 * e + ((l >> 4) & 1)) ^ vswz(from));
+  };
   auto read_v = [&](const uint8_t* slot, int kk, int e) {
-    return read_transposed(slot + SIDE + 16 * kk * D + vrow * D + 8 * (i16 & 1) + 16 * ((2 * e + dhalf) ^ vswz(vrow)));
+    return read_transposed(v_of(slot, kk, e, vrow, lane));
   };
   constexpr int SAME = 8;
   float skc[4], lsv[4], inv[4];
@@ -293,6 +297,54 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
     asm volatile("" : : : "memory");
   };
 
+  // A tile that the first of the workgroup's rows does not see all of, with a NaN code of V in it: the rows that see the code
+  // are NaN, then it is taken out for the others.  (All waves look at the whole tile, so they agree on the barriers.)
+  auto nan_codes_of = [&](uint8_t* slot, int t0, uint64_t there) {
+    int own = lane, from = vrow;  // (unknown to the compiler, which keeps addresses of this way out of the loop's registers)
+    asm volatile("" : "+v"(own), "+v"(from));
+    u4* const v = (u4*)(slot + SIDE);
+    uint32_t nan = 0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const u4 w = v[64 * i + own];
+      nan |= has_nan_code(w[0]) | has_nan_code(w[1]) | has_nan_code(w[2]) | has_nan_code(w[3]);
+    }
+    if (__builtin_amdgcn_ballot_w64(nan != 0) == 0) return;
+    const uint64_t mine = there >> (4 * (own >> 5));
+    const int left = sees - t0 - 4 * (own >> 5);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      f16v n = f16v{};
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        __builtin_amdgcn_sched_barrier(0);  // (one at a time: registers are for the way that is taken)
+        const u2 w = read_transposed(v_of(slot, kk, e, from, own));
+        h8 seen;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int at = position(8 * kk + k) - 4 * half;  // (a constant)
+          seen[k] = ((mine >> at) & 1) && at < left ? (_Float16)1.0f : (_Float16)0.0f;
+        }
+        const h8 ones = codes_to_half(nan_codes(w[0]) & 0x38383838u, nan_codes(w[1]) & 0x38383838u);  // 0x38: 1
+        n = __builtin_amdgcn_mfma_f32_32x32x16_f16(ones, seen, n, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) n[i] = n[i] > 0.0f ? __builtin_nanf("") : 0.0f;
+      o[e] += n;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    barrier();
+#pragma unroll 1
+    for (int i = tid; i < SIDE / 16; i += PM_WAVES * 64) {
+      u4 w = v[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] &= ~nan_codes(w[j]);
+      v[i] = w;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    barrier();
+  };
+
   // ---- stretches of the split whose pages fit the table
   const int stretch = (int)min((long long)(PM_TABLE - 2) * a.page / PM_TILE * PM_TILE, (long long)a.many.split_len);
   for (int c0 = s0; c0 < s1; c0 += stretch) {
@@ -325,6 +377,7 @@ __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_ke
       barrier();
       uint64_t there2 = 0, fine2 = 0;
       if (it + 2 < nit) there2 = request(sl == 0 ? 2 : sl - 1, t0 + 2 * PM_TILE, fine2);
+      if (t0 + PM_TILE > all_see && s1 > all_see) nan_codes_of(ring[sl], t0, there);  // uniform
       if (t0 < wave_end && there) {
         read_scales(t0);
         scores(ring[sl]);

@@ -218,7 +218,7 @@ hipError_t launch_quantize_f8_pages(const w4_f8_pages_view& p, const w4_half* k,
   // units begin a run where there are more units than the card has places (up to 1024 tokens of 8 heads: one each).
   const long long pieces = (long long)p.page * p.D / (wide ? 8 : 4);
   const int L = pieces <= 32 ? 16 : pieces <= QP_KEEP * 64 ? 64 : 256;
-  a.chunk = (long long)tokens * 2 * p.H * L <= (1 << 20) || p.page == 1 ? 1 : L == 16 ? 4 : L == 64 ? 16 : 48;
+  a.chunk = (long long)tokens * 2 * p.H * L <= (1 << 20) || (p.page == 1 && tokens < (1 << 23) / p.H) ? 1 : L == 16 ? 4 : L == 64 ? 16 : 48;
   const long long units = ((long long)tokens + a.chunk - 1) / a.chunk * 2 * p.H;
   a.units = (uint32_t)units;
   a.by_page = divider(p.page), a.by_row = divider(p.D / (wide ? 8 : 4));
