@@ -405,6 +405,65 @@ def test_nan_of_one_query_stays_its_own(adds):
     assert np.array_equal(got[keep].view(np.uint16), clean.view(np.uint16).reshape(got.shape)[keep])
 
 
+@pytest.mark.parametrize("nseq", [64, 65, 200, 256, 257])
+@pytest.mark.parametrize("longest", [300, 2600])
+def test_many_sequences(nseq, longest):
+    """One long sequence among many short ones, some without tokens or positions."""
+    rng = np.random.default_rng(nseq)
+    lens, adds = rng.integers(0, 40, nseq), np.ones(nseq, np.int64)
+    lens[nseq // 2], lens[3], adds[5] = longest, 0, 0
+    Attn(nseq + longest, lens.tolist(), adds.tolist(), 1, 2, 64, 16).check()
+    if longest > 300:
+        adds[7:9], lens[7:9] = 5, 900
+        Attn(nseq, lens.tolist(), adds.tolist(), 1, 4, 64, 16).check()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("group, adds", [(33, [1, 1, 1]), (64, [1, 0, 1]), (4, [9, 16, 8]), (1, [33, 32, 65]), (7, [40, 1, 11])])
+def test_blocks_of_rows_in_splits(D, group, adds):
+    """More rows of a KV head than a workgroup takes, on caches that are cut over workgroups."""
+    Attn(D + group, [1900, 20, 700], adds, 1, group, D, 16).check()
+
+
+@pytest.mark.parametrize("adds", [[30, 21], [700, 90]])
+@pytest.mark.parametrize("page", [1, 3, 16])
+def test_a_call_of_either_kernel(adds, page):
+    """The same rows by one kernel, and by the other where the bounds of the call are far off."""
+    lens = [max(900, adds[0]), 200]
+    a = Attn(71, lens, adds, 1, 8, 128, page)
+    b = Attn(71, lens, adds, 1, 8, 128, page, max_q=adds[0] + 1000, max_len=10 ** 6)
+    a.check(), b.check()
+
+
+def test_batches_of_every_kind_in_one_workspace():
+    """Whatever a call leaves in the workspace, the next one of another shape finds what it needs."""
+    kinds = [([3000, 40], [1, 1], 2, 4, 128, 16), ([900, 800], [200, 1], 1, 4, 128, 16), ([5000], [2], 1, 7, 64, 24),
+             ([400] * 70, [1] * 70, 1, 1, 96, 16), ([2100], [1], 1, 1, 40, 16), ([700, 2000], [40, 33], 1, 2, 256, 64)]
+    calls = [Attn(80 + i, *k) for i, k in enumerate(kinds)]
+    want = [host(x.run()).copy() for x in calls]
+    space = torch.zeros(max(x.n for x in calls) + 16, dtype=torch.uint8, device=DEV)
+    order = np.random.default_rng(1).integers(0, len(calls), 60)
+    outs = [calls[i].run(space=space) for i in order]
+    assert all(np.array_equal(host(o), want[i]) for o, i in zip(outs, order))
+    for x in calls:
+        x.check()
+
+
+def test_more_rows_than_workgroups():
+    """Every row's only position is the first: its V."""
+    a = Attn(90, [1], [1], 2, 1, 4, 1, causal=False)
+    c, T, group = w4amd.capi(), 16500, 32
+    q = torch.zeros(T * 2 * group * 4, dtype=torch.float16, device=DEV)
+    out = torch.zeros_like(q)
+    cu = i32([0, T])
+    batch = c.paged_batch(1, T, T, 1, ptr(a.d[5]), a.bt.shape[1], ptr(a.d[6]), ptr(cu))
+    assert c.attention_f8_pages_workspace(a.view, batch, group) == 0
+    c.attention_f8_pages(a.view, batch, group, 0, ptr(q), 0, ptr(out))
+    got = out.cpu().numpy().reshape(T, 2, group, 4)
+    exact = pages_ref.VALUES[a.v[0][:, a.bt[0, 0], 0]] * a.v[1][:, a.bt[0, 0]].astype(np.float64)[:, None]
+    assert (np.abs(got - exact[None, :, None]) <= 2.0 ** -10 * np.abs(exact)[None, :, None]).all()
+
+
 @pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 7, 24), (256, 2, 64), (96, 16, 16), (128, 8, 1), (40, 2, 5)])
 @pytest.mark.parametrize("lens, adds", [([40, 33, 5], [4, 1, 5]), ([50, 300], [45, 150]), ([3000, 70], [1500, 70])])
 def test_nan_codes_reach_only_the_rows_that_see_them(D, group, page, lens, adds):
