@@ -644,3 +644,8 @@ def test_offsets_past_32_bits():
         want, tol = pages_ref.attention(q, np.vectorize(small.get)(ids), lens, cu, *sides, page, 4, 2, True, np.zeros(q.shape))
         got = host(out).view(np.float16).reshape(q.shape).astype(np.float64)
         assert (np.abs(got - want) <= tol).all()
+
+
+def test_serving_through_the_cpp_api():
+    from test_cpp_gates import _run
+    assert " 0 failures" in _run("test_pages", 100)

@@ -6,7 +6,9 @@ namespace {
 
 // ---- any head dimension, page size and alignment -----------------------------------------------
 // A workgroup takes rows of one split in turn, tiles of 256 positions: a thread forms one position's score, then owns
-// four columns of O for every (256 / (D / 4))-th position of the tile.
+// four columns of O for every (256 / (D / 4))-th position of the tile.  Nothing is shared between the heads of a group and
+// no matrix core is used: 8 x 32768 positions at D = 128 took it 1035 us (the kernel for few rows: 89), two prompts of 4096
+// tokens 34.5 ms (the one for many: 318 us).  Bound: the vector ALUs.
 __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
   __shared__ float qs[512], red[4], weight[256], o4[256][4];
   __shared__ long long at[256];  // offset of a position's row in the codes; -1: not seen
@@ -143,10 +145,11 @@ size_t plan(Pages& a) {
   a.few = FewPlan{};
   a.many = PagesPlan{a.max_len, 1};
   a.few_rows = 0;
-  // Decode and a few tokens per sequence are the kernel's for few rows.  So is everything up to FEW_WORK (what the
-  // scores of all rows come to at most): one launch that cuts rows into blocks of 32 and positions into splits takes 7 - 25 us
-  // there, the kernel for many rows, which waits for tile after tile, and its join 10 - 35 us (60 calls; above twice
-  // that many it is ahead by 1.3 - 2).
+  // Decode and a few tokens per sequence are the kernel's for few rows (8 x 32768 positions 89 us, 175 by the one for many; five
+  // tokens each in 16 sequences 19.2 and 24.5).  So is everything up to FEW_WORK (what the scores of all rows come to
+  // at most): one launch that cuts rows into blocks of 32 and positions into splits takes 7 to 25 us there; the kernel for
+  // many rows, which waits for tile after tile, and its join 10 to 35 us (60 calls; above that it falls behind, to 0.6 of the
+  // speed).  Decoding sequences next to prompts: 131 us with both kernels, 147 with the one for many alone.
   if (fast) a.few = pages_few_plan(a, rows);
   const double work = (double)a.tokens * a.H * a.group * a.max_len * a.D;
   if (fast && (rows <= 32 || a.max_q == 1 || (work <= FEW_WORK && !a.few.alone))) {

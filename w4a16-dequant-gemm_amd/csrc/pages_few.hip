@@ -1,7 +1,7 @@
 // Paged FP8 attention for few rows: one token per sequence, or a handful, for the query heads of one KV head.
 //
 // A workgroup takes one (sequence, KV head) and a split of its positions; its four waves take tiles of 32
-// positions in turn, each with a softmax of its own, and meet once at the end.  With up to 16 NT rows as columns:
+// positions in turn, each with a softmax of its own, and meet once at the end.  Blocks of 16 NT rows are the columns of
 //   scores  S[t][row] = sum_d K[t][d] q[row][d]   v_mfma_f32_16x16x32_f16, A = K rows, B = queries; the codes are converted
 //           by the hardware (two per instruction, exact) and the page's scale enters the scores, not the elements
 //   output  O^T[d][row] += sum_t V[t][d] w[t][row]  A = V transposed: ds_read_b64_tr_b8 takes 8 positions x 16 d out
@@ -9,7 +9,11 @@
 //           (lane (row, r): positions 4r .. 4r+3 and 16+4r .. 16+4r+3 of the tile, which the reads of V follow)
 // K and V tiles reach LDS as whole rows by direct loads (16 bytes a lane, two slots per wave), with pieces swapped
 // by row so that neither read has bank conflicts.  Page ids and scales of the split lie in a table in LDS.
-// Bound: HBM, 2 D bytes per position and KV head.
+// Workgroups find their splits from the lengths on the device; the last one of a unit joins its partial sums in place.
+// Bound: HBM, 2 D bytes per position and KV head: 8 sequences of 32768 positions, 8 KV heads of 4 query heads, D = 128:
+// 89 us, 6.0 TB/s.  Short or ragged caches are bound by the chain of lengths, page ids, scales, tiles, join: 29 sequences of 400
+// to 6007 positions, 4 KV heads, D = 64: 18.5 us, 2.7 TB/s; 4 of up to 300: 6.5 us; 5 tokens in each of 16 sequences of
+// up to 1505: 19.2 us.
 #include <type_traits>
 
 #include "pages.cuh"
@@ -98,8 +102,9 @@ __device__ __forceinline__ Share find_share(const Pages& a, int wg) {
   return x;
 }
 
-// PG4: pages of a multiple of 4 rows (four neighbouring positions have one page).
-// NB: how many times 64 sequences find_share() looks at; 0: no unit is split.
+// PG4: pages of a multiple of 4 rows (four neighbouring positions have one page, and one read of its scales: 18.5 us
+// against 19.5 without for the 29 ragged sequences).
+// NB: how many times 64 sequences find_share() looks at (1: 18.5 us for 29 of them, 4: 20.2); 0: no unit is split.
 template <int D, int NT, bool PG4, int NB>
 __global__ __launch_bounds__(PF_WAVES * 64) void pages_few_kernel(const Pages a) {
   constexpr int P = D / 16, NC = D / 32, NE = D / 16;  // 16-byte pieces of a row, MFMAs of a score, of an output
@@ -499,18 +504,22 @@ bool pages_few_applies(const PagesArgs& a) {
 }
 
 FewPlan pages_few_plan(const PagesArgs& a, long long rows) {
-  // What runs at a time: two workgroups per compute unit, one where LDS leaves no more.
+  // What runs at a time: two workgroups per compute unit (three at D = 64: 19.1 us for the ragged ones instead of 18.6), one
+  // where LDS leaves no more.
   const int places = a.D == 256 ? 256 : 512;
   FewPlan p{};
-  p.block = rows <= 16 ? 16 : 32;
+  p.block = rows <= 16 ? 16 : 32;  // 4 rows in blocks of 32: 91.9 us instead of 89.1 (8 x 32768), 7.5 instead of 6.5 (4 x 300)
   p.blocks = (int)((rows + p.block - 1) / p.block);
   p.rows = rows < p.block ? (int)rows : p.block;
   const long long units = (long long)a.nseq * a.H * p.blocks;
-  // Units are not split where many of them fill the card without it, and beyond 256 sequences a workgroup does not look for
-  // its share; nor up to 512 positions, which take less time than a split costs (partial sums, arrival, join: 3 us).
+  // Units are not split where many of them fill the card without it (256 sequences of 1000 positions, 32 heads: 321 us against
+  // 357 in splits; of 200 to 2000: 355 against 382), and beyond 256 sequences a workgroup does not look for its share; nor up to
+  // 512 positions, which take less time than a split costs (partial sums, arrival, join): 4 x 300 6.5 us against 8.2.
   p.step_least = a.max_len <= 512 ? 4 : 2;
   p.alone = (a.max_len <= 512 && p.blocks == 1) || a.nseq > 256 || units >= 8 * places ||
             units * ((a.max_len + PF_STEP - 1) / PF_STEP) >= (1ll << 28);  // (quotients of floats: see over())
+  // One round of workgroups where the units leave room in it, two where they do not: 384 units of 500 to 4000 positions
+  // take 53 us in one, 61 in two (units + places), 160 units 21.5 and 27.
   p.grid = (int)(p.alone ? units : units <= places * 3 / 4 ? places : units + places);
   return p;
 }

@@ -9,7 +9,10 @@
 // barrier per tile.  Codes are converted by each wave after it has read them: half the LDS traffic of
 // converted tiles, which would take as long as the matrix products.
 // Weights are formed as 2^(x + log2(sv) - M) at once; the denominator takes a page's sum times 1 / sv.
-// Bound: the vector ALUs (exponentials and what surrounds them) next to the matrix cores.
+// Bound: the vector ALUs -- 128 conversions of two codes, 32 exponentials and some 230 other instructions for a wave's tile
+// of 64 positions next to 32 matrix products; matrix cores are busy for a bit more than a third of the time.  Two prompts of 4096
+// and 3777 tokens, 8 KV heads of 4 query heads, D = 128: 318 us, 800 TFLOP/s (a large library product of halves on the same
+// card: 1330).
 #include "pages.cuh"
 
 namespace w4k {
@@ -27,7 +30,8 @@ __device__ __forceinline__ int tiles_of(const Pages& a, int s) {
 }
 
 // P16: pages of a multiple of 16 rows: eight of a lane's scores in a row have one page, the same in all lanes.  Otherwise
-// the scales of a tile's positions are laid out one by one when it is requested.
+// the scales of a tile's positions are laid out one by one when it is requested: 345 us for the two prompts instead of
+// 325 (same card).
 template <int D, bool P16>
 __global__ __launch_bounds__(PM_WAVES * 64, D <= 128 ? 2 : 1) void pages_many_kernel(const Pages a) {
   constexpr int P = D / 16, NE = D / 32;  // pieces of a row, 32-element blocks of it
@@ -437,7 +441,8 @@ hipError_t go(const Pages& a, hipStream_t s) {
 }  // namespace
 
 PagesPlan pages_many_plan(const PagesArgs& a) {
-  // two workgroups per compute unit where the rows do not give them, no split shorter than 512 positions
+  // two workgroups per compute unit where the rows do not give them, no split shorter than 512 positions (256: 150 calls take
+  // the same on average, from 0.9 to 1.3 times as long)
   const long long tiles = ((long long)a.tokens * a.group + PM_ROWS - 1) / PM_ROWS * a.H;
   const int most = (a.max_len + 511) / 512;
   long long n = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
