@@ -91,13 +91,18 @@ struct Pages : PagesArgs {
 constexpr int PG_COUNTERS = 16384;
 
 // pages_few.hip.  Whether its kernel takes this call's dimensions, and how it spreads sequences of up to so many rows
-// per KV head.
+// per KV head; half: over half of the card.
 bool pages_few_applies(const PagesArgs& a);
-FewPlan pages_few_plan(const PagesArgs& a, long long rows);
+FewPlan pages_few_plan(const PagesArgs& a, long long rows, bool half = false);
 hipError_t launch_pages_few(const Pages& a, hipStream_t s);
-// pages_many.hip
+// pages_many.hip.  Most tiles of a call's sequences: whole ones, and one that is not for each sequence that has more than
+// few_rows.
+long long pages_many_tiles(const PagesArgs& a, int few_rows);
 PagesPlan pages_many_plan(const PagesArgs& a);
 hipError_t launch_pages_many(const Pages& a, hipStream_t s);
+// pages_mixed.hip.  Whether one launch does the work of both.
+bool pages_mixed_applies(const Pages& a);
+hipError_t launch_pages_mixed(const Pages& a, hipStream_t s);
 
 __device__ __forceinline__ int page_of(const Pages& a, int t) { return a.by_page(t); }
 

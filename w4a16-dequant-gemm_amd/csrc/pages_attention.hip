@@ -156,7 +156,8 @@ size_t plan(Pages& a) {
     a.few_rows = (int)rows;
   } else if (fast && a.group <= 32 && a.nseq > 1) {  // decoding sequences next to prompts
     a.few_rows = (a.group + 15) / 16 * 16;
-    a.few = pages_few_plan(a, a.few_rows);
+    a.few = pages_few_plan(a, a.few_rows, true);
+    if (!pages_mixed_applies(a)) a.few = pages_few_plan(a, a.few_rows);
   }
   if (rows > a.few_rows) a.many = fast ? pages_many_plan(a) : general_plan(a);
   size_t floats = 0;
@@ -189,9 +190,11 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   const long long rows = (long long)a.tokens * a.H * a.group;
   const bool more = (long long)a.max_q * a.group > a.few_rows, fast = pages_few_applies(a);
   hipError_t e = hipSuccess;
-  if (a.few_rows) e = launch_pages_few(a, s);
+  const bool mixed = a.few_rows && more && pages_mixed_applies(a);
+  if (mixed) e = launch_pages_mixed(a, s);
+  else if (a.few_rows) e = launch_pages_few(a, s);
   if (e == hipSuccess && more && fast) {
-    e = launch_pages_many(a, s);
+    if (!mixed) e = launch_pages_many(a, s);
   } else if (e == hipSuccess && more) {
     pages_general_kernel<<<dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20), a.many.nsplit), 256, 0, s>>>(a);
     e = hipGetLastError();
