@@ -375,5 +375,7 @@ def attention_f8_pages_workspace(view, batch, group):
 
 
 def attention_f8_pages(view, batch, group, causal, q, q_stride, out, workspace=0, workspace_bytes=0, stream=0):
+    """Attention of packed queries over the pages.  `workspace`: attention_f8_pages_workspace() bytes, cleared once, one
+    for each call in flight."""
     check(load().w4_attention_f8_pages(C.byref(view), C.byref(batch), group, int(causal), _n(q), q_stride, _n(out),
                                        _n(workspace), workspace_bytes, _n(stream)))
