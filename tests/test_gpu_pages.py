@@ -435,6 +435,18 @@ def test_a_call_of_either_kernel(adds, page):
     a.check(), b.check()
 
 
+@pytest.mark.parametrize("nseq", [3, 70, 260])
+@pytest.mark.parametrize("D, group, page", [(64, 7, 16), (96, 4, 32), (128, 4, 16), (256, 2, 16), (128, 20, 16), (64, 4, 24)])
+def test_chunks_next_to_decoding_sequences(D, group, page, nseq):
+    """Calls whose bounds are past what one kernel takes alone; prompts, single tokens and idle sequences side by side."""
+    rng = np.random.default_rng(D + nseq)
+    lens, adds = rng.integers(1, 200, nseq), np.ones(nseq, np.int64)
+    lens[:3], adds[:3] = [1400, 900, 260], [130, 1, 70]
+    if nseq > 3:
+        adds[5], lens[9], adds[9] = 0, 1700, 16 // group + 1
+    Attn(nseq + D, lens.tolist(), adds.tolist(), 1, group, D, page, pad=6000).check()
+
+
 def test_batches_of_every_kind_in_one_workspace():
     """Whatever a call leaves in the workspace, the next one of another shape finds what it needs."""
     kinds = [([3000, 40], [1, 1], 2, 4, 128, 16), ([900, 800], [200, 1], 1, 4, 128, 16), ([5000], [2], 1, 7, 64, 24),
