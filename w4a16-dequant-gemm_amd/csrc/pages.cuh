@@ -98,7 +98,7 @@ hipError_t launch_pages_few(const Pages& a, hipStream_t s);
 // pages_many.hip.  Most tiles of a call's sequences: whole ones, and one that is not for each sequence that has more than
 // few_rows.
 long long pages_many_tiles(const PagesArgs& a, int few_rows);
-PagesPlan pages_many_plan(const PagesArgs& a);
+PagesPlan pages_many_plan(const PagesArgs& a, int few_rows);
 hipError_t launch_pages_many(const Pages& a, hipStream_t s);
 // pages_mixed.hip.  Whether one launch does the work of both.
 bool pages_mixed_applies(const Pages& a);

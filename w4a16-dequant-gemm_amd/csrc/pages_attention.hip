@@ -159,7 +159,7 @@ size_t plan(Pages& a) {
     a.few = pages_few_plan(a, a.few_rows, true);
     if (!pages_mixed_applies(a)) a.few = pages_few_plan(a, a.few_rows);
   }
-  if (rows > a.few_rows) a.many = fast ? pages_many_plan(a) : general_plan(a);
+  if (rows > a.few_rows) a.many = fast ? pages_many_plan(a, a.few_rows) : general_plan(a);
   size_t floats = 0;
   a.count = nullptr;
   if (a.few_rows && !a.few.alone) {

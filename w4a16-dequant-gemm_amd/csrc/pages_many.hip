@@ -1,4 +1,6 @@
 // Paged FP8 attention for many rows: the kernel by itself, and how its work is spread.
+#include <math.h>
+
 #include "pages_many.cuh"
 
 namespace w4k {
@@ -27,15 +29,33 @@ long long pages_many_tiles(const PagesArgs& a, int few_rows) {
   return packed < each * a.nseq ? packed : each * a.nseq;
 }
 
-PagesPlan pages_many_plan(const PagesArgs& a) {
-  // two workgroups per compute unit where the rows do not give them, no split shorter than 512 positions (256: 150 calls take
-  // the same on average, from 0.9 to 1.3 times as long)
-  const long long tiles = ((long long)a.tokens * a.group + PM_ROWS - 1) / PM_ROWS * a.H;
-  const int most = (a.max_len + 511) / 512;
-  long long n = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
-  n = n > most ? most : n < 1 ? 1 : n;
+// One round of workgroups (a little less, or a little more), no split shorter than 512 positions, if that takes less time than no
+// splits: splits cost what they write and read again and a launch, and shorten the chain of tiles of a workgroup, 1.55 us for
+// 64 positions at D = 128 alone on a compute unit, 2.25 next to another one.  1024 tokens of 32 heads take 33 us in one split, 47 in
+// two; 512 behind 1500 54 in one, 44 in four; 1024 behind 8000 220 in one, 193 in two.  256 positions at least instead of 512: 150
+// calls take the same on average, from 0.9 to 1.3 times as long.
+PagesPlan pages_many_plan(const PagesArgs& a, int few_rows) {
+  // (next to a prompt the other sequences have a token each, which is not this kernel's, as far as the host can tell)
+  const long long tokens = few_rows && a.tokens - (a.nseq - 1) > a.max_q ? a.tokens - (a.nseq - 1) : few_rows ? a.max_q : a.tokens;
+  const long long tiles = (tokens * a.group + PM_ROWS - 1) / PM_ROWS * a.H;
+  const long long steps = (a.max_len + PM_TILE - 1) / PM_TILE, most = (a.max_len + 511) / 512;
+  const int each = a.D <= 128 ? 2 : 1;  // workgroups of a compute unit
+  const double us = 0.4 + 0.6 * a.D / 128;
+  auto takes = [&](long long n) {
+    // whole rounds, and what is left over: rows of a prompt differ in length, so a few workgroups more are not a whole round more
+    const long long full = tiles * n / (256 * each), rest = tiles * n % (256 * each);
+    const double last = rest > 256 ? 2.25 : full ? 1.55 * sqrt(rest / 256.0) : 1.55;
+    const double chain = (steps + n - 1) / n * us * (full * (each == 2 ? 2.25 : 1.55) + last);
+    return n > 1 ? chain + 3.5 + tiles * PM_ROWS * n * (a.D + 2) * 8 / 5e6 : chain;
+  };
+  const long long down = tiles > 0 ? 256 * each / tiles : 1;
+  long long best = 1;
+  for (long long n = down; n <= down + 1; ++n) {
+    const long long k = n > most ? most : n;
+    if (k > 1 && takes(k) < takes(best)) best = k;
+  }
   PagesPlan p;
-  p.split_len = (int)(((a.max_len + n - 1) / n + PM_TILE - 1) / PM_TILE * PM_TILE);
+  p.split_len = (int)((steps + best - 1) / best * PM_TILE);
   p.nsplit = (a.max_len + p.split_len - 1) / p.split_len;
   return p;
 }
