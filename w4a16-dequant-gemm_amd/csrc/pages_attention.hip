@@ -147,8 +147,8 @@ size_t plan(Pages& a) {
   a.few_rows = 0;
   // Decode and a few tokens per sequence are the kernel's for few rows (8 x 32768 positions 89 us, 175 by the one for many; five
   // tokens each in 16 sequences 19.2 and 24.5).  So is everything up to FEW_WORK (what the scores of all rows come to
-  // at most): one launch that cuts rows into blocks of 32 and positions into splits takes 0.56 to 1.2 of the time there that the
-  // kernel for many rows, which waits for tile after tile, and its join take, above that 0.7 to 2.4 (70 calls of 1e8
+  // at most): one launch that cuts rows into blocks of 32 and positions into splits takes 0.5 to 1.2 of the time there that the
+  // kernel for many rows, which waits for tile after tile, and its join take, above that 0.7 to 2.4 (140 calls of 1e8
   // to 2.5e9).  Decoding sequences next to prompts: 125 us with the work of both kernels, 147 with the one for many alone.
   if (fast) a.few = pages_few_plan(a, rows);
   const double work = (double)a.tokens * a.H * a.group * a.max_len * a.D;
