@@ -104,9 +104,6 @@ __device__ __forceinline__ Share find_share(const Pages& a, int wg) {
   return x;
 }
 
-// PG4: pages of a multiple of 4 rows (four neighbouring positions have one page, and one read of its scales: 18.5 us
-// against 19.5 without for the 29 ragged sequences).
-// NB: how many times 64 sequences find_share() looks at (1: 18.5 us for 29 of them, 4: 20.2); 0: no unit is split.
 template <int D>
 struct FewShared {
   __attribute__((aligned(16))) uint8_t ring[PF_WAVES][PF_RING * 2 * PF_TILE * D];
@@ -114,6 +111,9 @@ struct FewShared {
   int scaleless;  // a page of the split has a V scale of 0
   uint32_t arrived;
 };
+// Workgroup wg.  PG4: pages of a multiple of 4 rows (four neighbouring positions have one page, and one read of its scales: 18.5 us
+// against 19.5 without for the 29 ragged sequences).
+// NB: how many times 64 sequences find_share() looks at (1: 18.5 us for 29 of them, 4: 20.2); 0: no unit is split.
 template <int D, int NT, bool PG4, int NB>
 __device__ __forceinline__ void few_rows(const Pages& a, const int wg, FewShared<D>& sh) {
   constexpr int P = D / 16, NC = D / 32, NE = D / 16;  // 16-byte pieces of a row, MFMAs of a score, of an output

@@ -31,9 +31,6 @@ __device__ __forceinline__ int tiles_of(const Pages& a, int s) {
   return rows <= a.few_rows ? 0 : (rows + PM_ROWS - 1) / PM_ROWS;
 }
 
-// P16: pages of a multiple of 16 rows: eight of a lane's scores in a row have one page, the same in all lanes.  Otherwise
-// the scales of a tile's positions are laid out one by one when it is requested: 345 us for the two prompts instead of
-// 325 (same card).
 template <int D, bool P16>
 struct ManyShared {
   __attribute__((aligned(16))) uint8_t ring[PM_SLOTS][2 * PM_TILE * D];
@@ -42,6 +39,9 @@ struct ManyShared {
   int odd;  // a page of the table is none of the pool, or has a V scale of 0
 };
 // Workgroup wg of a split.
+// P16: pages of a multiple of 16 rows: eight of a lane's scores in a row have one page, the same in all lanes.  Otherwise
+// the scales of a tile's positions are laid out one by one when it is requested: 345 us for the two prompts instead of
+// 325 (same card).
 template <int D, bool P16>
 __device__ __forceinline__ void many_rows(const Pages& a, const int wg, const int split, ManyShared<D, P16>& sh) {
   constexpr int P = D / 16, NE = D / 32;  // pieces of a row, 32-element blocks of it
