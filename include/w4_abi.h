@@ -336,6 +336,12 @@ int w4_attention_f8_pages(const w4_f8_pages_view* view, const w4_paged_batch* ba
 /* Plain arithmetic: needs no GPU, reads no device memory. */
 int w4_attention_f8_pages_workspace(const w4_f8_pages_view* view, const w4_paged_batch* batch,
                                     int group, size_t* bytes);
+/* How a call would run.  plan[0]: 0 vector kernel, 1 the matrix-core kernel for few rows, 2 the one
+ * for many rows, 3 both, a launch each, 4 both in one launch;  plan[1]: sequences of up to so many rows
+ * (new tokens times group) are the kernel's for few rows;  plan[2]: positions per split of the others;
+ * plan[3]: splits of a sequence of max_len positions there.  Plain arithmetic, as the workspace's. */
+int w4_attention_f8_pages_plan_for(const w4_f8_pages_view* view, const w4_paged_batch* batch, int group,
+                                   int* plan);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,44 @@
+"""Which kernels a call of paged FP8 attention runs, and how it splits positions (no GPU)."""
+import pytest
+
+import w4amd
+
+A = 64  # an address that no check may touch
+
+
+def plan(H=8, D=128, page=16, npages=100, nseq=1, tokens=1, max_q=1, max_len=1000, stride=1 << 16, group=4, cu=A, q_k=A):
+    c = w4amd.capi()
+    view = c.f8_pages_view(H, D, page, npages, q_k, A, A, A)
+    return c.attention_f8_pages_plan_for(view, c.paged_batch(nseq, tokens, max_q, max_len, A, stride, A, cu), group)
+
+
+def test_kernels_of_a_call():
+    assert plan(nseq=8, tokens=8, max_len=32768)[:2] == (1, 4)                 # a token each
+    assert plan(nseq=8, tokens=40, max_q=5, max_len=32768)[:2] == (1, 20)      # a few each
+    assert plan(tokens=100, max_q=100, max_len=100)[:2] == (1, 400)            # a small prompt
+    assert plan(tokens=4096, max_q=4096, max_len=4096)[:2] == (2, 0)           # a prompt
+    assert plan(nseq=16, tokens=527, max_q=512, max_len=8192)[:2] == (4, 16)   # a chunk next to decoding sequences
+    assert plan(nseq=16, tokens=527, max_q=512, max_len=8192, page=24)[:2] == (3, 16)
+    assert plan(nseq=16, tokens=527, max_q=512, max_len=8192, group=20)[:2] == (3, 32)
+    assert plan(nseq=16, tokens=527, max_q=512, max_len=8192, group=40)[:2] == (2, 0)
+    for other in (dict(D=80), dict(D=512), dict(q_k=A + 4)):                   # nothing but the vector kernel takes these
+        assert plan(nseq=16, tokens=527, max_q=512, max_len=8192, **other)[:2] == (0, 0)
+
+
+def test_splits_cover_the_longest_sequence():
+    for kernel in ({}, {"D": 80}, {"page": 24}):
+        for tokens in (1, 40, 128, 512, 1024, 5000):
+            for nseq in (1, 2, 16):
+                for max_len in (1, 63, 64, 65, 512, 1000, 8192, 100_000, 1_000_000):
+                    _, few, length, splits = plan(nseq=nseq, tokens=tokens, max_q=tokens, max_len=max_len, **kernel)
+                    case = (kernel, tokens, nseq, max_len)
+                    assert splits >= 1 and length >= 1 and (splits - 1) * length < max_len <= splits * length, case
+
+
+def test_a_plan_refuses_what_the_call_refuses():
+    for change, text in (({"D": 516}, "512"), ({"group": 65}, "query group"), ({"max_len": 0}, "bad dims"), ({"cu": 0, "tokens": 2}, "need cu_q")):
+        with pytest.raises(ValueError, match=text):
+            plan(**change)
+    c = w4amd.capi()
+    view, batch = c.f8_pages_view(8, 128, 16, 100, A, A, A, A), c.paged_batch(1, 1, 1, 100, A, 100, A, A)
+    assert c.load().w4_attention_f8_pages_plan_for(view, batch, 4, None) != 0

@@ -102,6 +102,7 @@ SIGNATURES = {
                                C.c_size_t, vp], C.c_int),
     "w4_attention_f8_pages_workspace": ([C.POINTER(F8PagesView), C.POINTER(PagedBatch), C.c_int,
                                          C.POINTER(C.c_size_t)], C.c_int),
+    "w4_attention_f8_pages_plan_for": ([C.POINTER(F8PagesView), C.POINTER(PagedBatch), C.c_int, C.POINTER(C.c_int)], C.c_int),
 }
 
 _lib = None
@@ -372,6 +373,13 @@ def attention_f8_pages_workspace(view, batch, group):
     n = C.c_size_t()
     check(load().w4_attention_f8_pages_workspace(C.byref(view), C.byref(batch), group, C.byref(n)))
     return n.value
+
+
+def attention_f8_pages_plan_for(view, batch, group):
+    """(kernels, rows of the kernel for few rows, positions per split, splits) of a call (include/w4_abi.h)"""
+    plan = (C.c_int * 4)()
+    check(load().w4_attention_f8_pages_plan_for(C.byref(view), C.byref(batch), group, plan))
+    return tuple(plan)
 
 
 def attention_f8_pages(view, batch, group, causal, q, q_stride, out, workspace=0, workspace_bytes=0, stream=0):

@@ -702,6 +702,14 @@ int w4_attention_f8_pages_workspace(const w4_f8_pages_view* p, const w4_paged_ba
   return W4_OK;
 }
 
+int w4_attention_f8_pages_plan_for(const w4_f8_pages_view* p, const w4_paged_batch* b, int group, int* plan) {
+  w4k::PagesArgs a;
+  if (int rc = pages_args(a, p, b, group)) return rc;
+  REQUIRE(plan != nullptr, "attention f8 pages: null pointer");
+  w4k::pages_attention_plan(a, plan);
+  return W4_OK;
+}
+
 int w4_attention_f8_pages(const w4_f8_pages_view* p, const w4_paged_batch* b, int group, int causal, const w4_half* q,
                           int q_stride, w4_half* out, void* workspace, size_t workspace_bytes, w4_stream stream) {
   w4k::PagesArgs a;

@@ -216,6 +216,7 @@ struct PagesArgs {
   char* space;
 };
 size_t pages_attention_space(const PagesArgs& a);
+void pages_attention_plan(const PagesArgs& a, int* plan);  // w4_attention_f8_pages_plan_for
 hipError_t launch_pages_attention(const PagesArgs& a, hipStream_t s);
 
 }  // namespace w4k

@@ -182,6 +182,17 @@ size_t pages_attention_space(const PagesArgs& args) {
   return plan(a);
 }
 
+void pages_attention_plan(const PagesArgs& args, int* out) {
+  Pages a;
+  (PagesArgs&)a = args;
+  plan(a);
+  const bool more = (long long)a.max_q * a.group > a.few_rows;
+  out[0] = !pages_few_applies(a) ? 0 : !more ? 1 : !a.few_rows ? 2 : pages_mixed_applies(a) ? 4 : 3;
+  out[1] = a.few_rows;
+  out[2] = a.many.split_len;
+  out[3] = a.many.nsplit;
+}
+
 hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   Pages a;
   (PagesArgs&)a = args;
