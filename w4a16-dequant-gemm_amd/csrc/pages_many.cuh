@@ -379,6 +379,9 @@ __device__ __forceinline__ void many_rows(const Pages& a, const int wg, const in
     uint64_t there = 0, fine = 0, there1 = 0, fine1 = 0;
     there = request(0, c0, fine);
     if (1 < nit) there1 = request(1, c0 + PM_TILE, fine1);
+    // (a wave's scales are read by the others behind the next barrier, which waits for no store by itself; later tiles' are
+    // waited for at the end of the tile that requests them)
+    if constexpr (!P16) asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     int sl = 0;
 #pragma unroll 1
     for (int it = 0; it < nit; ++it) {
