@@ -93,7 +93,8 @@ typedef struct w4_paged_batch {
   int tokens;     /* places for packed tokens (queries, slots); those behind the last
                      sequence's are padding                                             */
   int max_q;      /* no sequence has more new tokens than this                          */
-  int max_len;    /* no sequence has more tokens than this                              */
+  int max_len;    /* no sequence has more tokens than this; attention takes up to 2^30
+                     (more only where bt_stride * page is not)                          */
   int bt_stride;  /* entries of a sequence's block table                                */
   const int* bt;  /* [nseq][bt_stride] pages in order; an entry outside [0, npages)
                      names no page                                                      */

@@ -1,9 +1,11 @@
 """The kernel of paged FP8 attention for many rows, by calls whose bounds are past what the one for few rows takes."""
 import numpy as np
 import pytest
+import torch
 
 import w4amd
-from test_gpu_pages import Attn
+from devutil import DEV, ptr, to_dev
+from test_gpu_pages import Attn, host, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +30,65 @@ def test_pages_that_are_no_multiple_of_16(D, page):
     prompts(D + page, [449, 512, 64, 40, 960], [120, 64, 64, 33, 50], 1, 4, D, page).check()
     prompts(D + page + 1, [64], [64], 2, 4, D, page).check()
     prompts(D + page + 2, [500], [90], 1, 4, D, page).check()
+
+
+# ---- far positions -------------------------------------------------------------------------
+
+
+def with_tables(a, bt, max_len, lens=None):
+    """The calls of `a` with other tables, a bound and lengths."""
+    c = w4amd.capi()
+    H, group, D, page, causal = a.args
+    a.bt, a.d[5] = bt, i32(bt)
+    if lens is not None:
+        a.lens, a.d[6] = np.array(lens), i32(lens)
+    a.batch = c.paged_batch(len(bt), len(a.q), int(max(a.adds)), max_len, ptr(a.d[5]), bt.shape[1], ptr(a.d[6]), ptr(a.cu_d))
+    a.n = c.attention_f8_pages_workspace(a.view, a.batch, group)
+    a.space = torch.zeros(a.n + 16, dtype=torch.uint8, device=DEV)
+    return a
+
+
+@pytest.mark.parametrize("adds", [[1, 1], [5, 2], [300, 1], [90, 64]])
+@pytest.mark.parametrize("D", [128, 40])
+def test_short_sequences_under_the_largest_bound(D, adds):
+    """Tables and a bound of 2^30 positions: prompts and single tokens are computed as under a bound of their own."""
+    a = Attn(D, [400, 200], adds, 1, 4, D, 1024)
+    bt = np.full((2, 1 << 20), -1, np.int32)
+    bt[:, :a.bt.shape[1]] = a.bt
+    with_tables(a, bt, 2 ** 31 - 1).check()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_the_longest_sequence(causal, n):
+    """2^30 - 3 positions whose table names page 0 in its first half, page 1 in its second and page 2 at its end.  Scores are
+    0 but for the last page, whose 2^20 positions (three of them behind the end) have as much weight as all others."""
+    H, group, D, page = 1, 4, 64, 1 << 20
+    L = (1 << 30) - 3
+    a = Attn(7, [64], [n], H, group, D, 64, causal)
+    a.args, entries = (H, group, D, page, causal), 1 << 10
+    q = np.zeros_like(a.q)
+    q[..., 0] = 8.0
+    codes = [np.zeros((H, 3, page, D), np.uint8) for _ in range(2)]
+    codes[0][:, 2, :, 0] = 0x38                            # 1
+    for p, one in enumerate((0x38, 0x40, 0x48)):           # 1, 2, 4
+        codes[1][:, p] = one
+    # 8 sk / sqrt(64) nats; (2^30 - 2^20) / 2^20 = 1023 times as many others
+    sk = float(np.float16(np.log(1023)))
+    scales = [np.full((H, 3), sk, np.float16), np.ones((H, 3), np.float16)]
+    a.k, a.v = [codes[0], scales[0]], [codes[1], scales[1]]
+    a.d[0:5] = [to_dev(x) for x in (q, codes[0], scales[0], codes[1], scales[1])]
+    c = w4amd.capi()
+    a.view = c.f8_pages_view(H, D, page, 3, *[ptr(t) for t in a.d[1:5]])
+    bt = np.repeat(np.array([0, 1], np.int32), entries // 2)
+    bt[-1] = 2
+    with_tables(a, bt[None], L, [L])
+    got = host(a.run()).view(np.float16).reshape(q.shape).astype(np.float64)
+    half = entries // 2 * page
+    for i in range(n):
+        last = (L - n + i + 1 if causal else L) - (entries - 1) * page
+        w = np.array([half, half - page, last * np.exp(sk)])
+        want = w @ np.array([1.0, 2.0, 4.0]) / w.sum()
+        # A lane adds its weights, and a matrix product its sums, at most 2^17 times (2^30 positions over 512 workgroups in
+        # tiles of 64, four additions each); an addition is off by 2^-24 of the sum.  Weights and the output are halves.
+        assert (np.abs(got[i] - want) <= want * (2 * 2.0 ** (17 - 24) + 2.0 ** -10)).all(), (i, got[i].min(), got[i].max(), want)

@@ -42,3 +42,28 @@ def test_a_plan_refuses_what_the_call_refuses():
     c = w4amd.capi()
     view, batch = c.f8_pages_view(8, 128, 16, 100, A, A, A, A), c.paged_batch(1, 1, 1, 100, A, 100, A, A)
     assert c.load().w4_attention_f8_pages_plan_for(view, batch, 4, None) != 0
+
+
+def test_bounds_of_positions():
+    """max_len counts as far as the tables reach.  Up to 2^30 positions every plan covers them; what is more is refused."""
+    for kernel in ({}, {"D": 80}, {"page": 1000}, {"nseq": 2, "tokens": 40}, {"nseq": 2, "tokens": 40, "group": 20}):
+        for tokens, max_q in ((2, 1), (40, 30), (1000, 990), (300_000, 300_000)):
+            base = {"nseq": 2, "page": 1024, "stride": 1 << 21, "H": 1, **kernel, "tokens": tokens, "max_q": max_q}
+            for max_len in (1 << 30, (1 << 30) - 1, (1 << 30) - 127):
+                _, _, length, splits = plan(max_len=max_len, **base)
+                assert 1 <= length <= max_len + 255 and (splits - 1) * length < max_len <= splits * length, (base, max_len)
+            for max_len in ((1 << 30) + 1, 2147483000, 2 ** 31 - 1):
+                with pytest.raises(ValueError, match="pass 2.30 positions"):
+                    plan(max_len=max_len, **base)
+            short = {**base, "stride": 50}
+            assert plan(max_len=2 ** 31 - 1, **short) == plan(max_len=50 * short["page"], **short)
+    assert plan(max_len=2 ** 31 - 1, page=1024, stride=1 << 20)[3] >= 1   # a table of 2^30 positions
+
+
+def test_calls_past_the_bounds_of_positions_are_refused():
+    c = w4amd.capi()
+    view, batch = c.f8_pages_view(1, 128, 1024, 100, A, A, A, A), c.paged_batch(2, 41, 40, 2 ** 31 - 1, A, 1 << 21, A, A)
+    with pytest.raises(ValueError, match="pass 2.30 positions"):
+        c.attention_f8_pages(view, batch, 4, 1, A, 0, A, A, 1 << 40)
+    with pytest.raises(ValueError, match="pass 2.30 positions"):
+        c.attention_f8_pages_workspace(view, batch, 4)

@@ -686,9 +686,11 @@ static int pages_args(w4k::PagesArgs& a, const w4_f8_pages_view* p, const w4_pag
   a.nseq = b->nseq; a.tokens = b->tokens;
   a.max_q = b->max_q < b->tokens || b->tokens == 0 ? b->max_q : b->tokens;
   a.stride = b->bt_stride;
-  // (no position past a table is looked at)
+  // No position past a table is looked at.  Positions are ints, of plans and kernels: a length rounded up to a tile, and a
+  // split behind it, have to be ones too.
   const long long in_table = (long long)b->bt_stride * p->page;
   a.max_len = in_table < b->max_len ? (int)in_table : b->max_len;
+  REQUIRE(a.max_len <= 1 << 30, "attention f8 pages: max_len and the block tables pass 2^30 positions");
   a.bt = b->bt; a.lens = b->lens; a.cu = b->cu_q;
   a.group = group;
   return W4_OK;
