@@ -77,7 +77,8 @@ typedef struct w4_act_mx8_view {
 /* Paged FP8 cache, device view: H pools (one per KV head) of npages pages of `page` rows of D
  * E4M3 bytes, q[H][npages][page][D], and one FP16 scale per page and head, s[H][npages].  The
  * values are E4M3 (OCP: 0x7F and 0xFF are NaN, which w4_quantize_f8_pages never writes) times the
- * page's scale, which is finite and not negative.  No counterpart in the reference. */
+ * page's scale, which is finite and not negative; a NaN is one under a scale of 0 too.  No counterpart
+ * in the reference. */
 typedef struct w4_f8_pages_view {
   int H, D, page, npages;
   const uint8_t* q_k;

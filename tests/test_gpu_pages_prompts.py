@@ -1,4 +1,5 @@
-"""The kernel of paged FP8 attention for many rows, by calls whose bounds are past what the one for few rows takes."""
+"""Paged FP8 attention where tests of small calls do not reach: the kernel for many rows, by calls whose bounds are past what
+the one for few rows takes, far positions, values that are not finite."""
 import numpy as np
 import pytest
 import torch
@@ -92,3 +93,42 @@ def test_the_longest_sequence(causal, n):
         # A lane adds its weights, and a matrix product its sums, at most 2^17 times (2^30 positions over 512 workgroups in
         # tiles of 64, four additions each); an addition is off by 2^-24 of the sum.  Weights and the output are halves.
         assert (np.abs(got[i] - want) <= want * (2 * 2.0 ** (17 - 24) + 2.0 ** -10)).all(), (i, got[i].min(), got[i].max(), want)
+
+
+# ---- NaN codes -----------------------------------------------------------------------------
+
+
+def with_nan_codes(a, rng):
+    """NaN codes of V in every second page of each sequence and in one of its last tokens, half of these pages under a scale
+    of 0; codes of K under a scale of 0."""
+    H, group, D, page, _ = a.args
+    for s, (n, m) in enumerate(zip(a.lens, a.adds)):
+        for j, t in enumerate([*range(page // 2, n - m, 2 * page)][:3] + [n - m // 2 - 1]):
+            pg = a.bt[s, t // page]
+            a.v[0][rng.integers(H), pg, t % page, rng.integers(0, D, 2)] = [0x7F, 0xFF]
+            if j % 2 == s % 2:
+                a.v[1][:, pg] = 0.0
+    a.k[1][:, a.bt[0, 0]] = 0.0
+    for at, x in ((2, a.k[1]), (3, a.v[0]), (4, a.v[1])):
+        a.d[at].copy_(to_dev(x).view(a.d[at].shape))
+    return a
+
+
+def check_nan(a):
+    got = host(a.run()).view(np.float16).reshape(a.before.shape).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want, tol = a.want()
+    nan = np.isnan(want)
+    assert nan.any() and not nan.all()
+    assert np.array_equal(np.isnan(got), nan), np.argwhere(np.isnan(got) != nan)[:4].tolist()
+    assert (np.abs(got - want)[~nan] <= tol[~nan]).all()
+
+
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 7, 24), (256, 2, 64), (96, 16, 16), (128, 8, 1), (40, 2, 5)])
+@pytest.mark.parametrize("lens, adds", [([40, 333, 5], [1, 1, 1]), ([50, 600], [5, 3]), ([300, 170], [60, 80])])
+def test_nan_codes_under_a_scale_of_0(D, group, page, lens, adds):
+    """A NaN stays one under a scale of 0, wherever in a tile it stands and whichever kernel reads it."""
+    check_nan(with_nan_codes(Attn(D, lens, adds, 2, group, D, page), np.random.default_rng(3)))
+    if D != 40 and max(adds) > 1:
+        many = [n * 40 // max(adds) for n in adds] if max(adds) < 40 else adds
+        check_nan(with_nan_codes(prompts(D, lens, many, 2, group, D, page), np.random.default_rng(4)))

@@ -204,7 +204,7 @@ __device__ __forceinline__ float* part_of(const Pages& a, long long row, int spl
   return a.part + (row * a.many.nsplit + split) * (a.D + 2);
 }
 
-// A page of a split or a stretch of one, in LDS.  Where the V scale is 0 the kernels read zeros for the codes.
+// A page of a split or a stretch of one, in LDS.  Where the V scale is 0 the kernels read zeros for the codes that are numbers.
 struct PageEntry {
   int row0;   // first row of the page in its head's pool; -1: no page of the pool
   float skc;  // scale of K times c, not 0 (a masked score, -infinity, stays that when multiplied)
@@ -242,6 +242,19 @@ __device__ __forceinline__ uint32_t has_nan_code(uint32_t w) { return ((w & 0x7F
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // 0xFF at each
   const uint32_t x = has_nan_code(w) >> 7;
   return (x << 8) - x;
+}
+
+// What is left of a row of V in LDS that does not count: zeros where no position is there (it may hold anything, and 0
+// times that may be NaN), the NaN codes under a scale of 0, which are NaN all the same.
+template <int PIECES>
+__device__ __forceinline__ void clear_row(uint8_t* row, bool there) {
+#pragma unroll 1
+  for (int i = 0; i < PIECES; ++i) {
+    u4 w = *(const u4*)(row + 16 * i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] &= there ? nan_codes(w[j]) : 0u;
+    *(u4*)(row + 16 * i) = w;
+  }
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr;

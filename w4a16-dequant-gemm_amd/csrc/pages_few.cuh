@@ -299,12 +299,9 @@ __device__ __forceinline__ void few_rows(const Pages& a, const int wg, FewShared
       }
     }
     if (there != ~0u || no_scales) {
-      // rows of V that are not there may hold anything, and 0 times that may be NaN: zeros in their place, and in that
-      // of rows under a scale of 0
       const int t = min(t0 + (lane & 31), s1 - 1);
-      if (lane < PF_TILE && (!((there >> lane) & 1) || !has_scale(table[page_of(a, t) - j0])))
-#pragma unroll 1
-        for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
+      const bool here = (there >> (lane & 31)) & 1;
+      if (lane < PF_TILE && (!here || !has_scale(table[page_of(a, t) - j0]))) clear_row<P>(slot + SIDE + lane * D, here);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
     const int last = (s1 - 1) - t0;  // (positions past the split have the last one's entry)

@@ -212,11 +212,8 @@ __device__ __forceinline__ void many_rows(const Pages& a, const int wg, const in
   auto weights = [&](int sl, int t0, uint64_t there, uint64_t fine) {
     uint8_t* const slot = ring[sl];
     if (fine != ~0ull) {
-      // rows of V that do not count may hold anything, and 0 times that may be NaN: zeros in their place (every wave
-      // writes the same ones, before its own reads)
-      if (!((fine >> lane) & 1))
-#pragma unroll 1
-        for (int i = 0; i < P; ++i) *(u4*)(slot + SIDE + lane * D + 16 * i) = u4{0u, 0u, 0u, 0u};
+      // (every wave writes the same, also what it makes of what another one wrote, before its own reads)
+      if (!((fine >> lane) & 1)) clear_row<P>(slot + SIDE + lane * D, (there >> lane) & 1);
       asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
 #pragma unroll
