@@ -132,3 +132,19 @@ def test_nan_codes_under_a_scale_of_0(D, group, page, lens, adds):
     if D != 40 and max(adds) > 1:
         many = [n * 40 // max(adds) for n in adds] if max(adds) < 40 else adds
         check_nan(with_nan_codes(prompts(D, lens, many, 2, group, D, page), np.random.default_rng(4)))
+
+
+# ---- kernels side by side ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("nseq, H, kind", [(255, 8, 4), (256, 8, 4), (257, 8, 3), (256, 16, 3)])
+def test_many_sequences_next_to_a_chunk(nseq, H, kind):
+    """One launch with workgroups for half of the card, for all of it, and two launches."""
+    rng = np.random.default_rng(nseq)
+    lens, adds = rng.integers(1, 30, nseq), np.ones(nseq, np.int64)
+    lens[3], adds[3], lens[100], adds[7] = 600, 40, 500, 0
+    a = prompts(nseq, lens.tolist(), adds.tolist(), H, 1, 64, 16)
+    assert a.plan[0] == kind
+    a.check()
+    first = host(a.run()).copy()
+    assert np.array_equal(host(a.run()), first)

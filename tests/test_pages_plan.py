@@ -67,3 +67,13 @@ def test_calls_past_the_bounds_of_positions_are_refused():
         c.attention_f8_pages(view, batch, 4, 1, A, 0, A, A, 1 << 40)
     with pytest.raises(ValueError, match="pass 2.30 positions"):
         c.attention_f8_pages_workspace(view, batch, 4)
+
+
+def test_one_launch_or_two():
+    """Decoding sequences next to a chunk: one launch as long as units of the few-rows kernel are split, over half of the card
+    or over all of it."""
+    many = dict(tokens=5000, max_q=512, max_len=8192)
+    for nseq, H, D, kind in ((2, 8, 128, 4), (255, 8, 128, 4), (256, 8, 128, 4), (256, 15, 64, 4), (256, 16, 64, 3), (257, 1, 128, 3),
+                             (255, 8, 256, 4), (256, 8, 256, 3), (255, 16, 96, 4)):
+        assert plan(nseq=nseq, H=H, D=D, **many)[:2] == (kind, 16), (nseq, H, D)
+    assert plan(nseq=256, H=8, tokens=200_000, max_q=512, max_len=512)[0] == 3  # (up to 512 positions no unit is split)

@@ -78,6 +78,7 @@ struct FewPlan {
 struct Pages : PagesArgs {
   Divider by_page;
   int few_rows;
+  bool mixed;  // both kernels' work in one launch
   FewPlan few;
   PagesPlan many;
   uint32_t* count;  // few rows: arrivals of a unit, at its first workgroup's number << count_shift
@@ -100,7 +101,7 @@ hipError_t launch_pages_few(const Pages& a, hipStream_t s);
 long long pages_many_tiles(const PagesArgs& a, int few_rows);
 PagesPlan pages_many_plan(const PagesArgs& a, int few_rows);
 hipError_t launch_pages_many(const Pages& a, hipStream_t s);
-// pages_mixed.hip.  Whether one launch does the work of both.
+// pages_mixed.hip.  Whether one launch can do the work of both, as a.few spreads it.
 bool pages_mixed_applies(const Pages& a);
 hipError_t launch_pages_mixed(const Pages& a, hipStream_t s);
 

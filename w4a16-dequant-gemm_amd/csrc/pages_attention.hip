@@ -145,6 +145,7 @@ size_t plan(Pages& a) {
   a.few = FewPlan{};
   a.many = PagesPlan{a.max_len, 1};
   a.few_rows = 0;
+  a.mixed = false;
   // Decode and a few tokens per sequence are the kernel's for few rows (8 x 32768 positions 89 us, 175 by the one for many; five
   // tokens each in 16 sequences 19.2 and 24.5).  So is everything up to FEW_WORK (what the scores of all rows come to
   // at most): one launch that cuts rows into blocks of 32 and positions into splits takes 0.5 to 1.2 of the time there that the
@@ -156,8 +157,14 @@ size_t plan(Pages& a) {
     a.few_rows = (int)rows;
   } else if (fast && a.group <= 32 && a.nseq > 1) {  // decoding sequences next to prompts
     a.few_rows = (a.group + 15) / 16 * 16;
+    // over half of the card where its units are split then, else over all of it (256 sequences of 900 to 7680 positions and 8 KV
+    // heads, one with a chunk of 512: 508 us so in one launch, 529 in two); two launches where they are split in neither
     a.few = pages_few_plan(a, a.few_rows, true);
-    if (!pages_mixed_applies(a)) a.few = pages_few_plan(a, a.few_rows);
+    a.mixed = pages_mixed_applies(a);
+    if (!a.mixed) {
+      a.few = pages_few_plan(a, a.few_rows);
+      a.mixed = pages_mixed_applies(a);
+    }
   }
   if (rows > a.few_rows) a.many = fast ? pages_many_plan(a, a.few_rows) : general_plan(a);
   size_t floats = 0;
@@ -187,7 +194,7 @@ void pages_attention_plan(const PagesArgs& args, int* out) {
   (PagesArgs&)a = args;
   plan(a);
   const bool more = (long long)a.max_q * a.group > a.few_rows;
-  out[0] = !pages_few_applies(a) ? 0 : !more ? 1 : !a.few_rows ? 2 : pages_mixed_applies(a) ? 4 : 3;
+  out[0] = !pages_few_applies(a) ? 0 : !more ? 1 : !a.few_rows ? 2 : a.mixed ? 4 : 3;
   out[1] = a.few_rows;
   out[2] = a.many.split_len;
   out[3] = a.many.nsplit;
@@ -201,11 +208,10 @@ hipError_t launch_pages_attention(const PagesArgs& args, hipStream_t s) {
   const long long rows = (long long)a.tokens * a.H * a.group;
   const bool more = (long long)a.max_q * a.group > a.few_rows, fast = pages_few_applies(a);
   hipError_t e = hipSuccess;
-  const bool mixed = a.few_rows && more && pages_mixed_applies(a);
-  if (mixed) e = launch_pages_mixed(a, s);
+  if (a.mixed) e = launch_pages_mixed(a, s);
   else if (a.few_rows) e = launch_pages_few(a, s);
   if (e == hipSuccess && more && fast) {
-    if (!mixed) e = launch_pages_many(a, s);
+    if (!a.mixed) e = launch_pages_many(a, s);
   } else if (e == hipSuccess && more) {
     pages_general_kernel<<<dim3((unsigned)(rows < (1 << 20) ? rows : 1 << 20), a.many.nsplit), 256, 0, s>>>(a);
     e = hipGetLastError();

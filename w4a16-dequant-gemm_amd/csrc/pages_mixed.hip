@@ -1,6 +1,7 @@
 // Paged FP8 attention of decoding sequences next to prompts: the work of both kernels in one launch.
 //
-// Workgroups for few rows come first, half a round of them: they wait for memory, those for many rows for the vector ALUs.
+// Workgroups for few rows come first, half a round of them (plan() has where it is more): they wait for memory, those for many
+// rows for the vector ALUs.
 // Where no sequence has few rows (only the device knows), they end at once and cost no launch.  A chunk of 512 tokens at 8192
 // next to 15 decoding sequences: 125.6 us, 129.6 in two launches, 153 with workgroups of both kinds in turn, eight by eight (one
 // kind to one half of the compute units); 36 calls of prompts and chunks: 0.89 of the time of two launches on average, 0.92
