@@ -328,7 +328,9 @@ int w4_quantize_f8_pages(const w4_f8_pages_view* view, const w4_half* k, const w
  * tokens: with `causal` the i-th sees positions up to lens[s] - n + i, without it all
  * lens[s].  Positions whose table entry is no page of the pool are not seen (pages that
  * were given back).  A query that sees nothing gives zeros; rows of `out` behind the last
- * sequence's are left as they are.  Scores are scaled by 1 / sqrt(D).
+ * sequence's are left as they are.  Scores are scaled by 1 / sqrt(D).  Scores, softmax statistics and
+ * sums are FP32; where matrix cores run, a weight (times its page's V scale) is rounded to FP16
+ * first, to 11 bits down to 2^-20 of the largest, to a step of 2^-30 of it below.
  * workspace: device memory of w4_attention_f8_pages_workspace() bytes, 16-byte aligned
  * (NULL when that is 0); cleared once by the caller before its first use, every call
  * leaves it ready for the next.  Calls that overlap (streams, graphs) need one each. */

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+import pages_ref
 import w4amd
 from devutil import DEV, ptr, to_dev
 from test_gpu_pages import Attn, host, i32
@@ -148,3 +149,38 @@ def test_many_sequences_next_to_a_chunk(nseq, H, kind):
     a.check()
     first = host(a.run()).copy()
     assert np.array_equal(host(a.run()), first)
+
+
+# ---- weights far apart ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n, many", [(1, False), (5, False), (20, False), (60, True)])
+def test_small_weights_next_to_a_token_without_values(D, n, many):
+    """A first token that takes nearly all of the softmax and has no values (an attention sink): the others, 2^25 to 2^27
+    times below it, are all of the output."""
+    a = (prompts if many else Attn)(D + n, [400], [n], 1, 4, D, 16)
+    H, group, D, page, _ = a.args
+    rng = np.random.default_rng(n)
+    first = a.bt[0, 0]
+    a.q[...] = 0
+    a.q[..., 0] = np.sqrt(D)
+    a.q[..., 1] = np.sqrt(D) / 16
+    a.k[0][...] = 0
+    a.k[0][0, first, 0, 0] = 0x38                                                        # 1: sk nats
+    a.k[0][..., 1] = rng.choice(np.array([0x00, 0x38, 0xB8], np.uint8), a.k[0].shape[:3])  # 0, 1, -1: sk / 16 nats = 1.6 binades
+    a.k[1][...] = np.float16(26 * np.log(2))
+    a.v[0][...] = pages_ref.encode(100 + 100 * rng.random(a.v[0].shape))
+    a.v[0][0, first, 0] = 0
+    a.v[1][...] = 1.0
+    q = np.zeros((len(a.q), a.row), np.float16)
+    q[:] = a.q.reshape(len(a.q), -1)
+    for at, x in ((0, q), (1, a.k[0]), (2, a.k[1]), (3, a.v[0]), (4, a.v[1])):
+        a.d[at].copy_(to_dev(x).view(a.d[at].shape))
+    got = host(a.run()).view(np.float16).reshape(a.before.shape).astype(np.float64)[:n]
+    want = a.want()[0][:n]
+    # Weights are kept at 2^6 times what they are to the largest one, so those below halves' normal range are off by 2^-31 of
+    # that at most; values are positive and at most 200.  Others' are rounded by 2^-11, as is the output; exponents of up to 26
+    # are off by 2^-21 times 26.
+    assert (want > 1e-4).all()
+    assert (np.abs(got - want) <= 2.0 ** -31 * 400 * 200 + (2.0 ** -10 + 2.0 ** -16) * want).all(), float((np.abs(got - want) / want).max())

@@ -4,8 +4,12 @@
 // A row is one query token and head.  For position t on page p with scales sk, sv and a row's raw dot product s of
 // codes, its score in units of log2 is x = s sk c, c = log2(e) / sqrt(D), and its weight on the raw V codes is
 // 2^x sv.  Sums are kept relative to M, the running maximum of x + log2(sv): the weights that enter the matrix
-// product in FP16 then stay at most 1 whatever the scales are, and the denominators, 2^(x - M), stay in FP32.
+// product in FP16 then have one range whatever the scales are, and the denominators, 2^(x - M), stay in FP32.
 // (Relative to the maximum of x alone, weights of pages whose V scale is small would fall below FP16's range.)
+// Both are kept 2^PG_LIFT times as large, which falls out of their quotient: M may lag behind by PG_SLACK, so weights go up
+// to 2^14 of the 2^16 that a half holds (room for what rounding does to exponents as long as scores are below 2^24), and
+// only those 2^-20 of the largest and less lose bits.  A token that takes nearly all of the softmax and has no values
+// is ordinary; without the lift, others 2^-25 below it were lost in the numerator and there in the denominator.
 #pragma once
 
 #include "dq.cuh"
@@ -212,7 +216,8 @@ struct PageEntry {
   float lsv;  // log2 of the scale of V (at least -24: a half); PG_NO_SCALE where it is 0
   float inv;  // 2^-lsv
 };
-constexpr float PG_SLACK = 8.0f;  // sums are rescaled only when the maximum has risen by this (weights stay below 2^9)
+constexpr float PG_SLACK = 8.0f;  // sums are rescaled only when the maximum has risen by this
+constexpr float PG_LIFT = 6.0f;
 constexpr float PG_NO_SCALE = -25.0f;
 __device__ __forceinline__ bool has_scale(const PageEntry& e) { return e.lsv > -24.5f; }
 __device__ __forceinline__ void set_scales(PageEntry& e, float sk, float sv, float c) {

@@ -332,7 +332,7 @@ __device__ __forceinline__ void few_rows(const Pages& a, const int wg, FewShared
         l[t] *= alpha;
         M[t] = m_new;
       }
-      const float use = M[t] == -INFINITY ? 0.0f : M[t];
+      const float use = M[t] == -INFINITY ? 0.0f : M[t] - PG_LIFT;
 #pragma unroll
       for (int k = 0; k < 8; k += SAME) {
         const float add = lsv[k / SAME] - use;

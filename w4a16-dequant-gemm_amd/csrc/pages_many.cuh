@@ -260,7 +260,7 @@ __device__ __forceinline__ void many_rows(const Pages& a, const int wg, const in
       l *= alpha;
       M = m_new;
     }
-    const float use = M == -INFINITY ? 0.0f : M;
+    const float use = M == -INFINITY ? 0.0f : M - PG_LIFT;
     // (denominators take the weights as they are in FP32: under a small scale of V the halves lose what they need)
     if constexpr (P16) {
 #pragma unroll
