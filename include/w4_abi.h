@@ -310,7 +310,8 @@ int w4_paged_tables(const w4_paged_batch* batch, int page, int npages, const int
 /* Writes new tokens into the cache: k, v are FP16, token t's rows of H * D elements at
  * t * row_stride (0: H * D).  Token t goes to row slots[t] of each head's pool; negative
  * slots and slots past the pool are skipped.  Tokens of one page stand side by side with
- * ascending slots, as w4_paged_tables gives them, and no page appears twice.
+ * ascending slots, as w4_paged_tables gives them, and no page appears twice.  A page has at most
+ * 2^32 bytes.
  *   scale(a) = the smallest half that is at least a / 448, a: the largest finite magnitude
  *   a page begun in this call (its first new token is its row 0): s = scale(a)
  *   an older page: s = s_old * 2^k, the smallest k >= 0 with s >= scale(a) (scale(a) where

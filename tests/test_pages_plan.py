@@ -1,4 +1,5 @@
-"""Which kernels a call of paged FP8 attention runs, and how it splits positions (no GPU)."""
+"""Which kernels a call of paged FP8 attention runs, how it splits positions, and bounds that calls are refused past
+(no GPU)."""
 import pytest
 
 import w4amd
@@ -77,3 +78,15 @@ def test_one_launch_or_two():
                              (255, 8, 256, 4), (256, 8, 256, 3), (255, 16, 96, 4)):
         assert plan(nseq=nseq, H=H, D=D, **many)[:2] == (kind, 16), (nseq, H, D)
     assert plan(nseq=256, H=8, tokens=200_000, max_q=512, max_len=512)[0] == 3  # (up to 512 positions no unit is split)
+
+
+def test_append_refuses_pages_past_what_it_counts():
+    c = w4amd.capi()
+
+    def append(D, page):
+        c.quantize_f8_pages(c.f8_pages_view(1, D, page, 1, A, A, A, A), A, A, 0, 0, 0, A)
+
+    append(512, 1 << 23), append(4, 1 << 30), append(128, 1 << 25)
+    for D, page in ((512, (1 << 23) + 1), (512, (1 << 31) - 1), (8, (1 << 29) + 1)):
+        with pytest.raises(ValueError, match="2.32 bytes"):
+            append(D, page)

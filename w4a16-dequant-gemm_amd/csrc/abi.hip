@@ -661,6 +661,8 @@ int w4_quantize_f8_pages(const w4_f8_pages_view* p, const w4_half* k, const w4_h
                          const int* slots, int tokens, int* status, w4_stream stream) {
   if (int rc = check_pages(p, "quantize_f8_pages")) return rc;
   REQUIRE(tokens >= 0, "quantize_f8_pages: bad dims");
+  // (a page's words and pieces are counted in ints)
+  REQUIRE((long long)p->page * p->D <= 1LL << 32, "quantize_f8_pages: a page has more than 2^32 bytes");
   REQUIRE(k && v && status && (slots || tokens == 0), "quantize_f8_pages: null io pointer");
   REQUIRE(row_stride == 0 || row_stride >= (long long)p->H * p->D, "quantize_f8_pages: row_stride is shorter than a row");
   REQUIRE((long long)tokens * 2 * p->H < (1LL << 29), "quantize_f8_pages: too many rows");
