@@ -301,8 +301,8 @@ int w4_gemm_mx_plan_for(int x8, int M, int N, int K, int* plan);
  * zero or past its table, bit 2 more tokens than places.  A sequence that runs into one
  * of these gets no page: its tokens have no slot, its length stays max(cached, 0), and
  * its packed tokens keep their places.  A token whose page's entry is no page of the pool
- * has no slot either.  max_q and max_len are not looked at; `cached` must not be the array
- * lens.  slots and positions may be NULL when tokens == 0. */
+ * has no slot either.  max_q and max_len are not looked at; nseq is at most 2^30; `cached` must
+ * not be the array lens.  slots and positions may be NULL when tokens == 0. */
 int w4_paged_tables(const w4_paged_batch* batch, int page, int npages, const int* cached,
                     const int* added, const int* free_pages, const int* free_range,
                     int* slots, int* positions, int* result, w4_stream stream);

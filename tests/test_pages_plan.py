@@ -90,3 +90,10 @@ def test_append_refuses_pages_past_what_it_counts():
     for D, page in ((512, (1 << 23) + 1), (512, (1 << 31) - 1), (8, (1 << 29) + 1)):
         with pytest.raises(ValueError, match="2.32 bytes"):
             append(D, page)
+
+
+def test_tables_refuse_sequences_past_what_they_count():
+    c = w4amd.capi()
+    for nseq in ((1 << 30) + 1, 2 ** 31 - 1000, 2 ** 31 - 1):
+        with pytest.raises(ValueError, match="2.30 sequences"):
+            c.paged_tables(c.paged_batch(nseq, 3, 1, 100, A, 8, A, A), 16, 8, 128, 192, A, A, A, A, A)

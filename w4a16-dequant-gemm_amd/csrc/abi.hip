@@ -647,6 +647,7 @@ int w4_paged_tables(const w4_paged_batch* b, int page, int npages, const int* ca
                     w4_stream stream) {
   REQUIRE(b != nullptr, "paged tables: null batch");
   REQUIRE(b->nseq >= 1 && b->tokens >= 0 && b->bt_stride >= 1, "paged tables: bad dims");
+  REQUIRE(b->nseq <= 1 << 30, "paged tables: more than 2^30 sequences");  // (a thread's run of them ends at an int)
   REQUIRE(page >= 1 && npages >= 1 && (long long)npages * page < (1LL << 31), "paged tables: bad page geometry");
   REQUIRE(b->bt && b->lens && b->cu_q && cached && added && free_pages && free_range && result,
           "paged tables: null pointer");
