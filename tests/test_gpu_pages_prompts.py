@@ -7,7 +7,7 @@ import torch
 import pages_ref
 import w4amd
 from devutil import DEV, ptr, to_dev
-from test_gpu_pages import Attn, host, i32
+from test_gpu_pages import Attn, Step, host, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -184,3 +184,182 @@ def test_small_weights_next_to_a_token_without_values(D, n, many):
     # are off by 2^-21 times 26.
     assert (want > 1e-4).all()
     assert (np.abs(got - want) <= 2.0 ** -31 * 400 * 200 + (2.0 ** -10 + 2.0 ** -16) * want).all(), float((np.abs(got - want) / want).max())
+
+
+# ---- the kernel for many rows on what tests of small calls give the one for few -------------
+
+SHAPES = [(128, 4, 16), (64, 7, 24), (256, 2, 64), (96, 3, 16), (128, 1, 1), (96, 5, 7), (256, 4, 24), (64, 1, 16), (128, 40, 16)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D, group, page", SHAPES)
+def test_prompts_of_any_length(D, group, page, causal):
+    prompts(D * group + page, [131, 400, 64, 90], [131, 150, 63, 0], 1, group, D, page, causal=causal).check()
+    prompts(D * group + page + 1, [777], [1 + 40 // group], 2, group, D, page, causal=causal).check()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D, group, page", SHAPES)
+def test_prompts_over_pages_that_were_given_back(D, group, page, causal):
+    """Table entries outside the pool, in the first tile and the last, all of a sequence's, and next to scales of 0."""
+    a = prompts(D + group, [300, 290, 260], [90, 40, 200], 1, group, D, page, causal=causal, holes=2 + 40 // page)
+    a.check()
+    a.bt[1] = -1                                        # a sequence that has none left
+    a.bt[0, 0] = a.bt[0, 299 // page] = a.npages
+    a.d[5].copy_(i32(a.bt))
+    got = a.check()
+    assert (got[a.cu[1]:a.cu[2]] == 0).all()
+    for side in (a.k, a.v):
+        side[1][:, ::2] = 0.0
+    a.d[2].copy_(to_dev(a.k[1])), a.d[4].copy_(to_dev(a.v[1]))
+    a.check()
+
+
+@pytest.mark.parametrize("lens, adds", [([3, 40], [50, 48]), ([0, 45], [70, 40]), ([0, 400], [70, 1]), ([30, 200], [100, 250])])
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 2, 24), (256, 1, 16), (96, 8, 1)])
+def test_prompts_that_see_nothing(D, group, page, lens, adds):
+    """More queries than positions: the first of them lie before position 0; sequences without any."""
+    got = prompts(sum(lens) + D, lens, adds, 2, group, D, page).check()
+    assert (got[:max(0, adds[0] - lens[0])] == 0).all()
+
+
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 4, 24), (256, 1, 16), (96, 8, 1)])
+def test_prompts_under_scales_far_apart(D, group, page):
+    lens, adds = [300, 50, 128], [120, 1, 64]
+    prompts(21, lens, adds, 1, group, D, page, scale_spread=9).check()
+    prompts(22, lens, adds, 1, group, D, page, scales=(2.0 ** -22, 2.0 ** -22)).check()
+    a = prompts(23, lens, adds, 1, group, D, page)
+    for side in (a.k, a.v):
+        side[1][:, ::2] = 0.0  # pages of zeros
+    a.d[2].copy_(to_dev(a.k[1])), a.d[4].copy_(to_dev(a.v[1]))
+    a.check()
+
+
+def test_prompts_of_peaked_and_flat_scores():
+    prompts(32, [700, 90], [40, 70], 1, 4, 128, 16, q_scale=30.0).check()
+    prompts(33, [700, 90], [40, 70], 1, 4, 128, 16, q_scale=0.0).check()
+    prompts(34, [700, 90], [40, 70], 1, 4, 64, 24, q_scale=30.0).check()
+
+
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 4, 24), (256, 1, 16), (96, 8, 1)])
+def test_nan_of_one_query_of_a_prompt_stays_its_own(D, group, page):
+    a = prompts(41, [200, 90], [44, 40], 2, group, D, page)
+    clean = host(a.run()).copy()
+    q = a.q.copy()
+    q[0, 1, 5] = np.nan
+    a.d[0].copy_(to_dev(q).view(-1))
+    got = host(a.run()).view(np.float16).reshape(a.before.shape)
+    assert np.isnan(got[0, 1]).all()
+    keep = np.ones(got.shape[:2], bool)
+    keep[0, 1] = False
+    assert np.array_equal(got[keep].view(np.uint16), clean.view(np.uint16).reshape(got.shape)[keep])
+
+
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 7, 24), (256, 2, 64), (96, 16, 16), (128, 8, 1), (96, 5, 7), (256, 3, 24)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_nan_codes_of_prompts_reach_only_the_rows_that_see_them(D, group, page, causal):
+    lens, adds = [150, 300, 90], [145, 150, 90]
+    a = prompts(D + group, lens, adds, 1, group, D, page, causal=causal)
+    rng = np.random.default_rng(7)
+    for s, (n, m) in enumerate(zip(lens, adds)):
+        if s < 2 or causal:  # (without a mask all rows see what the third sequence has: it keeps none)
+            for back in (1, 2, m // 2, m - 1):
+                t = n - back
+                a.v[0].reshape(-1, D)[a.bt[s, t // page] * page + t % page, rng.integers(0, D, 2)] = [0x7F, 0xFF]
+    a.k[0].reshape(-1, D)[a.bt[1, 298 // page] * page + 298 % page, 3] = 0x7F
+    a.d[1].copy_(to_dev(a.k[0]).view(a.d[1].shape)), a.d[3].copy_(to_dev(a.v[0]).view(a.d[3].shape))
+    check_nan(a)
+
+
+def test_prompts_strides_and_bounds():
+    for stride in (1000, 1001):                          # rows at odd addresses
+        got = prompts(8, [100, 260], [80, 40], 2, 2, 128, 16, stride=stride).check()
+        assert (got[120:] == 7.0).all()
+    prompts(9, [100, 260], [80, 40], 2, 2, 128, 16, max_len=5000, max_q=1000).check()
+    # lengths past the bound of the call are cut
+    a = prompts(12, [100, 260], [80, 40], 2, 2, 128, 16, max_len=128)
+    out = a.run()
+    a.lens = np.array([100, 128])
+    got = host(out).view(np.float16).reshape(a.before.shape).astype(np.float64)
+    want, tol = a.want()
+    assert (np.abs(got - want)[:80] <= tol[:80]).all()
+    a.args = (*a.args[:4], False)                       # (the second one's queries lie past what is kept: they see all of it)
+    want, tol = a.want()
+    assert (np.abs(got - want)[80:120] <= tol[80:120]).all()
+
+
+@pytest.mark.parametrize("D, group, page", [(128, 4, 16), (64, 7, 24), (256, 1, 64), (96, 3, 7), (64, 4, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompts_in_splits(D, group, page, causal):
+    """One tile of rows behind many positions, and shorter sequences next to it whose last splits have nothing."""
+    a = prompts(D + page, [6000, 300, 1400], [1 + 100 // group, 34, 40], 1, group, D, page, causal=causal)
+    assert a.plan[3] > 1
+    a.check()
+
+
+@pytest.mark.parametrize("D, group, page", [(128, 8, 16), (64, 8, 24), (96, 2, 3), (256, 4, 16)])
+def test_the_same_rows_by_either_kernel(D, group, page):
+    """A call that the kernel for few rows takes, and one with more places whose prompt is the other's."""
+    lens, adds = [400, 200], [60, 21]
+    a, b = Attn(71, lens, adds, 1, group, D, page), prompts(71, lens, adds, 1, group, D, page)
+    plan = w4amd.capi().attention_f8_pages_plan_for(a.view, a.batch, group)
+    assert plan[0] == 1 and b.plan[0] >= 3
+    assert all(np.array_equal(x, y) for x, y in ((a.bt, b.bt), (a.k[0], b.k[0]), (a.v[0], b.v[0]), (a.q, b.q[:81])))
+    a.check(), b.check()
+
+
+@pytest.mark.parametrize("page", [64, 24])
+def test_prompts_on_pages_past_32_bits(page):
+    """A pool of more than 2^32 bytes a side: the bytes of the call over a small one."""
+    c = w4amd.capi()
+    H, group, D = 2, 2, 128
+    a = prompts(page, [300, 700], [90, 64], H, group, D, page)
+    want = a.run()
+    a.check(want)
+    npages = 300_000 * 64 // page
+    pools = []
+    for small in a.d[1:5]:
+        big = torch.zeros(H, npages, *small.shape[2:], dtype=small.dtype, device=DEV)
+        big[:, npages - a.npages:] = small.flip(1)
+        pools.append(big)
+    assert pools[0][0].numel() > 1 << 31 and pools[0].numel() > 1 << 32
+    a.view = c.f8_pages_view(H, D, page, npages, *[ptr(t) for t in pools])
+    a.d[5].copy_(i32(npages - 1 - a.bt))
+    assert np.array_equal(host(a.run()), host(want))
+
+
+def test_prompts_of_every_kind_in_one_workspace():
+    kinds = [([3000, 40], [64, 1], 2, 4, 128, 16), ([900, 800], [200, 1], 1, 4, 128, 24), ([5000], [40], 1, 7, 64, 24),
+             ([400] * 70, [1] * 69 + [50], 1, 1, 96, 16), ([700, 2000], [40, 33], 1, 2, 256, 64)]
+    calls = [prompts(80 + i, *k) for i, k in enumerate(kinds)]
+    calls += [Attn(90, [3000, 40], [1, 1], 2, 4, 128, 16), Attn(91, [900], [40], 1, 4, 40, 16)]
+    want = [host(x.run()).copy() for x in calls]
+    space = torch.zeros(max(x.n for x in calls) + 16, dtype=torch.uint8, device=DEV)
+    order = np.random.default_rng(1).integers(0, len(calls), 60)
+    outs = [calls[i].run(space=space) for i in order]
+    assert all(np.array_equal(host(o), want[i]) for o, i in zip(outs, order))
+    for x in calls:
+        x.check()
+
+
+# ---- a step whose bounds are a serving loop's ------------------------------------------------
+
+
+@pytest.mark.parametrize("group, page, kind", [(4, 16, 4), (4, 24, 3), (20, 16, 3)])
+def test_a_captured_step_of_prompts_and_tokens_replayed(group, page, kind):
+    """Bounds past what the kernel for few rows takes: prompts, chunks and single tokens under one graph."""
+    s = Step(73, 4, 1, group, 128, page, 80, 640 // page, 2300, 300)
+    assert w4amd.capi().attention_f8_pages_plan_for(s.view, s.batch, group)[0] == kind
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        s.launch(side.cuda_stream)
+
+    def replay():
+        graph.replay()
+        torch.cuda.synchronize()
+
+    for added in ([150, 3, 1, 0], [1, 1, 1, 1], [40, 60, 0, 100], [1, 1, 1, 1], [100, 1, 9, 2]):
+        assert s.step(np.array(added), replay)[1] == 0
+        torch.ones(1000, device=DEV).sum().item()  # the program's own work between replays
+    s.step(np.array([1, 40, 1, 1]), s.launch)
