@@ -251,15 +251,21 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) {  // 0xFF at each
 }
 
 // What is left of a row of V in LDS that does not count: zeros where no position is there (it may hold anything, and 0
-// times that may be NaN), the NaN codes under a scale of 0, which are NaN all the same.
+// times that may be NaN), the NaN codes under a scale of 0, which are NaN all the same.  (The end of every short sequence
+// comes this way: zeros are stored without a read, 4 x 300 positions 6.4 us against 7.1.)
 template <int PIECES>
 __device__ __forceinline__ void clear_row(uint8_t* row, bool there) {
+  if (!there) {
 #pragma unroll 1
-  for (int i = 0; i < PIECES; ++i) {
-    u4 w = *(const u4*)(row + 16 * i);
+    for (int i = 0; i < PIECES; ++i) *(u4*)(row + 16 * i) = u4{0u, 0u, 0u, 0u};
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < PIECES; ++i) {
+      u4 w = *(const u4*)(row + 16 * i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] &= there ? nan_codes(w[j]) : 0u;
-    *(u4*)(row + 16 * i) = w;
+      for (int j = 0; j < 4; ++j) w[j] &= nan_codes(w[j]);
+      *(u4*)(row + 16 * i) = w;
+    }
   }
 }
 
