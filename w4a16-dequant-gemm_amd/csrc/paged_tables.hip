@@ -8,7 +8,7 @@
 // tokens by a search in LDS.
 //
 // Bound: latency.  The two sums are four trips through LDS and barriers behind one load; the tokens add a
-// search, one dependent load (a free page or an old entry) and their stores.  64 sequences with a token each: 3.0 us on the
+// search, one dependent load (a free page or an old entry) and their stores.  64 sequences with a token each: 2.8 us on the
 // device, 4.0 us a call when calls follow each other; 333 prompts with 67317 tokens: 5.6 us.
 #include "pages.cuh"
 

@@ -7,8 +7,8 @@ namespace {
 // ---- any head dimension, page size and alignment -----------------------------------------------
 // A workgroup takes rows of one split in turn, tiles of 256 positions: a thread forms one position's score, then owns
 // four columns of O for every (256 / (D / 4))-th position of the tile.  Nothing is shared between the heads of a group and
-// no matrix core is used: 8 x 32768 positions at D = 128 took it 1035 us (the kernel for few rows: 89), two prompts of 4096
-// tokens 34.5 ms (the one for many: 318 us).  Bound: the vector ALUs.
+// no matrix core is used: 8 x 32768 positions at D = 128 took it 1035 us (the kernel for few rows: 90), two prompts of 4096
+// tokens 34.5 ms (the one for many: 313 us).  Bound: the vector ALUs.
 __global__ __launch_bounds__(256) void pages_general_kernel(const Pages a) {
   __shared__ float qs[512], red[4], weight[256], o4[256][4];
   __shared__ long long at[256];  // offset of a position's row in the codes; -1: not seen

@@ -11,9 +11,9 @@
 // by row so that neither read has bank conflicts.  Page ids and scales of the split lie in a table in LDS.
 // Workgroups find their splits from the lengths on the device; the last one of a unit joins its partial sums in place.
 // Bound: HBM, 2 D bytes per position and KV head: 8 sequences of 32768 positions, 8 KV heads of 4 query heads, D = 128:
-// 89 us, 6.0 TB/s.  Short or ragged caches are bound by the chain of lengths, page ids, scales, tiles, join: 29 sequences of 400
-// to 6007 positions, 4 KV heads, D = 64: 18.5 us, 2.7 TB/s; 4 of up to 300: 6.5 us; 5 tokens in each of 16 sequences of
-// up to 1505: 19.2 us.
+// 90 us, 6.0 TB/s (a large read: 7.0).  Short or ragged caches are bound by the chain of lengths, page ids, scales, tiles, join: 29 sequences of 400
+// to 6007 positions, 4 KV heads, D = 64: 18.5 us, 2.7 TB/s; 4 of up to 300: 6.4 us; 5 tokens in each of 16 sequences of
+// up to 1505: 19.2 us.  (On one pool again and again, which the last-level cache holds; cold 1 to 2 us more.)
 #pragma once
 
 #include <type_traits>

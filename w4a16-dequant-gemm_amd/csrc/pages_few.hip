@@ -45,7 +45,8 @@ FewPlan pages_few_plan(const PagesArgs& a, long long rows, bool half) {
   p.rows = rows < p.block ? (int)rows : p.block;
   const long long units = (long long)a.nseq * a.H * p.blocks;
   // Units are not split where many of them fill the card without it (256 sequences of 1000 positions, 32 heads: 321 us against
-  // 357 in splits; of 200 to 2000: 355 against 382), and beyond 256 sequences a workgroup does not look for its share; nor up to
+  // 357 in splits; of 200 to 2000: 355 against 382), and beyond 256 sequences a workgroup does not look for its share (what that
+  // costs where one is much longer than the rest: 100000 positions next to 50 .. 1000 973 us, 103 with 256 sequences); nor up to
   // 512 positions, which take less time than a split costs (partial sums, arrival, join): 4 x 300 6.5 us against 8.2.
   p.step_least = a.max_len <= 512 ? 4 : 2;
   p.alone = (a.max_len <= 512 && p.blocks == 1) || a.nseq > 256 || units >= 8 * places ||

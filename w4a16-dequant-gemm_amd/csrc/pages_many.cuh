@@ -9,10 +9,10 @@
 // barrier per tile.  Codes are converted by each wave after it has read them: half the LDS traffic of
 // converted tiles, which would take as long as the matrix products.
 // Weights are formed as 2^(x + log2(sv) - M) at once; the denominator takes a page's sum times 1 / sv.
-// Bound: the vector ALUs -- 128 conversions of two codes, 32 exponentials and some 230 other instructions for a wave's tile
-// of 64 positions next to 32 matrix products; matrix cores are busy for a bit more than a third of the time.  Two prompts of 4096
-// and 3777 tokens, 8 KV heads of 4 query heads, D = 128: 318 us, 800 TFLOP/s (a large library product of halves on the same
-// card: 1330).
+// Bound: vector ALUs and matrix cores in turn -- 128 conversions of two codes, 32 exponentials and some 230 other instructions for
+// a wave's tile of 64 positions, then 32 matrix products: the first are busy 0.62 of the time, the second 0.38, and little of
+// one runs beside the other.  Two prompts of 4096 and 3777 tokens, 8 KV heads of 4 query heads, D = 128: 313 to 323 us by
+// card, 800 TFLOP/s (a large library product of halves: 1330).
 #pragma once
 
 #include "pages.cuh"

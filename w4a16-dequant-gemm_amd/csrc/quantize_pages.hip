@@ -9,7 +9,7 @@
 //   code: RNE(x / s).  Quotients of two halves are exact ties or 2^-17 away from one, so a quotient that is right
 //   to the last bit of an FP32 is enough; x * (1 / s) with one residual step is.
 // Bound: HBM for prompts (3 bytes per element), behind the chain of slots, rows, scale and codes: 4096 tokens of 8 heads, D = 128,
-// on pages of 16 take 8.6 us, 2.9 TB/s (at the rate of a large copy: 4.9 us).  Latency for a decode step: 64 tokens 4.0 us.
+// on pages of 16 take 8.6 us, 2.9 TB/s (at the rate of a large copy: 4.9 us).  Latency for a decode step: 64 tokens 4.5 us.
 #include "pages.cuh"
 
 namespace w4k {
