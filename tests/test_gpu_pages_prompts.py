@@ -363,3 +363,66 @@ def test_a_captured_step_of_prompts_and_tokens_replayed(group, page, kind):
         assert s.step(np.array(added), replay)[1] == 0
         torch.ones(1000, device=DEV).sum().item()  # the program's own work between replays
     s.step(np.array([1, 40, 1, 1]), s.launch)
+
+
+# ---- where things lie ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("adds", [[1, 1], [5, 2], [80, 40]])
+@pytest.mark.parametrize("off", [4, 8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pools_that_are_not_16_byte_aligned(D, off, adds):
+    """Nothing but the vector kernel takes these; head dimensions are the matrix cores'."""
+    a = Attn(D + off, [300, 90], adds, 2, 4, D, 16)
+    c = w4amd.capi()
+    moved = []
+    for t in (a.d[1], a.d[3]):
+        buf = torch.empty(t.numel() + 16, dtype=torch.uint8, device=DEV)
+        moved.append(buf[off:off + t.numel()])
+        moved[-1].copy_(t.reshape(-1))
+    a.view = c.f8_pages_view(2, D, 16, a.npages, ptr(moved[0]), ptr(a.d[2]), ptr(moved[1]), ptr(a.d[4]))
+    assert c.attention_f8_pages_plan_for(a.view, a.batch, 4)[0] == 0
+    a.n = c.attention_f8_pages_workspace(a.view, a.batch, 4)
+    a.space = torch.zeros(a.n + 16, dtype=torch.uint8, device=DEV)
+    a.check()
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("adds", [[1, 1], [70, 40]])
+def test_offsets_that_do_not_begin_at_0(D, adds):
+    """Packed tokens ahead of the first sequence's are no query, and their rows of `out` stay as they are."""
+    before = 9
+    a = (prompts if max(adds) > 1 and D != 80 else Attn)(D, [200, 90], adds, 2, 4, D, 16)
+    plain = host(a.run()).copy()
+    T = len(a.q)
+    q = torch.zeros((T + before) * a.row, dtype=torch.int16, device=DEV)
+    q[before * a.row:] = a.d[0].view(torch.int16).reshape(-1)
+    out = to_dev(np.full((T + before, *a.before.shape[1:]), 7.0, np.float16))
+    cu = i32(a.cu + before)
+    c = w4amd.capi()
+    batch = c.paged_batch(2, T + before, int(max(adds)), 200, ptr(a.d[5]), a.bt.shape[1], ptr(a.d[6]), ptr(cu))
+    n = c.attention_f8_pages_workspace(a.view, batch, 4)
+    space = torch.zeros(n + 16, dtype=torch.uint8, device=DEV)
+    c.attention_f8_pages(a.view, batch, 4, 1, ptr(q), 0, ptr(out), ptr(space), n)
+    got = host(out).view(np.float16)
+    assert (got[:before] == 7.0).all()
+    a.check(out[before:])
+    assert np.array_equal(got[before:].reshape(-1).view(np.int16), plain.reshape(-1))
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("adds", [[1, 1, 1, 1], [5, 4, 6, 3], [60, 40, 50, 45]])
+def test_offsets_past_the_places(D, adds):
+    """More tokens than places: sequences that fit are computed, and nothing is written behind the places."""
+    a = (prompts if max(adds) > 8 and D != 80 else Attn)(D, [200, 90, 120, 60], adds, 1, 4, D, 16)
+    fit = int(a.cu[2])
+    want, tol = (x[:fit] for x in a.want())
+    c = w4amd.capi()
+    for tokens in (fit, fit + (adds[2] + 1) // 2):
+        for max_len in (200, 1000):
+            batch = c.paged_batch(4, tokens, int(max(adds)), max_len, ptr(a.d[5]), a.bt.shape[1], ptr(a.d[6]), ptr(a.cu_d))
+            n = c.attention_f8_pages_workspace(a.view, batch, 4)
+            space, out = torch.zeros(n + 16, dtype=torch.uint8, device=DEV), to_dev(a.before)
+            c.attention_f8_pages(a.view, batch, 4, 1, ptr(a.d[0]), 0, ptr(out), ptr(space), n)
+            got = host(out).view(np.float16).reshape(a.before.shape).astype(np.float64)
+            assert (np.abs(got[:fit] - want) <= tol).all() and (got[tokens:] == 7.0).all()
