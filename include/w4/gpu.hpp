@@ -458,4 +458,55 @@ inline void attention_f8_pages(const DeviceF8Pages& p, const DevicePagedBatch& b
                                       detail::h(out), workspace, workspace_bytes, stream));
 }
 
+// ---- a feed-forward block of experts (additive; no reference counterpart) ------------
+// The structs are w4_abi.h's own: their pointers are device memory.
+using Router = w4_router;
+using DeviceExpertRows = w4_expert_rows;
+using DeviceBlockNorm = w4_block_norm;
+enum class Act { none = 0, silu = 1, gelu = 2 };
+
+inline size_t route_experts_workspace(const Router& r, int tokens) {
+  size_t bytes = 0;
+  detail::raise(w4_route_experts_workspace(&r, tokens, &bytes));
+  return bytes;
+}
+inline void route_experts(const Router& r, const float* logits, int row_stride, int tokens,
+                          const int* count, int* experts, float* weights, int* order, int* offsets,
+                          void* workspace, size_t workspace_bytes, hipStream_t stream = 0) {
+  detail::raise(w4_route_experts(&r, logits, 1, row_stride, tokens, count, experts, weights, order,
+                                 offsets, workspace, workspace_bytes, stream));
+}
+inline void route_experts(const Router& r, const __half* logits, int row_stride, int tokens,
+                          const int* count, int* experts, float* weights, int* order, int* offsets,
+                          void* workspace, size_t workspace_bytes, hipStream_t stream = 0) {
+  detail::raise(w4_route_experts(&r, logits, 0, row_stride, tokens, count, experts, weights, order,
+                                 offsets, workspace, workspace_bytes, stream));
+}
+inline void gemm_experts(const DevicePackedW& p, const DeviceExpertRows& rows, Act act,
+                         const __half* x, bool from_tokens, __half* out, bool to_pairs,
+                         hipStream_t stream = 0) {
+  const auto v = detail::abi(p);
+  detail::raise(w4_gemm_experts(&v, &rows, (int)act, detail::h(x), from_tokens, detail::h(out),
+                                to_pairs, stream));
+}
+inline void gemm_experts(const DevicePackedWm& p, const DeviceExpertRows& rows, Act act,
+                         const __half* x, bool from_tokens, __half* out, bool to_pairs,
+                         hipStream_t stream = 0) {
+  const auto v = detail::abi(p);
+  detail::raise(w4_gemm_experts_mx(&v, &rows, (int)act, detail::h(x), from_tokens, detail::h(out),
+                                   to_pairs, stream));
+}
+inline void residual_norm(const DeviceBlockNorm& n, int tokens, int terms, const __half* y,
+                          const float* weights, const __half* shared, const float* residual,
+                          float* residual_out, __half* h, hipStream_t stream = 0) {
+  detail::raise(w4_residual_norm(&n, tokens, terms, detail::h(y), weights, detail::h(shared),
+                                 residual, 1, residual_out, detail::h(h), stream));
+}
+inline void residual_norm(const DeviceBlockNorm& n, int tokens, int terms, const __half* y,
+                          const float* weights, const __half* shared, const __half* residual,
+                          __half* residual_out, __half* h, hipStream_t stream = 0) {
+  detail::raise(w4_residual_norm(&n, tokens, terms, detail::h(y), weights, detail::h(shared),
+                                 residual, 0, residual_out, detail::h(h), stream));
+}
+
 }  // namespace w4::gpu

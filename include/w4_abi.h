@@ -104,6 +104,42 @@ typedef struct w4_paged_batch {
                       one token each (tokens == nseq, max_q == 1)                       */
 } w4_paged_batch;
 
+/* How a row of logits becomes a choice of experts (no counterpart in the reference). */
+typedef struct w4_router {
+  int experts;       /* logits of a row, up to 1024                                        */
+  int top_k;         /* experts chosen per token, up to 32 and no more than experts        */
+  int score;         /* 0: softmax over the row, 1: 1 / (1 + e^-logit) of each             */
+  int groups;        /* experts lie in so many groups of experts / groups side by side     */
+  int top_groups;    /* groups kept                                                        */
+  int group_best;    /* a group is worth the sum of its best one or two                    */
+  int renorm;        /* weights of a token are divided by their sum                        */
+  float scale;       /* and multiplied by this                                             */
+  const float* bias; /* [experts], added to the scores for the choice only; may be NULL    */
+} w4_router;
+
+/* Tokens and the experts they are sent to (no counterpart in the reference).  Pair t * top_k + j
+ * is token t's j-th choice.  Both arrays are device memory, as w4_route_experts writes them. */
+typedef struct w4_expert_rows {
+  int experts, tokens, top_k;
+  const int* offsets; /* [experts + 1] ascending, from 0: an expert's places in `order`     */
+  const int* order;   /* [tokens * top_k] the pair at each place                            */
+} w4_expert_rows;
+
+/* The norms around a block, its gate and its way into the residual stream (no counterpart in the
+ * reference).  Vectors of dim halves; a NULL weight is no norm, a NULL bias or gate none. */
+typedef struct w4_block_norm {
+  int dim;              /* up to 32768                                                      */
+  int centred;          /* 0: x / sqrt(mean(x^2) + eps), 1: the mean is subtracted first    */
+  float eps;
+  float residual_scale;
+  const w4_half* post;  /* weight of the norm behind the block                              */
+  const w4_half* post_bias;
+  const w4_half* gate;  /* factor of each channel; rows per token where gate_stride is not 0 */
+  int gate_stride;      /* elements between a token's gates and the next's                  */
+  const w4_half* pre;   /* weight of the norm ahead of the next block; NULL: no h           */
+  const w4_half* pre_bias;
+} w4_block_norm;
+
 const char* w4_last_error(void);
 
 /* M at or above this goes to the matrix-core kernel in w4_gemm / w4_gemm_mx.
@@ -347,6 +383,57 @@ int w4_attention_f8_pages_workspace(const w4_f8_pages_view* view, const w4_paged
  * plan[3]: splits of a sequence of max_len positions there.  Plain arithmetic, as the workspace's. */
 int w4_attention_f8_pages_plan_for(const w4_f8_pages_view* view, const w4_paged_batch* batch, int group,
                                    int* plan);
+
+/* ---- a feed-forward block of experts (no counterpart in the reference) ------------
+ * w4_route_experts chooses each token's experts and sorts the pairs of token and expert,
+ * w4_gemm_experts multiplies the pairs' rows with their experts' packed matrices (once for the gate and
+ * the way up, once for the way down), w4_residual_norm joins a token's rows to the residual stream.  None of
+ * them reads anything back to the host, allocates or synchronises: a block can be captured. */
+
+/* logits: `tokens` rows of r->experts halves, or floats (logits_f32), row_stride (0: r->experts)
+ * elements apart.
+ *   score  s of a row: softmax, or the sigmoid of each logit
+ *   choice c = s + bias in 64 bits; the logit itself where there is neither a bias nor more than one group
+ *   groups are worth the sum of their best group_best c; the top_groups best stay
+ *   the top_k best c of what stays are chosen, best first; of equals, the lowest index, groups too
+ *   weight = s, divided by the sum of the chosen if renorm, times scale; in FP32
+ * A logit of +inf counts as the type's largest; one of -inf or NaN has no score.  Such an expert, and one whose c is
+ * -inf or NaN, is never chosen and adds nothing to its group; a group of such is not kept.  Places left have expert
+ * -1 and weight 0, and so have all of the tokens from *count on (a device int; NULL: all tokens are there).
+ * Writes experts and weights [tokens][top_k], order [tokens * top_k]: the pairs that have an expert, by expert, then
+ * by token; -1 behind them; and offsets [experts + 1] of the experts in it.  No float of it depends on
+ * the order in which workgroups run.
+ * At most 2^25 tokens, 2^30 pairs.
+ * workspace: device memory of w4_route_experts_workspace() bytes, 16-byte aligned (NULL when that is 0);
+ * cleared once by the caller before its first use, every call leaves it ready for the next.  Calls that
+ * overlap (streams, graphs) need one each. */
+int w4_route_experts(const w4_router* r, const void* logits, int logits_f32, int row_stride, int tokens,
+                     const int* count, int* experts, float* weights, int* order, int* offsets,
+                     void* workspace, size_t workspace_bytes, w4_stream stream);
+/* Plain arithmetic: needs no GPU, reads no device memory. */
+int w4_route_experts_workspace(const w4_router* r, int tokens, size_t* bytes);
+
+/* The view holds rows->experts matrices of R = N / experts rows one after the other.  The pair at place i of
+ * expert e's places is multiplied with e's matrix: y = x_row * W_e^T, W as w4_dequant gives it, sums in FP32.
+ *   x    from_tokens 1: [tokens][K], the pair's token; 0: [tokens * top_k][K], row i
+ *   act  0: y is the row of outputs, R wide; 1, 2: R is even, an expert's rows are those of the gate, then those of
+ *        the way up, and act(y[j]) * y[R / 2 + j] is the row, R / 2 wide; 1 SiLU, 2 GELU in its tanh form
+ *   out  to_pairs 1: the row goes to the pair's index; 0: to row i; one rounding to FP16
+ * Rows of `out` that no place names are left as they are; places whose `order` is no pair are not multiplied. */
+int w4_gemm_experts(const w4_packed_view* p, const w4_expert_rows* rows, int act, const w4_half* x,
+                    int from_tokens, w4_half* out, int to_pairs, w4_stream stream);
+int w4_gemm_experts_mx(const w4_packed_mx_view* p, const w4_expert_rows* rows, int act, const w4_half* x,
+                       int from_tokens, w4_half* out, int to_pairs, w4_stream stream);
+
+/* Per token:  b = sum_j weights[j] * y[j] + shared  (weights NULL: the sum; shared may be NULL)
+ *             b = norm(b) * post + post_bias;  r = residual + residual_scale * gate * b;
+ *             residual_out = r;  h = norm(r) * pre + pre_bias
+ * y: [tokens][terms][dim]; weights: floats [tokens][terms]; a row under a weight of 0 is not read.  residual and
+ * residual_out: halves, or floats (residual_f32), and may be the same array; h: halves; rows [tokens][dim].  FP32
+ * inside, h from r before it is rounded.  terms is up to 64. */
+int w4_residual_norm(const w4_block_norm* n, int tokens, int terms, const w4_half* y, const float* weights,
+                     const w4_half* shared, const void* residual, int residual_f32, void* residual_out, w4_half* h,
+                     w4_stream stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,162 @@
+"""Calls of the entry points for a block of experts that are refused, and their 64-bit definitions against independent
+ones (no GPU)."""
+import numpy as np
+import pytest
+import torch
+
+import experts_ref
+import w4amd
+
+A = 64  # an address that no check may touch
+
+
+def _router(c, experts=8, top_k=2, **more):
+    return c.router(experts, top_k, **more)
+
+
+def test_routing_refuses_what_it_cannot_do():
+    c = w4amd.capi()
+    good = dict(logits=A, logits_f32=1, row_stride=0, tokens=3, count=0, experts=A, weights=A, order=A, offsets=A,
+                workspace=A, workspace_bytes=1 << 20)
+
+    def refused(text, router=None, **change):
+        with pytest.raises(ValueError, match=text):
+            c.route_experts(router if router is not None else _router(c), **{**good, **change})
+
+    for text, change in (("number of experts", {"experts": 0}), ("number of experts", {"experts": 1025}),
+                         ("top_k", {"top_k": 0}), ("top_k", {"top_k": 9}), ("top_k", {"experts": 64, "top_k": 33}),
+                         ("score", {"score": 2}), ("groups do not divide", {"groups": 3}), ("groups do not divide", {"groups": 0}),
+                         ("top_groups", {"groups": 4, "top_groups": 0}), ("top_groups", {"groups": 4, "top_groups": 5}),
+                         ("more than 64 groups", {"experts": 256, "groups": 128}), ("group_best", {"group_best": 0}),
+                         ("group_best", {"group_best": 3})):
+        refused(text, _router(c, **change))
+        with pytest.raises(ValueError, match=text):
+            c.route_experts_workspace(_router(c, **change), 3)
+    for name in ("logits", "experts", "weights", "order", "offsets"):
+        refused("null pointer", **{name: 0})
+    refused("number of tokens", tokens=-1)
+    refused("number of tokens", tokens=(1 << 25) + 1)
+    refused("logits_f32", logits_f32=2)
+    refused("row_stride", row_stride=7)
+    refused("row_stride", row_stride=-8)
+    refused("misaligned", logits=A + 2)
+    refused("misaligned", logits=A + 1, logits_f32=0)
+    refused("16-byte aligned", workspace=A + 8)
+    need = c.route_experts_workspace(_router(c), 3)
+    if need:
+        refused("workspace too small", workspace_bytes=need - 1)
+        refused("workspace too small", workspace=0)
+
+
+def test_products_refuse_what_they_cannot_do():
+    c = w4amd.capi()
+    call = dict(act=1, x=A, from_tokens=1, out=A, to_pairs=0)
+
+    def refused(text, N=32, experts=4, tokens=3, top_k=2, offsets=A, order=A, **change):
+        rows = c.expert_rows(experts, tokens, top_k, offsets, order)
+        with pytest.raises(ValueError, match=text):
+            c.gemm_experts(c.packed_view(N, 64, 32, 2, 1, A, A), rows, **{**call, **change})
+        with pytest.raises(ValueError, match=text):
+            c.gemm_experts_mx(c.packed_mx_view(N, 64, 2, A, A), rows, **{**call, **change})
+
+    refused("number of experts", experts=0)
+    refused("number of experts", N=1025, experts=1025)
+    refused("not a multiple", N=33)
+    refused("even number of rows", N=36)
+    refused("number of tokens", tokens=-1)
+    refused("number of tokens", top_k=0)
+    refused("number of tokens", tokens=1 << 29)
+    refused("act", act=3)
+    refused("act", act=-1)
+    refused("from_tokens", from_tokens=2)
+    refused("from_tokens", to_pairs=-1)
+    refused("null pointer", offsets=0)
+    refused("null pointer", order=0)
+    refused("null pointer", x=0)
+    refused("null pointer", out=0)
+    rows = c.expert_rows(4, 3, 2, A, A)
+    with pytest.raises(ValueError, match="gs must be"):
+        c.gemm_experts(c.packed_view(32, 64, 12, 6, 1, A, A), rows, **call)
+    with pytest.raises(ValueError, match="null pointer"):
+        c.gemm_experts_mx(c.packed_mx_view(32, 64, 2, A, 0), rows, **call)
+    # no tokens: nothing to do
+    c.gemm_experts(c.packed_view(32, 64, 32, 2, 1, A, A), c.expert_rows(4, 0, 2, A, 0), 1, 0, 1, 0, 0)
+
+
+def test_norms_refuse_what_they_cannot_do():
+    c = w4amd.capi()
+    good = dict(tokens=3, terms=2, y=A, weights=A, shared=0, residual=A, residual_f32=1, residual_out=A, h=A)
+
+    def refused(text, norm=None, **change):
+        n = c.block_norm(**{**dict(dim=64, pre=A), **(norm or {})})
+        with pytest.raises(ValueError, match=text):
+            c.residual_norm(n, **{**good, **change})
+
+    refused("dim is", {"dim": 0})
+    refused("dim is", {"dim": 32769})
+    refused("negative eps", {"eps": -1e-6})
+    refused("negative eps", {"eps": float("nan")})
+    refused("bias without", {"post_bias": A})
+    refused("bias without", {"pre": 0, "pre_bias": A}, h=0)
+    refused("gate_stride", {"gate": A, "gate_stride": 63})
+    refused("gate_stride", {"gate_stride": 64})
+    refused("bad dims", tokens=-1)
+    refused("bad dims", terms=0)
+    refused("bad dims", terms=65)
+    refused("residual_f32", residual_f32=2)
+    refused("h goes with", {"pre": 0})
+    refused("h goes with", h=0)
+    for name in ("y", "residual", "residual_out"):
+        refused("null pointer", **{name: 0})
+    refused("misaligned", residual=A + 2)
+    refused("misaligned", residual_out=A + 1, residual_f32=0)
+    c.residual_norm(c.block_norm(64, pre=A), 0, 1, 0, 0, 0, 0, 1, 0, 0)
+
+
+# ---- the definitions -----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_routing_by_definition(sigmoid):
+    rng = np.random.default_rng(1)
+    l = rng.normal(size=(40, 24)).astype(np.float32)
+    ids, w, _, order, offsets = experts_ref.route(l, 5, sigmoid=sigmoid)
+    t = torch.from_numpy(l).double()
+    s = torch.sigmoid(t) if sigmoid else torch.softmax(t, 1)
+    top = s.topk(5, dim=1)
+    assert np.array_equal(top.indices.numpy(), ids)
+    np.testing.assert_allclose(w, (top.values / top.values.sum(1, keepdim=True)).numpy(), rtol=1e-12)
+    assert sorted(order) == list(range(200)) and offsets[-1] == 200
+    for e in range(24):
+        places = order[offsets[e]:offsets[e + 1]]
+        assert (ids.reshape(-1)[places] == e).all() and (np.diff(places) > 0).all()
+
+
+def test_products_by_definition():
+    rng = np.random.default_rng(2)
+    for fmt in (0, 1, 2):
+        m = experts_ref.Experts(rng, 3, 8, 40, fmt, 16)
+        assert m.w.shape == (24, 40) and np.isfinite(m.w).all()
+        ids = np.array([[0, 2], [2, 1], [2, 0]])
+        flat = ids.reshape(-1)
+        order = np.argsort(flat, kind="stable").astype(np.int32)
+        offsets = np.concatenate([[0], np.cumsum(np.bincount(flat, minlength=3))]).astype(np.int32)
+        x = rng.normal(size=(3, 40)).astype(np.float16)
+        got, _ = experts_ref.gemm_experts(m, x, order, offsets, 2, 1, True, True, np.zeros((6, 4)))
+        for p in range(6):
+            y = torch.from_numpy(m.w.astype(np.float64)[flat[p] * 8:flat[p] * 8 + 8] @ x[p // 2].astype(np.float64))
+            want = torch.nn.functional.silu(y[:4]) * y[4:]
+            np.testing.assert_allclose(got[p], want.numpy(), rtol=1e-12, atol=1e-14)
+
+
+def test_norms_by_definition():
+    rng = np.random.default_rng(3)
+    y, r = rng.normal(size=(4, 2, 33)), rng.normal(size=(4, 33))
+    post, pre, bias = rng.normal(size=33), rng.normal(size=33), rng.normal(size=33)
+    got, _, h, _ = experts_ref.residual_norm(y, None, None, r, post, bias, None, pre, bias, True, 1e-5, 0.5)
+    ln = torch.nn.functional.layer_norm
+    T = torch.from_numpy
+    b = ln(T(y.sum(1)), (33,), T(post), T(bias), 1e-5)
+    want = T(r) + 0.5 * b
+    np.testing.assert_allclose(got, want.numpy(), rtol=1e-12)
+    np.testing.assert_allclose(h, ln(want, (33,), T(pre), T(bias), 1e-5).numpy(), rtol=1e-10)

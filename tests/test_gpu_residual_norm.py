@@ -1,0 +1,166 @@
+"""Joined rows, norms and the residual stream on the GPU, against their definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import experts_ref
+import w4amd
+from devutil import DEV, ptr, to_dev
+
+pytestmark = pytest.mark.gpu
+
+
+class Norm:
+    def __init__(self, seed, T, k, D, centred=False, post=True, biases=False, gate=0, pre=True, f32=False, shared=False,
+                 weights=True, scale=1.0, eps=1e-6, in_place=False, skew=0, gate_stride=0):
+        c = w4amd.capi()
+        rng = np.random.default_rng(seed)
+
+        def half(*shape):
+            return rng.normal(size=shape).astype(np.float16)
+
+        self.y = half(T, k, D)
+        self.w = rng.uniform(0, 1, (T, k)).astype(np.float32) if weights else None
+        self.shared = half(T, D) if shared else None
+        self.r = rng.normal(size=(T, D)).astype(np.float32 if f32 else np.float16)
+        self.post, self.pre = half(D) if post else None, half(D) if pre else None
+        self.post_bias = half(D) if post and biases else None
+        self.pre_bias = half(D) if pre and biases else None
+        self.gate = None if gate == 0 else half(D) if gate == 1 else half(T, max(gate_stride, D))
+        self.T, self.k, self.D, self.f32, self.scale, self.eps, self.centred = T, k, D, f32, scale, eps, centred
+        self.skew, self.in_place = skew, in_place
+        self.dev = {}
+
+        def put(name, a, fill=None):
+            if a is None:
+                return 0
+            flat = np.concatenate([np.zeros(skew, a.dtype), a.reshape(-1), np.full(8, 9, a.dtype)])
+            self.dev[name] = to_dev(flat)
+            return ptr(self.dev[name]) + skew * a.itemsize
+
+        self.put = put
+        at = {n: put(n, getattr(self, n)) for n in ("y", "shared", "r", "post", "pre", "post_bias", "pre_bias", "gate")}
+        self.dev["w"] = None if self.w is None else to_dev(self.w)
+        at["w"] = ptr(self.dev["w"])
+        at["r_out"] = at["r"] if in_place else put("r_out", np.full((T, D), 7, self.r.dtype))
+        at["h"] = put("h", np.full((T, D), 7, np.float16)) if pre else 0
+        self.at = at
+        stride = 0 if gate != 2 else self.gate.shape[1]
+        self.n = c.block_norm(D, centred=centred, eps=eps, residual_scale=scale, post=at["post"], post_bias=at["post_bias"],
+                              gate=at["gate"], gate_stride=stride, pre=at["pre"], pre_bias=at["pre_bias"])
+
+    def call(self, stream=0):
+        a = self.at
+        w4amd.capi().residual_norm(self.n, self.T, self.k, a["y"], a["w"], a["shared"], a["r"], int(self.f32), a["r_out"],
+                                   a["h"], stream)
+        return self
+
+    def host(self, name, dtype):
+        torch.cuda.synchronize()
+        flat = self.dev[name].cpu().numpy().view(dtype)
+        assert (flat[:self.skew] == 0).all() and (flat[self.skew + self.T * self.D:] == 9).all(), "written outside"
+        return flat[self.skew:self.skew + self.T * self.D].reshape(self.T, self.D).astype(np.float64)
+
+    def check(self):
+        gate = self.gate if self.gate is None or self.gate.ndim == 1 else self.gate[:, :self.D]
+        r, off, h, err = experts_ref.residual_norm(self.y, self.w, self.shared, self.r, self.post, self.post_bias, gate,
+                                                   self.pre, self.pre_bias, self.centred, self.eps, np.float64(np.float32(self.scale)))
+        far = np.abs(self.host("r" if self.in_place else "r_out", self.r.dtype) - r)
+        bound = experts_ref.rounded(r, off, self.f32)
+        assert (far <= bound).all(), float((far / bound).max())
+        if h is not None:
+            far, bound = np.abs(self.host("h", np.float16) - h), experts_ref.rounded(h, err)
+            assert (far <= bound).all(), float((far / bound).max())
+        return self
+
+
+DIMS = [1, 2, 7, 8, 9, 63, 64, 100, 511, 512, 513, 520, 1000, 2047, 2048, 2049, 4096, 4097, 5120, 8191, 8192, 8200, 16384, 20001, 32767, 32768]
+
+
+@pytest.mark.parametrize("D", DIMS)
+@pytest.mark.parametrize("f32", [False, True])
+def test_lengths(D, f32):
+    Norm(D, 3, 1, D, f32=f32).call().check()
+    Norm(D + 1, 2, 3, D, f32=f32, centred=True, biases=True, gate=1).call().check()
+
+
+@pytest.mark.parametrize("T", [1, 2, 5, 63, 300])
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 8, 13, 64])
+def test_terms(T, k):
+    Norm(T + k, T, k, 264).call().check()
+    Norm(T + k, T, k, 101, weights=False, shared=True, f32=True).call().check()
+
+
+@pytest.mark.parametrize("centred", [False, True])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("pre", [False, True])
+@pytest.mark.parametrize("gate", [0, 1, 2])
+@pytest.mark.parametrize("f32", [False, True])
+def test_ways(centred, post, pre, gate, f32):
+    for n, (biases, shared, weights, in_place) in enumerate(((True, False, True, False), (False, True, False, True))):
+        Norm(n, 9, 2, 300, centred, post, biases, gate, pre, f32, shared, weights, scale=(1.0, 0.22)[n], eps=(1e-6, 1e-2)[n],
+             in_place=in_place, gate_stride=(300, 333)[n]).call().check()
+
+
+@pytest.mark.parametrize("skew", [1, 2, 4])
+@pytest.mark.parametrize("D", [64, 1001])
+def test_arrays_at_any_address(skew, D):
+    for f32 in (False, True):
+        Norm(D, 5, 2, D, gate=2, f32=f32, shared=True, skew=skew, centred=True, biases=True).call().check()
+
+
+def test_rows_under_a_weight_of_0_are_not_read():
+    p = Norm(1, 6, 4, 200)
+    p.w[0, 1], p.w[1], p.w[2, :3], p.w[3, 3] = 0.0, 0.0, 0.0, -0.0
+    y = p.y.copy()
+    y[p.w == 0] = np.nan
+    p.dev["w"].copy_(to_dev(p.w))
+    p.dev["y"][:y.size].copy_(to_dev(y.reshape(-1)))
+    p.call().check()
+
+
+@pytest.mark.parametrize("k", [1, 4])
+def test_zero_rows_and_large_values(k):
+    p = Norm(2, 8, k, 333, f32=True, weights=False)
+    p.y[0], p.r[0] = 0, 0
+    p.y[1], p.y[2], p.r[2] = 60000 / k, 1e-7, 1e-20
+    p.r[3] = 1e18  # (its square is still an FP32 number)
+    p.dev["y"][:p.y.size].copy_(to_dev(p.y.reshape(-1)))
+    p.dev["r"][:p.r.size].copy_(to_dev(p.r.reshape(-1)))
+    p.call().check()
+
+
+def test_nothing_finite_stays_in_its_row():
+    p = Norm(3, 5, 2, 130)
+    p.y[2, 1, 7] = np.nan
+    p.dev["y"][:p.y.size].copy_(to_dev(p.y.reshape(-1)))
+    p.call()
+    r, h = p.host("r_out", np.float16), p.host("h", np.float16)
+    assert np.isnan(r[2]).all() and np.isnan(h[2]).all()
+    assert np.isfinite(np.delete(r, 2, 0)).all() and np.isfinite(np.delete(h, 2, 0)).all()
+
+
+def test_many_tokens_and_the_same_bytes_again():
+    p = Norm(4, 4000, 2, 260, gate=1).call().check()
+    h = p.dev["h"].clone()
+    s = torch.cuda.Stream()
+    p.dev["h"].zero_()
+    torch.cuda.synchronize()
+    p.call(s.cuda_stream)
+    torch.cuda.synchronize()
+    n = p.T * p.D
+    assert torch.equal(h[:n], p.dev["h"][:n])
+
+
+def test_a_captured_call():
+    p = Norm(5, 7, 3, 500, f32=True).call().check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        p.call(torch.cuda.current_stream().cuda_stream)
+    for seed in range(3):
+        p.y = np.random.default_rng(seed).normal(size=p.y.shape).astype(np.float16)
+        p.dev["y"][:p.y.size].copy_(to_dev(p.y.reshape(-1)))
+        graph.replay()
+        p.check()
+        Norm(seed, 3, 1, 64).call().check()
+    assert DEV

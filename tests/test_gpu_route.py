@@ -1,0 +1,208 @@
+"""Routing to experts on the GPU against its definition in 64 bits: choices, orders and offsets are equal, weights within
+what FP32 arithmetic may lose."""
+import numpy as np
+import pytest
+import torch
+
+import experts_ref
+import w4amd
+from devutil import DEV, ptr, to_dev
+
+pytestmark = pytest.mark.gpu
+
+
+class Route:
+    def __init__(self, logits, top_k, stride=0, count=None, pad_rows=0, **router):
+        c = w4amd.capi()
+        self.logits, self.top_k, self.count, self.more = logits, top_k, count, router
+        T, E = logits.shape
+        self.T, self.E = T, E
+        wide = np.full((T, stride or E), np.inf, logits.dtype)  # what lies between rows is not looked at
+        wide[:, :E] = logits
+        self.d = to_dev(wide) if T else torch.zeros(8, device=DEV)
+        bias = router.get("bias")
+        self.bias = None if bias is None else to_dev(bias)
+        self.count_d = None if count is None else to_dev(np.array([count], np.int32))
+        self.r = c.router(E, top_k, score=int(router.get("sigmoid", False)), groups=router.get("groups", 1),
+                          top_groups=router.get("top_groups", 1), group_best=router.get("group_best", 1),
+                          renorm=router.get("renorm", True), scale=router.get("scale", 1.0), bias=ptr(self.bias))
+        self.stride, self.f32 = stride, int(logits.dtype == np.float32)
+        self.n = c.route_experts_workspace(self.r, T)
+        self.space = torch.zeros(self.n + 16, dtype=torch.uint8, device=DEV)
+        self.fresh()
+
+    def fresh(self):
+        T, k, E = self.T, self.top_k, self.E
+        self.ids, self.order = (torch.full((T * k + 4,), 77, dtype=torch.int32, device=DEV) for _ in range(2))
+        self.w = torch.full((T * k + 4,), 7.0, device=DEV)
+        self.offsets = torch.full((E + 5,), 77, dtype=torch.int32, device=DEV)
+
+    def call(self, stream=0):
+        w4amd.capi().route_experts(self.r, ptr(self.d), self.f32, self.stride, self.T, ptr(self.count_d), ptr(self.ids),
+                                   ptr(self.w), ptr(self.order), ptr(self.offsets), ptr(self.space) if self.n else 0, self.n,
+                                   stream)
+        return self
+
+    def check(self):
+        torch.cuda.synchronize()
+        T, k, E = self.T, self.top_k, self.E
+        ids, w, bound, order, offsets = experts_ref.route(self.logits, k, count=self.count, **self.more)
+        got = [t.cpu().numpy() for t in (self.ids, self.w, self.order, self.offsets)]
+        assert np.array_equal(got[0][:T * k].reshape(T, k), ids)
+        off = np.abs(got[1][:T * k].reshape(T, k) - w)
+        assert (off <= bound).all(), float((off / bound).max())
+        assert np.array_equal(got[2][:T * k], order)
+        assert np.array_equal(got[3][:E + 1], offsets)
+        assert (got[0][T * k:] == 77).all() and (got[1][T * k:] == 7).all() and (got[2][T * k:] == 77).all()
+        assert (got[3][E + 1:] == 77).all()
+        return self
+
+
+def logits(seed, T, E, dtype=np.float32, spread=1.5):
+    rng = np.random.default_rng(seed)
+    return (spread * rng.normal(size=(T, E)) + 0.7 * rng.normal(size=E)).astype(dtype)
+
+
+@pytest.mark.parametrize("E,k", [(1, 1), (2, 2), (7, 3), (8, 2), (60, 4), (64, 6), (65, 6), (128, 8), (160, 6), (256, 8), (384, 8),
+                                 (512, 32), (1000, 9), (1024, 32)])
+@pytest.mark.parametrize("T", [1, 2, 17, 64, 130])
+def test_sizes(T, E, k):
+    for n, (dtype, sigmoid) in enumerate(((np.float32, False), (np.float16, False), (np.float32, True), (np.float16, True))):
+        Route(logits(T * E + n, T, E, dtype), k, sigmoid=sigmoid, renorm=n % 2 == 0, scale=1.0 + n).call().check()
+
+
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("E,groups,top_groups,best", [(16, 4, 2, 2), (64, 8, 3, 1), (160, 8, 3, 2), (256, 8, 4, 2), (256, 8, 8, 2),
+                                                     (64, 64, 9, 2), (96, 3, 1, 2), (1024, 64, 16, 2), (24, 1, 1, 1), (250, 2, 1, 2)])
+def test_groups_and_bias(E, groups, top_groups, best, bias, sigmoid):
+    rng = np.random.default_rng(E + groups)
+    b = (0.2 * rng.normal(size=E)).astype(np.float32) if bias else None
+    for dtype in (np.float32, np.float16):
+        Route(logits(E, 70, E, dtype), min(8, top_groups * (E // groups)), sigmoid=sigmoid, bias=b, groups=groups,
+              top_groups=top_groups, group_best=best, scale=2.5).call().check()
+
+
+@pytest.mark.parametrize("T", [4099, 16384, 70000])
+def test_many_tokens(T):
+    """Several blocks of tokens; past 65536 a block has more than 64."""
+    a = logits(T, 97, 64)
+    l = a[np.random.default_rng(T).integers(0, 97, T)]  # (rows repeat, so that the definition stays quick)
+    r = Route(l, 6).call()
+    torch.cuda.synchronize()
+    ids, w, bound, _, _ = experts_ref.route(a, 6)
+    _, back = np.unique(l, axis=0, return_index=True)
+    which = {l_.tobytes(): i for i, l_ in enumerate(a)}
+    rows = np.array([which[x.tobytes()] for x in l])
+    flat = ids[rows].reshape(-1)
+    assert np.array_equal(r.ids.cpu().numpy()[:T * 6], flat)
+    assert (np.abs(r.w.cpu().numpy()[:T * 6].reshape(T, 6) - w[rows]) <= bound[rows]).all()
+    assert np.array_equal(r.order.cpu().numpy()[:T * 6], np.argsort(flat, kind="stable"))
+    assert np.array_equal(r.offsets.cpu().numpy()[:65], np.concatenate([[0], np.cumsum(np.bincount(flat, minlength=64))]))
+
+
+def test_no_tokens():
+    r = Route(np.zeros((0, 24), np.float32), 4).call()
+    torch.cuda.synchronize()
+    assert (r.offsets.cpu().numpy()[:25] == 0).all()
+
+
+@pytest.mark.parametrize("count", [0, 1, 63, 64, 65, 99, 100, 1000, -5])
+def test_tokens_that_are_not_there(count):
+    Route(logits(3, 100, 32), 4, count=count).call().check()
+
+
+def test_rows_apart():
+    for dtype in (np.float32, np.float16):
+        Route(logits(4, 33, 60, dtype), 4, stride=67).call().check()
+
+
+@pytest.mark.parametrize("E,groups", [(8, 1), (48, 1), (64, 4), (256, 8)])
+@pytest.mark.parametrize("sigmoid", [False, True])
+def test_equal_logits_go_to_the_lowest(E, groups, sigmoid):
+    l = np.random.default_rng(E).integers(-2, 3, (200, E)).astype(np.float32)
+    l[0] = 0
+    l[1] = -3e38
+    more = dict(sigmoid=sigmoid, groups=groups, top_groups=max(1, groups // 2), group_best=2)
+    Route(l, 4, **more).call().check()
+    Route(np.clip(l, -100, 100).astype(np.float16), 4, **more).call().check()
+    bias = np.repeat(np.float32([0.25, -0.5]), E // 2)
+    Route(np.clip(l, -100, 100), 4, bias=bias, **more).call().check()
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("sigmoid,groups,bias", [(False, 1, False), (True, 1, False), (True, 4, True), (False, 4, True)])
+def test_logits_that_are_not_finite(dtype, sigmoid, groups, bias):
+    rng = np.random.default_rng(7)
+    l = logits(8, 300, 64, dtype)
+    bad = rng.random(l.shape)
+    l[bad < 0.2] = -np.inf
+    l[(bad > 0.2) & (bad < 0.3)] = np.nan
+    l[(bad > 0.3) & (bad < 0.32)] = np.inf
+    l[0], l[1], l[2] = -np.inf, np.nan, np.inf
+    l[3] = -np.inf
+    l[3, 40] = 0.5                      # one expert is left
+    l[4, :16], l[4, 16:] = np.nan, -np.inf
+    l[5] = np.finfo(dtype).min          # the type's lowest value is a logit like others
+    l[6, 3:] = np.finfo(dtype).min
+    b = None
+    if bias:
+        b = (0.1 * rng.normal(size=64)).astype(np.float32)
+        b[5], b[9], b[33] = -np.inf, np.nan, np.inf
+    Route(l, 6, sigmoid=sigmoid, groups=groups, top_groups=max(1, groups // 2), group_best=2, bias=b).call().check()
+
+
+def test_choices_next_to_a_border():
+    """Sums of score and bias that 32 bits do not tell apart."""
+    rng = np.random.default_rng(11)
+    E, T = 32, 400
+    bias = rng.normal(size=E).astype(np.float32)
+    l = np.zeros((T, E), np.float32)
+    for t in range(T):
+        level = rng.uniform(1.6, 1.8)
+        want = np.clip(level - bias.astype(np.float64), 1e-3, 1 - 1e-3)  # every score + bias at about one level
+        l[t] = np.log(want / (1 - want))
+    ids = experts_ref.route(l, 4, sigmoid=True, bias=bias)[0]
+    s = (np.float32(1) / (np.float32(1) + np.exp(-l))) + bias
+    assert (np.argsort(-s, axis=1, kind="stable")[:, :4] != ids).any(), "the case is not next to a border"
+    Route(l, 4, sigmoid=True, bias=bias).call().check()
+    Route(l, 4, sigmoid=True, bias=bias, groups=4, top_groups=2, group_best=2).call().check()
+
+
+def test_a_captured_call_is_replayed_on_other_logits():
+    c = w4amd.capi()
+    for T in (5, 40, 900):
+        r = Route(logits(12, T, 64), 4, count=T)
+        stream = torch.cuda.Stream()
+        r.call().check()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            r.call(torch.cuda.current_stream().cuda_stream)
+        for seed, count in ((13, T), (14, T // 2), (15, 0), (16, T)):
+            r.logits, r.count = logits(seed, T, 64), count
+            r.d.copy_(to_dev(r.logits))
+            r.count_d.fill_(count)
+            graph.replay()
+            r.check()
+            Route(logits(seed + 50, T + 3, 64), 4).call().check()  # eager work in between
+    assert c is not None
+
+
+def test_one_workspace_for_calls_of_every_size():
+    a = [Route(logits(20 + T, T, E), 4) for T, E in ((3000, 256), (1, 64), (130, 1024), (17, 8), (5000, 64))]
+    big = max(a, key=lambda r: r.n)
+    for r in a * 3:
+        r.space = big.space
+        r.fresh()
+        r.call().check()
+
+
+def test_two_streams():
+    rs = [Route(logits(30 + i, 300 + i, 128), 8) for i in range(4)]
+    streams = [torch.cuda.Stream() for _ in rs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for r, s in zip(rs, streams):
+            r.call(s.cuda_stream)
+    for r in rs:
+        r.check()

@@ -58,6 +58,20 @@ class PagedBatch(C.Structure):
                 ("bt", vp), ("lens", vp), ("cu_q", vp)]
 
 
+class Router(C.Structure):
+    _fields_ = [("experts", C.c_int), ("top_k", C.c_int), ("score", C.c_int), ("groups", C.c_int), ("top_groups", C.c_int),
+                ("group_best", C.c_int), ("renorm", C.c_int), ("scale", C.c_float), ("bias", vp)]
+
+
+class ExpertRows(C.Structure):
+    _fields_ = [("experts", C.c_int), ("tokens", C.c_int), ("top_k", C.c_int), ("offsets", vp), ("order", vp)]
+
+
+class BlockNorm(C.Structure):
+    _fields_ = [("dim", C.c_int), ("centred", C.c_int), ("eps", C.c_float), ("residual_scale", C.c_float), ("post", vp),
+                ("post_bias", vp), ("gate", vp), ("gate_stride", C.c_int), ("pre", vp), ("pre_bias", vp)]
+
+
 # every symbol include/w4_abi.h declares, with its argument types
 SIGNATURES = {
     "w4_last_error": ([], C.c_char_p),
@@ -103,6 +117,11 @@ SIGNATURES = {
     "w4_attention_f8_pages_workspace": ([C.POINTER(F8PagesView), C.POINTER(PagedBatch), C.c_int,
                                          C.POINTER(C.c_size_t)], C.c_int),
     "w4_attention_f8_pages_plan_for": ([C.POINTER(F8PagesView), C.POINTER(PagedBatch), C.c_int, C.POINTER(C.c_int)], C.c_int),
+    "w4_route_experts": ([C.POINTER(Router), vp, C.c_int, C.c_int, C.c_int] + [vp] * 6 + [C.c_size_t, vp], C.c_int),
+    "w4_route_experts_workspace": ([C.POINTER(Router), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "w4_gemm_experts": ([C.POINTER(PackedView), C.POINTER(ExpertRows), C.c_int, vp, C.c_int, vp, C.c_int, vp], C.c_int),
+    "w4_gemm_experts_mx": ([C.POINTER(PackedMxView), C.POINTER(ExpertRows), C.c_int, vp, C.c_int, vp, C.c_int, vp], C.c_int),
+    "w4_residual_norm": ([C.POINTER(BlockNorm), C.c_int, C.c_int, vp, vp, vp, vp, C.c_int, vp, vp, vp], C.c_int),
 }
 
 _lib = None
@@ -150,6 +169,10 @@ _NATIVE = {
     "paged_tables": ("w4_paged_tables", None),
     "quantize_f8_pages": ("w4_quantize_f8_pages", None),
     "attention_f8_pages": ("w4_attention_f8_pages", None),
+    "route_experts": ("w4_route_experts", None),
+    "gemm_experts": ("w4_gemm_experts", None),
+    "gemm_experts_mx": ("w4_gemm_experts_mx", None),
+    "residual_norm": ("w4_residual_norm", None),
 }
 
 
@@ -387,3 +410,52 @@ def attention_f8_pages(view, batch, group, causal, q, q_stride, out, workspace=0
     for each call in flight."""
     check(load().w4_attention_f8_pages(C.byref(view), C.byref(batch), group, int(causal), _n(q), q_stride, _n(out),
                                        _n(workspace), workspace_bytes, _n(stream)))
+
+
+def router(experts, top_k, score=0, groups=1, top_groups=1, group_best=1, renorm=True, scale=1.0, bias=0):
+    """How logits become a choice of experts; score 0 softmax, 1 sigmoid (include/w4_abi.h)"""
+    return Router(experts, top_k, score, groups, top_groups, group_best, int(bool(renorm)), scale, bias or None)
+
+
+def expert_rows(experts, tokens, top_k, offsets, order):
+    return ExpertRows(experts, tokens, top_k, offsets or None, order or None)
+
+
+def block_norm(dim, centred=False, eps=1e-6, residual_scale=1.0, post=0, post_bias=0, gate=0, gate_stride=0, pre=0,
+               pre_bias=0):
+    """The norms around a block, its gate and its way into the residual stream (include/w4_abi.h)"""
+    return BlockNorm(dim, int(bool(centred)), eps, residual_scale, post or None, post_bias or None, gate or None, gate_stride,
+                     pre or None, pre_bias or None)
+
+
+def route_experts_workspace(router, tokens):
+    """Bytes of device memory that route_experts needs, cleared once before its first call."""
+    n = C.c_size_t()
+    check(load().w4_route_experts_workspace(C.byref(router), tokens, C.byref(n)))
+    return n.value
+
+
+def route_experts(router, logits, logits_f32, row_stride, tokens, count, experts, weights, order, offsets, workspace=0,
+                  workspace_bytes=0, stream=0):
+    """Each token's experts and weights, the pairs sorted by expert, the experts' offsets.  `workspace`:
+    route_experts_workspace() bytes, cleared once, one for each call in flight."""
+    check(load().w4_route_experts(C.byref(router), _n(logits), int(logits_f32), row_stride, tokens, _n(count), _n(experts),
+                                  _n(weights), _n(order), _n(offsets), _n(workspace), workspace_bytes, _n(stream)))
+
+
+def gemm_experts(view, rows, act, x, from_tokens, out, to_pairs, stream=0):
+    """Rows of pairs times their experts' W4 matrices; act 0 none, 1 SiLU(gate) * up, 2 GELU(gate) * up."""
+    check(load().w4_gemm_experts(C.byref(view), C.byref(rows), act, _n(x), int(from_tokens), _n(out), int(to_pairs),
+                                 _n(stream)))
+
+
+def gemm_experts_mx(view, rows, act, x, from_tokens, out, to_pairs, stream=0):
+    """gemm_experts over MXFP4 matrices"""
+    check(load().w4_gemm_experts_mx(C.byref(view), C.byref(rows), act, _n(x), int(from_tokens), _n(out), int(to_pairs),
+                                    _n(stream)))
+
+
+def residual_norm(norm, tokens, terms, y, weights, shared, residual, residual_f32, residual_out, h, stream=0):
+    """Weighted sum of a token's rows, norm, gate, residual and the next block's norm."""
+    check(load().w4_residual_norm(C.byref(norm), tokens, terms, _n(y), _n(weights), _n(shared), _n(residual),
+                                  int(residual_f32), _n(residual_out), _n(h), _n(stream)))

@@ -733,6 +733,99 @@ int w4_attention_f8_pages(const w4_f8_pages_view* p, const w4_paged_batch* b, in
   return done("attention_f8_pages", w4k::launch_pages_attention(a, (hipStream_t)stream));
 }
 
+// ---- a feed-forward block of experts --------------------------------------------------
+
+static int check_router(const w4_router* r, int tokens) {
+  REQUIRE(r != nullptr, "route experts: null router");
+  REQUIRE(r->experts >= 1 && r->experts <= 1024, "route experts: bad number of experts");
+  REQUIRE(r->top_k >= 1 && r->top_k <= 32 && r->top_k <= r->experts, "route experts: bad top_k");
+  REQUIRE(r->score == 0 || r->score == 1, "route experts: score is 0 or 1");
+  REQUIRE(r->groups >= 1 && r->experts % r->groups == 0, "route experts: groups do not divide the experts");
+  REQUIRE(r->top_groups >= 1 && r->top_groups <= r->groups, "route experts: bad top_groups");
+  REQUIRE(r->groups <= 64, "route experts: more than 64 groups");
+  REQUIRE(r->group_best == 1 || r->group_best == 2, "route experts: group_best is 1 or 2");
+  REQUIRE(r->renorm == 0 || r->renorm == 1, "route experts: renorm is 0 or 1");
+  REQUIRE(tokens >= 0 && tokens <= 1 << 25 && (long long)tokens * r->top_k < (1LL << 30),
+          "route experts: bad number of tokens");
+  return W4_OK;
+}
+
+int w4_route_experts_workspace(const w4_router* r, int tokens, size_t* bytes) {
+  if (int rc = check_router(r, tokens)) return rc;
+  REQUIRE(bytes != nullptr, "route experts: null pointer");
+  *bytes = w4k::route_space(*r, tokens);
+  return W4_OK;
+}
+
+int w4_route_experts(const w4_router* r, const void* logits, int logits_f32, int row_stride, int tokens, const int* count,
+                     int* experts, float* weights, int* order, int* offsets, void* workspace, size_t workspace_bytes,
+                     w4_stream stream) {
+  if (int rc = check_router(r, tokens)) return rc;
+  REQUIRE(offsets && (tokens == 0 || (logits && experts && weights && order)), "route experts: null pointer");
+  REQUIRE(logits_f32 == 0 || logits_f32 == 1, "route experts: logits_f32 is 0 or 1");
+  REQUIRE(row_stride == 0 || row_stride >= r->experts, "route experts: row_stride is shorter than a row");
+  REQUIRE(((uintptr_t)logits & (logits_f32 ? 3 : 1)) == 0, "route experts: misaligned logits");
+  const size_t need = w4k::route_space(*r, tokens);
+  REQUIRE(workspace_bytes >= need && (workspace || !need), "route experts: workspace too small");
+  REQUIRE(((uintptr_t)workspace & 15) == 0, "route experts: workspace 16-byte aligned");
+  const w4k::RouteArgs a{*r, logits, logits_f32, tokens, row_stride ? row_stride : r->experts, count, experts, weights,
+                         order, offsets, (char*)workspace};
+  return done("route_experts", w4k::launch_route_experts(a, (hipStream_t)stream));
+}
+
+static int run_gemm_experts(const w4k::WView& v, const w4_expert_rows* rows, int act, const w4_half* x, int from_tokens,
+                            w4_half* out, int to_pairs, w4_stream stream) {
+  REQUIRE(rows != nullptr, "gemm experts: null rows");
+  REQUIRE(rows->experts >= 1 && rows->experts <= 1024, "gemm experts: bad number of experts");
+  REQUIRE(rows->top_k >= 1 && rows->tokens >= 0 && (long long)rows->tokens * rows->top_k < (1LL << 30),
+          "gemm experts: bad number of tokens");
+  REQUIRE(v.N % rows->experts == 0, "gemm experts: N is not a multiple of the experts");
+  REQUIRE(act >= 0 && act <= 2, "gemm experts: act is 0, 1 or 2");
+  REQUIRE(act == 0 || v.N / rows->experts % 2 == 0, "gemm experts: a gated expert has an even number of rows");
+  REQUIRE((from_tokens == 0 || from_tokens == 1) && (to_pairs == 0 || to_pairs == 1),
+          "gemm experts: from_tokens and to_pairs are 0 or 1");
+  REQUIRE(rows->offsets && (rows->tokens == 0 || (rows->order && x && out)), "gemm experts: null pointer");
+  if (rows->tokens == 0) return W4_OK;
+  const w4k::ExpertArgs a{v, rows->experts, rows->tokens, rows->top_k, act, from_tokens, to_pairs, rows->offsets,
+                          rows->order, x, out};
+  const hipError_t e = w4k::launch_gemm_experts(a, (hipStream_t)stream);
+  REQUIRE(e != hipErrorInvalidConfiguration, "gemm experts: launch grid out of range");
+  return done("gemm_experts", e);
+}
+
+int w4_gemm_experts(const w4_packed_view* p, const w4_expert_rows* rows, int act, const w4_half* x, int from_tokens,
+                    w4_half* out, int to_pairs, w4_stream stream) {
+  if (int rc = check_packed(p, "gemm experts")) return rc;
+  return run_gemm_experts(w4k::view_of(*p), rows, act, x, from_tokens, out, to_pairs, stream);
+}
+
+int w4_gemm_experts_mx(const w4_packed_mx_view* p, const w4_expert_rows* rows, int act, const w4_half* x, int from_tokens,
+                       w4_half* out, int to_pairs, w4_stream stream) {
+  if (int rc = check_mx(p)) return rc;
+  return run_gemm_experts(w4k::view_of(*p), rows, act, x, from_tokens, out, to_pairs, stream);
+}
+
+int w4_residual_norm(const w4_block_norm* n, int tokens, int terms, const w4_half* y, const float* weights,
+                     const w4_half* shared, const void* residual, int residual_f32, void* residual_out, w4_half* h,
+                     w4_stream stream) {
+  REQUIRE(n != nullptr, "residual norm: null norm");
+  REQUIRE(n->dim >= 1 && n->dim <= 32768, "residual norm: dim is 1 to 32768");
+  REQUIRE(n->centred == 0 || n->centred == 1, "residual norm: centred is 0 or 1");
+  REQUIRE(n->eps >= 0.f, "residual norm: negative eps");
+  REQUIRE(n->post || !n->post_bias, "residual norm: a bias without its norm");
+  REQUIRE(n->pre || !n->pre_bias, "residual norm: a bias without its norm");
+  REQUIRE(n->gate_stride == 0 || (n->gate && n->gate_stride >= n->dim), "residual norm: gate_stride is shorter than a row");
+  REQUIRE(tokens >= 0 && terms >= 1 && terms <= 64, "residual norm: bad dims");
+  REQUIRE(residual_f32 == 0 || residual_f32 == 1, "residual norm: residual_f32 is 0 or 1");
+  REQUIRE((n->pre != nullptr) == (h != nullptr) || tokens == 0, "residual norm: h goes with the norm ahead");
+  REQUIRE(tokens == 0 || (y && residual && residual_out), "residual norm: null pointer");
+  REQUIRE((((uintptr_t)residual | (uintptr_t)residual_out) & (residual_f32 ? 3 : 1)) == 0,
+          "residual norm: misaligned residual");
+  if (tokens == 0) return W4_OK;
+  const w4k::NormArgs a{*n, tokens, terms, y, weights, shared, residual, residual_f32, residual_out, h};
+  return done("residual_norm", w4k::launch_residual_norm(a, (hipStream_t)stream));
+}
+
 }  // extern "C"
 
 // ---- two-pass baseline -------------------------------------------------------------

@@ -1,0 +1,97 @@
+// Products of pairs' rows with their experts' packed matrices (w4_gemm_experts, w4_gemm_experts_mx).
+//
+// This file: the kernel for every K, group size and alignment, and the rule that says which kernel a call runs.
+#include "experts.cuh"
+
+namespace w4k {
+namespace {
+
+constexpr int EG_WAVES = 4, EG_ROWS = 8;
+
+// The host's dequantization step of element k of a row, as a float.
+template <int FMT>
+__device__ __forceinline__ void expert_word(const ExpertArgs& a, long long row, int word, float w[8]) {
+  const WView& v = a.v;
+  const uint32_t q = v.q[row * words(v.K) + word];
+  if constexpr (FMT == 2) {
+    const float s = mx_scale(((const uint8_t*)v.scales)[row * v.B + word / 4]);
+    h2 n[4];
+    dq_mx(q, s, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = (float)n[e >> 1][e & 1];
+  } else {
+    const int g = word * 8 / v.gs;  // (gs is a multiple of 8: a word lies in one group)
+    int z = 8;
+    if constexpr (FMT == 1) z = v.zeros[row * words(v.G) + (g >> 3)] >> (4 * (g & 7)) & 0xF;
+    const float s = half_bits_to_float(((const uint16_t*)v.scales)[row * v.G + g]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = (float)(_Float16)(s * (float)((int)(q >> (4 * e) & 0xF) - z));
+  }
+}
+
+// A wave: one output column (gated: a gate row and an up row) of up to EG_ROWS places; a lane takes every 64th word.
+template <int FMT, bool GATED>
+__global__ __launch_bounds__(64 * EG_WAVES) void experts_general_kernel(ExpertArgs a, int tiles_n) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int pairs = a.tokens * a.top_k;
+  const ExpertTile t = find_expert_tile<EG_ROWS>(a.offsets, a.experts, pairs, blockIdx.x / tiles_n);
+  const int R = a.v.N / a.experts, width = GATED ? R / 2 : R;
+  const int col = blockIdx.x % tiles_n * EG_WAVES + wave;
+  if (t.rows == 0 || col >= width) return;
+  const long long row = (long long)t.expert * R + col;
+  int pair[EG_ROWS];
+  const uint16_t* x[EG_ROWS];
+  float sum[GATED ? 2 : 1][EG_ROWS] = {};
+#pragma unroll
+  for (int m = 0; m < EG_ROWS; ++m) {
+    const int place = t.first + min(m, t.rows - 1);
+    pair[m] = a.order[place];
+    const bool there = m < t.rows && pair[m] >= 0 && pair[m] < pairs;
+    const int from = a.from_tokens ? (there ? pair[m] : 0) / a.top_k : place;
+    x[m] = a.x + (long long)from * a.v.K;
+    if (!there) pair[m] = -1;
+  }
+  for (int w = lane; w < words(a.v.K); w += 64) {
+    float gate[8], up[8];
+    expert_word<FMT>(a, row, w, gate);
+    if constexpr (GATED) expert_word<FMT>(a, row + width, w, up);
+    const int n = min(8, a.v.K - 8 * w);
+#pragma unroll
+    for (int m = 0; m < EG_ROWS; ++m) {
+      if (m >= t.rows) break;
+      for (int e = 0; e < n; ++e) {
+        const float xv = half_bits_to_float(x[m][8 * w + e]);
+        sum[0][m] += gate[e] * xv;
+        if constexpr (GATED) sum[1][m] += up[e] * xv;
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < EG_ROWS; ++m) {
+    if (m >= t.rows) break;
+    float y = wave_sum_to_lane63(sum[0][m]);
+    if constexpr (GATED) y = expert_act(a.act, y) * wave_sum_to_lane63(sum[1][m]);
+    if (lane == 63 && pair[m] >= 0)
+      a.out[(long long)(a.to_pairs ? pair[m] : t.first + m) * width + col] = __builtin_bit_cast(uint16_t, (_Float16)y);
+  }
+}
+
+template <int FMT>
+hipError_t go_general(const ExpertArgs& a, hipStream_t s) {
+  const int R = a.v.N / a.experts, width = a.act ? R / 2 : R;
+  const int tiles_n = (width + EG_WAVES - 1) / EG_WAVES;
+  const long long grid = most_expert_tiles(a, EG_ROWS) * tiles_n;
+  if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  if (a.act) experts_general_kernel<FMT, true><<<(unsigned)grid, 64 * EG_WAVES, 0, s>>>(a, tiles_n);
+  else experts_general_kernel<FMT, false><<<(unsigned)grid, 64 * EG_WAVES, 0, s>>>(a, tiles_n);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_gemm_experts(const ExpertArgs& a, hipStream_t s) {
+  if (a.v.mx) return go_general<2>(a, s);
+  return a.v.symmetric ? go_general<0>(a, s) : go_general<1>(a, s);
+}
+
+}  // namespace w4k

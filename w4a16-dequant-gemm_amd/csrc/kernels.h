@@ -219,4 +219,44 @@ size_t pages_attention_space(const PagesArgs& a);
 void pages_attention_plan(const PagesArgs& a, int* plan);  // w4_attention_f8_pages_plan_for
 hipError_t launch_pages_attention(const PagesArgs& a, hipStream_t s);
 
+// ---- a feed-forward block of experts -----------------------------------------------------
+// experts_route.hip
+struct RouteArgs {
+  w4_router r;  // (bias: device memory)
+  const void* logits;
+  int f32, tokens;
+  long long stride;
+  const int* count;
+  int* experts;
+  float* weights;
+  int *order, *offsets;
+  char* space;
+};
+size_t route_space(const w4_router& r, int tokens);
+hipError_t launch_route_experts(const RouteArgs& a, hipStream_t s);
+
+// gemm_experts.hip
+struct ExpertArgs {
+  WView v;  // N = experts * R rows
+  int experts, tokens, top_k, act, from_tokens, to_pairs;
+  const int *offsets, *order;
+  const w4_half* x;
+  w4_half* out;
+};
+hipError_t launch_gemm_experts(const ExpertArgs& a, hipStream_t s);
+
+// residual_norm.hip
+struct NormArgs {
+  w4_block_norm n;
+  int tokens, terms;
+  const w4_half* y;
+  const float* weights;
+  const w4_half* shared;
+  const void* residual;
+  int f32;
+  void* residual_out;
+  w4_half* h;
+};
+hipError_t launch_residual_norm(const NormArgs& a, hipStream_t s);
+
 }  // namespace w4k
