@@ -17,7 +17,7 @@ CALLS = os.path.join(PKG, "lib", "w4calls" + (sysconfig.get_config_var("EXT_SUFF
 CALLS_SRC = os.path.join(CSRC, "pycalls.cpp")
 PY_INCLUDE = sysconfig.get_paths()["include"]
 SOURCES = ["abi.hip", "dequant.hip", "gemm_simt.hip", "gemm_mfma.hip", "flash.hip", "flash_mfma.hip", "quantize.hip", "gemm_mxnative.hip", "gemm_tile_dma.hip", "gemm_tile_any.hip", "gemm_tile256.hip", "gemm_decode_resident.hip", "gemm_decode_general.hip", "gemm_decode_longk.hip", "gemm_block.hip",
-           "baseline.hip", "paged_tables.hip", "quantize_pages.hip", "pages_attention.hip", "pages_few.hip", "pages_many.hip", "pages_mixed.hip", "experts_route.hip", "gemm_experts.hip", "residual_norm.hip"]
+           "baseline.hip", "paged_tables.hip", "quantize_pages.hip", "pages_attention.hip", "pages_few.hip", "pages_many.hip", "pages_mixed.hip", "experts_route.hip", "gemm_experts.hip", "gemm_experts_tile.hip", "residual_norm.hip"]
 HEADERS = ["dq.cuh", "experts.cuh", "kernels.h", "pages.cuh", "pages_few.cuh", "pages_many.cuh", "simt_rows4.cuh", "tile_dma.cuh", "bench_kernels.hip", os.path.join("..", "..", "include", "w4_abi.h")]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
@@ -35,13 +35,14 @@ FLAGS = [
 # vector-ALU multiplies between matrix instructions: with the accumulators in
 # the AGPR half of the register file the compiler copies all 36 of them across
 # every loop edge, so keep its MFMA results in ordinary VGPRs.
-# The tile kernels for any group unroll eight steps that are longer than the
-# threshold allows (the LDS addresses in their loads are immediates).
+# The tile kernels for any group, and those of experts, unroll steps that are longer than
+# the threshold allows (the LDS addresses in their loads are immediates).
 EXTRA_FLAGS = {"flash_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "pages_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "pages_many.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "pages_mixed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-               "gemm_tile_any.hip": ["-mllvm", "-pragma-unroll-threshold=100000"]}
+               "gemm_tile_any.hip": ["-mllvm", "-pragma-unroll-threshold=100000"],
+               "gemm_experts_tile.hip": ["-mllvm", "-pragma-unroll-threshold=100000"]}
 
 
 def _calls_stale():

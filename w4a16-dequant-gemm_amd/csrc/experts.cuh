@@ -6,38 +6,71 @@
 
 namespace w4k {
 
-// One tile of up to TM places of one expert.
+// Some places of one expert, of which a workgroup takes up to TM.
 struct ExpertTile {
-  int expert, first, rows;  // rows 0: there is no such tile
-  int tiles;                // of all experts
+  int expert, first, rows;  // of the tile; rows 0: there is no such tile
+  int column;               // its turn among the tiles of W
 };
 
-// Tile `tile` of the experts' tiles of TM places, in the experts' order; `tile` may be any number.  Every wave of a
-// workgroup finds it for itself: lane l sums the tiles of experts l, l + 64 ... in turns of 64 experts, a scan of a wave
-// each.  Offsets are cut to what `order` has, so that no plan leads outside the arrays.
-template <int TM>
-__device__ __forceinline__ ExpertTile find_expert_tile(const int* __restrict__ offsets, int experts, int pairs, int tile) {
+// Lane l looks after experts e0 + l: where their places begin and end.  Offsets are cut to what `order` has, so that no
+// plan leads outside the arrays.
+__device__ __forceinline__ void expert_places(const int* __restrict__ offsets, int experts, int pairs, int e0, int& lo, int& hi) {
+  const int e = e0 + (int)(threadIdx.x & 63), at = min(e, experts - 1);
+  lo = min(max(offsets[at], 0), pairs);
+  hi = e < experts ? min(max(offsets[at + 1], lo), pairs) : lo;
+}
+
+__device__ __forceinline__ int wave_upto(int v) {  // sum over the lanes up to this one
   const int lane = threadIdx.x & 63;
-  ExpertTile r{0, 0, 0, 0};
-  for (int e0 = 0; e0 < experts; e0 += 64) {
-    const int e = min(e0 + lane, experts - 1);
-    const int lo = min(max(offsets[e], 0), pairs), hi = min(max(offsets[e + 1], lo), pairs);
-    const int n = e0 + lane < experts ? (hi - lo + TM - 1) / TM : 0;
-    int upto = n;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int v = __shfl_up(upto, o);
-      if (lane >= o) upto += v;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Tile L of the experts' tiles of TM places times `columns` tiles of W, in the experts' order, an expert's places
+// fastest: workgroups side by side read the same codes.  L may be any number.  Every wave finds it for itself.
+// EVEN: an expert's places are shared out over its tiles in steps of 32.
+// SPREAD: consecutive workgroup ids land on different XCDs, each with an L2 of its own: L is turned round so that each
+// XCD has a run of the order, whose length is that of the tiles there are, not of the grid.
+template <int TM, bool EVEN, bool SPREAD>
+__device__ __forceinline__ ExpertTile find_expert_tile(const int* __restrict__ offsets, int experts, int pairs, int columns,
+                                                       int L) {
+  ExpertTile r{0, 0, 0, 0};
+  int lo, hi;
+  if constexpr (SPREAD) {
+    int all = 0;
+    for (int e0 = 0; e0 < experts; e0 += 64) {
+      expert_places(offsets, experts, pairs, e0, lo, hi);
+      all += (hi - lo + TM - 1) / TM;
     }
-    const int t = tile - r.tiles - (upto - n);  // the tile's number in this lane's expert
-    const unsigned long long hit = __ballot(t >= 0 && t < n);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
+    const int run = (all * columns + 7) >> 3;
+    if (L >> 3 >= run) return r;
+    L = (L & 7) * run + (L >> 3);
+  }
+  const int tile = L / columns;  // an expert's tiles times columns begin at a multiple of columns
+  int before = 0;
+  for (int e0 = 0; e0 < experts; e0 += 64) {
+    expert_places(offsets, experts, pairs, e0, lo, hi);
+    const int n = (hi - lo + TM - 1) / TM, upto = wave_upto(n);
+    const int first = before + upto - n;  // of this lane's expert
+    const unsigned long long hit = __ballot(tile >= first && tile < first + n);
     if (hit) {
       const int l = __builtin_ctzll(hit);
+      const int count = __shfl(n, l), places = __shfl(hi - lo, l), turn = L - __shfl(first, l) * columns;
+      const int per = EVEN ? ((places + count - 1) / count + 31) / 32 * 32 : TM;
+      const int m = turn % count * per;
       r.expert = e0 + l;
-      r.first = __shfl(lo + t * TM, l);
-      r.rows = __shfl(min(hi - (lo + t * TM), TM), l);
+      r.first = __shfl(lo, l) + m;
+      r.rows = min(places - m, per);
+      r.column = turn / count;
+      break;
     }
-    r.tiles += __shfl(upto, 63);
+    before += __shfl(upto, 63);
   }
   return r;
 }
@@ -54,5 +87,8 @@ __device__ __forceinline__ float expert_act(int act, float x) {
   const float u = act == 1 ? x : 1.5957691216057308f * x * (1.f + 0.044715f * x * x);
   return x / (1.f + __expf(-u));
 }
+
+// gemm_experts_tile.hip: false (nothing launched) when the arguments are not its.
+bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err);
 
 }  // namespace w4k

@@ -34,9 +34,9 @@ template <int FMT, bool GATED>
 __global__ __launch_bounds__(64 * EG_WAVES) void experts_general_kernel(ExpertArgs a, int tiles_n) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int pairs = a.tokens * a.top_k;
-  const ExpertTile t = find_expert_tile<EG_ROWS>(a.offsets, a.experts, pairs, blockIdx.x / tiles_n);
+  const ExpertTile t = find_expert_tile<EG_ROWS, false, false>(a.offsets, a.experts, pairs, tiles_n, blockIdx.x);
   const int R = a.v.N / a.experts, width = GATED ? R / 2 : R;
-  const int col = blockIdx.x % tiles_n * EG_WAVES + wave;
+  const int col = t.column * EG_WAVES + wave;
   if (t.rows == 0 || col >= width) return;
   const long long row = (long long)t.expert * R + col;
   int pair[EG_ROWS];
@@ -90,6 +90,8 @@ hipError_t go_general(const ExpertArgs& a, hipStream_t s) {
 }  // namespace
 
 hipError_t launch_gemm_experts(const ExpertArgs& a, hipStream_t s) {
+  hipError_t err = hipSuccess;
+  if (try_experts_tile(a, s, &err)) return err;
   if (a.v.mx) return go_general<2>(a, s);
   return a.v.symmetric ? go_general<0>(a, s) : go_general<1>(a, s);
 }

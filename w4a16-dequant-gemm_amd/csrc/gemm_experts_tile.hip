@@ -1,0 +1,392 @@
+// Products of many rows per expert with the experts' packed matrices, on the matrix cores.
+//
+// A workgroup multiplies up to 256 (or 128) places of one expert with 256 of its rows:
+//   * packed words and rows of x go global -> LDS (global_load_lds_dwordx4, no registers), a stage is 64 k: 32 bytes of
+//     a row of W, 128 of a row of x, wherever in x the place's token has it; three stage buffers, one barrier a stage;
+//   * v_mfma_f32_32x32x16_f16: a wave holds 64 rows of W against all rows of x.  Lane l brings row l % 32 and k
+//     32 (l / 32) + 8 u .. + 7 in step u of a stage: its words of W are one 16-byte read per stage and 32 rows;
+//   * a word becomes eight halves in registers, bit for bit those of w4_dequant, under the products of the step before:
+//     the order of the main loop is fixed by hand, one phase of the expansion behind each product, because with one
+//     wave per SIMD nothing else hides an instruction's latency;
+//   * gated experts: of a wave's two tiles of 32 rows the first is the gate's and the second the way up's for the same
+//     columns, so both sums of an output lie in one lane and the gate is taken in registers.
+// A tile with few places runs a loop of its own for 64, 128 or 192 of them: products of rows that are not there would
+// take as long as the others.  An expert's places are shared out evenly over its tiles.
+#include <atomic>
+
+#include "experts.cuh"
+
+namespace w4k {
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+constexpr int ET_THREADS = 256, ET_WAVES = 4, ET_STAGES = 3;
+constexpr int ET_W_BYTES = 256 * 32;
+constexpr int et_tile(int mj) { return ET_W_BYTES + mj * 32 * 128; }
+constexpr int et_stage(int mj) { return et_tile(mj) + 2 * 256 * 4; }  // + a scale dword and a zero-point word per row of W
+constexpr int ET_PITCH = 128 + 16;                                     // a wave's outputs of one place, padded
+constexpr int et_lds(int mj) {
+  return ET_STAGES * et_stage(mj) > ET_WAVES * mj * 32 * ET_PITCH ? ET_STAGES * et_stage(mj) : ET_WAVES * mj * 32 * ET_PITCH;
+}
+static_assert(et_lds(8) <= 160 * 1024 && 2 * et_lds(4) <= 160 * 1024, "one workgroup, or two, of a compute unit");
+
+extern __shared__ __attribute__((aligned(16))) uint8_t et_lds_mem[];
+
+// Position of 16-byte piece p of row R of x in a stage buffer.  A load instruction writes lane l's 16 bytes at 16 l, so
+// it covers eight whole rows; which piece a lane fetches is chosen so that the sixteen consecutive rows that one phase
+// of a ds_read_b128 touches (same p) fall on sixteen distinct 16-byte bank groups.
+__device__ __forceinline__ int et_x_key(int R) { return (R >> 1) & 7; }
+__device__ __forceinline__ int et_x_at(int R, int p) { return (R >> 3) * 1024 + ((R & 7) * 8 + (p ^ et_x_key(R))) * 16; }
+// rows of W are two pieces each: the 32 rows x 2 pieces that a wave reads are one contiguous KB
+__device__ __forceinline__ int et_w_at(int R, int p) { return (R * 2 + p) * 16; }
+
+// The loads are asm so that the compiler neither tracks them (it would wait for all of them before any LDS read) nor moves
+// LDS reads across them; the vmcnt waits are by hand.  M0 carries the wave-uniform LDS address.
+__device__ __forceinline__ void et_dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void et_dma4(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+
+// FMT: 0 W4 symmetric, 1 W4 with zero-points, 2 MXFP4.  GS32: W4 groups of 32 (a lane's 32 k of a stage are one group, the
+// stage two); otherwise gs is a multiple of 64 and a stage lies in one group.  MJ: 32-row tiles of x.
+template <int FMT, bool GS32, bool GATED, int MJ>
+__device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTile& tile) {
+  constexpr bool ASYM = FMT == 1, MX = FMT == 2;
+  constexpr int NI = 2;
+  constexpr int WI = 8 / ET_WAVES, XI = 4 * MJ / ET_WAVES;  // 1 KB load instructions of W and of x per wave and stage
+  constexpr int LOADS = WI + XI + 1 + (ASYM ? 1 : 0);
+  constexpr int CH = NI * MJ / 4;  // chunks of four products per 16-k step
+  constexpr int PPC = (LOADS + 4 * CH - 1) / (4 * CH);  // load instructions of a chunk
+  constexpr int TILE = et_tile(MJ), STAGE = et_stage(MJ);
+  static_assert(2 * LOADS < 64, "a stage's requests fit the counter");
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // in an SGPR: LDS addresses go to M0
+  const int r = lane & 31, h = lane >> 5;
+  const int K = a.v.K, G = MX ? a.v.B : a.v.G, gs = a.v.gs, wg = words(G), pairs = a.tokens * a.top_k;
+  const int R = a.v.N / a.experts, width = GATED ? R / 2 : R;
+  const int c0 = tile.column * (GATED ? 128 : 256);  // first output column
+  // row of the expert that row n of the tile is; columns past the last repeat it and are not stored
+  auto row_of = [&](int n) {
+    if (GATED) return min(c0 + (n >> 6) * 32 + (n & 31), width - 1) + (n & 32 ? width : 0);
+    return min(c0 + n, width - 1);
+  };
+
+  // What this lane fetches (byte offsets of 32 bits from scalar bases; the launcher bounds the operands).
+  const char* const wqb = (const char*)a.v.q + (size_t)tile.expert * R * (K >> 1);
+  const char* const xb = (const char*)(a.from_tokens ? a.x : a.x + (size_t)tile.first * K);
+  uint32_t wo[WI], xo[XI];
+#pragma unroll
+  for (int i = 0; i < WI; ++i)
+    wo[i] = (uint32_t)row_of((wave + ET_WAVES * i) * 32 + (lane >> 1)) * (uint32_t)(K >> 1) + (lane & 1) * 16;
+#pragma unroll
+  for (int i = 0; i < XI; ++i) {
+    const int m = (wave + ET_WAVES * i) * 8 + (lane >> 3), place = min(m, tile.rows - 1);
+    uint32_t from = place;
+    if (a.from_tokens) {
+      const int pair = a.order[tile.first + place];
+      from = pair >= 0 && pair < pairs ? (uint32_t)pair / (uint32_t)a.top_k : 0u;
+    }
+    xo[i] = from * (uint32_t)(K * 2) + (((lane & 7) ^ et_x_key(m)) * 16);
+  }
+  // per stage: the dword that holds the scale(s) of row 64 wave + lane, and (ASYM) the word that holds its zero-point
+  const uint32_t row0 = (uint32_t)tile.expert * (uint32_t)R;
+  const uint32_t sn = row0 + row_of(wave * 64 + lane);
+  const uint32_t sc_base = sn * (uint32_t)G, zw_base = sn * (uint32_t)wg;
+  const int stages = K >> 6;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)et_lds_mem;
+  auto group_of = [&](uint32_t d) { return GS32 ? 2u * d : (d * 64u) / (uint32_t)gs; };  // of the stage's first k (W4)
+  // Load instruction `part` (0 .. LOADS - 1) of stage d into the buffer at byte offset buf.  A stage past the last is
+  // fetched from the last one and never used.
+  auto request_part = [&](int d, uint32_t buf, int part) {
+    const uint32_t dd = (uint32_t)(d < stages ? d : stages - 1);
+    const uint32_t st = lds0 + buf;
+    if (part < WI) {  // the stage's offset goes into the scalar base: no vector arithmetic
+      et_dma16(wqb + dd * 32u, wo[part], st + (wave + ET_WAVES * part) * 1024);
+    } else if (part < WI + XI) {
+      et_dma16(xb + dd * 128u, xo[part - WI], st + ET_W_BYTES + (wave + ET_WAVES * (part - WI)) * 1024);
+    } else if (part == WI + XI) {
+      // MXFP4: the dword around the stage's two E8M0 bytes; gs = 32: the dword of its two scales; else the one around its scale
+      const uint32_t off = MX ? ((sc_base + 2u * dd) & ~3u)
+                              : GS32 ? (sc_base + 2u * dd) * 2u : ((sc_base + group_of(dd)) >> 1) * 4u;
+      et_dma4(a.v.scales, off, st + TILE + wave * 256);
+    } else if (ASYM && part == WI + XI + 1) {
+      et_dma4(a.v.zeros, (zw_base + (group_of(dd) >> 3)) * 4u, st + TILE + 1024 + wave * 256);
+    }
+  };
+
+  // this lane's rows of the two tiles of its wave, and where their first scale sits in the dword fetched around it
+  const int wrow0 = wave * 64 + r;
+  uint32_t par[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) par[i] = ((row0 + row_of(wrow0 + 32 * i)) * (uint32_t)G) & (MX ? 3u : 1u);
+  uint32_t mask = 0x00F0000Fu, magic = 0x54006400u;
+  asm volatile("" : "+s"(mask));   // opaque: otherwise they come back as literals of two
+  asm volatile("" : "+v"(magic));  // separate instructions
+
+  u4 xv[2][MJ];  // operands of x of the step in hand and of the next
+  u4 wv[NI];     // the stage's packed words: word = step
+  u4 av[2][NI];  // expanded operands of the step in hand and of the next
+  uint32_t sc[NI], zw[NI];
+  h2 cneg[NI], s2v[NI];
+  float sf[NI];
+  uint32_t xoff[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) xoff[u] = ET_W_BYTES + et_x_at(r, 4 * h + u);
+  const uint32_t woff = et_w_at(wrow0, h), scoff = TILE + wrow0 * 4;
+  auto read_x = [&](u4* dst, uint32_t buf, int u, int j0, int j1) {
+    const uint8_t* p = et_lds_mem + (buf + xoff[u]);
+#pragma unroll
+    for (int j = j0; j < j1; ++j) dst[j] = *(const u4*)(p + j * 4096);
+  };
+  auto read_w = [&](uint32_t buf) {
+    const uint8_t* p = et_lds_mem + (buf + woff);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) wv[i] = *(const u4*)(p + i * 1024);
+    p = et_lds_mem + (buf + scoff);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      sc[i] = *(const uint32_t*)(p + i * 128);
+      if (ASYM) zw[i] = *(const uint32_t*)(p + 1024 + i * 128);
+    }
+  };
+  auto set_group = [&](int d) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if constexpr (MX) {  // block 2 d + h of the row
+        sf[i] = mx_scale((sc[i] >> (8 * (((par[i] + 2u * d) & 3u) + h))) & 0xFFu);
+      } else {
+        const uint32_t g = group_of((uint32_t)d) + (GS32 ? h : 0);
+        const bool hi = GS32 ? h != 0 : ((par[i] + g) & 1u) != 0;
+        s2v[i] = splat_bits(hi ? (sc[i] >> 16) : (sc[i] & 0xFFFFu));
+        const uint32_t z = ASYM ? ((zw[i] >> (4 * (g & 7))) & 0xFu) : 8u;
+        cneg[i] = as_h2(0xD400E400u | (z << 20) | z);
+      }
+    }
+  };
+  // Phase ph (0 .. 3) of registers q0 .. q0 + n - 1 of the eight (four of each tile) that step u multiplies: byte e to bytes 0
+  // and 2; the low nibble into the significand of 1024.0, the high one into that of 64.0; minus (1024 + z), (64 + z):
+  // exact; times the scale: one rounding.  tmp: the values in between.
+  auto expand_phase = [&](int ph, u4* dst, uint32_t* tmp, int u, int q0, int n) {
+#pragma unroll
+    for (int p = 0; p < n; ++p) {
+      const int i = (q0 + p) >> 2, e = (q0 + p) & 3;
+      const uint32_t w = wv[i][u];
+      if constexpr (MX) {
+        if (ph == (p & 3))
+          dst[i][e] = as_u32(e == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sf[i], 0)
+                             : e == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sf[i], 1)
+                             : e == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sf[i], 2)
+                                      : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sf[i], 3));
+      } else {
+        if (ph == 0) tmp[p] = __builtin_amdgcn_perm(0u, w, 0x0c000c00u | (uint32_t)(e << 16) | (uint32_t)e);
+        if (ph == 1) tmp[p] = (tmp[p] & mask) | magic;
+        if (ph == 2) tmp[p] = as_u32(as_h2(tmp[p]) + cneg[i]);
+        if (ph == 3) dst[i][e] = as_u32(as_h2(tmp[p]) * s2v[i]);
+      }
+    }
+  };
+
+  uint32_t tmp[8];
+  f16v acc[NI][MJ];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  // A stage is 4 CH chunks of four products.  A chunk issues up to PPC load instructions, reads two tiles of x and expands its
+  // share of the next step's registers.  The barrier at the start of step 3 of stage d frees that stage's buffer; the
+  // chunks from there (step 3 of stage d, steps 0 .. 2 of stage d + 1) request stage d + 3 into it.  b0, b1, b2: byte
+  // offsets of the buffers of stages d, d + 1, d + 2 (d + 3 takes b0 again).
+  uint32_t b0 = 0, b1 = STAGE, b2 = 2 * STAGE;
+  constexpr int AHEAD = PPC * CH < LOADS ? PPC * CH : LOADS;
+#pragma unroll
+  for (int part = 0; part < LOADS; ++part) request_part(0, b0, part);
+#pragma unroll
+  for (int part = 0; part < LOADS; ++part) request_part(1, b1, part);
+#pragma unroll
+  for (int part = 0; part < AHEAD; ++part) request_part(2, b2, part);
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS + AHEAD));  // stage 0 has landed
+  __syncthreads();
+  read_x(xv[0], b0, 0, 0, MJ);
+  read_w(b0);
+  set_group(0);
+#pragma unroll
+  for (int ph = 0; ph < 4; ++ph) expand_phase(ph, av[0], tmp, 0, 0, 8);
+  auto mfma1 = [&](int cur, int c, int k) {  // product 4 c + k of a step
+    const int i = (4 * c + k) / MJ, j = (4 * c + k) % MJ;
+    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, av[cur][i]), __builtin_bit_cast(h8, xv[cur][j]),
+                                                       acc[i][j], 0, 0, 0);
+  };
+#pragma unroll 1
+  for (int d = 0; d < stages; ++d) {
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+      const int cur = u & 1, nxt = cur ^ 1;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+#pragma unroll
+        for (int p = 0; p < PPC; ++p)
+          if (PPC * (CH + CH * u + c) + p < LOADS) request_part(d + 2, b2, PPC * (CH + CH * u + c) + p);
+        __builtin_amdgcn_sched_barrier(0);
+        read_x(xv[nxt], b0, u + 1, 2 * c, 2 * c + 2);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          expand_phase(k, av[nxt], tmp, u + 1, 8 * c / CH, 8 * (c + 1) / CH - 8 * c / CH);
+          mfma1(cur, c, k);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    // Step 3.  Every LDS read of stage d has been issued (the operands of x of this step during step 2, the words at the
+    // stage's start): once all waves are here its buffer can take stage d + 3, and stage d + 1 has landed for everyone
+    // (outstanding: all of stage d + 2).
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS));
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+#pragma unroll
+      for (int p = 0; p < PPC; ++p)
+        if (PPC * c + p < LOADS) request_part(d + 3, b0, PPC * c + p);
+      __builtin_amdgcn_sched_barrier(0);
+      if (c == 0) {  // operands of step 0 of stage d + 1: the words, their scales, x
+        read_w(b1);
+        read_x(xv[0], b1, 0, 0, MJ < 4 ? MJ : 4);
+      }
+      if (c == 1) {
+        if constexpr (MJ > 4) read_x(xv[0], b1, 0, 4, MJ);
+        set_group(d + 1);
+      }
+      // the expansion goes under the last chunks: the words have only just been asked for
+      constexpr int FROM = CH >= 2 ? (CH + 1) / 2 : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (CH >= 2 && c >= FROM) expand_phase(k, av[0], tmp, 0, 8 * (c - FROM) / (CH - FROM), 8 / (CH - FROM));
+        mfma1(1, c, k);
+        if (CH >= 2 && c >= FROM) __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (CH == 1) {
+      set_group(d + 1);
+#pragma unroll
+      for (int ph = 0; ph < 4; ++ph) expand_phase(ph, av[0], tmp, 0, 0, 8);
+    }
+    const uint32_t first = b0;
+    b0 = b1;
+    b1 = b2;
+    b2 = first;
+  }
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // nothing may still be writing LDS at exit
+
+  // A lane holds, of each 32 x 32 tile, rows 8 q + 4 h + e of W for row r of x.  The outputs go through LDS (free by now) so
+  // that every store instruction writes whole lines: a wave lays its block out a place a row and reads it back 16 bytes a lane.
+  __syncthreads();  // no wave reads a stage buffer any more, no load is landing in one
+  constexpr int BYTES = GATED ? 64 : 128, PITCH = BYTES + 16, PIECES = BYTES / 16;
+  uint8_t* mine = et_lds_mem + wave * (32 * MJ * PITCH);
+#pragma unroll
+  for (int j = 0; j < MJ; ++j) {
+    // the sums of a tile leave the accumulator registers only when its turn comes (256 of them copied out at once would not
+    // fit beside everything else)
+    if constexpr (MJ > 4) asm volatile("" : "+a"(acc[0][j]), "+a"(acc[1][j]));
+#pragma unroll
+    for (int i = 0; i < (GATED ? 1 : NI); ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        h4 out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y = acc[i][j][4 * q + e];
+          out[e] = (_Float16)(GATED ? expert_act(a.act, y) * acc[1][j][4 * q + e] : y);
+        }
+        *(h4*)(mine + (j * 32 + r) * PITCH + i * 64 + q * 16 + h * 8) = out;
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const int piece = lane % PIECES, col = c0 + wave * (BYTES / 2) + piece * 8, n = min(8, width - col);
+  for (int row = lane / PIECES; row < tile.rows; row += 64 / PIECES) {
+    const int place = tile.first + row;
+    int to = place;
+    if (a.to_pairs) to = a.order[place];
+    const u4 v = *(const u4*)(mine + row * PITCH + piece * 16);
+    if (n <= 0 || to < 0 || to >= pairs || (!a.to_pairs && (uint32_t)a.order[place] >= (uint32_t)pairs)) continue;
+    w4_half* const dst = a.out + (size_t)to * width + col;
+    if (n == 8) {
+      __builtin_memcpy(dst, &v, 16);  // (the card stores 16 bytes to any address)
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < n) dst[e] = (w4_half)(v[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
+// TM: places of a tile at most, 256 (one workgroup a compute unit) or 128 (two).
+template <int FMT, bool GS32, bool GATED, int TM>
+__global__ __launch_bounds__(ET_THREADS, TM == 256 ? 1 : 2) void experts_tile_kernel(ExpertArgs a, int columns) {
+  const ExpertTile tile = find_expert_tile<TM, true, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
+  const int rows = __builtin_amdgcn_readfirstlane(tile.rows);
+  if (rows == 0) return;
+  const ExpertTile u{__builtin_amdgcn_readfirstlane(tile.expert), __builtin_amdgcn_readfirstlane(tile.first), rows,
+                     __builtin_amdgcn_readfirstlane(tile.column)};
+  if constexpr (TM == 256) {
+    if (rows > 192) return experts_tile<FMT, GS32, GATED, 8>(a, u);
+    if (rows > 128) return experts_tile<FMT, GS32, GATED, 6>(a, u);
+  }
+  if (rows > 64) return experts_tile<FMT, GS32, GATED, 4>(a, u);
+  experts_tile<FMT, GS32, GATED, 2>(a, u);
+}
+
+template <int FMT, bool GS32, bool GATED, int TM>
+hipError_t go(const ExpertArgs& a, hipStream_t s) {
+  // more than 64 KB of LDS has to be granted per device, once
+  constexpr int LDS = et_lds(TM / 32);
+  static std::atomic<bool> granted[64] = {};
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+  if (dev < 0 || dev >= 64 || !granted[dev]) {
+    const hipError_t e = hipFuncSetAttribute((const void*)experts_tile_kernel<FMT, GS32, GATED, TM>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return e;
+    if (dev >= 0 && dev < 64) granted[dev] = true;
+  }
+  const int R = a.v.N / a.experts, columns = GATED ? (R / 2 + 127) / 128 : (R + 255) / 256;
+  const long long grid = (most_expert_tiles(a, TM) * columns + 7) / 8 * 8;  // (an eighth of the tiles, rounded up, per XCD)
+  if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  experts_tile_kernel<FMT, GS32, GATED, TM><<<dim3((unsigned)grid), dim3(ET_THREADS), LDS, s>>>(a, columns);
+  return hipGetLastError();
+}
+
+template <int FMT, bool GS32>
+hipError_t go_rows(const ExpertArgs& a, hipStream_t s) {
+  const long long pairs = (long long)a.tokens * a.top_k;
+  const bool wide = pairs >= 160LL * a.experts;
+  if (a.act) return wide ? go<FMT, GS32, true, 256>(a, s) : go<FMT, GS32, true, 128>(a, s);
+  return wide ? go<FMT, GS32, false, 256>(a, s) : go<FMT, GS32, false, 128>(a, s);
+}
+
+}  // namespace
+
+bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
+  const WView& v = a.v;
+  const long long G = v.mx ? v.B : v.G, pairs = (long long)a.tokens * a.top_k;
+  if (v.K % 64 || (!v.mx && v.gs != 32 && v.gs % 64)) return false;
+  // the dword around a scale lies inside the array
+  if ((v.mx && v.N * G % 4) || (!v.mx && v.gs != 32 && v.N * G % 2)) return false;
+  // offsets of 32 bits: codes of an expert, scales of all, rows of x (of a tile, or of all tokens)
+  if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32 || v.N * G * 4 >= 1LL << 32) return false;
+  if (v.K >= 1 << 23 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
+  if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
+  if (pairs < 8LL * a.experts) return false;
+  if (v.mx) *err = go_rows<2, false>(a, s);
+  else if (v.symmetric) *err = v.gs == 32 ? go_rows<0, true>(a, s) : go_rows<0, false>(a, s);
+  else *err = v.gs == 32 ? go_rows<1, true>(a, s) : go_rows<1, false>(a, s);
+  return true;
+}
+
+}  // namespace w4k
