@@ -382,7 +382,7 @@ bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32 || v.N * G * 4 >= 1LL << 32) return false;
   if (v.K >= 1 << 23 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
-  if (pairs < 8LL * a.experts) return false;
+  if (pairs < 32LL * a.experts) return false;
   if (v.mx) *err = go_rows<2, false>(a, s);
   else if (v.symmetric) *err = v.gs == 32 ? go_rows<0, true>(a, s) : go_rows<0, false>(a, s);
   else *err = v.gs == 32 ? go_rows<1, true>(a, s) : go_rows<1, false>(a, s);
