@@ -1,62 +1,53 @@
 // Products of a few rows per expert with the experts' packed matrices: decode steps, whose time is the reading of codes.
 //
-// A workgroup multiplies up to 16 MT places of one expert with 32 of its rows (gated: 16 of the gate and the 16 of the way
-// up for the same columns).  Its four waves share K out in chunks of 128; a wave asks for all codes, scales and rows of x of four
-// chunks at once and waits for no other wave before the end, where the four sums are added in the waves' order.
+// A wave multiplies up to 16 MT places of one expert with 32 of its rows (gated: 16 of the gate and the 16 of the way up for
+// the same columns), over all of K or one of `parts` shares of it.  It walks K in chunks of 128 k and asks for the codes
+// and the rows of x of a chunk three chunks ahead; scales and zero-points come for four chunks at a time.
 // v_mfma_f32_16x16x32_f16: lane l brings row l % 16 and eight consecutive k; of a chunk it has k 32 (l / 16) .. + 31, so that
 // its codes are one 16-byte load and lie in one group of 32 or more, and its part of a row of x is 64 bytes side by side.
+// Rows of x that are not there are asked for past the end of a buffer: the card returns zeros and fetches nothing.
 #include "experts.cuh"
 
 namespace w4k {
 namespace {
 
 constexpr int EF_WAVES = 4;
+constexpr uint32_t EF_NOWHERE = 0xF0000000u;  // past every buffer, with room for the offsets added to it
 
-template <int FMT, bool GATED, int MT>
-__global__ __launch_bounds__(64 * EF_WAVES) void experts_few_kernel(ExpertArgs a, int columns) {
-  constexpr bool MX = FMT == 2;
-  constexpr int U = 4 / MT;  // chunks asked for at once
-  __shared__ float sums[EF_WAVES][2][MT][4][64];
+typedef __amdgpu_buffer_rsrc_t rsrc;
+__device__ __forceinline__ rsrc ef_buffer(const void* p, size_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(bytes < 0xE0000000u ? bytes : 0xE0000000u), 0x00020000);
+}
+__device__ __forceinline__ u4 ef_load(rsrc b, uint32_t off, uint32_t scalar) {
+  return __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(b, off, scalar, 0));
+}
+
+// How the groups of W4 lie in a chunk (GM): 0 one (gs 128), 1 two, 2 four (gs 32, and MXFP4's blocks), 3 any gs that is a
+// multiple of 32.  Parameters of four chunks of a row: so many dwords, which begin at any half (MXFP4: byte).
+constexpr int ef_params(int fmt, int gm) { return fmt == 2 ? 4 : gm == 0 ? 2 : gm == 2 ? 8 : 4; }
+
+template <int FMT, bool GATED, int GM, int MT>
+__global__ __launch_bounds__(64 * EF_WAVES) void experts_few_kernel(ExpertArgs a, int columns, int parts, uint32_t group_mul) {
+  constexpr bool MX = FMT == 2, ASYM = FMT == 1;
+  constexpr int S = MT == 1 ? 4 : 2;  // chunks in registers
+  constexpr int NP = ef_params(FMT, GM), NZ = !ASYM ? 0 : GM == 3 ? 4 : GM == 2 ? 2 : 1;
+  constexpr int COLS = GATED ? 16 : 32;  // output columns of a wave
+  __shared__ float sums[EF_WAVES][2 * MT * 4][64];
   const int pairs = a.tokens * a.top_k;
   const ExpertTile tile = find_expert_tile<16 * MT, false, true>(a.offsets, a.experts, pairs, columns, blockIdx.x);
   const int rows = __builtin_amdgcn_readfirstlane(tile.rows);
   if (rows == 0) return;
   const int expert = __builtin_amdgcn_readfirstlane(tile.expert), first = __builtin_amdgcn_readfirstlane(tile.first);
-  const int c0 = __builtin_amdgcn_readfirstlane(tile.column) * (GATED ? 16 : 32);
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int K = a.v.K, G = MX ? a.v.B : a.v.G, gs = a.v.gs;
+  const int K = a.v.K, G = MX ? a.v.B : a.v.G, wg = words(G);
   const int R = a.v.N / a.experts, width = GATED ? R / 2 : R;
-  const int chunks = (K + 127) >> 7, per = (chunks + EF_WAVES - 1) / EF_WAVES;
-  const int c_end = min(chunks, (wave + 1) * per);
-
-  // this lane's rows of W (columns past the last repeat it and are not stored)
-  const char* const codes = (const char*)a.v.q + (size_t)expert * R * (K >> 1);
-  uint32_t wo[2];
-  size_t so[2], zo[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = GATED ? min(c0 + r, width - 1) + i * width : min(c0 + 16 * i + r, width - 1);
-    wo[i] = (uint32_t)row * (uint32_t)(K >> 1);
-    so[i] = ((size_t)expert * R + row) * G;
-    zo[i] = ((size_t)expert * R + row) * words(G);
-  }
-  const w4_half* xr[MT];
-  bool there[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int place = first + min(16 * m + r, rows - 1);
-    int from = place;
-    if (a.from_tokens) {
-      const int pair = a.order[place];
-      from = pair >= 0 && pair < pairs ? (uint32_t)pair / (uint32_t)a.top_k : 0;
-    }
-    there[m] = 16 * m + r < rows;
-    xr[m] = a.x + (size_t)from * K + 32 * q;
-  }
-  uint32_t mask = 0x00F0000Fu, magic = 0x54006400u;
-  asm volatile("" : "+s"(mask));   // opaque: otherwise they come back as literals of two
-  asm volatile("" : "+v"(magic));  // separate instructions
+  const int part = wave & (parts - 1);
+  const int c0 = (__builtin_amdgcn_readfirstlane(tile.column) * (EF_WAVES / parts) + wave / parts) * COLS;
+  const int chunks = (K + 127) >> 7;
+  // (four chunks of 32-groups take two whole words of zero-points from even chunks on)
+  const int per = GM == 2 ? ((chunks + parts - 1) / parts + 1) & ~1 : (chunks + parts - 1) / parts;
+  const int c_begin = part * per, c_end = min(chunks, c_begin + per);
 
   f4 acc[2][MT];
 #pragma unroll
@@ -64,104 +55,233 @@ __global__ __launch_bounds__(64 * EF_WAVES) void experts_few_kernel(ExpertArgs a
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[i][m] = f4{0.f, 0.f, 0.f, 0.f};
 
-  for (int cb = wave * per; cb < c_end; cb += U) {
-    u4 w[U][2], xv[U][MT][4];
-    uint32_t sc[U][2], z[U][2];
+  if (c0 < width && c_begin < c_end) {
+    // this lane's rows of W (columns past the last repeat it and are not stored)
+    const rsrc codes = ef_buffer((const char*)a.v.q + (size_t)expert * R * (K >> 1), (size_t)R * (K >> 1));
+    const char* const scales = (const char*)a.v.scales + (size_t)expert * R * G * (MX ? 1 : 2);
+    const uint32_t* const zeros = a.v.zeros + (size_t)expert * R * wg;
+    // entries of the arrays from this expert on
+    const size_t left = (size_t)(a.v.N - expert * R);
+    const uint32_t sc_end = left * G < 0xFFFFFF00u ? (uint32_t)(left * G) : 0xFFFFFF00u;
+    const uint32_t zw_last = left * wg < 0xFFFFFF00u ? (uint32_t)(left * wg) - 1 : 0xFFFFFF00u;
+    uint32_t wo[2], so[2], zo[2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      // (a slice of 32 k behind the end of K, or a chunk behind the wave's last: fetched from the row's start, times 0)
-      const int k = (cb + u) * 128 + 32 * q;
-      const bool inside = cb + u < c_end && k < K;
-      const int kk = inside ? k : 0;
+    for (int i = 0; i < 2; ++i) {
+      const int row = GATED ? min(c0 + r, width - 1) + i * width : min(c0 + 16 * i + r, width - 1);
+      wo[i] = (uint32_t)row * (uint32_t)(K >> 1) + 16 * q;
+      so[i] = (uint32_t)row * (uint32_t)G;
+      zo[i] = (uint32_t)row * (uint32_t)wg;
+    }
+    const rsrc xb = a.from_tokens ? ef_buffer(a.x, (size_t)a.tokens * K * 2) : ef_buffer(a.x + (size_t)first * K, (size_t)rows * K * 2);
+    uint32_t xo[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int place = 16 * m + r;
+      xo[m] = EF_NOWHERE;
+      if (place < rows) {
+        uint32_t from = place;
+        if (a.from_tokens) {
+          const int pair = a.order[first + place];
+          from = pair >= 0 && pair < pairs ? (uint32_t)pair / (uint32_t)a.top_k : 0;
+        }
+        xo[m] = from * (uint32_t)(K * 2) + 64 * q;
+      }
+    }
+    uint32_t mask = 0x00F0000Fu, magic = 0x54006400u;
+    asm volatile("" : "+s"(mask));   // opaque: otherwise they come back as literals of two
+    asm volatile("" : "+v"(magic));  // separate instructions
+
+    // Parameters of the four chunks from c on.
+    struct Params {
+      uint32_t p[NP], z[NZ + 1];
+    };
+    auto params = [&](Params (&out)[2], int c) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        w[u][i] = *(const u4*)(codes + (wo[i] + (kk >> 1)));
-        if constexpr (MX) {
-          sc[u][i] = ((const uint8_t*)a.v.scales)[so[i] + (kk >> 5)];
+        if constexpr (GM == 3 && !MX) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t g = min(__umulhi(2u * (4 * (c + e) + q), group_mul), (uint32_t)G - 1);
+            out[i].p[e] = *(const uint16_t*)(scales + 2 * (so[i] + g));
+            if (ASYM) out[i].z[e] = zeros[zo[i] + (g >> 3)] >> (4 * (g & 7));
+          }
         } else {
-          const int g = kk / gs;
-          sc[u][i] = ((const uint16_t*)a.v.scales)[so[i] + g];
-          z[u][i] = FMT == 1 ? a.v.zeros[zo[i] + (g >> 3)] >> (4 * (g & 7)) & 0xFu : 8u;
+          const uint32_t g = (MX ? 4u : 1u << GM) * c, at = so[i] + g;
+          constexpr uint32_t N = MX ? 16 : 2 * NP;
+          if (__any(at + N > sc_end)) {  // the end of the array: one by one
+#pragma unroll
+            for (uint32_t e = 0; e < N; ++e) {
+              const uint32_t j = min(at + e, sc_end - 1);
+              if (MX) out[i].p[e >> 2] = (e & 3 ? out[i].p[e >> 2] : 0u) | (uint32_t)((const uint8_t*)scales)[j] << (8 * (e & 3));
+              else out[i].p[e >> 1] = (e & 1 ? out[i].p[e >> 1] : 0u) | (uint32_t)((const uint16_t*)scales)[j] << (16 * (e & 1));
+            }
+          } else {
+            __builtin_memcpy(out[i].p, scales + (size_t)at * (MX ? 1 : 2), 4 * NP);
+          }
+          if constexpr (ASYM && GM == 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) out[i].z[e] = zeros[min(zo[i] + (g >> 3) + e, zw_last)];
+          } else if constexpr (ASYM) {
+            const uint32_t lo = zeros[min(zo[i] + (g >> 3), zw_last)], hi = zeros[min(zo[i] + (g >> 3) + 1, zw_last)];
+            out[i].z[0] = __builtin_amdgcn_alignbit(hi, lo, 4 * (g & 7));
+          }
         }
       }
+    };
+    u4 w[S][2], xv[S][MT][4];
+    auto request = [&](int s, int c) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int i = 0; i < 2; ++i) w[s][i] = ef_load(codes, wo[i], c * 64);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          xv[u][m][j] = u4{0u, 0u, 0u, 0u};
-          if (there[m] && inside) xv[u][m][j] = *(const u4*)(xr[m] + (cb + u) * 128 + 8 * j);
+      for (int m = 0; m < MT; ++m) {
+        // (behind the end of K: nowhere)
+        const uint32_t off = c * 128 + 128 > K && c * 128 + 32 * q >= K ? EF_NOWHERE : xo[m];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) xv[s][m][j] = ef_load(xb, off + 16 * j, c * 256);
+      }
+    };
+    const uint32_t sel = GM == 1 ? (q >> 1 ? 0x03020302u : 0x01000100u) : 0x01000100u + 0x02020202u * q;
+    const uint32_t zsh = GM == 1 ? 4 * (q >> 1) : GM == 2 ? 4 * q : 0;
+    auto multiply = [&](int s, const Params (&pp)[2], int ci, int c) {
+      const bool past = c * 128 + 128 > K && c * 128 + 32 * q >= K;  // what was fetched there counts as 0
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Params& p = pp[i];
+        h2 s2{}, cneg{};
+        float sf = 0.f;
+        if constexpr (MX) {
+          sf = mx_scale(p.p[ci] >> (8 * q) & 0xFFu);
+          if (past) sf = 0.f;
+        } else {
+          uint32_t v = GM == 0   ? __builtin_amdgcn_perm(0u, p.p[ci >> 1], ci & 1 ? 0x03020302u : 0x01000100u)
+                       : GM == 1 ? __builtin_amdgcn_perm(0u, p.p[ci], sel)
+                       : GM == 2 ? __builtin_amdgcn_perm(p.p[2 * ci + 1], p.p[2 * ci], sel)
+                                 : __builtin_amdgcn_perm(0u, p.p[ci], 0x01000100u);
+          if (past) v = 0u;
+          s2 = as_h2(v);
+          const uint32_t z = !ASYM     ? 8u
+                             : GM == 0 ? p.z[0] >> (4 * ci) & 0xFu
+                             : GM == 1 ? p.z[0] >> (8 * ci + zsh) & 0xFu
+                             : GM == 2 ? p.z[ci >> 1] >> (16 * (ci & 1) + zsh) & 0xFu
+                                       : p.z[ci] & 0xFu;
+          cneg = as_h2(0xD400E400u + z * 0x00100001u);
         }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           h8 av;
           if constexpr (MX) {
             h2 n[4];
-            dq_mx(w[u][i][j], mx_scale(sc[u][i]), n);
+            dq_mx(w[s][i][j], sf, n);
             av = __builtin_bit_cast(h8, u4{as_u32(n[0]), as_u32(n[1]), as_u32(n[2]), as_u32(n[3])});
           } else {
-            av = expand_word(w[u][i][j], as_h2(0xD400E400u | (z[u][i] << 20) | z[u][i]), splat_bits(sc[u][i]), mask, magic);
+            av = expand_word(w[s][i][j], cneg, s2, mask, magic);
           }
 #pragma unroll
           for (int m = 0; m < MT; ++m)
-            acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(h8, xv[u][m][j]), acc[i][m], 0, 0, 0);
+            acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(h8, xv[s][m][j]), acc[i][m], 0, 0, 0);
         }
-  }
+      }
+    };
+    // A chunk past the wave's last is fetched from the last one and not multiplied.
+    Params now[2], next[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int s = 0; s < S - 1; ++s) request(s, min(c_begin + s, c_end - 1));
+    params(now, c_begin);
+    for (int cb = c_begin; cb < c_end; cb += 4) {
+      if (cb + 4 < c_end) params(next, cb + 4);
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+      for (int ci = 0; ci < 4; ++ci) {
+        if (cb + ci >= c_end) break;
+        request((ci + S - 1) % S, min(cb + ci + S - 1, c_end - 1));
+        multiply(ci % S, now, ci, cb + ci);
+      }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[wave][i][m][e][lane] = acc[i][m][e];
-  __syncthreads();
-  // lane l of a 16 x 16 tile holds columns 4 (l / 16) + e of place l % 16
-  constexpr int COLS = GATED ? 16 : 32;
-  for (int o = t; o < COLS * 16 * MT; o += 64 * EF_WAVES) {
-    const int col = o % COLS, m = o / COLS;  // column and place of the tile
-    if (m >= rows || c0 + col >= width) continue;
-    const int e = col & 3, l = (col >> 2 & 3) * 16 + (m & 15), i = GATED ? 0 : col >> 4;
-    float y = 0.f, up = 0.f;
-#pragma unroll
-    for (int w = 0; w < EF_WAVES; ++w) {
-      y += sums[w][i][m >> 4][e][l];
-      if (GATED) up += sums[w][1][m >> 4][e][l];
+      for (int i = 0; i < 2; ++i) now[i] = next[i];
     }
-    if (GATED) y = expert_act(a.act, y) * up;
-    const int pair = a.order[first + m];
+  }
+  if (parts > 1) {  // the shares of K are added in their order
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[wave][(i * MT + m) * 4 + e][lane] = acc[i][m][e];
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          for (int w = 1; w < parts; ++w) acc[i][m][e] += sums[wave + w][(i * MT + m) * 4 + e][lane];
+  }
+  // lane l of a 16 x 16 tile holds columns 4 (l / 16) + e of place l % 16
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int place = first + 16 * m + r;
+    if (16 * m + r >= rows) continue;
+    const int pair = a.order[place];
     if (pair < 0 || pair >= pairs) continue;
-    a.out[(size_t)(a.to_pairs ? pair : first + m) * width + c0 + col] = __builtin_bit_cast(uint16_t, (_Float16)y);
+    w4_half* const out = a.out + (size_t)(a.to_pairs ? pair : place) * width;
+#pragma unroll
+    for (int i = 0; i < (GATED ? 1 : 2); ++i) {
+      const int col = c0 + 16 * i + 4 * q;
+      h4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = (_Float16)(GATED ? expert_act(a.act, acc[0][m][e]) * acc[1][m][e] : acc[i][m][e]);
+      if (col + 4 <= width) {
+        __builtin_memcpy(out + col, &y, 8);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < width) out[col + e] = __builtin_bit_cast(uint16_t, (_Float16)y[e]);
+      }
+    }
   }
 }
 
-template <int FMT, bool GATED, int MT>
+template <int FMT, bool GATED, int GM, int MT>
 hipError_t go(const ExpertArgs& a, hipStream_t s) {
-  const int R = a.v.N / a.experts, columns = GATED ? (R / 2 + 15) / 16 : (R + 31) / 32;
-  const long long grid = (most_expert_tiles(a, 16 * MT) * columns + 7) / 8 * 8;
+  const int R = a.v.N / a.experts, tiles = GATED ? (R / 2 + 15) / 16 : (R + 31) / 32;
+  const long long pairs = (long long)a.tokens * a.top_k, most = most_expert_tiles(a, 16 * MT);
+  const long long waves = (pairs < a.experts ? pairs : a.experts) * tiles;
+  const int parts = waves >= 3000 ? 1 : waves >= 1500 ? 2 : 4;
+  const int columns = (tiles + EF_WAVES / parts - 1) / (EF_WAVES / parts);
+  const long long grid = (most * columns + 7) / 8 * 8;
   if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-  experts_few_kernel<FMT, GATED, MT><<<dim3((unsigned)grid), dim3(64 * EF_WAVES), 0, s>>>(a, columns);
+  // the group of slice n of 32 k is (2 n group_mul) >> 32
+  const uint32_t d = a.v.mx ? 1 : a.v.gs / 32, mul = (uint32_t)(((1ull << 31) + d - 1) / d);
+  experts_few_kernel<FMT, GATED, GM, MT><<<dim3((unsigned)grid), dim3(64 * EF_WAVES), 0, s>>>(a, columns, parts, mul);
   return hipGetLastError();
 }
 
-template <int FMT>
+template <int FMT, int GM>
 hipError_t go_rows(const ExpertArgs& a, hipStream_t s) {
   const long long pairs = (long long)a.tokens * a.top_k;
   const bool two = pairs >= 12LL * a.experts;
-  if (a.act) return two ? go<FMT, true, 2>(a, s) : go<FMT, true, 1>(a, s);
-  return two ? go<FMT, false, 2>(a, s) : go<FMT, false, 1>(a, s);
+  if (a.act) return two ? go<FMT, true, GM, 2>(a, s) : go<FMT, true, GM, 1>(a, s);
+  return two ? go<FMT, false, GM, 2>(a, s) : go<FMT, false, GM, 1>(a, s);
+}
+
+template <int FMT>
+hipError_t go_groups(const ExpertArgs& a, hipStream_t s) {
+  if (a.v.gs == 128) return go_rows<FMT, 0>(a, s);
+  if (a.v.gs == 64) return go_rows<FMT, 1>(a, s);
+  if (a.v.gs == 32) return go_rows<FMT, 2>(a, s);
+  return go_rows<FMT, 3>(a, s);
 }
 
 }  // namespace
 
 bool try_experts_few(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   const WView& v = a.v;
-  if (v.K % 32 || (!v.mx && v.gs % 32)) return false;
-  if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32) return false;  // offsets of 32 bits into an expert's codes
+  if (v.K % 32 || (!v.mx && v.gs % 32) || v.K >= 1 << 20) return false;
+  // offsets of 32 bits: an expert's codes and parameters, rows of x
+  const long long R = v.N / a.experts;
+  if (R * v.K / 2 >= 0xE0000000LL || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 0xE0000000LL)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 1) || ((uintptr_t)v.zeros & 3)) return false;
-  *err = v.mx ? go_rows<2>(a, s) : v.symmetric ? go_rows<0>(a, s) : go_rows<1>(a, s);
+  *err = v.mx ? go_rows<2, 2>(a, s) : v.symmetric ? go_groups<0>(a, s) : go_groups<1>(a, s);
   return true;
 }
 
