@@ -74,7 +74,8 @@ def test_sizes(T, E, k):
 @pytest.mark.parametrize("sigmoid", [False, True])
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("E,groups,top_groups,best", [(16, 4, 2, 2), (64, 8, 3, 1), (160, 8, 3, 2), (256, 8, 4, 2), (256, 8, 8, 2),
-                                                     (64, 64, 9, 2), (96, 3, 1, 2), (1024, 64, 16, 2), (24, 1, 1, 1), (250, 2, 1, 2)])
+                                                     (64, 64, 9, 2), (96, 3, 1, 2), (1024, 64, 16, 2), (24, 1, 1, 1), (250, 2, 1, 2), (1023, 33, 7, 2), (1020, 60, 9, 1),
+                                                     (204, 17, 4, 2), (63, 21, 5, 2), (1000, 8, 3, 2)])
 def test_groups_and_bias(E, groups, top_groups, best, bias, sigmoid):
     rng = np.random.default_rng(E + groups)
     b = (0.2 * rng.normal(size=E)).astype(np.float32) if bias else None

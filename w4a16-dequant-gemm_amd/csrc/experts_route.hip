@@ -1,251 +1,435 @@
 // Routing of tokens to experts: scores, choice, weights, and the pairs sorted by expert (w4_route_experts).
 //
-// Two launches.  The first has a workgroup for a block of tokens, a wave for a token: it chooses experts and counts
-// how often the block chose each.  The second sorts: a block's pairs of expert e begin where all pairs of the
-// experts before e end, plus what the blocks before it have of e; inside the block they follow by token, and since a token
-// chooses an expert once, a pair's place among 64 tokens is the number of bits below its token's in the set of
-// those that chose e.  Nothing in it depends on which workgroup comes first.
+// A token belongs to LANES lanes of a wave, each with NE experts side by side, so a wave routes 64 / LANES tokens at once and the
+// choice is k rounds of: the largest of a lane, of the token's lanes (DPP), the lowest expert that has it, out with it.  What
+// is compared are the logits themselves where neither a bias nor groups take part; else scores plus bias in 64 bits,
+// whose arithmetic runs at the rate of 32 bits on this card, so no choice hangs on a rounding.
+//
+// Sorting: a block's pairs of expert e begin where all pairs of the experts before e end, plus what the blocks before
+// it have of e; inside the block they follow by token, and since a token chooses an expert once, a pair's place among 64
+// tokens is the number of bits below its token's in the set of those that chose e.  Nothing in it depends on which
+// workgroup comes first.  Up to 64 tokens one workgroup does both; else the first launch leaves how often each block of
+// tokens chose each expert, and the workgroups of the second sum all blocks' counts, each for itself.
+#include <algorithm>
+#include <type_traits>
+
 #include "dq.cuh"
 #include "kernels.h"
 
 namespace w4k {
 namespace {
 
-constexpr int RT_THREADS = 256, RT_WAVES = RT_THREADS / 64;
-constexpr int RT_MAX_E = 1024;
-constexpr int RT_MAX_BLOCKS = 1024;  // of tokens: a sorting block reads all blocks' counts
+constexpr int RT_MAX_E = 1024, RT_MAX_K = 32;
+constexpr int RT_THREADS = 256;      // of a block of many
+constexpr int RT_ONE = 64;           // tokens up to which one workgroup does all
+constexpr int RT_MAX_BLOCKS = 1024;  // a sorting workgroup reads all blocks' counts
 
-int route_block(int tokens) {  // tokens of a block, a multiple of 64
-  const int units = (tokens + 63) / 64;
-  return 64 * ((units + RT_MAX_BLOCKS - 1) / RT_MAX_BLOCKS);
+// ---- reductions over the lanes of a token ------------------------------------------------
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
-
-// The larger of two choices (c, index): of equals, the lower index.
-__device__ __forceinline__ bool ahead(double c, int i, double d, int j) { return c > d || (c == d && i < j); }
-
-__device__ __forceinline__ void wave_best(double& c, int& i) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const double d = __shfl_xor(c, o);
-    const int j = __shfl_xor(i, o);
-    if (ahead(d, j, c, i)) c = d, i = j;
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)dpp<CTRL>((int)(uint32_t)u), hi = (uint32_t)dpp<CTRL>((int)(u >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// f over all LANES lanes (a power of two), in every one of them; f does not care about order
+template <int LANES, class T, class F>
+__device__ __forceinline__ T lanes_all(T v, F f) {
+  if constexpr (LANES > 1) v = f(v, dpp<0xB1>(v));    // quad_perm [1,0,3,2]
+  if constexpr (LANES > 2) v = f(v, dpp<0x4E>(v));    // quad_perm [2,3,0,1]
+  if constexpr (LANES > 4) v = f(v, dpp<0x141>(v));   // row_half_mirror
+  if constexpr (LANES > 8) v = f(v, dpp<0x140>(v));   // row_mirror
+  if constexpr (LANES > 16) v = f(v, __shfl_xor(v, 16));
+  if constexpr (LANES > 32) v = f(v, __shfl_xor(v, 32));
+  return v;
+}
+struct Most {
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const {
+    if constexpr (std::is_same_v<T, int>) return a > b ? a : b;
+    else if constexpr (std::is_same_v<T, float>) return fmaxf(a, b);
+    else return fmax(a, b);
   }
-}
+};
+struct Least {
+  __device__ __forceinline__ int operator()(int a, int b) const { return a < b ? a : b; }
+};
+// (each lane's sum is of two sums in one order: a + b and b + a are the same number)
+struct Sum {
+  template <class T>
+  __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
 
-// Lane l has experts l, l + 64 ...; a lane of NE of them.  c of an expert that is not to be chosen is -inf.
-template <int NE>
-__global__ __launch_bounds__(RT_THREADS) void route_kernel(RouteArgs a, int block, uint16_t* __restrict__ counts) {
-  __shared__ int count_lds[RT_MAX_E];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int E = a.r.experts, k = a.r.top_k;
-  const int per = E / a.r.groups;
-  for (int e = t; e < E; e += RT_THREADS) count_lds[e] = 0;
-  __syncthreads();
-  const int there = a.count ? min(*a.count, a.tokens) : a.tokens;
-  const long long first = (long long)blockIdx.x * block;
-  const int end = (int)min((long long)a.tokens, first + block);
-  for (int tok = (int)first + wave; tok < end; tok += RT_WAVES) {
-    int* const ids = a.experts + (long long)tok * k;
-    float* const ws = a.weights + (long long)tok * k;
-    if (tok >= there) {
-      if (lane < k) ids[lane] = -1, ws[lane] = 0.f;
-      continue;
-    }
-    double c[NE];
-    float l[NE], top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = lane + 64 * i;
-      l[i] = -INFINITY;
-      if (e < E) {
-        const long long at = (long long)tok * a.stride + e;
-        const float raw = a.f32 ? ((const float*)a.logits)[at] : (float)((const _Float16*)a.logits)[at];
-        l[i] = raw != raw ? -INFINITY : fminf(raw, a.f32 ? 3.4028234663852886e38f : 65504.f);
-      }
-      top = fmaxf(top, l[i]);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const bool exact = a.r.bias || a.r.groups > 1;
-    float total = 0.f;  // of e^(l - top)
-    double total_d = 0.0;
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const bool has = l[i] > -INFINITY;
-      c[i] = l[i];
-      if (a.r.score == 0) {
-        total += has ? expf(l[i] - top) : 0.f;
-        if (exact && has) c[i] = exp((double)l[i] - (double)top), total_d += c[i];
-      } else if (exact && has) {
-        c[i] = 1.0 / (1.0 + exp(-(double)l[i]));
-      }
-    }
-    if (a.r.score == 0) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o), total_d += __shfl_xor(total_d, o);
-    }
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const int e = lane + 64 * i;
-      if (a.r.score == 0 && exact && c[i] > -INFINITY) c[i] /= total_d;
-      if (a.r.bias && e < E && c[i] > -INFINITY) c[i] += (double)a.r.bias[e];
-      if (!(c[i] > -INFINITY)) c[i] = -INFINITY;
-    }
-    if (a.r.groups > 1) {
-      // every group's value by its best two, group g's held by lane g; then the groups that stay
-      double mine = -INFINITY;
-      for (int g = 0; g < a.r.groups; ++g) {
-        double sum = -INFINITY;
-        int skip = -1;
-        for (int n = 0; n < a.r.group_best; ++n) {
-          double b = -INFINITY;
-          int at = E;
-#pragma unroll
-          for (int i = 0; i < NE; ++i) {
-            const int e = lane + 64 * i;
-            if (e < E && e / per == g && e != skip && ahead(c[i], e, b, at)) b = c[i], at = e;
-          }
-          wave_best(b, at);
-          if (b > -INFINITY) sum = n == 0 ? b : sum + b;
-          skip = at;
-        }
-        if (lane == g) mine = sum;
-      }
-      unsigned long long kept = 0;
-      for (int n = 0; n < a.r.top_groups; ++n) {
-        double b = kept >> lane & 1 ? -INFINITY : mine;
-        int at = lane;
-        wave_best(b, at);
-        if (b > -INFINITY) kept |= 1ull << at;
-      }
-#pragma unroll
-      for (int i = 0; i < NE; ++i) {
-        const int e = lane + 64 * i;
-        if (e < E && !(kept >> (e / per) & 1)) c[i] = -INFINITY;
-      }
-    }
-    // lane j keeps the j-th choice and its logit
-    int id = -1;
-    float lj = -INFINITY;
-    for (int j = 0; j < k; ++j) {
-      double b = -INFINITY;
-      int at = E;
-#pragma unroll
-      for (int i = 0; i < NE; ++i)
-        if (ahead(c[i], lane + 64 * i, b, at)) b = c[i], at = lane + 64 * i;
-      wave_best(b, at);
-      if (!(b > -INFINITY)) break;
-      float v = 0.f;
-#pragma unroll
-      for (int i = 0; i < NE; ++i)
-        if (lane + 64 * i == at) v = l[i], c[i] = -INFINITY;
-      v = __shfl(v, at & 63);
-      if (lane == j) id = at, lj = v;
-    }
-    // Weights that are divided by their sum are taken relative to the largest chosen score: however far below
-    // the row's others the chosen ones lie (a bias may choose them), their ratios are kept.
-    float most = lj;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
-    float w = 0.f;
-    if (a.r.score == 0) {
-      if (id >= 0) w = a.r.renorm ? expf(lj - most) : expf(lj - top) / total;
-    } else if (id >= 0) {  // e^min(l, 0) / (1 + e^-|l|)
-      w = expf(fminf(lj, 0.f) - (a.r.renorm ? fminf(most, 0.f) : 0.f)) / (1.f + expf(-fabsf(lj)));
-    }
-    if (a.r.renorm) {
-      float sum = w;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-      w = id >= 0 ? w / sum : 0.f;
-    }
-    if (lane < k) {
-      ids[lane] = id;
-      ws[lane] = w * a.r.scale;
-      if (id >= 0) atomicAdd(&count_lds[id], 1);
-    }
-  }
-  __syncthreads();
-  for (int e = t; e < E; e += RT_THREADS) counts[(size_t)blockIdx.x * E + e] = (uint16_t)count_lds[e];
-}
+// ---- sorting ------------------------------------------------------------------------------------
 
-constexpr int SORT_THREADS = 1024;
+struct SortSpace {
+  int base[RT_MAX_E];                  // where an expert's next pair goes
+  unsigned long long chose[RT_MAX_E];  // tokens of 64 that chose it
+  int wave_sum[16];
+};
 
-__global__ __launch_bounds__(SORT_THREADS) void route_sort_kernel(RouteArgs a, int block, int blocks,
-                                                                  const uint16_t* __restrict__ counts) {
-  __shared__ int base[RT_MAX_E];                   // where the block's next pair of an expert goes
-  __shared__ unsigned long long chose[RT_MAX_E];   // tokens of 64 that chose it
-  __shared__ int wave_sum[SORT_THREADS / 64];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int E = a.r.experts, k = a.r.top_k;
-  int before = 0, total = 0;
-  if (t < E)
-    for (int b = 0; b < blocks; ++b) {
-      const int n = counts[(size_t)b * E + t];
-      if (b < (int)blockIdx.x) before += n;
-      total += n;
-    }
-  int run = total;  // sums over the experts up to this one
+// base[e] = pairs of the experts before e + before[e] (null: none), from every expert's total.  Returns all pairs.
+__device__ __forceinline__ int sort_bases(SortSpace& s, int E, const int* total, const int* before, int* offsets) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, waves = blockDim.x >> 6;
+  const int per = (E + blockDim.x - 1) / blockDim.x, e0 = t * per;  // experts of a thread, side by side
+  int mine = 0;
+  for (int i = 0; i < per; ++i) mine += e0 + i < E ? total[e0 + i] : 0;
+  int run = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int v = __shfl_up(run, o);
     if (lane >= o) run += v;
   }
-  if (lane == 63) wave_sum[wave] = run;
+  if (lane == 63) s.wave_sum[wave] = run;
   __syncthreads();
   int all = 0;
-  for (int w = 0; w < SORT_THREADS / 64; ++w) {
-    if (w < wave) run += wave_sum[w];
-    all += wave_sum[w];
+  run -= mine;
+  for (int w = 0; w < waves; ++w) {
+    if (w < wave) run += s.wave_sum[w];
+    all += s.wave_sum[w];
   }
-  if (t < E) {
-    base[t] = run - total + before;
-    if (blockIdx.x == 0) a.offsets[t] = run - total;
+  for (int e = e0; e < e0 + per && e < E; ++e) {
+    s.base[e] = run + (before ? before[e] : 0);
+    if (offsets) offsets[e] = run;
+    run += total[e];
   }
-  if (blockIdx.x == 0 && t == 0) a.offsets[E] = all;
+  if (offsets && t == 0) offsets[E] = all;
+  return all;
+}
+
+// Pairs of tokens t0 .. t0 + n - 1 (n <= 64) into the order; ids: their choices.
+__device__ __forceinline__ void sort_tokens(SortSpace& s, int E, int k, int t0, int n, const int* ids, int* order, bool more) {
+  const int t = threadIdx.x;
+  for (int e = t; e < E; e += blockDim.x) s.chose[e] = 0;
+  __syncthreads();
+  for (int i = t; i < n * k; i += blockDim.x)
+    if (ids[i] >= 0) atomicOr(&s.chose[ids[i]], 1ull << (i / k));
+  __syncthreads();
+  for (int i = t; i < n * k; i += blockDim.x) {
+    const int e = ids[i];
+    if (e >= 0) order[s.base[e] + __popcll(s.chose[e] & ((1ull << (i / k)) - 1))] = t0 * k + i;
+  }
+  if (!more) return;
+  __syncthreads();
+  for (int e = t; e < E; e += blockDim.x) s.base[e] += __popcll(s.chose[e]);
+}
+
+// ---- one token ----------------------------------------------------------------------------------
+
+// Routes token `tok` with the LANES lanes that call it together, lane `l` of them; ids, ls: room for its k choices in
+// LDS, which it leaves in ids.  KEY: what is compared.
+template <class KEY, int LANES, int NE>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, bool there, int* ids, float* ls) {
+  constexpr bool EXACT = std::is_same_v<KEY, double>;
+  const int E = a.r.experts, k = a.r.top_k;
+  // a group has `wide` lanes of its own, of which the last may have fewer than NE
+  const int per = E / a.r.groups, wide = (per + NE - 1) / NE, group = a.r.groups > 1 ? l / wide : 0;
+  const int e0 = a.r.groups > 1 ? group * per + (l - group * wide) * NE : l * NE;
+  const int mine = a.r.groups > 1 ? (group < a.r.groups ? (group + 1) * per - e0 : 0) : E - e0;  // experts of this lane, or more
+  const KEY NONE = -INFINITY;
+  float lg[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) lg[i] = -INFINITY;
+  if (there) {
+    const long long at = (long long)tok * a.stride + e0;
+    const float most = a.f32 ? 3.4028234663852886e38f : 65504.f;
+    if (mine >= NE) {
+      if (a.f32) {
+        __builtin_memcpy(lg, (const float*)a.logits + at, 4 * NE);
+      } else {
+        _Float16 h[NE];
+        __builtin_memcpy(h, (const _Float16*)a.logits + at, 2 * NE);
+#pragma unroll
+        for (int i = 0; i < NE; ++i) lg[i] = (float)h[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (i < mine) lg[i] = a.f32 ? ((const float*)a.logits)[at + i] : (float)((const _Float16*)a.logits)[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < NE; ++i) lg[i] = lg[i] != lg[i] ? -INFINITY : fminf(lg[i], most);
+  }
+  float top = -INFINITY, total = 0.f;  // largest logit, sum of e^(logit - top)
+  if (a.r.score == 0 && (EXACT || !a.r.renorm)) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) top = fmaxf(top, lg[i]);
+    top = lanes_all<LANES>(top, Most());
+  }
+  KEY c[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) c[i] = lg[i];
+  if (a.r.score == 0 && !a.r.renorm) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) total += lg[i] > -INFINITY ? expf(lg[i] - top) : 0.f;
+    total = lanes_all<LANES>(total, Sum());
+  }
+  if constexpr (EXACT) {
+    if (a.r.score == 0) {
+      double sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (lg[i] > -INFINITY) c[i] = exp((double)lg[i] - (double)top), sum += c[i];
+      sum = lanes_all<LANES>(sum, Sum());
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (lg[i] > -INFINITY) c[i] /= sum;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (lg[i] > -INFINITY) c[i] = 1.0 / (1.0 + exp(-(double)lg[i]));
+    }
+    if (a.r.bias) {
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
+        if (i < mine && lg[i] > -INFINITY) c[i] += (double)a.r.bias[e0 + i];
+    }
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (!(c[i] > NONE)) c[i] = NONE;
+    if (a.r.groups > 1) {
+      const int first = group * wide;
+      KEY b1 = NONE, b2 = NONE;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        b2 = fmax(b2, fmin(b1, c[i]));
+        b1 = fmax(b1, c[i]);
+      }
+      const int lane = threadIdx.x & 63, of = lane - l;
+      const KEY m1 = b1, m2 = b2;
+      for (int o = 1; o < wide; ++o) {
+        const int from = of + min(first + (l - first + o) % wide, LANES - 1);
+        const KEY d1 = __shfl(m1, from), d2 = __shfl(m2, from);
+        b2 = fmax(fmax(b2, d2), fmin(b1, d1));
+        b1 = fmax(b1, d1);
+      }
+      KEY value = group < a.r.groups ? b1 : NONE;
+      if (a.r.group_best == 2 && b2 > NONE) value += b2;
+      bool kept = false;
+      for (int n = 0; n < a.r.top_groups; ++n) {
+        const KEY v = kept ? NONE : value;
+        const KEY m = lanes_all<LANES>(v, Most());
+        const int win = lanes_all<LANES>(v == m && m > NONE ? group : RT_MAX_E, Least());
+        if (group == win) kept = true;
+      }
+      if (!kept) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i) c[i] = NONE;
+      }
+    }
+  }
+  for (int j = 0; j < k; ++j) {
+    KEY m = c[0];
+#pragma unroll
+    for (int i = 1; i < NE; ++i) m = Most()(m, c[i]);
+    m = lanes_all<LANES>(m, Most());
+    int at = RT_MAX_E;
+#pragma unroll
+    for (int i = NE - 1; i >= 0; --i)
+      if (c[i] == m) at = e0 + i;
+    const int own = at;
+    at = lanes_all<LANES>(at, Least());
+    const bool found = m > NONE;
+    float v = -INFINITY;
+    const int out = own == at ? at - e0 : -1;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (i == out) v = lg[i], c[i] = NONE;
+    if (found && own == at) ids[j] = at, ls[j] = v;
+    if (!found && l == 0) ids[j] = -1, ls[j] = -INFINITY;
+  }
+  __builtin_amdgcn_wave_barrier();  // (a wave's LDS writes are read by the same wave, in order)
+  // Weights.  Those that are divided by their sum are taken relative to the largest chosen score: however far below the
+  // row's others the chosen ones lie (a bias may choose them), their ratios are kept.
+  float most = -INFINITY;
+  if (a.r.renorm) {
+    for (int j = l; j < k; j += LANES) most = fmaxf(most, ls[j]);
+    most = lanes_all<LANES>(most, Most());
+  }
+  float w[(RT_MAX_K + LANES - 1) / LANES], sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < (RT_MAX_K + LANES - 1) / LANES; ++n) {
+    const int j = l + n * LANES;
+    w[n] = 0.f;
+    if (j >= k || ids[j] < 0) continue;
+    if (a.r.score == 0) w[n] = a.r.renorm ? expf(ls[j] - most) : expf(ls[j] - top) / total;
+    else w[n] = expf(fminf(ls[j], 0.f) - (a.r.renorm ? fminf(most, 0.f) : 0.f)) / (1.f + expf(-fabsf(ls[j])));
+    sum += w[n];
+  }
+  if (a.r.renorm) sum = lanes_all<LANES>(sum, Sum());
+#pragma unroll
+  for (int n = 0; n < (RT_MAX_K + LANES - 1) / LANES; ++n) {
+    const int j = l + n * LANES;
+    if (j >= k || tok >= a.tokens) continue;
+    a.experts[(long long)tok * k + j] = ids[j];
+    a.weights[(long long)tok * k + j] = ids[j] < 0 ? 0.f : (a.r.renorm ? w[n] / sum : w[n]) * a.r.scale;
+  }
+}
+
+// Threads of the workgroup that does all: fewer where a lane holds many experts in 64 bits and so needs more registers.
+template <class KEY, int NE>
+constexpr int one_threads() {
+  return std::is_same_v<KEY, float> || NE <= 8 ? 1024 : NE == 16 ? 512 : 256;
+}
+
+// `passes` times blockDim.x / LANES tokens a workgroup.  ONE: a single workgroup, which sorts as well.
+template <class KEY, int LANES, int NE, bool ONE>
+__global__ __launch_bounds__((ONE ? one_threads<KEY, NE>() : RT_THREADS)) void route_kernel(RouteArgs a, int passes, uint16_t* counts, int padded) {
+  constexpr int SLOTS = ONE ? RT_ONE : RT_THREADS / LANES;
+  __shared__ int ids[SLOTS * RT_MAX_K];
+  __shared__ float ls[(ONE ? one_threads<KEY, NE>() / LANES : SLOTS) * RT_MAX_K];
+  __shared__ int chosen[RT_MAX_E];
+  __shared__ SortSpace sort[ONE ? 1 : 0 + 1];
+  const int t = threadIdx.x, l = t % LANES, E = a.r.experts, k = a.r.top_k;
+  const int at_once = blockDim.x / LANES, first = blockIdx.x * passes * at_once;
+  const int there = a.count ? min(max(*a.count, 0), a.tokens) : a.tokens;
+  for (int e = t; e < E; e += blockDim.x) chosen[e] = 0;
+  __syncthreads();
+  for (int p = 0; p < passes; ++p) {
+    const int slot = t / LANES, mine = ONE ? p * at_once + slot : slot, tok = first + p * at_once + slot;
+    if (ONE && mine >= RT_ONE) continue;
+    int* const my_ids = ids + mine * k;
+    route_token<KEY, LANES, NE>(a, tok, l, tok < there, my_ids, ls + slot * k);
+    if (tok < there)
+      for (int j = l; j < k; j += LANES)
+        if (my_ids[j] >= 0) atomicAdd(&chosen[my_ids[j]], 1);
+  }
+  __syncthreads();
+  if constexpr (!ONE) {
+    for (int e = t; e < padded; e += RT_THREADS) counts[(size_t)blockIdx.x * padded + e] = e < E ? (uint16_t)chosen[e] : 0;
+  } else {
+    const int all = sort_bases(sort[0], E, chosen, nullptr, a.offsets);
+    for (int p = all + t; p < a.tokens * k; p += blockDim.x) a.order[p] = -1;
+    sort_tokens(sort[0], E, k, 0, a.tokens, ids, a.order, false);
+  }
+}
+
+constexpr int SORT_THREADS = 1024;
+
+// `tokens` of a workgroup, a multiple of 64 and of a block; counts: [blocks][padded].
+__global__ __launch_bounds__(SORT_THREADS) void route_sort_kernel(RouteArgs a, int tokens, int block, int blocks, int padded,
+                                                                  const uint16_t* __restrict__ counts) {
+  __shared__ SortSpace s;
+  __shared__ int total[RT_MAX_E], before[RT_MAX_E];
+  const int t = threadIdx.x, E = a.r.experts, k = a.r.top_k;
+  total[t] = 0, before[t] = 0;
+  __syncthreads();
+  {  // eight experts of every step-th block a thread
+    const int cols = padded / 8, col = t % cols, step = SORT_THREADS / cols;
+    const int mine = blockIdx.x * (tokens / block);
+    int all[8] = {}, pre[8] = {};
+    if (t < step * cols)
+#pragma unroll 4
+      for (int b = t / cols; b < blocks; b += step) {
+        const u4 v = *(const u4*)(counts + (size_t)b * padded + 8 * col);
+        const bool ahead = b < mine;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int n = v[e >> 1] >> (16 * (e & 1)) & 0xFFFF;
+          all[e] += n;
+          pre[e] += ahead ? n : 0;
+        }
+      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (all[e]) atomicAdd(&total[8 * col + e], all[e]);
+      if (pre[e]) atomicAdd(&before[8 * col + e], pre[e]);
+    }
+  }
+  __syncthreads();
+  const int all = sort_bases(s, E, total, before, blockIdx.x ? nullptr : a.offsets);
   const long long P = (long long)a.tokens * k;
-  for (long long p = all + (long long)blockIdx.x * SORT_THREADS + t; p < P; p += (long long)blocks * SORT_THREADS)
+  for (long long p = all + (long long)blockIdx.x * SORT_THREADS + t; p < P; p += (long long)gridDim.x * SORT_THREADS)
     a.order[p] = -1;
-  const long long first = (long long)blockIdx.x * block;
-  for (int u = 0; u < block; u += 64) {
-    const int t0 = (int)min(first + u, (long long)a.tokens), n = min(64, a.tokens - t0);
-    for (int e = t; e < E; e += SORT_THREADS) chose[e] = 0;
-    __syncthreads();
-    for (int i = t; i < n * k; i += SORT_THREADS) {
-      const int e = a.experts[(long long)t0 * k + i];
-      if (e >= 0) atomicOr(&chose[e], 1ull << (i / k));
-    }
-    __syncthreads();
-    for (int i = t; i < n * k; i += SORT_THREADS) {
-      const int e = a.experts[(long long)t0 * k + i];
-      if (e >= 0) a.order[base[e] + __popcll(chose[e] & ((1ull << (i / k)) - 1))] = t0 * k + i;
-    }
-    __syncthreads();
-    if (t < E) base[t] += __popcll(chose[t]);
+  const long long first = (long long)blockIdx.x * tokens;
+  for (int u = 0; u < tokens && first + u < a.tokens; u += 64)
+    sort_tokens(s, E, k, (int)first + u, min(64, a.tokens - ((int)first + u)), a.experts + (first + u) * k, a.order, true);
+}
+
+// ---- which -----------------------------------------------------------------------------------------
+
+struct RoutePlan {
+  int lanes, ne;
+  int at_once, passes, blocks;  // of many tokens: tokens of a pass, passes of a block, blocks
+  int padded;                   // experts in the counts, a multiple of eight
+  int sort_tokens, sort_blocks;
+};
+
+// Lanes and experts a lane.  With few tokens a wave has one: the rounds are a chain, and the fewer experts a lane goes
+// through the shorter it is; else a lane has eight or sixteen, which costs the least instructions a token.  Each group
+// of experts takes a whole number of lanes; 64 lanes of 32 experts hold any.
+RoutePlan route_plan(const w4_router& r, int tokens) {
+  RoutePlan p{};
+  static const int few[][2] = {{64, 1}, {64, 2}, {64, 4}, {64, 8}, {64, 16}, {64, 32}};
+  static const int many[][2] = {{8, 8}, {16, 8}, {16, 16}, {32, 16}, {64, 16}, {64, 32}};
+  const int per = r.experts / r.groups;
+  for (const auto& shape : tokens <= 16 ? few : many) {
+    p.lanes = shape[0], p.ne = shape[1];
+    if (r.groups * ((per + p.ne - 1) / p.ne) <= p.lanes) break;
+  }
+  p.at_once = RT_THREADS / p.lanes;
+  p.passes = 1;
+  while ((long long)p.at_once * p.passes * RT_MAX_BLOCKS < tokens) p.passes *= 2;
+  const int block = p.at_once * p.passes;
+  p.blocks = (tokens + block - 1) / block;
+  p.padded = (r.experts + 7) / 8 * 8;
+  p.sort_tokens = block > 64 ? block : 64;
+  while (p.sort_tokens < 256 && (tokens + p.sort_tokens - 1) / p.sort_tokens > 256) p.sort_tokens *= 2;
+  p.sort_blocks = (tokens + p.sort_tokens - 1) / p.sort_tokens;
+  return p;
+}
+
+template <class KEY, int LANES, int NE>
+hipError_t go(const RouteArgs& a, const RoutePlan& p, uint16_t* counts, hipStream_t s) {
+  if (a.tokens <= RT_ONE) {
+    constexpr int MOST = one_threads<KEY, NE>();
+    const int threads = std::min(MOST, (std::max(a.tokens * LANES, a.r.experts) + 63) / 64 * 64);
+    const int passes = (a.tokens * LANES + threads - 1) / threads;
+    route_kernel<KEY, LANES, NE, true><<<1, threads, 0, s>>>(a, passes, nullptr, 0);
+    return hipGetLastError();
+  }
+  route_kernel<KEY, LANES, NE, false><<<p.blocks, RT_THREADS, 0, s>>>(a, p.passes, counts, p.padded);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  route_sort_kernel<<<p.sort_blocks, SORT_THREADS, 0, s>>>(a, p.sort_tokens, p.at_once * p.passes, p.blocks, p.padded, counts);
+  return hipGetLastError();
+}
+
+template <class KEY>
+hipError_t go_shape(const RouteArgs& a, const RoutePlan& p, uint16_t* c, hipStream_t s) {
+  switch (p.lanes * 100 + p.ne) {
+    case 808: return go<KEY, 8, 8>(a, p, c, s);
+    case 1608: return go<KEY, 16, 8>(a, p, c, s);
+    case 1616: return go<KEY, 16, 16>(a, p, c, s);
+    case 3216: return go<KEY, 32, 16>(a, p, c, s);
+    case 6401: return go<KEY, 64, 1>(a, p, c, s);
+    case 6402: return go<KEY, 64, 2>(a, p, c, s);
+    case 6404: return go<KEY, 64, 4>(a, p, c, s);
+    case 6408: return go<KEY, 64, 8>(a, p, c, s);
+    case 6416: return go<KEY, 64, 16>(a, p, c, s);
+    default: return go<KEY, 64, 32>(a, p, c, s);
   }
 }
 
 }  // namespace
 
 size_t route_space(const w4_router& r, int tokens) {
-  const int block = tokens ? route_block(tokens) : 64;
-  return (((size_t)(tokens + block - 1) / block * r.experts * 2) + 15) / 16 * 16;
+  if (tokens <= RT_ONE) return 0;
+  const RoutePlan p = route_plan(r, tokens);
+  return ((size_t)p.blocks * p.padded * 2 + 15) / 16 * 16;
 }
 
 hipError_t launch_route_experts(const RouteArgs& a, hipStream_t s) {
-  const int block = a.tokens ? route_block(a.tokens) : 64, blocks = (a.tokens + block - 1) / block;
-  uint16_t* const counts = (uint16_t*)a.space;
-  const int E = a.r.experts;
-  if (blocks) {
-    if (E <= 64) route_kernel<1><<<blocks, RT_THREADS, 0, s>>>(a, block, counts);
-    else if (E <= 128) route_kernel<2><<<blocks, RT_THREADS, 0, s>>>(a, block, counts);
-    else if (E <= 256) route_kernel<4><<<blocks, RT_THREADS, 0, s>>>(a, block, counts);
-    else if (E <= 512) route_kernel<8><<<blocks, RT_THREADS, 0, s>>>(a, block, counts);
-    else route_kernel<16><<<blocks, RT_THREADS, 0, s>>>(a, block, counts);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  route_sort_kernel<<<blocks ? blocks : 1, SORT_THREADS, 0, s>>>(a, block, blocks, counts);
-  return hipGetLastError();
+  const RoutePlan p = route_plan(a.r, a.tokens);
+  const bool exact = a.r.bias || a.r.groups > 1;
+  return exact ? go_shape<double>(a, p, (uint16_t*)a.space, s) : go_shape<float>(a, p, (uint16_t*)a.space, s);
 }
 
 }  // namespace w4k
