@@ -12,65 +12,67 @@ struct ExpertTile {
   int column;               // its turn among the tiles of W
 };
 
-// Lane l looks after experts e0 + l: where their places begin and end.  Offsets are cut to what `order` has, so that no
-// plan leads outside the arrays.
-__device__ __forceinline__ void expert_places(const int* __restrict__ offsets, int experts, int pairs, int e0, int& lo, int& hi) {
-  const int e = e0 + (int)(threadIdx.x & 63), at = min(e, experts - 1);
-  lo = min(max(offsets[at], 0), pairs);
-  hi = e < experts ? min(max(offsets[at + 1], lo), pairs) : lo;
-}
-
 __device__ __forceinline__ int wave_upto(int v) {  // sum over the lanes up to this one
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    if (lane >= o) v += u;
-  }
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // row_shr:1, 2, 4, 8: inside rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);   // row_bcast15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);   // row_bcast31 into rows 2 and 3
   return v;
 }
 
 // Tile L of the experts' tiles of TM places times `columns` tiles of W, in the experts' order, an expert's places
-// fastest: workgroups side by side read the same codes.  L may be any number.  Every wave finds it for itself.
+// fastest: workgroups side by side read the same codes.  L may be any number.  Every wave finds it for itself: lane l
+// looks after `per` experts side by side, and what its experts need is read lane by lane into scalars.
+// Offsets are cut to what `order` has, so that no plan leads outside the arrays.
 // EVEN: an expert's places are shared out over its tiles in steps of 32.
 // SPREAD: consecutive workgroup ids land on different XCDs, each with an L2 of its own: L is turned round so that each
 // XCD has a run of the order, whose length is that of the tiles there are, not of the grid.
 template <int TM, bool EVEN, bool SPREAD>
 __device__ __forceinline__ ExpertTile find_expert_tile(const int* __restrict__ offsets, int experts, int pairs, int columns,
                                                        int L) {
-  ExpertTile r{0, 0, 0, 0};
-  int lo, hi;
-  if constexpr (SPREAD) {
-    int all = 0;
-    for (int e0 = 0; e0 < experts; e0 += 64) {
-      expert_places(offsets, experts, pairs, e0, lo, hi);
-      all += (hi - lo + TM - 1) / TM;
-    }
+  constexpr int HELD = 4;  // experts of a lane whose offsets it keeps
+  const int lane = threadIdx.x & 63, per = (experts + 63) >> 6, e0 = lane * per;
+  auto cut = [&](int e) { return min(max(offsets[min(e, experts)], 0), pairs); };
+  auto tiles_of = [](int lo, int hi) { return hi > lo ? (hi - lo + TM - 1) / TM : 0; };
+  int at[HELD + 1], mine = 0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
-    const int run = (all * columns + 7) >> 3;
+  for (int i = 0; i <= HELD; ++i) at[i] = i <= per ? cut(e0 + i) : 0;
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (i < per) mine += tiles_of(at[i], at[i + 1]);
+  for (int i = HELD; i < per; ++i) mine += tiles_of(cut(e0 + i), cut(e0 + i + 1));
+  const int upto = wave_upto(mine), all = __builtin_amdgcn_readlane(upto, 63);
+  ExpertTile r{0, 0, 0, 0};
+  if constexpr (SPREAD) {
+    const int run = (int)(((long long)all * columns + 7) >> 3);
     if (L >> 3 >= run) return r;
     L = (L & 7) * run + (L >> 3);
   }
   const int tile = L / columns;  // an expert's tiles times columns begin at a multiple of columns
-  int before = 0;
-  for (int e0 = 0; e0 < experts; e0 += 64) {
-    expert_places(offsets, experts, pairs, e0, lo, hi);
-    const int n = (hi - lo + TM - 1) / TM, upto = wave_upto(n);
-    const int first = before + upto - n;  // of this lane's expert
-    const unsigned long long hit = __ballot(tile >= first && tile < first + n);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int count = __shfl(n, l), places = __shfl(hi - lo, l), turn = L - __shfl(first, l) * columns;
-      const int per = EVEN ? ((places + count - 1) / count + 31) / 32 * 32 : TM;
-      const int m = turn % count * per;
-      r.expert = e0 + l;
-      r.first = __shfl(lo, l) + m;
-      r.rows = min(places - m, per);
-      r.column = turn / count;
-      break;
+  const unsigned long long hit = __ballot(tile >= upto - mine && tile < upto);
+  if (!hit) return r;
+  const int l = __builtin_ctzll(hit);
+  int before = __builtin_amdgcn_readlane(upto - mine, l);  // tiles of the experts before
+  auto take = [&](int e, int lo, int hi) {  // scalars
+    const int count = tiles_of(lo, hi);
+    if (tile >= before + count) {
+      before += count;
+      return false;
     }
-    before += __shfl(upto, 63);
+    const int places = hi - lo, turn = L - before * columns;
+    const int each = EVEN ? ((places + count - 1) / count + 31) / 32 * 32 : TM;
+    const int m = turn % count * each;
+    r = ExpertTile{e, lo + m, min(places - m, each), turn / count};
+    return true;
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; ++i)
+    if (i < per && take(l * per + i, __builtin_amdgcn_readlane(at[i], l), __builtin_amdgcn_readlane(at[i + 1], l))) return r;
+  for (int i = HELD; i < per; ++i) {
+    const int e = l * per + i;
+    if (take(e, __builtin_amdgcn_readfirstlane(cut(e)), __builtin_amdgcn_readfirstlane(cut(e + 1)))) return r;
   }
   return r;
 }

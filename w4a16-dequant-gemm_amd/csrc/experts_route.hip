@@ -13,15 +13,19 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "dq.cuh"
-#include "kernels.h"
+#include "experts.cuh"
 
 namespace w4k {
 namespace {
 
 constexpr int RT_MAX_E = 1024, RT_MAX_K = 32;
-constexpr int RT_THREADS = 256;      // of a block of many
-constexpr int RT_ONE = 64;           // tokens up to which one workgroup does all
+// Threads of a block of many tokens, which go through 16 tokens of 16 and more lanes or 32 of 8: at once, or where a lane
+// holds many experts and so needs more registers in several passes.
+constexpr int rt_threads(int lanes, int ne) {
+  const int all = lanes <= 16 ? 256 : 16 * lanes, most = ne <= 8 ? 1024 : ne == 16 ? 512 : 256;
+  return all < most ? all : most;
+}
+constexpr int RT_ONE = 64, RT_ONE_EXACT = 16;  // tokens up to which one workgroup does all
 constexpr int RT_MAX_BLOCKS = 1024;  // a sorting workgroup reads all blocks' counts
 
 // ---- reductions over the lanes of a token ------------------------------------------------
@@ -40,6 +44,32 @@ __device__ __forceinline__ double dpp(double v) {
   const uint32_t lo = (uint32_t)dpp<CTRL>((int)(uint32_t)u), hi = (uint32_t)dpp<CTRL>((int)(u >> 32));
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+// f over a lane and the one N (16, 32) lanes from it: the swap of a register with its copy leaves the one half in both
+// halves (of 32 or 64 lanes) of the first and the other in both of the second
+template <int N>
+__device__ __forceinline__ void swap_halves(uint32_t v, uint32_t& a, uint32_t& b) {
+  if constexpr (N == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    a = r[0], b = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    a = r[0], b = r[1];
+  }
+}
+template <int N, class T, class F>
+__device__ __forceinline__ T swapped(T v, F f) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t a, b;
+    swap_halves<N>(__builtin_bit_cast(uint32_t, v), a, b);
+    return f(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    uint32_t a, b, c, d;
+    swap_halves<N>((uint32_t)u, a, b);
+    swap_halves<N>((uint32_t)(u >> 32), c, d);
+    return f(__builtin_bit_cast(T, (uint64_t)c << 32 | a), __builtin_bit_cast(T, (uint64_t)d << 32 | b));
+  }
+}
 // f over all LANES lanes (a power of two), in every one of them; f does not care about order
 template <int LANES, class T, class F>
 __device__ __forceinline__ T lanes_all(T v, F f) {
@@ -47,8 +77,8 @@ __device__ __forceinline__ T lanes_all(T v, F f) {
   if constexpr (LANES > 2) v = f(v, dpp<0x4E>(v));    // quad_perm [2,3,0,1]
   if constexpr (LANES > 4) v = f(v, dpp<0x141>(v));   // row_half_mirror
   if constexpr (LANES > 8) v = f(v, dpp<0x140>(v));   // row_mirror
-  if constexpr (LANES > 16) v = f(v, __shfl_xor(v, 16));
-  if constexpr (LANES > 32) v = f(v, __shfl_xor(v, 32));
+  if constexpr (LANES > 16) v = swapped<16>(v, f);
+  if constexpr (LANES > 32) v = swapped<32>(v, f);
   return v;
 }
 struct Most {
@@ -82,12 +112,7 @@ __device__ __forceinline__ int sort_bases(SortSpace& s, int E, const int* total,
   const int per = (E + blockDim.x - 1) / blockDim.x, e0 = t * per;  // experts of a thread, side by side
   int mine = 0;
   for (int i = 0; i < per; ++i) mine += e0 + i < E ? total[e0 + i] : 0;
-  int run = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(run, o);
-    if (lane >= o) run += v;
-  }
+  int run = wave_upto(mine);
   if (lane == 63) s.wave_sum[wave] = run;
   __syncthreads();
   int all = 0;
@@ -105,11 +130,9 @@ __device__ __forceinline__ int sort_bases(SortSpace& s, int E, const int* total,
   return all;
 }
 
-// Pairs of tokens t0 .. t0 + n - 1 (n <= 64) into the order; ids: their choices.
+// Pairs of tokens t0 .. t0 + n - 1 (n <= 64) into the order; ids: their choices, in LDS.  s.chose is cleared.
 __device__ __forceinline__ void sort_tokens(SortSpace& s, int E, int k, int t0, int n, const int* ids, int* order, bool more) {
   const int t = threadIdx.x;
-  for (int e = t; e < E; e += blockDim.x) s.chose[e] = 0;
-  __syncthreads();
   for (int i = t; i < n * k; i += blockDim.x)
     if (ids[i] >= 0) atomicOr(&s.chose[ids[i]], 1ull << (i / k));
   __syncthreads();
@@ -119,15 +142,27 @@ __device__ __forceinline__ void sort_tokens(SortSpace& s, int E, int k, int t0, 
   }
   if (!more) return;
   __syncthreads();
-  for (int e = t; e < E; e += blockDim.x) s.base[e] += __popcll(s.chose[e]);
+  for (int e = t; e < E; e += blockDim.x) {
+    s.base[e] += __popcll(s.chose[e]);
+    s.chose[e] = 0;
+  }
+  __syncthreads();
+}
+
+// 1 / d for d >= 1, to a step of 64 bits.
+__device__ __forceinline__ double one_over(double d) {
+  double r = __builtin_amdgcn_rcp(d);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+  return d < INFINITY ? r : 0.0;
 }
 
 // ---- one token ----------------------------------------------------------------------------------
 
-// Routes token `tok` with the LANES lanes that call it together, lane `l` of them; ids, ls: room for its k choices in
-// LDS, which it leaves in ids.  KEY: what is compared.
+// Routes token `tok` with the LANES lanes that call it together, lane `l` of them; its k choices are left in ids, in
+// LDS.  KEY: what is compared.
 template <class KEY, int LANES, int NE>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, bool there, int* ids, float* ls) {
+__device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, bool there, int* ids) {
   constexpr bool EXACT = std::is_same_v<KEY, double>;
   const int E = a.r.experts, k = a.r.top_k;
   // a group has `wide` lanes of its own, of which the last may have fewer than NE
@@ -179,13 +214,14 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
       for (int i = 0; i < NE; ++i)
         if (lg[i] > -INFINITY) c[i] = exp((double)lg[i] - (double)top), sum += c[i];
       sum = lanes_all<LANES>(sum, Sum());
+      const double per_sum = one_over(sum);
 #pragma unroll
       for (int i = 0; i < NE; ++i)
-        if (lg[i] > -INFINITY) c[i] /= sum;
+        if (lg[i] > -INFINITY) c[i] = c[i] * per_sum;
     } else {
 #pragma unroll
       for (int i = 0; i < NE; ++i)
-        if (lg[i] > -INFINITY) c[i] = 1.0 / (1.0 + exp(-(double)lg[i]));
+        if (lg[i] > -INFINITY) c[i] = one_over(1.0 + exp(-(double)lg[i]));
     }
     if (a.r.bias) {
 #pragma unroll
@@ -204,12 +240,24 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
         b1 = fmax(b1, c[i]);
       }
       const int lane = threadIdx.x & 63, of = lane - l;
-      const KEY m1 = b1, m2 = b2;
-      for (int o = 1; o < wide; ++o) {
-        const int from = of + min(first + (l - first + o) % wide, LANES - 1);
-        const KEY d1 = __shfl(m1, from), d2 = __shfl(m2, from);
-        b2 = fmax(fmax(b2, d2), fmin(b1, d1));
-        b1 = fmax(b1, d1);
+      if ((wide & (wide - 1)) == 0) {  // the group's lanes are an aligned power of two
+        auto join = [&](KEY d1, KEY d2) {
+          b2 = fmax(fmax(b2, d2), fmin(b1, d1));
+          b1 = fmax(b1, d1);
+        };
+        if (LANES > 1 && wide > 1) join(dpp<0xB1>(b1), dpp<0xB1>(b2));
+        if (LANES > 2 && wide > 2) join(dpp<0x4E>(b1), dpp<0x4E>(b2));
+        if (LANES > 4 && wide > 4) join(dpp<0x141>(b1), dpp<0x141>(b2));
+        if (LANES > 8 && wide > 8) join(dpp<0x140>(b1), dpp<0x140>(b2));
+        if (LANES > 16 && wide > 16) join(__shfl_xor(b1, 16), __shfl_xor(b2, 16));
+      } else {
+        const KEY m1 = b1, m2 = b2;
+        for (int o = 1; o < wide; ++o) {
+          const int from = of + min(first + (l - first + o) % wide, LANES - 1);
+          const KEY d1 = __shfl(m1, from), d2 = __shfl(m2, from);
+          b2 = fmax(fmax(b2, d2), fmin(b1, d1));
+          b1 = fmax(b1, d1);
+        }
       }
       KEY value = group < a.r.groups ? b1 : NONE;
       if (a.r.group_best == 2 && b2 > NONE) value += b2;
@@ -226,42 +274,69 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
       }
     }
   }
+  // The rounds compare FP32: what is larger rounded is larger.  Where several are the same the 64 bits decide, then the
+  // index.  (As integers in the same order: FP32 maxima cost an instruction more each, for NaNs that are not there.)
+  int f[NE];
+  constexpr int NOTHING = (int)0x80000000;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int u = __builtin_bit_cast(int, (float)c[i] + 0.f);  // (-0 is 0)
+    f[i] = c[i] > NONE ? u ^ (u >> 31 & 0x7FFFFFFF) : NOTHING;
+  }
   for (int j = 0; j < k; ++j) {
-    KEY m = c[0];
+    int m = f[0];
 #pragma unroll
-    for (int i = 1; i < NE; ++i) m = Most()(m, c[i]);
+    for (int i = 1; i < NE; ++i) m = max(m, f[i]);
     m = lanes_all<LANES>(m, Most());
-    int at = RT_MAX_E;
+    const bool found = m > NOTHING;
+    int out = NE;  // this lane's first that has it
+    bool twice = false;
 #pragma unroll
-    for (int i = NE - 1; i >= 0; --i)
-      if (c[i] == m) at = e0 + i;
-    const int own = at;
-    at = lanes_all<LANES>(at, Least());
-    const bool found = m > NONE;
-    float v = -INFINITY;
-    const int out = own == at ? at - e0 : -1;
+    for (int i = NE - 1; i >= 0; --i) {
+      if (EXACT) twice |= f[i] == m && out < NE;
+      out = f[i] == m ? i : out;
+    }
+    if constexpr (EXACT) {
+      const unsigned long long have = __ballot(out < NE && found);
+      const unsigned long long lanes = LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1) << (threadIdx.x & 63 & ~(LANES - 1));
+      if (__any((twice && found) || __popcll(have & lanes) > 1)) {
+        KEY d = NONE;
 #pragma unroll
-    for (int i = 0; i < NE; ++i)
-      if (i == out) v = lg[i], c[i] = NONE;
-    if (found && own == at) ids[j] = at, ls[j] = v;
-    if (!found && l == 0) ids[j] = -1, ls[j] = -INFINITY;
+        for (int i = 0; i < NE; ++i) d = f[i] == m ? fmax(d, c[i]) : d;
+        d = lanes_all<LANES>(d, Most());
+        out = NE;
+#pragma unroll
+        for (int i = NE - 1; i >= 0; --i) out = f[i] == m && c[i] == d ? i : out;
+      }
+    }
+    const int own = out < NE ? e0 + out : RT_MAX_E, at = lanes_all<LANES>(own, Least());
+    out = own == at ? out : NE;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) f[i] = i == out ? NOTHING : f[i];
+    if (l == 0) ids[j] = found ? at : -1;
   }
   __builtin_amdgcn_wave_barrier();  // (a wave's LDS writes are read by the same wave, in order)
   // Weights.  Those that are divided by their sum are taken relative to the largest chosen score: however far below the
   // row's others the chosen ones lie (a bias may choose them), their ratios are kept.
-  float most = -INFINITY;
-  if (a.r.renorm) {
-    for (int j = l; j < k; j += LANES) most = fmaxf(most, ls[j]);
-    most = lanes_all<LANES>(most, Most());
+  float lj[(RT_MAX_K + LANES - 1) / LANES], most = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < (RT_MAX_K + LANES - 1) / LANES; ++n) {
+    const int j = l + n * LANES;
+    lj[n] = -INFINITY;
+    if (j >= k || ids[j] < 0) continue;
+    const long long at = (long long)tok * a.stride + ids[j];
+    lj[n] = a.f32 ? fminf(((const float*)a.logits)[at], 3.4028234663852886e38f) : fminf((float)((const _Float16*)a.logits)[at], 65504.f);
+    most = fmaxf(most, lj[n]);
   }
+  if (a.r.renorm) most = lanes_all<LANES>(most, Most());
   float w[(RT_MAX_K + LANES - 1) / LANES], sum = 0.f;
 #pragma unroll
   for (int n = 0; n < (RT_MAX_K + LANES - 1) / LANES; ++n) {
     const int j = l + n * LANES;
     w[n] = 0.f;
     if (j >= k || ids[j] < 0) continue;
-    if (a.r.score == 0) w[n] = a.r.renorm ? expf(ls[j] - most) : expf(ls[j] - top) / total;
-    else w[n] = expf(fminf(ls[j], 0.f) - (a.r.renorm ? fminf(most, 0.f) : 0.f)) / (1.f + expf(-fabsf(ls[j])));
+    if (a.r.score == 0) w[n] = a.r.renorm ? expf(lj[n] - most) : expf(lj[n] - top) / total;
+    else w[n] = expf(fminf(lj[n], 0.f) - (a.r.renorm ? fminf(most, 0.f) : 0.f)) / (1.f + expf(-fabsf(lj[n])));
     sum += w[n];
   }
   if (a.r.renorm) sum = lanes_all<LANES>(sum, Sum());
@@ -282,52 +357,61 @@ constexpr int one_threads() {
 
 // `passes` times blockDim.x / LANES tokens a workgroup.  ONE: a single workgroup, which sorts as well.
 template <class KEY, int LANES, int NE, bool ONE>
-__global__ __launch_bounds__((ONE ? one_threads<KEY, NE>() : RT_THREADS)) void route_kernel(RouteArgs a, int passes, uint16_t* counts, int padded) {
-  constexpr int SLOTS = ONE ? RT_ONE : RT_THREADS / LANES;
+__global__ __launch_bounds__((ONE ? one_threads<KEY, NE>() : rt_threads(LANES, NE))) void route_kernel(RouteArgs a, int passes, uint16_t* counts, int padded) {
+  constexpr int SLOTS = ONE ? RT_ONE : rt_threads(LANES, NE) / LANES;
   __shared__ int ids[SLOTS * RT_MAX_K];
-  __shared__ float ls[(ONE ? one_threads<KEY, NE>() / LANES : SLOTS) * RT_MAX_K];
   __shared__ int chosen[RT_MAX_E];
   __shared__ SortSpace sort[ONE ? 1 : 0 + 1];
   const int t = threadIdx.x, l = t % LANES, E = a.r.experts, k = a.r.top_k;
   const int at_once = blockDim.x / LANES, first = blockIdx.x * passes * at_once;
   const int there = a.count ? min(max(*a.count, 0), a.tokens) : a.tokens;
-  for (int e = t; e < E; e += blockDim.x) chosen[e] = 0;
+  for (int e = t; e < E; e += blockDim.x) {
+    chosen[e] = 0;
+    if (ONE) sort[0].chose[e] = 0;
+  }
   __syncthreads();
   for (int p = 0; p < passes; ++p) {
     const int slot = t / LANES, mine = ONE ? p * at_once + slot : slot, tok = first + p * at_once + slot;
     if (ONE && mine >= RT_ONE) continue;
     int* const my_ids = ids + mine * k;
-    route_token<KEY, LANES, NE>(a, tok, l, tok < there, my_ids, ls + slot * k);
+    route_token<KEY, LANES, NE>(a, tok, l, tok < there, my_ids);
     if (tok < there)
       for (int j = l; j < k; j += LANES)
         if (my_ids[j] >= 0) atomicAdd(&chosen[my_ids[j]], 1);
   }
   __syncthreads();
   if constexpr (!ONE) {
-    for (int e = t; e < padded; e += RT_THREADS) counts[(size_t)blockIdx.x * padded + e] = e < E ? (uint16_t)chosen[e] : 0;
+    for (int e = t; e < padded; e += blockDim.x) counts[(size_t)blockIdx.x * padded + e] = e < E ? (uint16_t)chosen[e] : 0;
   } else {
     const int all = sort_bases(sort[0], E, chosen, nullptr, a.offsets);
     for (int p = all + t; p < a.tokens * k; p += blockDim.x) a.order[p] = -1;
+    __syncthreads();
     sort_tokens(sort[0], E, k, 0, a.tokens, ids, a.order, false);
   }
 }
 
-constexpr int SORT_THREADS = 1024;
+constexpr int SORT_THREADS = 256;
 
 // `tokens` of a workgroup, a multiple of 64 and of a block; counts: [blocks][padded].
 __global__ __launch_bounds__(SORT_THREADS) void route_sort_kernel(RouteArgs a, int tokens, int block, int blocks, int padded,
                                                                   const uint16_t* __restrict__ counts) {
   __shared__ SortSpace s;
-  __shared__ int total[RT_MAX_E], before[RT_MAX_E];
+  __shared__ int total[RT_MAX_E], before[RT_MAX_E], ids[64 * RT_MAX_K];
   const int t = threadIdx.x, E = a.r.experts, k = a.r.top_k;
-  total[t] = 0, before[t] = 0;
+  const long long first = (long long)blockIdx.x * tokens;
+  auto fetch = [&](int u) {  // choices of 64 tokens
+    const int n = (int)min(64ll, a.tokens - (first + u)) * k;
+    for (int i = t; i < n; i += SORT_THREADS) ids[i] = a.experts[(first + u) * k + i];
+  };
+  fetch(0);
+  for (int e = t; e < padded; e += SORT_THREADS) total[e] = 0, before[e] = 0, s.chose[e] = 0;
   __syncthreads();
   {  // eight experts of every step-th block a thread
     const int cols = padded / 8, col = t % cols, step = SORT_THREADS / cols;
     const int mine = blockIdx.x * (tokens / block);
     int all[8] = {}, pre[8] = {};
     if (t < step * cols)
-#pragma unroll 4
+#pragma unroll 8
       for (int b = t / cols; b < blocks; b += step) {
         const u4 v = *(const u4*)(counts + (size_t)b * padded + 8 * col);
         const bool ahead = b < mine;
@@ -349,9 +433,14 @@ __global__ __launch_bounds__(SORT_THREADS) void route_sort_kernel(RouteArgs a, i
   const long long P = (long long)a.tokens * k;
   for (long long p = all + (long long)blockIdx.x * SORT_THREADS + t; p < P; p += (long long)gridDim.x * SORT_THREADS)
     a.order[p] = -1;
-  const long long first = (long long)blockIdx.x * tokens;
-  for (int u = 0; u < tokens && first + u < a.tokens; u += 64)
-    sort_tokens(s, E, k, (int)first + u, min(64, a.tokens - ((int)first + u)), a.experts + (first + u) * k, a.order, true);
+  __syncthreads();
+  for (int u = 0; u < tokens && first + u < a.tokens; u += 64) {
+    if (u) {
+      fetch(u);
+      __syncthreads();
+    }
+    sort_tokens(s, E, k, (int)first + u, (int)min(64ll, a.tokens - (first + u)), ids, a.order, u + 64 < tokens);
+  }
 }
 
 // ---- which -----------------------------------------------------------------------------------------
@@ -363,40 +452,42 @@ struct RoutePlan {
   int sort_tokens, sort_blocks;
 };
 
-// Lanes and experts a lane.  With few tokens a wave has one: the rounds are a chain, and the fewer experts a lane goes
-// through the shorter it is; else a lane has eight or sixteen, which costs the least instructions a token.  Each group
-// of experts takes a whole number of lanes; 64 lanes of 32 experts hold any.
+bool route_exact(const w4_router& r) { return r.bias || r.groups > 1; }
+
+// Lanes and experts a lane.  The fewer experts a lane goes through the shorter is the chain of the rounds, the more it
+// has the fewer instructions a token costs.  One or two tokens: a wave each (E 128: 5.0 us, 5.4 with 16 lanes); else
+// eight experts a lane (16384 tokens 17.6 us, 30 with 64 lanes of two).  Choices in 64 bits, whose scores take most of the
+// time: a wave each up to eight tokens (E 256, groups: 9.1 us, 13.3 with 16 lanes), then eight experts a lane (4099 tokens
+// 19.9; 21.3 with 16 a lane, 27 with four).  Each group of experts takes a whole number of lanes; 64 lanes of 32 experts hold any.
 RoutePlan route_plan(const w4_router& r, int tokens) {
   RoutePlan p{};
-  static const int few[][2] = {{64, 1}, {64, 2}, {64, 4}, {64, 8}, {64, 16}, {64, 32}};
-  static const int many[][2] = {{8, 8}, {16, 8}, {16, 16}, {32, 16}, {64, 16}, {64, 32}};
+  static const int shapes[][2] = {{8, 8}, {16, 8}, {32, 8}, {64, 1}, {64, 2}, {64, 4}, {64, 8}, {64, 16}, {64, 32}};
   const int per = r.experts / r.groups;
-  for (const auto& shape : tokens <= 16 ? few : many) {
-    p.lanes = shape[0], p.ne = shape[1];
+  for (int i = tokens <= (route_exact(r) ? 8 : 2) ? 3 : 0; i < 9; ++i) {
+    p.lanes = shapes[i][0], p.ne = shapes[i][1];
     if (r.groups * ((per + p.ne - 1) / p.ne) <= p.lanes) break;
   }
-  p.at_once = RT_THREADS / p.lanes;
-  p.passes = 1;
+  p.at_once = rt_threads(p.lanes, p.ne) / p.lanes;
+  p.passes = p.at_once < 16 ? 16 / p.at_once : 1;
   while ((long long)p.at_once * p.passes * RT_MAX_BLOCKS < tokens) p.passes *= 2;
   const int block = p.at_once * p.passes;
   p.blocks = (tokens + block - 1) / block;
   p.padded = (r.experts + 7) / 8 * 8;
   p.sort_tokens = block > 64 ? block : 64;
-  while (p.sort_tokens < 256 && (tokens + p.sort_tokens - 1) / p.sort_tokens > 256) p.sort_tokens *= 2;
   p.sort_blocks = (tokens + p.sort_tokens - 1) / p.sort_tokens;
   return p;
 }
 
 template <class KEY, int LANES, int NE>
 hipError_t go(const RouteArgs& a, const RoutePlan& p, uint16_t* counts, hipStream_t s) {
-  if (a.tokens <= RT_ONE) {
+  if (a.tokens <= (route_exact(a.r) ? RT_ONE_EXACT : RT_ONE)) {
     constexpr int MOST = one_threads<KEY, NE>();
     const int threads = std::min(MOST, (std::max(a.tokens * LANES, a.r.experts) + 63) / 64 * 64);
     const int passes = (a.tokens * LANES + threads - 1) / threads;
     route_kernel<KEY, LANES, NE, true><<<1, threads, 0, s>>>(a, passes, nullptr, 0);
     return hipGetLastError();
   }
-  route_kernel<KEY, LANES, NE, false><<<p.blocks, RT_THREADS, 0, s>>>(a, p.passes, counts, p.padded);
+  route_kernel<KEY, LANES, NE, false><<<p.blocks, rt_threads(LANES, NE), 0, s>>>(a, p.passes, counts, p.padded);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   route_sort_kernel<<<p.sort_blocks, SORT_THREADS, 0, s>>>(a, p.sort_tokens, p.at_once * p.passes, p.blocks, p.padded, counts);
   return hipGetLastError();
@@ -407,8 +498,7 @@ hipError_t go_shape(const RouteArgs& a, const RoutePlan& p, uint16_t* c, hipStre
   switch (p.lanes * 100 + p.ne) {
     case 808: return go<KEY, 8, 8>(a, p, c, s);
     case 1608: return go<KEY, 16, 8>(a, p, c, s);
-    case 1616: return go<KEY, 16, 16>(a, p, c, s);
-    case 3216: return go<KEY, 32, 16>(a, p, c, s);
+    case 3208: return go<KEY, 32, 8>(a, p, c, s);
     case 6401: return go<KEY, 64, 1>(a, p, c, s);
     case 6402: return go<KEY, 64, 2>(a, p, c, s);
     case 6404: return go<KEY, 64, 4>(a, p, c, s);
@@ -421,15 +511,14 @@ hipError_t go_shape(const RouteArgs& a, const RoutePlan& p, uint16_t* c, hipStre
 }  // namespace
 
 size_t route_space(const w4_router& r, int tokens) {
-  if (tokens <= RT_ONE) return 0;
+  if (tokens <= (route_exact(r) ? RT_ONE_EXACT : RT_ONE)) return 0;
   const RoutePlan p = route_plan(r, tokens);
   return ((size_t)p.blocks * p.padded * 2 + 15) / 16 * 16;
 }
 
 hipError_t launch_route_experts(const RouteArgs& a, hipStream_t s) {
   const RoutePlan p = route_plan(a.r, a.tokens);
-  const bool exact = a.r.bias || a.r.groups > 1;
-  return exact ? go_shape<double>(a, p, (uint16_t*)a.space, s) : go_shape<float>(a, p, (uint16_t*)a.space, s);
+  return route_exact(a.r) ? go_shape<double>(a, p, (uint16_t*)a.space, s) : go_shape<float>(a, p, (uint16_t*)a.space, s);
 }
 
 }  // namespace w4k
