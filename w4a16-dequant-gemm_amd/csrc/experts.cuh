@@ -26,53 +26,65 @@ __device__ __forceinline__ int wave_upto(int v) {  // sum over the lanes up to t
 // fastest: workgroups side by side read the same codes.  L may be any number.  Every wave finds it for itself: lane l
 // looks after `per` experts side by side, and what its experts need is read lane by lane into scalars.
 // Offsets are cut to what `order` has, so that no plan leads outside the arrays.
-// EVEN: an expert's places are shared out over its tiles in steps of 32.
+// FULL_FIRST: all tiles of TM places come before the experts' last, shorter ones: they take longest, and what is left of the
+// last round of workgroups is filled by short ones.
 // SPREAD: consecutive workgroup ids land on different XCDs, each with an L2 of its own: L is turned round so that each
 // XCD has a run of the order, whose length is that of the tiles there are, not of the grid.
-template <int TM, bool EVEN, bool SPREAD>
+template <int TM, bool FULL_FIRST, bool SPREAD>
 __device__ __forceinline__ ExpertTile find_expert_tile(const int* __restrict__ offsets, int experts, int pairs, int columns,
                                                        int L) {
   constexpr int HELD = 4;  // experts of a lane whose offsets it keeps
   const int lane = threadIdx.x & 63, per = (experts + 63) >> 6, e0 = lane * per;
   auto cut = [&](int e) { return min(max(offsets[min(e, experts)], 0), pairs); };
-  auto tiles_of = [](int lo, int hi) { return hi > lo ? (hi - lo + TM - 1) / TM : 0; };
-  int at[HELD + 1], mine = 0;
+  bool rest = false;  // the shorter tiles are looked through
+  auto tiles_of = [&](int lo, int hi) {
+    if (hi <= lo) return 0;
+    return FULL_FIRST ? (rest ? (hi - lo) % TM != 0 : (hi - lo) / TM) : (hi - lo + TM - 1) / TM;
+  };
+  int at[HELD + 1];
 #pragma unroll
   for (int i = 0; i <= HELD; ++i) at[i] = i <= per ? cut(e0 + i) : 0;
-#pragma unroll
-  for (int i = 0; i < HELD; ++i)
-    if (i < per) mine += tiles_of(at[i], at[i + 1]);
-  for (int i = HELD; i < per; ++i) mine += tiles_of(cut(e0 + i), cut(e0 + i + 1));
-  const int upto = wave_upto(mine), all = __builtin_amdgcn_readlane(upto, 63);
   ExpertTile r{0, 0, 0, 0};
-  if constexpr (SPREAD) {
-    const int run = (int)(((long long)all * columns + 7) >> 3);
-    if (L >> 3 >= run) return r;
-    L = (L & 7) * run + (L >> 3);
-  }
-  const int tile = L / columns;  // an expert's tiles times columns begin at a multiple of columns
-  const unsigned long long hit = __ballot(tile >= upto - mine && tile < upto);
-  if (!hit) return r;
-  const int l = __builtin_ctzll(hit);
-  int before = __builtin_amdgcn_readlane(upto - mine, l);  // tiles of the experts before
-  auto take = [&](int e, int lo, int hi) {  // scalars
-    const int count = tiles_of(lo, hi);
-    if (tile >= before + count) {
-      before += count;
-      return false;
-    }
-    const int places = hi - lo, turn = L - before * columns;
-    const int each = EVEN ? ((places + count - 1) / count + 31) / 32 * 32 : TM;
-    const int m = turn % count * each;
-    r = ExpertTile{e, lo + m, min(places - m, each), turn / count};
-    return true;
-  };
+  for (int turn_of = 0; turn_of < (FULL_FIRST ? 2 : 1); ++turn_of) {
+    rest = turn_of;
+    int mine = 0;
 #pragma unroll
-  for (int i = 0; i < HELD; ++i)
-    if (i < per && take(l * per + i, __builtin_amdgcn_readlane(at[i], l), __builtin_amdgcn_readlane(at[i + 1], l))) return r;
-  for (int i = HELD; i < per; ++i) {
-    const int e = l * per + i;
-    if (take(e, __builtin_amdgcn_readfirstlane(cut(e)), __builtin_amdgcn_readfirstlane(cut(e + 1)))) return r;
+    for (int i = 0; i < HELD; ++i)
+      if (i < per) mine += tiles_of(at[i], at[i + 1]);
+    for (int i = HELD; i < per; ++i) mine += tiles_of(cut(e0 + i), cut(e0 + i + 1));
+    const int upto = wave_upto(mine), all = __builtin_amdgcn_readlane(upto, 63);
+    if constexpr (SPREAD) {
+      const int run = (int)(((long long)all * columns + 7) >> 3);
+      if (L >> 3 >= run) {
+        L -= 8 * run;  // (the other tiles' turn, if there are any)
+        continue;
+      }
+      L = (L & 7) * run + (L >> 3);
+    }
+    const int tile = L / columns;  // an expert's tiles times columns begin at a multiple of columns
+    const unsigned long long hit = __ballot(tile >= upto - mine && tile < upto);
+    if (!hit) return r;
+    const int l = __builtin_ctzll(hit);
+    int before = __builtin_amdgcn_readlane(upto - mine, l);  // tiles of the experts before
+    auto take = [&](int e, int lo, int hi) {  // scalars
+      const int count = tiles_of(lo, hi);
+      if (tile >= before + count) {
+        before += count;
+        return false;
+      }
+      const int turn = L - before * columns;
+      const int m = rest ? (hi - lo) / TM * TM : turn % count * TM;
+      r = ExpertTile{e, lo + m, min(hi - lo - m, TM), turn / count};
+      return true;
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; ++i)
+      if (i < per && take(l * per + i, __builtin_amdgcn_readlane(at[i], l), __builtin_amdgcn_readlane(at[i + 1], l))) return r;
+    for (int i = HELD; i < per; ++i) {
+      const int e = l * per + i;
+      if (take(e, __builtin_amdgcn_readfirstlane(cut(e)), __builtin_amdgcn_readfirstlane(cut(e + 1)))) return r;
+    }
+    return r;
   }
   return r;
 }

@@ -4,8 +4,9 @@
 // A workgroup multiplies up to 16 places of one expert with 128 of its rows, 32 a wave (gated: 16 of the gate and the 16 of
 // the way up for the same columns), in stages of 256 k.  Everything goes global -> LDS (no registers) in whole lines: a
 // load instruction that takes 16 bytes of each of 64 rows, as the operands need them, holds the memory path four times as
-// long.  The rows of x are fetched once for the four waves; a wave's codes, scales and zero-points are its own.  Three stage
-// buffers, one barrier a stage.
+// long.  The rows of x are fetched once for the four waves; a wave's codes, scales and zero-points are its own.  Two stage
+// buffers and one barrier a stage: with at most 52.5 KB a compute unit has three workgroups, whose waits and arithmetic overlap (three
+// buffers and two workgroups: 56 us against 51 for 61 tokens, 6 of 64 experts, K 2048, width 1408).
 // v_mfma_f32_16x16x32_f16: lane l brings row l % 16 and eight consecutive k; of a stage it has k 64 (l / 16) .. + 63, two
 // 16-byte pieces of codes and eight of x.
 #include <atomic>
@@ -17,18 +18,24 @@ namespace {
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
-constexpr int ES_WAVES = 4, ES_STAGES = 3;
+constexpr int ES_WAVES = 4;
 constexpr int ES_W = 4096;            // a wave's codes of a stage: 32 rows of 128 bytes
 constexpr int ES_X = 16 * 512;        // rows of x
-constexpr int ES_X_AT = ES_WAVES * ES_W, ES_P_AT = ES_X_AT + ES_X;
+constexpr int ES_X_AT = ES_WAVES * ES_W, ES_STAGE = ES_X_AT + ES_X, ES_P_AT = 2 * ES_STAGE;
 
-// How the groups of W4 lie in a stage (GM): 0 two (gs 128), 1 four, 2 eight (gs 32, and MXFP4's blocks), 3 at most four of any
-// size that is a multiple of 32, from 96 on.  What a row needs of a stage: a run of dwords of scales, which begins at any
-// half (MXFP4: byte) of its first, and words of zero-points; one dword of 32 rows is half a load instruction.
-constexpr int es_scales(int fmt, int gm) { return fmt == 2 ? 3 : gm == 0 ? 2 : gm == 2 ? 5 : 3; }
-constexpr int es_zeros(int fmt, int gm) { return fmt != 1 ? 0 : gm == 3 ? 2 : 1; }
-constexpr int es_param_loads(int fmt, int gm) { return (es_scales(fmt, gm) + es_zeros(fmt, gm) + 1) / 2; }
-constexpr int es_stage(int fmt, int gm) { return ES_P_AT + ES_WAVES * es_param_loads(fmt, gm) * 256; }
+// Scales and zero-points come for two stages at a time, a row's side by side: 64 dwords that touch as few lines as they can.
+// How the groups of W4 lie (GM): 0 gs 128, 1 gs 64, 2 gs 32 (and MXFP4's blocks), 3 any size that is a multiple of 32, from 96
+// on.  Groups of two stages; dwords of their scales, one more where a run may begin at an odd half (MXFP4: at any byte);
+// words of their zero-points.
+constexpr int es_groups(int fmt, int gm) { return fmt == 2 || gm == 2 ? 16 : gm == 1 ? 8 : gm == 0 ? 4 : 7; }
+constexpr int es_zeros(int fmt, int gm) { return fmt != 1 ? 0 : gm >= 2 ? 2 : 1; }
+constexpr int es_most(int fmt, int gm) {
+  return (fmt == 2 ? 5 : (es_groups(fmt, gm) + 1) / 2 + (gm == 3 ? 0 : 1)) + es_zeros(fmt, gm);
+}
+int es_dwords(const ExpertArgs& a, int fmt, int gm) {
+  const bool whole = fmt == 2 ? a.v.B % 4 == 0 : gm != 3 && a.v.G % 2 == 0;
+  return es_most(fmt, gm) - (whole ? 1 : 0);
+}
 
 extern __shared__ __attribute__((aligned(16))) uint8_t es_lds[];
 
@@ -48,10 +55,9 @@ __device__ __forceinline__ void es_dma4(const void* at, uint32_t lds) {
 
 // XI: load instructions of x per wave and stage, for up to 8 XI places.
 template <int FMT, bool GATED, int GM, int XI>
-__device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTile& tile, uint32_t group_mul) {
+__device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTile& tile, uint32_t group_mul, int dwords) {
   constexpr bool MX = FMT == 2, ASYM = FMT == 1;
-  constexpr int PS = es_scales(FMT, GM), PZ = es_zeros(FMT, GM), PI = es_param_loads(FMT, GM);
-  constexpr int LOADS = 4 + XI + PI, STAGE = es_stage(FMT, GM);
+  constexpr int PZ = es_zeros(FMT, GM), PI = (es_most(FMT, GM) + 1) / 2;  // load instructions of parameters at most
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int K = a.v.K, G = MX ? a.v.B : a.v.G, wg = words(G), pairs = a.tokens * a.top_k;
@@ -85,33 +91,43 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
     xp[i] = (lane & 31) ^ (m & 15);
     xo[i] = from * (uint32_t)(K * 2) + 16 * xp[i];
   }
-  // parameters: this lane's dwords of a stage (entry e: dword e / 32 of row e % 32)
+  // parameters: entry e of a wave's is dword e % dwords of row e / dwords, scales first
   const size_t row0 = (size_t)tile.expert * R;
   const size_t sc_last = ((size_t)a.v.N * G >> (MX ? 2 : 1)) - 1, zw_last = (size_t)a.v.N * wg - 1;
-  auto first_group = [&](uint32_t d) { return MX ? 8 * d : GM == 3 ? __umulhi(16 * d, group_mul) : (2u << GM) * d; };
-  const size_t pn = row0 + row_of(lane & 31);
-  auto request = [&](int d, uint32_t buf) {
-    const uint32_t dd = (uint32_t)min(d, stages - 1), st = lds0 + buf;
-    const bool tail = dd * 256 + 256 > (uint32_t)K;  // pieces behind the end of a row are fetched from its part that is there
+  const int ps = dwords - PZ;
+  auto first_group = [&](uint32_t w) { return MX ? 16 * w : GM == 3 ? __umulhi(32 * w, group_mul) : (4u << GM) * w; };
+  size_t pe[PI];  // the lane's entry in the row's scales or words
+  int pd[PI];
+#pragma unroll
+  for (int i = 0; i < PI; ++i) {
+    const int e = min(64 * i + lane, 32 * dwords - 1), n = e / dwords;
+    pd[i] = e - n * dwords;
+    pe[i] = (row0 + row_of(n)) * (size_t)(pd[i] < ps ? G : wg);
+  }
+  const uint32_t p_at = lds0 + ES_P_AT + wave * dwords * 128;
+  auto request = [&](int d, int buf) {
+    const uint32_t st = lds0 + buf * ES_STAGE;
+    const bool tail = d * 256 + 256 > K;  // pieces behind the end of a row are fetched from its part that is there
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint32_t off = wo[i];
-      if (tail && dd * 256 + 32 * wp[i] >= (uint32_t)K) off -= 16 * wp[i];
-      es_dma16(wb + dd * 128, off, st + wave * ES_W + i * 1024);
+      if (tail && d * 256 + 32 * wp[i] >= K) off -= 16 * wp[i];
+      es_dma16(wb + d * 128, off, st + wave * ES_W + i * 1024);
     }
 #pragma unroll
     for (int i = 0; i < XI; ++i) {
       uint32_t off = xo[i];
-      if (tail && dd * 256 + 8 * xp[i] >= (uint32_t)K) off -= 16 * xp[i];
-      es_dma16(xb + dd * 512, off, st + ES_X_AT + (wave + ES_WAVES * i) * 1024);
+      if (tail && d * 256 + 8 * xp[i] >= K) off -= 16 * xp[i];
+      es_dma16(xb + (size_t)d * 512, off, st + ES_X_AT + (wave + ES_WAVES * i) * 1024);
     }
-    const uint32_t g = first_group(dd);
+    if (d & 1) return;
+    const uint32_t g = first_group(d >> 1);
 #pragma unroll
     for (int i = 0; i < PI; ++i) {
-      const int e = 2 * i + (lane >> 5);
-      const uint32_t* at = (const uint32_t*)a.v.scales + min(((pn * G + g) >> (MX ? 2 : 1)) + min(e, PS - 1), sc_last);
-      if (ASYM && e >= PS) at = a.v.zeros + min(pn * wg + (g >> 3) + min(e - PS, PZ - 1), zw_last);
-      es_dma4(at, st + ES_P_AT + (wave * PI + i) * 256);
+      if (64 * i + lane >= 32 * dwords) continue;
+      const uint32_t* at = (const uint32_t*)a.v.scales + min(((pe[i] + g) >> (MX ? 2 : 1)) + pd[i], sc_last);
+      if (ASYM && pd[i] >= ps) at = a.v.zeros + min(pe[i] + (g >> 3) + (pd[i] - ps), zw_last);
+      es_dma4(at, p_at + i * 256);
     }
   };
 
@@ -124,42 +140,54 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
   for (int i = 0; i < 2; ++i) first[i] = (uint32_t)((row0 + row_of(16 * i + r)) * G);
   const uint8_t* const mine = es_lds + wave * ES_W;
   const uint8_t* const xs = es_lds + ES_X_AT;
-  const uint8_t* const ps = es_lds + ES_P_AT + wave * PI * 256;
-  uint32_t b0 = 0, b1 = STAGE, b2 = 2 * STAGE;
-  request(0, b0);
-  request(1, b1);
-#pragma unroll 1
-  for (int d = 0; d < stages; ++d) {
-    // stage d has landed (outstanding: stage d + 1), for every wave behind the barrier, where nobody reads stage d - 1 any more
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS));
+  const uint8_t* const params = es_lds + ES_P_AT + wave * (dwords * 128);
+  uint32_t sc[2][2][2], zw[2][2][2];  // of two stages: of the lane's two pieces of a row
+  // Scales and zero-points of both stages go into registers at the first: their place is free for the next two.
+  auto read_params = [&](int d) {
+    const uint32_t g0 = first_group(d >> 1);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          // group of the piece, counted from the first of the two stages
+          const uint32_t n = MX || GM == 2 ? 8 * half + 2 * q + p
+                             : GM == 1     ? 4 * half + q
+                             : GM == 0     ? 2 * half + (q >> 1)
+                                           : __umulhi(2 * (8 * (d + half) + 2 * q + p), group_mul) - g0;
+          if (p && !MX && GM < 2) {
+            sc[half][i][1] = sc[half][i][0], zw[half][i][1] = zw[half][i][0];
+            continue;
+          }
+          const uint8_t* const row = params + (16 * i + r) * (dwords * 4);
+          const uint32_t at = n + ((first[i] + g0) & (MX ? 3 : 1));
+          if constexpr (MX) {
+            sc[half][i][p] = row[at];
+          } else {
+            sc[half][i][p] = *(const uint16_t*)(row + 2 * at);
+            const uint32_t g = g0 + n;
+            zw[half][i][p] = 8;
+            if (ASYM) zw[half][i][p] = *(const uint32_t*)(row + 4 * (ps + (g >> 3) - (g0 >> 3))) >> (4 * (g & 7)) & 0xFu;
+          }
+        }
+  };
+  auto stage = [&](int d, int half) {
+    // stage d has landed, for every wave behind the barrier, where nobody reads stage d - 1 any more
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     __syncthreads();
-    request(d + 2, b2);
+    if (half == 0) {
+      read_params(d);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (d + 1 < stages) request(d + 1, half ^ 1);
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t g0 = first_group(d);
+    const uint32_t b0 = half * ES_STAGE;
     u4 w[2][2];
-    uint32_t sc[2][2], zw[2][2];  // of the lane's two pieces of a row
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        w[i][p] = *(const u4*)(mine + b0 + es_w_at(16 * i + r, 2 * q + p));
-        // group of the piece, counted from the stage's first
-        const uint32_t n = MX || GM == 2 ? 2 * q + p : GM == 1 ? q : GM == 0 ? q >> 1 : __umulhi(2 * (8 * d + 2 * q + p), group_mul) - g0;
-        if (p && !MX && GM < 2) {
-          sc[i][1] = sc[i][0], zw[i][1] = zw[i][0];
-          continue;
-        }
-        const uint32_t at = n + ((first[i] + g0) & (MX ? 3 : 1));
-        if constexpr (MX) {
-          sc[i][p] = ps[b0 + (at >> 2) * 128 + (16 * i + r) * 4 + (at & 3)];
-        } else {
-          sc[i][p] = *(const uint16_t*)(ps + b0 + (at >> 1) * 128 + (16 * i + r) * 4 + (at & 1) * 2);
-          const uint32_t g = g0 + n;
-          zw[i][p] = 8;
-          if (ASYM)
-            zw[i][p] = *(const uint32_t*)(ps + b0 + (PS + (GM == 3 ? (g >> 3) - (g0 >> 3) : 0)) * 128 + (16 * i + r) * 4) >> (4 * (g & 7)) & 0xFu;
-        }
-      }
+      for (int p = 0; p < 2; ++p) w[i][p] = *(const u4*)(mine + b0 + es_w_at(16 * i + r, 2 * q + p));
     const bool tail = d * 256 + 256 > K;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
@@ -172,21 +200,21 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
         h8 av;
         if constexpr (MX) {
           h2 n[4];
-          dq_mx(w[i][p][s & 3], tail && past ? 0.f : mx_scale(sc[i][p]), n);
+          dq_mx(w[i][p][s & 3], tail && past ? 0.f : mx_scale(sc[half][i][p]), n);
           av = __builtin_bit_cast(h8, u4{as_u32(n[0]), as_u32(n[1]), as_u32(n[2]), as_u32(n[3])});
         } else {
-          av = expand_word(w[i][p][s & 3], as_h2(0xD400E400u + zw[i][p] * 0x00100001u), splat_bits(tail && past ? 0u : sc[i][p]), mask, magic);
+          av = expand_word(w[i][p][s & 3], as_h2(0xD400E400u + zw[half][i][p] * 0x00100001u), splat_bits(tail && past ? 0u : sc[half][i][p]), mask, magic);
         }
         acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(h8, x), acc[i], 0, 0, 0);
       }
     }
-    const uint32_t old = b0;
-    b0 = b1;
-    b1 = b2;
-    b2 = old;
+  };
+  request(0, 0);
+#pragma unroll 1
+  for (int d = 0; d < stages; d += 2) {
+    stage(d, 0);
+    if (d + 1 < stages) stage(d + 1, 1);
   }
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // nothing may still be writing LDS at exit
-
   // lane l of a 16 x 16 tile holds columns 4 (l / 16) + e of place l % 16
   if (r >= tile.rows) return;
   const int place = tile.first + r, pair = a.order[place];
@@ -209,26 +237,27 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
 }
 
 template <int FMT, bool GATED, int GM>
-__global__ __launch_bounds__(64 * ES_WAVES, 2) void experts_step_kernel(ExpertArgs a, int columns, uint32_t group_mul) {
+__global__ __launch_bounds__(64 * ES_WAVES, 3) void experts_step_kernel(ExpertArgs a, int columns, uint32_t group_mul, int dwords) {
   const ExpertTile tile = find_expert_tile<16, false, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
   const int rows = __builtin_amdgcn_readfirstlane(tile.rows);
   if (rows == 0) return;
   const ExpertTile u{__builtin_amdgcn_readfirstlane(tile.expert), __builtin_amdgcn_readfirstlane(tile.first), rows,
                      __builtin_amdgcn_readfirstlane(tile.column)};
-  if (rows > 8) return experts_step<FMT, GATED, GM, 2>(a, u, group_mul);
-  experts_step<FMT, GATED, GM, 1>(a, u, group_mul);
+  if (rows > 8) return experts_step<FMT, GATED, GM, 2>(a, u, group_mul, dwords);
+  experts_step<FMT, GATED, GM, 1>(a, u, group_mul, dwords);
 }
 
 template <int FMT, bool GATED, int GM>
 hipError_t go(const ExpertArgs& a, hipStream_t s) {
   // more than 64 KB of LDS has to be granted per device, once
-  constexpr int LDS = ES_STAGES * es_stage(FMT, GM);
+  constexpr int MOST = ES_P_AT + ES_WAVES * es_most(FMT, GM) * 128;
+  const int dwords = es_dwords(a, FMT, GM), LDS = ES_P_AT + ES_WAVES * dwords * 128;
   static std::atomic<bool> granted[64] = {};
   int dev = 0;
   if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
   if (dev < 0 || dev >= 64 || !granted[dev]) {
     const hipError_t e = hipFuncSetAttribute((const void*)experts_step_kernel<FMT, GATED, GM>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, MOST);
     if (e != hipSuccess) return e;
     if (dev >= 0 && dev < 64) granted[dev] = true;
   }
@@ -237,7 +266,7 @@ hipError_t go(const ExpertArgs& a, hipStream_t s) {
   if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   // the group of slice n of 32 k is (2 n group_mul) >> 32
   const uint32_t d = a.v.mx ? 1 : a.v.gs / 32, mul = (uint32_t)(((1ull << 31) + d - 1) / d);
-  experts_step_kernel<FMT, GATED, GM><<<dim3((unsigned)grid), dim3(64 * ES_WAVES), LDS, s>>>(a, columns, mul);
+  experts_step_kernel<FMT, GATED, GM><<<dim3((unsigned)grid), dim3(64 * ES_WAVES), LDS, s>>>(a, columns, mul, dwords);
   return hipGetLastError();
 }
 

@@ -11,11 +11,14 @@
 //   * gated experts: of a wave's two tiles of 32 rows the first is the gate's and the second the way up's for the same
 //     columns, so both sums of an output lie in one lane and the gate is taken in registers.
 // A tile with few places runs a loop of its own for 64, 128 or 192 of them: products of rows that are not there would
-// take as long as the others.  An expert's places are shared out evenly over its tiles.
+// take as long as the others.
 #include <atomic>
 
 #include "experts.cuh"
 
+#ifndef WIDE
+#define WIDE 160LL
+#endif
 namespace w4k {
 namespace {
 
@@ -356,7 +359,7 @@ hipError_t go(const ExpertArgs& a, hipStream_t s) {
     if (dev >= 0 && dev < 64) granted[dev] = true;
   }
   const int R = a.v.N / a.experts, columns = GATED ? (R / 2 + 127) / 128 : (R + 255) / 256;
-  const long long grid = (most_expert_tiles(a, TM) * columns + 7) / 8 * 8;  // (an eighth of the tiles, rounded up, per XCD)
+  const long long grid = (most_expert_tiles(a, TM) * columns + 15) / 8 * 8;  // (an eighth per XCD, rounded up, of either kind)
   if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   experts_tile_kernel<FMT, GS32, GATED, TM><<<dim3((unsigned)grid), dim3(ET_THREADS), LDS, s>>>(a, columns);
   return hipGetLastError();
@@ -365,7 +368,7 @@ hipError_t go(const ExpertArgs& a, hipStream_t s) {
 template <int FMT, bool GS32>
 hipError_t go_rows(const ExpertArgs& a, hipStream_t s) {
   const long long pairs = (long long)a.tokens * a.top_k;
-  const bool wide = pairs >= 160LL * a.experts;
+  const bool wide = pairs >= WIDE * a.experts;
   if (a.act) return wide ? go<FMT, GS32, true, 256>(a, s) : go<FMT, GS32, true, 128>(a, s);
   return wide ? go<FMT, GS32, false, 256>(a, s) : go<FMT, GS32, false, 128>(a, s);
 }
