@@ -17,7 +17,7 @@ CALLS = os.path.join(PKG, "lib", "w4calls" + (sysconfig.get_config_var("EXT_SUFF
 CALLS_SRC = os.path.join(CSRC, "pycalls.cpp")
 PY_INCLUDE = sysconfig.get_paths()["include"]
 SOURCES = ["abi.hip", "dequant.hip", "gemm_simt.hip", "gemm_mfma.hip", "flash.hip", "flash_mfma.hip", "quantize.hip", "gemm_mxnative.hip", "gemm_tile_dma.hip", "gemm_tile_any.hip", "gemm_tile256.hip", "gemm_decode_resident.hip", "gemm_decode_general.hip", "gemm_decode_longk.hip", "gemm_block.hip",
-           "baseline.hip", "paged_tables.hip", "quantize_pages.hip", "pages_attention.hip", "pages_few.hip", "pages_many.hip", "pages_mixed.hip", "experts_route.hip", "gemm_experts.hip", "gemm_experts_tile.hip", "gemm_experts_step.hip", "gemm_experts_few.hip", "residual_norm.hip"]
+           "baseline.hip", "paged_tables.hip", "quantize_pages.hip", "pages_attention.hip", "pages_few.hip", "pages_many.hip", "pages_mixed.hip", "experts_route.hip", "gemm_experts.hip", "gemm_experts_tile.hip", "gemm_experts_token.hip", "gemm_experts_step.hip", "gemm_experts_few.hip", "residual_norm.hip"]
 HEADERS = ["dq.cuh", "experts.cuh", "kernels.h", "pages.cuh", "pages_few.cuh", "pages_many.cuh", "simt_rows4.cuh", "tile_dma.cuh", "bench_kernels.hip", os.path.join("..", "..", "include", "w4_abi.h")]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

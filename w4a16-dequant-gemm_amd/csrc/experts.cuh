@@ -105,6 +105,7 @@ __device__ __forceinline__ float expert_act(int act, float x) {
 // gemm_experts_tile.hip: false (nothing launched) when the arguments are not its.
 bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err);
 // gemm_experts_step.hip, gemm_experts_few.hip: the same for few rows per expert, of many experts and of few.
+bool try_experts_token(const ExpertArgs& a, hipStream_t s, hipError_t* err);
 bool try_experts_step(const ExpertArgs& a, hipStream_t s, hipError_t* err);
 bool try_experts_few(const ExpertArgs& a, hipStream_t s, hipError_t* err);
 

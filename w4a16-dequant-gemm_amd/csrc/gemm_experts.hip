@@ -91,7 +91,7 @@ hipError_t go_general(const ExpertArgs& a, hipStream_t s) {
 
 hipError_t launch_gemm_experts(const ExpertArgs& a, hipStream_t s) {
   hipError_t err = hipSuccess;
-  if (try_experts_tile(a, s, &err) || try_experts_step(a, s, &err) || try_experts_few(a, s, &err)) return err;
+  if (try_experts_tile(a, s, &err) || try_experts_token(a, s, &err) || try_experts_step(a, s, &err) || try_experts_few(a, s, &err)) return err;
   if (a.v.mx) return go_general<2>(a, s);
   return a.v.symmetric ? go_general<0>(a, s) : go_general<1>(a, s);
 }

@@ -1,0 +1,202 @@
+// Products of one to four rows per expert with the experts' packed matrices, on the vector ALUs: single tokens.
+//
+// A wave multiplies up to four places of one expert with eight (K up to 1024: sixteen) of its rows (gated: half of them the
+// gate's, half the way up's, for the same columns).  Lanes lie along K, 32 k each, so that a load instruction takes a whole
+// row's codes, or two rows', side by side; all rows' codes of 2048 k are asked for at once, ahead of anything that waits
+// for `order`.  Rows of x come to LDS in whole lines, once for the workgroup's four waves.  A word is expanded to the halves of
+// w4_dequant and multiplied by v_dot2_f32_f16, whose sums are FP32; lanes are added by DPP at the end.
+#include "experts.cuh"
+
+namespace w4k {
+namespace {
+
+constexpr int EK_WAVES = 4, EK_ROWS = 8;  // load instructions of codes of a wave
+constexpr int EK_PLACES = 4;
+
+// 16-byte piece p of a row of x in LDS: lane l reads pieces 4 l + j, which for 16 lanes (same j) lie on 16 distinct bank groups.
+__device__ __forceinline__ int ek_x_at(int p) { return (p ^ (p >> 4 & 3)) * 16; }
+
+// LPR: lanes of a row, 64 or 32.  NM: places.
+template <int FMT, bool GATED, int LPR, int NM>
+__device__ __forceinline__ void experts_token(const ExpertArgs& a, const ExpertTile& tile, uint32_t group_mul, uint8_t* xs) {
+  constexpr bool MX = FMT == 2, ASYM = FMT == 1;
+  constexpr int RPI = 64 / LPR;             // rows of an instruction
+  constexpr int SPAN = 32 * LPR;            // k of a segment
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int l = lane & (LPR - 1), sub = lane / LPR;
+  const int K = a.v.K, G = MX ? a.v.B : a.v.G, wg = words(G), pairs = a.tokens * a.top_k;
+  const int R = a.v.N / a.experts, width = GATED ? R / 2 : R;
+  constexpr int COLS = EK_ROWS * RPI / (GATED ? 2 : 1);  // output columns of a wave
+  const int c0 = tile.column * (EK_WAVES * COLS) + wave * COLS;
+  const size_t row0 = (size_t)tile.expert * R;
+  // load instruction i's rows; gated: instructions 0 .. 3 the gate's, 4 .. 7 the way up's for the same columns.  Columns
+  // past the last repeat it and are not stored.
+  auto col_of = [&](int i) { return c0 + (GATED ? i % (EK_ROWS / 2) : i) * RPI + sub; };
+  uint32_t row[EK_ROWS];
+#pragma unroll
+  for (int i = 0; i < EK_ROWS; ++i) row[i] = min(col_of(i), width - 1) + (GATED && i >= EK_ROWS / 2 ? width : 0);
+  const char* const codes = (const char*)a.v.q + row0 * (K >> 1);
+  const int segments = (K + SPAN - 1) / SPAN;
+  u4 w[EK_ROWS];
+  uint32_t sc[EK_ROWS], zw[EK_ROWS];
+  auto request = [&](int s, int i) {  // the rows of instruction i, segment s
+    const int k = s * SPAN + 32 * l, kk = k < K ? k : 0;  // (behind the end of K: from the row's start, not multiplied)
+    const uint32_t g = MX ? kk >> 5 : __umulhi(2u * (kk >> 5), group_mul);
+    w[i] = *(const u4*)(codes + (row[i] * (uint32_t)(K >> 1) + (kk >> 1)));
+    if (MX) sc[i] = ((const uint8_t*)a.v.scales)[(row0 + row[i]) * G + g];
+    else sc[i] = ((const uint16_t*)a.v.scales)[(row0 + row[i]) * G + g];
+    if (ASYM) zw[i] = a.v.zeros[(row0 + row[i]) * wg + (g >> 3)] >> (4 * (g & 7)) & 0xFu;
+  };
+  const w4_half* x[NM];
+  int pair[NM];
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {  // (scalar loads: they wait for no codes)
+    const int place = tile.first + min(m, tile.rows - 1);
+    pair[m] = a.order[place];
+  }
+  // The first half of the codes, then x, which needs `order`, then the second half: what is asked for comes back in
+  // order, and the first rows are multiplied while the others are on their way.
+#pragma unroll
+  for (int i = 0; i < EK_ROWS / 2; ++i) request(0, i);
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    const bool there = pair[m] >= 0 && pair[m] < pairs;
+    const int place = tile.first + min(m, tile.rows - 1);
+    x[m] = a.x + (size_t)(a.from_tokens ? (uint32_t)(there ? pair[m] : 0) / (uint32_t)a.top_k : place) * K;
+    if (!there || m >= tile.rows) pair[m] = -1;
+  }
+  uint32_t mask = 0x00F0000Fu, magic = 0x54006400u;
+  asm volatile("" : "+s"(mask));   // opaque: otherwise they come back as literals of two
+  asm volatile("" : "+v"(magic));  // separate instructions
+  float acc[EK_ROWS][NM];
+#pragma unroll
+  for (int i = 0; i < EK_ROWS; ++i)
+#pragma unroll
+    for (int m = 0; m < NM; ++m) acc[i][m] = 0.f;
+  // 16-byte pieces of x of a segment: the workgroup's threads have one each of a place, or of two places (LPR 32)
+  constexpr int PIECES = SPAN / 8, AT_ONCE = 64 * EK_WAVES / PIECES, XN = (NM + AT_ONCE - 1) / AT_ONCE;
+  static_assert(AT_ONCE == 1 || AT_ONCE == 2, "threads for whole places");
+  const int piece = t % PIECES, second = t / PIECES;
+  u4 xp[XN];
+  auto fetch_x = [&](int s) {
+    const int k = s * SPAN + 8 * piece;
+#pragma unroll
+    for (int e = 0; e < XN; ++e) {
+      const w4_half* from = x[AT_ONCE * e];
+      if (AT_ONCE == 2 && second) from = x[2 * e + 1 < NM ? 2 * e + 1 : 2 * e];
+      xp[e] = u4{0u, 0u, 0u, 0u};
+      if (k < K) xp[e] = *(const u4*)(from + k);
+    }
+  };
+  fetch_x(0);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = EK_ROWS / 2; i < EK_ROWS; ++i) request(0, i);
+  __builtin_amdgcn_sched_barrier(0);
+  for (int s = 0; s < segments; ++s) {
+    if (s) __syncthreads();  // nobody reads the last segment any more
+#pragma unroll
+    for (int e = 0; e < XN; ++e) {
+      const int m = AT_ONCE * e + second;
+      if (m < NM) *(u4*)(xs + m * (SPAN * 2) + ek_x_at(piece)) = xp[e];
+    }
+    __syncthreads();
+    const bool past = s * SPAN + 32 * l >= K, more = s + 1 < segments;
+    if (more) fetch_x(s + 1);
+    u4 xv[NM][4];
+#pragma unroll
+    for (int m = 0; m < NM; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xv[m][j] = *(const u4*)(xs + m * (SPAN * 2) + ek_x_at(4 * l + j));
+#pragma unroll
+    for (int i = 0; i < EK_ROWS; ++i) {
+      const uint32_t si = past ? 0u : sc[i], zi = ASYM ? zw[i] : 8u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u4 av;
+        if constexpr (MX) {
+          h2 n[4];
+          dq_mx(w[i][j], mx_scale(si), n);
+          av = u4{as_u32(n[0]), as_u32(n[1]), as_u32(n[2]), as_u32(n[3])};
+        } else {
+          av = __builtin_bit_cast(u4, expand_word(w[i][j], as_h2(0xD400E400u + zi * 0x00100001u), splat_bits(si), mask, magic));
+        }
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][m] = dot2(as_h2(av[e]), as_h2(xv[m][j][e]), acc[i][m]);
+      }
+      if (more) request(s + 1, i);  // (its registers are free)
+    }
+  }
+  // the last lane of a row has its sum
+#pragma unroll
+  for (int i = 0; i < EK_ROWS; ++i)
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      float v = acc[i][m];
+      v = dpp_add<0xB1, 0xF>(v);   // (as wave_sum_to_lane63)
+      v = dpp_add<0x4E, 0xF>(v);
+      v = dpp_add<0x141, 0xF>(v);
+      v = dpp_add<0x140, 0xF>(v);
+      v = dpp_add<0x142, 0xA>(v);
+      if (LPR == 64) v = dpp_add<0x143, 0xC>(v);
+      acc[i][m] = v;
+    }
+  if (l != LPR - 1) return;
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+    if (pair[m] < 0) continue;
+    w4_half* const out = a.out + (size_t)(a.to_pairs ? pair[m] : tile.first + m) * width;
+#pragma unroll
+    for (int i = 0; i < EK_ROWS / (GATED ? 2 : 1); ++i) {
+      const float y = GATED ? expert_act(a.act, acc[i][m]) * acc[(i + EK_ROWS / 2) % EK_ROWS][m] : acc[i][m];
+      if (col_of(i) < width) out[col_of(i)] = __builtin_bit_cast(uint16_t, (_Float16)y);
+    }
+  }
+}
+
+template <int FMT, bool GATED, int LPR>
+__global__ __launch_bounds__(64 * EK_WAVES) void experts_token_kernel(ExpertArgs a, int columns, uint32_t group_mul) {
+  __shared__ __attribute__((aligned(16))) uint8_t xs[EK_PLACES * LPR * 64];
+  const ExpertTile tile = find_expert_tile<EK_PLACES, false, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
+  if (tile.rows == 0) return;
+  if (tile.rows == 1) return experts_token<FMT, GATED, LPR, 1>(a, tile, group_mul, xs);
+  if (tile.rows == 2) return experts_token<FMT, GATED, LPR, 2>(a, tile, group_mul, xs);
+  experts_token<FMT, GATED, LPR, 4>(a, tile, group_mul, xs);
+}
+
+template <int FMT, bool GATED, int LPR>
+hipError_t go(const ExpertArgs& a, hipStream_t s) {
+  const int R = a.v.N / a.experts, per = EK_WAVES * EK_ROWS * (64 / LPR) / (GATED ? 2 : 1);
+  const int columns = ((GATED ? R / 2 : R) + per - 1) / per;
+  const long long grid = (most_expert_tiles(a, EK_PLACES) * columns + 7) / 8 * 8;
+  if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
+  // the group of slice n of 32 k is (2 n group_mul) >> 32
+  const uint32_t d = a.v.mx ? 1 : a.v.gs / 32, mul = (uint32_t)(((1ull << 31) + d - 1) / d);
+  experts_token_kernel<FMT, GATED, LPR><<<dim3((unsigned)grid), dim3(64 * EK_WAVES), 0, s>>>(a, columns, mul);
+  return hipGetLastError();
+}
+
+template <int FMT>
+hipError_t go_shape(const ExpertArgs& a, hipStream_t s) {
+  if (a.v.K <= 1024) return a.act ? go<FMT, true, 32>(a, s) : go<FMT, false, 32>(a, s);
+  return a.act ? go<FMT, true, 64>(a, s) : go<FMT, false, 64>(a, s);
+}
+
+}  // namespace
+
+bool try_experts_token(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
+  const WView& v = a.v;
+  const long long R = v.N / a.experts, pairs = (long long)a.tokens * a.top_k;
+  if (v.K % 32 || (!v.mx && v.gs % 32) || v.K >= 1 << 20) return false;
+  if (R * v.K / 2 >= 1LL << 32) return false;  // offsets of 32 bits into an expert's codes
+  if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 1) || ((uintptr_t)v.zeros & 3)) return false;
+  // One row an expert mostly, and few enough rows of W that the time is latency: the vector ALUs do more for a word than the
+  // matrix cores' operands need (K 2048, 16384 rows of W in all 8.9 us against 11.0, 32768 15.9 against 12.2).
+  if (pairs > a.experts || pairs * R > 30000) return false;
+  *err = v.mx ? go_shape<2>(a, s) : v.symmetric ? go_shape<0>(a, s) : go_shape<1>(a, s);
+  return true;
+}
+
+}  // namespace w4k
