@@ -1,7 +1,7 @@
 // Products of some rows per expert with the experts' packed matrices, where many experts have a few: decode steps of many
 // sequences, whose time is the reading of codes.
 //
-// A workgroup multiplies up to 16 places of one expert with 128 of its rows, 32 a wave (gated: 16 of the gate and the 16 of
+// A workgroup multiplies up to 16 (or 32) places of one expert with 128 of its rows, 32 a wave (gated: 16 of the gate and the 16 of
 // the way up for the same columns), in stages of 256 k.  Everything goes global -> LDS (no registers) in whole lines: a
 // load instruction that takes 16 bytes of each of 64 rows, as the operands need them, holds the memory path four times as
 // long.  The rows of x are fetched once for the four waves; a wave's codes, scales and zero-points are its own.  Two stage
@@ -20,8 +20,9 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 
 constexpr int ES_WAVES = 4;
 constexpr int ES_W = 4096;            // a wave's codes of a stage: 32 rows of 128 bytes
-constexpr int ES_X = 16 * 512;        // rows of x
-constexpr int ES_X_AT = ES_WAVES * ES_W, ES_STAGE = ES_X_AT + ES_X, ES_P_AT = 2 * ES_STAGE;
+constexpr int ES_X_AT = ES_WAVES * ES_W;                                // then rows of x, 512 bytes each
+constexpr int es_stage(int tm) { return ES_X_AT + tm * 512; }           // tm: places of a tile, 16 or 32
+constexpr int es_params_at(int tm) { return 2 * es_stage(tm); }
 
 // Scales and zero-points come for two stages at a time, a row's side by side: 64 dwords that touch as few lines as they can.
 // How the groups of W4 lie (GM): 0 gs 128, 1 gs 64, 2 gs 32 (and MXFP4's blocks), 3 any size that is a multiple of 32, from 96
@@ -53,10 +54,11 @@ __device__ __forceinline__ void es_dma4(const void* at, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(at), "s"(lds) : "memory", "m0");
 }
 
-// XI: load instructions of x per wave and stage, for up to 8 XI places.
-template <int FMT, bool GATED, int GM, int XI>
+// XI: load instructions of x per wave and stage, for up to 8 XI places; TM: places that the buffers have room for.
+template <int FMT, bool GATED, int GM, int TM, int XI>
 __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTile& tile, uint32_t group_mul, int dwords) {
   constexpr bool MX = FMT == 2, ASYM = FMT == 1;
+  constexpr int MT = (XI + 1) / 2, STAGE = es_stage(TM), PARAMS = es_params_at(TM);  // tiles of 16 places
   constexpr int PZ = es_zeros(FMT, GM), PI = (es_most(FMT, GM) + 1) / 2;  // load instructions of parameters at most
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -104,9 +106,9 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
     pd[i] = e - n * dwords;
     pe[i] = (row0 + row_of(n)) * (size_t)(pd[i] < ps ? G : wg);
   }
-  const uint32_t p_at = lds0 + ES_P_AT + wave * dwords * 128;
+  const uint32_t p_at = lds0 + PARAMS + wave * dwords * 128;
   auto request = [&](int d, int buf) {
-    const uint32_t st = lds0 + buf * ES_STAGE;
+    const uint32_t st = lds0 + buf * STAGE;
     const bool tail = d * 256 + 256 > K;  // pieces behind the end of a row are fetched from its part that is there
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -134,13 +136,17 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
   uint32_t mask = 0x00F0000Fu, magic = 0x54006400u;
   asm volatile("" : "+s"(mask));   // opaque: otherwise they come back as literals of two
   asm volatile("" : "+v"(magic));  // separate instructions
-  f4 acc[2] = {f4{0.f, 0.f, 0.f, 0.f}, f4{0.f, 0.f, 0.f, 0.f}};
+  f4 acc[2][MT];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[i][m] = f4{0.f, 0.f, 0.f, 0.f};
   uint32_t first[2];  // entry of the row's first scale in the whole array: its place in a dword
 #pragma unroll
   for (int i = 0; i < 2; ++i) first[i] = (uint32_t)((row0 + row_of(16 * i + r)) * G);
   const uint8_t* const mine = es_lds + wave * ES_W;
   const uint8_t* const xs = es_lds + ES_X_AT;
-  const uint8_t* const params = es_lds + ES_P_AT + wave * (dwords * 128);
+  const uint8_t* const params = es_lds + PARAMS + wave * (dwords * 128);
   uint32_t sc[2][2][2], zw[2][2][2];  // of two stages: of the lane's two pieces of a row
   // Scales and zero-points of both stages go into registers at the first: their place is free for the next two.
   auto read_params = [&](int d) {
@@ -182,7 +188,7 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
     }
     if (d + 1 < stages) request(d + 1, half ^ 1);
     __builtin_amdgcn_sched_barrier(0);
-    const uint32_t b0 = half * ES_STAGE;
+    const uint32_t b0 = half * STAGE;
     u4 w[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -191,10 +197,14 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
     const bool tail = d * 256 + 256 > K;
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      u4 x = *(const u4*)(xs + b0 + es_x_at(r, 8 * q + s));
+      u4 x[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[m] = *(const u4*)(xs + b0 + es_x_at(16 * m + r, 8 * q + s));
       const int p = s >> 2;
       const bool past = d * 256 + 64 * q + 32 * p >= K;
-      if (tail && past) x = u4{0u, 0u, 0u, 0u};  // what was fetched there counts as 0, and so do its codes
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        if (tail && past) x[m] = u4{0u, 0u, 0u, 0u};  // what was fetched there counts as 0, and so do its codes
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         h8 av;
@@ -205,7 +215,9 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
         } else {
           av = expand_word(w[i][p][s & 3], as_h2(0xD400E400u + zw[half][i][p] * 0x00100001u), splat_bits(tail && past ? 0u : sc[half][i][p]), mask, magic);
         }
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(h8, x), acc[i], 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, __builtin_bit_cast(h8, x[m]), acc[i][m], 0, 0, 0);
       }
     }
   };
@@ -216,63 +228,71 @@ __device__ __forceinline__ void experts_step(const ExpertArgs& a, const ExpertTi
     if (d + 1 < stages) stage(d + 1, 1);
   }
   // lane l of a 16 x 16 tile holds columns 4 (l / 16) + e of place l % 16
-  if (r >= tile.rows) return;
-  const int place = tile.first + r, pair = a.order[place];
-  if (pair < 0 || pair >= pairs) return;
-  w4_half* const out = a.out + (size_t)(a.to_pairs ? pair : place) * width;
 #pragma unroll
-  for (int i = 0; i < (GATED ? 1 : 2); ++i) {
-    const int col = c0 + 16 * i + 4 * q;
-    h4 y;
+  for (int m = 0; m < MT; ++m) {
+    if (16 * m + r >= tile.rows) continue;
+    const int place = tile.first + 16 * m + r, pair = a.order[place];
+    if (pair < 0 || pair >= pairs) continue;
+    w4_half* const out = a.out + (size_t)(a.to_pairs ? pair : place) * width;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (_Float16)(GATED ? expert_act(a.act, acc[0][e]) * acc[1][e] : acc[i][e]);
-    if (col + 4 <= width) {
-      __builtin_memcpy(out + col, &y, 8);
-    } else {
+    for (int i = 0; i < (GATED ? 1 : 2); ++i) {
+      const int col = c0 + 16 * i + 4 * q;
+      h4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < width) out[col + e] = __builtin_bit_cast(uint16_t, (_Float16)y[e]);
+      for (int e = 0; e < 4; ++e) y[e] = (_Float16)(GATED ? expert_act(a.act, acc[0][m][e]) * acc[1][m][e] : acc[i][m][e]);
+      if (col + 4 <= width) {
+        __builtin_memcpy(out + col, &y, 8);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < width) out[col + e] = __builtin_bit_cast(uint16_t, (_Float16)y[e]);
+      }
     }
   }
 }
 
-template <int FMT, bool GATED, int GM>
-__global__ __launch_bounds__(64 * ES_WAVES, 3) void experts_step_kernel(ExpertArgs a, int columns, uint32_t group_mul, int dwords) {
-  const ExpertTile tile = find_expert_tile<16, false, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
-  const int rows = __builtin_amdgcn_readfirstlane(tile.rows);
-  if (rows == 0) return;
-  const ExpertTile u{__builtin_amdgcn_readfirstlane(tile.expert), __builtin_amdgcn_readfirstlane(tile.first), rows,
-                     __builtin_amdgcn_readfirstlane(tile.column)};
-  if (rows > 8) return experts_step<FMT, GATED, GM, 2>(a, u, group_mul, dwords);
-  experts_step<FMT, GATED, GM, 1>(a, u, group_mul, dwords);
+template <int FMT, bool GATED, int GM, int TM>
+__global__ __launch_bounds__(64 * ES_WAVES, TM == 16 ? 3 : 2) void experts_step_kernel(ExpertArgs a, int columns, uint32_t group_mul, int dwords) {
+  const ExpertTile tile = find_expert_tile<TM, false, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
+  if (tile.rows == 0) return;
+  if constexpr (TM == 32) {
+    if (tile.rows > 24) return experts_step<FMT, GATED, GM, TM, 4>(a, tile, group_mul, dwords);
+    if (tile.rows > 16) return experts_step<FMT, GATED, GM, TM, 3>(a, tile, group_mul, dwords);
+  }
+  if (tile.rows > 8) return experts_step<FMT, GATED, GM, TM, 2>(a, tile, group_mul, dwords);
+  experts_step<FMT, GATED, GM, TM, 1>(a, tile, group_mul, dwords);
 }
 
-template <int FMT, bool GATED, int GM>
+template <int FMT, bool GATED, int GM, int TM>
 hipError_t go(const ExpertArgs& a, hipStream_t s) {
   // more than 64 KB of LDS has to be granted per device, once
-  constexpr int MOST = ES_P_AT + ES_WAVES * es_most(FMT, GM) * 128;
-  const int dwords = es_dwords(a, FMT, GM), LDS = ES_P_AT + ES_WAVES * dwords * 128;
+  constexpr int MOST = es_params_at(TM) + ES_WAVES * es_most(FMT, GM) * 128;
+  const int dwords = es_dwords(a, FMT, GM), LDS = es_params_at(TM) + ES_WAVES * dwords * 128;
   static std::atomic<bool> granted[64] = {};
   int dev = 0;
   if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
   if (dev < 0 || dev >= 64 || !granted[dev]) {
-    const hipError_t e = hipFuncSetAttribute((const void*)experts_step_kernel<FMT, GATED, GM>,
+    const hipError_t e = hipFuncSetAttribute((const void*)experts_step_kernel<FMT, GATED, GM, TM>,
                                              hipFuncAttributeMaxDynamicSharedMemorySize, MOST);
     if (e != hipSuccess) return e;
     if (dev >= 0 && dev < 64) granted[dev] = true;
   }
   const int R = a.v.N / a.experts, columns = GATED ? (R / 2 + 63) / 64 : (R + 127) / 128;
-  const long long grid = (most_expert_tiles(a, 16) * columns + 7) / 8 * 8;
+  const long long grid = (most_expert_tiles(a, TM) * columns + 7) / 8 * 8;
   if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
   // the group of slice n of 32 k is (2 n group_mul) >> 32
   const uint32_t d = a.v.mx ? 1 : a.v.gs / 32, mul = (uint32_t)(((1ull << 31) + d - 1) / d);
-  experts_step_kernel<FMT, GATED, GM><<<dim3((unsigned)grid), dim3(64 * ES_WAVES), LDS, s>>>(a, columns, mul, dwords);
+  experts_step_kernel<FMT, GATED, GM, TM><<<dim3((unsigned)grid), dim3(64 * ES_WAVES), LDS, s>>>(a, columns, mul, dwords);
   return hipGetLastError();
 }
 
 template <int FMT, int GM>
 hipError_t go_act(const ExpertArgs& a, hipStream_t s) {
-  return a.act ? go<FMT, true, GM>(a, s) : go<FMT, false, GM>(a, s);
+  // Room for 32 places costs a third workgroup: K 2048, 64 experts of 2048 rows, 16 rows each 46.7 us against 47.2 (MXFP4 40.0
+  // against 38.7), 32 each 59 against 69 (49 against 52).
+  const bool wide = (long long)a.tokens * a.top_k > 16LL * a.experts;
+  if (a.act) return wide ? go<FMT, true, GM, 32>(a, s) : go<FMT, true, GM, 16>(a, s);
+  return wide ? go<FMT, false, GM, 32>(a, s) : go<FMT, false, GM, 16>(a, s);
 }
 
 template <int FMT>
@@ -293,7 +313,9 @@ bool try_experts_step(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   // offsets of 32 bits: an expert's codes, rows of x
   if (R * v.K / 2 >= 1LL << 32 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
-  if ((pairs < a.experts ? pairs : a.experts) * R < 256 * 128) return false;
+  // A long K over few workgroups is a chain of stages of a microsecond each: the kernel that shares K out is ahead (8 experts
+  // of 1024 rows, K 4096, 32 rows: 12.1 us against 20.5; of 2048 rows, K 2048: 12.3 against 11.5).
+  if (v.K > 2048 && (pairs < a.experts ? pairs : a.experts) * R < 256 * 128) return false;
   *err = v.mx ? go_act<2, 2>(a, s) : v.symmetric ? go_groups<0>(a, s) : go_groups<1>(a, s);
   return true;
 }

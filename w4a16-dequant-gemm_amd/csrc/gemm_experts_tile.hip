@@ -1,6 +1,6 @@
 // Products of many rows per expert with the experts' packed matrices, on the matrix cores.
 //
-// A workgroup multiplies up to 256 (or 128) places of one expert with 256 of its rows:
+// A workgroup multiplies up to 128 places of one expert with 256 of its rows:
 //   * packed words and rows of x go global -> LDS (global_load_lds_dwordx4, no registers), a stage is 64 k: 32 bytes of
 //     a row of W, 128 of a row of x, wherever in x the place's token has it; three stage buffers, one barrier a stage;
 //   * v_mfma_f32_32x32x16_f16: a wave holds 64 rows of W against all rows of x.  Lane l brings row l % 32 and k
@@ -10,15 +10,14 @@
 //     wave per SIMD nothing else hides an instruction's latency;
 //   * gated experts: of a wave's two tiles of 32 rows the first is the gate's and the second the way up's for the same
 //     columns, so both sums of an output lie in one lane and the gate is taken in registers.
-// A tile with few places runs a loop of its own for 64, 128 or 192 of them: products of rows that are not there would
-// take as long as the others.
+// A tile of up to 64 places runs a loop of its own: products of rows that are not there would take as long as the others.
+// Two workgroups a compute unit: one's first loads and last stores go beside the other's products (tiles of 256 places,
+// one workgroup: 4096 tokens, 8 of 64 experts, K 2048, width 1024 320 us against 298; 2053 tokens, 2 of 8, K 14336 604
+// against 580).
 #include <atomic>
 
 #include "experts.cuh"
 
-#ifndef WIDE
-#define WIDE 160LL
-#endif
 namespace w4k {
 namespace {
 
@@ -30,10 +29,9 @@ constexpr int ET_W_BYTES = 256 * 32;
 constexpr int et_tile(int mj) { return ET_W_BYTES + mj * 32 * 128; }
 constexpr int et_stage(int mj) { return et_tile(mj) + 2 * 256 * 4; }  // + a scale dword and a zero-point word per row of W
 constexpr int ET_PITCH = 128 + 16;                                     // a wave's outputs of one place, padded
-constexpr int et_lds(int mj) {
-  return ET_STAGES * et_stage(mj) > ET_WAVES * mj * 32 * ET_PITCH ? ET_STAGES * et_stage(mj) : ET_WAVES * mj * 32 * ET_PITCH;
-}
-static_assert(et_lds(8) <= 160 * 1024 && 2 * et_lds(4) <= 160 * 1024, "one workgroup, or two, of a compute unit");
+constexpr int ET_PLACES = 128, ET_LDS = ET_STAGES * et_stage(ET_PLACES / 32);
+static_assert(2 * ET_LDS <= 160 * 1024, "two workgroups of a compute unit");
+static_assert(ET_LDS >= ET_WAVES * ET_PLACES * ET_PITCH, "the outputs fit the stage buffers");
 
 extern __shared__ __attribute__((aligned(16))) uint8_t et_lds_mem[];
 
@@ -259,10 +257,9 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
       __builtin_amdgcn_sched_barrier(0);
       if (c == 0) {  // operands of step 0 of stage d + 1: the words, their scales, x
         read_w(b1);
-        read_x(xv[0], b1, 0, 0, MJ < 4 ? MJ : 4);
+        read_x(xv[0], b1, 0, 0, MJ);
       }
       if (c == 1) {
-        if constexpr (MJ > 4) read_x(xv[0], b1, 0, 4, MJ);
         set_group(d + 1);
       }
       // the expansion goes under the last chunks: the words have only just been asked for
@@ -294,9 +291,6 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
   uint8_t* mine = et_lds_mem + wave * (32 * MJ * PITCH);
 #pragma unroll
   for (int j = 0; j < MJ; ++j) {
-    // the sums of a tile leave the accumulator registers only when its turn comes (256 of them copied out at once would not
-    // fit beside everything else)
-    if constexpr (MJ > 4) asm volatile("" : "+a"(acc[0][j]), "+a"(acc[1][j]));
 #pragma unroll
     for (int i = 0; i < (GATED ? 1 : NI); ++i)
 #pragma unroll
@@ -329,48 +323,36 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
   }
 }
 
-// TM: places of a tile at most, 256 (one workgroup a compute unit) or 128 (two).
-template <int FMT, bool GS32, bool GATED, int TM>
-__global__ __launch_bounds__(ET_THREADS, TM == 256 ? 1 : 2) void experts_tile_kernel(ExpertArgs a, int columns) {
-  const ExpertTile tile = find_expert_tile<TM, true, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
-  const int rows = __builtin_amdgcn_readfirstlane(tile.rows);
-  if (rows == 0) return;
-  const ExpertTile u{__builtin_amdgcn_readfirstlane(tile.expert), __builtin_amdgcn_readfirstlane(tile.first), rows,
-                     __builtin_amdgcn_readfirstlane(tile.column)};
-  if constexpr (TM == 256) {
-    if (rows > 192) return experts_tile<FMT, GS32, GATED, 8>(a, u);
-    if (rows > 128) return experts_tile<FMT, GS32, GATED, 6>(a, u);
-  }
-  if (rows > 64) return experts_tile<FMT, GS32, GATED, 4>(a, u);
-  experts_tile<FMT, GS32, GATED, 2>(a, u);
+template <int FMT, bool GS32, bool GATED>
+__global__ __launch_bounds__(ET_THREADS, 2) void experts_tile_kernel(ExpertArgs a, int columns) {
+  const ExpertTile tile = find_expert_tile<ET_PLACES, true, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
+  if (tile.rows == 0) return;
+  if (tile.rows > 64) return experts_tile<FMT, GS32, GATED, 4>(a, tile);
+  experts_tile<FMT, GS32, GATED, 2>(a, tile);
 }
 
-template <int FMT, bool GS32, bool GATED, int TM>
+template <int FMT, bool GS32, bool GATED>
 hipError_t go(const ExpertArgs& a, hipStream_t s) {
   // more than 64 KB of LDS has to be granted per device, once
-  constexpr int LDS = et_lds(TM / 32);
   static std::atomic<bool> granted[64] = {};
   int dev = 0;
   if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
   if (dev < 0 || dev >= 64 || !granted[dev]) {
-    const hipError_t e = hipFuncSetAttribute((const void*)experts_tile_kernel<FMT, GS32, GATED, TM>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    const hipError_t e = hipFuncSetAttribute((const void*)experts_tile_kernel<FMT, GS32, GATED>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, ET_LDS);
     if (e != hipSuccess) return e;
     if (dev >= 0 && dev < 64) granted[dev] = true;
   }
   const int R = a.v.N / a.experts, columns = GATED ? (R / 2 + 127) / 128 : (R + 255) / 256;
-  const long long grid = (most_expert_tiles(a, TM) * columns + 15) / 8 * 8;  // (an eighth per XCD, rounded up, of either kind)
+  const long long grid = (most_expert_tiles(a, ET_PLACES) * columns + 15) / 8 * 8;  // (an eighth per XCD, rounded up, of either kind)
   if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-  experts_tile_kernel<FMT, GS32, GATED, TM><<<dim3((unsigned)grid), dim3(ET_THREADS), LDS, s>>>(a, columns);
+  experts_tile_kernel<FMT, GS32, GATED><<<dim3((unsigned)grid), dim3(ET_THREADS), ET_LDS, s>>>(a, columns);
   return hipGetLastError();
 }
 
 template <int FMT, bool GS32>
-hipError_t go_rows(const ExpertArgs& a, hipStream_t s) {
-  const long long pairs = (long long)a.tokens * a.top_k;
-  const bool wide = pairs >= WIDE * a.experts;
-  if (a.act) return wide ? go<FMT, GS32, true, 256>(a, s) : go<FMT, GS32, true, 128>(a, s);
-  return wide ? go<FMT, GS32, false, 256>(a, s) : go<FMT, GS32, false, 128>(a, s);
+hipError_t go_act(const ExpertArgs& a, hipStream_t s) {
+  return a.act ? go<FMT, GS32, true>(a, s) : go<FMT, GS32, false>(a, s);
 }
 
 }  // namespace
@@ -385,10 +367,11 @@ bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32 || v.N * G * 4 >= 1LL << 32) return false;
   if (v.K >= 1 << 23 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
-  if (pairs < 32LL * a.experts) return false;
-  if (v.mx) *err = go_rows<2, false>(a, s);
-  else if (v.symmetric) *err = v.gs == 32 ? go_rows<0, true>(a, s) : go_rows<0, false>(a, s);
-  else *err = v.gs == 32 ? go_rows<1, true>(a, s) : go_rows<1, false>(a, s);
+  // K 2048, 64 experts of 2048 rows: 32 places each 71 us against 59 by the kernel for some rows, 64 each 80 against 92.
+  if (pairs < 48LL * a.experts) return false;
+  if (v.mx) *err = go_act<2, false>(a, s);
+  else if (v.symmetric) *err = v.gs == 32 ? go_act<0, true>(a, s) : go_act<0, false>(a, s);
+  else *err = v.gs == 32 ? go_act<1, true>(a, s) : go_act<1, false>(a, s);
   return true;
 }
 

@@ -192,9 +192,9 @@ bool try_experts_token(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   if (v.K % 32 || (!v.mx && v.gs % 32) || v.K >= 1 << 20) return false;
   if (R * v.K / 2 >= 1LL << 32) return false;  // offsets of 32 bits into an expert's codes
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 1) || ((uintptr_t)v.zeros & 3)) return false;
-  // One row an expert mostly, and few enough rows of W that the time is latency: the vector ALUs do more for a word than the
-  // matrix cores' operands need (K 2048, 16384 rows of W in all 8.9 us against 11.0, 32768 15.9 against 12.2).
-  if (pairs > a.experts || pairs * R > 30000) return false;
+  // Experts with a row each, mostly, and so few rows of W that the time is latency.  K 2048, 8 of 128 experts of 2048 rows: 8.2 us
+  // against 11.0 by the kernel that shares K out; 16 of 64: 15.4 against 12.3.  K 4096, 8 pairs on 8 experts: 12.8 against 10.8.
+  if (2 * pairs > a.experts || pairs * R > 30000) return false;
   *err = v.mx ? go_shape<2>(a, s) : v.symmetric ? go_shape<0>(a, s) : go_shape<1>(a, s);
   return true;
 }
