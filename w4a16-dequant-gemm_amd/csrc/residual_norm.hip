@@ -8,28 +8,41 @@ namespace w4k {
 namespace {
 
 // A piece is eight consecutive elements.  Rows of any length begin at any half, and the card loads 16 bytes from any
-// address, so a piece is one load whatever its alignment; the last of a row is cut short.
-__device__ __forceinline__ void load_halves(const w4_half* p, int n, float v[8]) {
-  if (n == 8) {
-    h8 x;
-    __builtin_memcpy(&x, p, 16);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
+// address at about the same rate (777 rows of 4098, 4100 or 4104: within 2 %), so a piece is one load whatever its
+// alignment.  The last piece of a row ends with the row: its first `skip` elements are the piece before's, count as 0 and
+// are not stored (777 rows of 4097: 11.8 us; 12.8 with its elements one by one, each array waited for).
+// WHOLE: rows have eight elements at least; n: elements of a shorter one.
+template <bool WHOLE>
+__device__ __forceinline__ u4 load_halves(const w4_half* p, int n) {
+  u4 v{0u, 0u, 0u, 0u};
+  if constexpr (WHOLE) {
+    __builtin_memcpy(&v, p, 16);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? half_bits_to_float(p[e]) : 0.f;
+    for (int e = 0; e < 8; ++e)
+      if (e < n) v[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
   }
+  return v;
 }
-__device__ __forceinline__ void load_floats(const float* p, int n, float v[8]) {
-  if (n == 8) {
-    __builtin_memcpy(v, p, 32);
+__device__ __forceinline__ float half_of(u4 v, int e) { return (float)__builtin_bit_cast(h8, v)[e]; }
+struct Floats {
+  float v[8];
+};
+template <bool WHOLE>
+__device__ __forceinline__ Floats load_floats(const float* p, int n) {
+  Floats f{};
+  if constexpr (WHOLE) {
+    __builtin_memcpy(f.v, p, 32);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : 0.f;
+    for (int e = 0; e < 8; ++e)
+      if (e < n) f.v[e] = p[e];
   }
+  return f;
 }
-__device__ __forceinline__ void store_halves(w4_half* p, int n, const float v[8]) {
-  if (n == 8) {
+// elements skip .. end - 1
+__device__ __forceinline__ void store_halves(w4_half* p, int skip, int end, const float v[8]) {
+  if (skip == 0 && end == 8) {
     h8 x;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (_Float16)v[e];
@@ -37,135 +50,171 @@ __device__ __forceinline__ void store_halves(w4_half* p, int n, const float v[8]
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < n) p[e] = __builtin_bit_cast(uint16_t, (_Float16)v[e]);
+      if (e >= skip && e < end) p[e] = __builtin_bit_cast(uint16_t, (_Float16)v[e]);
   }
 }
-__device__ __forceinline__ void store_floats(float* p, int n, const float v[8]) {
-  if (n == 8) {
+__device__ __forceinline__ void store_floats(float* p, int skip, int end, const float v[8]) {
+  if (skip == 0 && end == 8) {
     __builtin_memcpy(p, v, 32);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < n) p[e] = v[e];
+      if (e >= skip && e < end) p[e] = v[e];
   }
 }
 
-constexpr int RN_MAX_THREADS = 1024;
+constexpr int RN_MAX_THREADS = 1024, RN_AHEAD_THREADS = 256;
 
-// Sum over the workgroup, in the same order for every thread.
+// Sum over the workgroup, in the same order for every thread; lds: 16 floats that no other sum of the call has.
 __device__ __forceinline__ float group_sum(float v, float* lds) {
-  const int waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   v = wave_sum_to_lane63(v);
-  if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
+  if (waves == 1) return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+  if (lane == 63) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  float sum = 0.f;
-  for (int w = 0; w < waves; ++w) sum += lds[w];
-  __syncthreads();
-  return sum;
+  float w = lane < waves ? lds[lane] : 0.f;  // (up to 16 waves: a row of lanes)
+  w = dpp_add<0xB1, 0xF>(w);
+  w = dpp_add<0x4E, 0xF>(w);
+  w = dpp_add<0x141, 0xF>(w);
+  w = dpp_add<0x140, 0xF>(w);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, w)));
 }
 
-// PIECES: of a thread, every blockDim-th.
-template <int PIECES>
-__global__ __launch_bounds__(RN_MAX_THREADS) void residual_norm_kernel(NormArgs a) {
-  __shared__ float lds[RN_MAX_THREADS / 64];
+// PIECES: of a thread, every blockDim-th.  F32: the residual stream.  AHEAD: everything that a row needs is asked for at
+// once, ahead of the sums (4096 rows of 2048, 8 terms: 46.3 us without, 42.8 with; 777 rows of 4096, 512 threads a row,
+// whose registers then leave fewer rows on a compute unit: 10.0 and 11.3).
+template <int PIECES, bool F32, bool AHEAD, bool WHOLE>
+__global__ __launch_bounds__(AHEAD ? RN_AHEAD_THREADS : RN_MAX_THREADS) void residual_norm_kernel(NormArgs a) {
+  static_assert(!AHEAD || PIECES == 1, "one piece a thread");
+  __shared__ float lds[4][16];
   const int D = a.n.dim, t = threadIdx.x, step = blockDim.x;
   const long long tok = blockIdx.x, row = tok * D;
+  auto at = [&](int i) { return WHOLE ? min(8 * (t + i * step), D - 8) : 8 * (t + i * step); };
+  auto skip = [&](int i) { return WHOLE ? 8 * (t + i * step) - at(i) : 0; };
+  auto end = [&](int i) { return WHOLE ? 8 : D - at(i); };
+  auto has = [&](int i, int e) { return e >= skip(i) && e < end(i); };
+  auto get = [&](const w4_half* p, int i) { return p ? load_halves<WHOLE>(p + at(i), end(i)) : u4{0u, 0u, 0u, 0u}; };
+  const w4_half* const gates = a.n.gate ? a.n.gate + tok * a.n.gate_stride : nullptr;
+  [[maybe_unused]] u4 post{}, post_bias{}, gate{}, pre{}, pre_bias{}, r16{};
+  [[maybe_unused]] Floats r32{};
+  auto residual = [&](int i) {
+    if constexpr (F32) return load_floats<WHOLE>((const float*)a.residual + row + at(i), end(i));
+    else return load_halves<WHOLE>((const w4_half*)a.residual + row + at(i), end(i));
+  };
   float b[PIECES][8];
-  auto left = [&](int i) { return min(8, D - 8 * (t + i * step)); };
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int n = left(i), at = 8 * (t + i * step);
 #pragma unroll
     for (int e = 0; e < 8; ++e) b[i][e] = 0.f;
-    if (n <= 0) continue;
-    for (int j = 0; j < a.terms; ++j) {
-      const float w = a.weights ? a.weights[tok * a.terms + j] : 1.f;
-      if (w == 0.f) continue;
-      float v[8];
-      load_halves(a.y + (tok * a.terms + j) * D + at, n, v);
+    for (int j0 = 0; j0 < a.terms; j0 += 4) {  // four terms at a time
+      u4 y[4];
+      float w[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b[i][e] += w * v[e];
+      for (int j = 0; j < 4; ++j) {
+        w[j] = j0 + j < a.terms ? (a.weights ? a.weights[tok * a.terms + j0 + j] : 1.f) : 0.f;
+        y[j] = u4{0u, 0u, 0u, 0u};
+        if (w[j] != 0.f) y[j] = get(a.y + (tok * a.terms + j0 + j) * D, i);
+      }
+      if (AHEAD && j0 == 0) {
+        if constexpr (F32) r32 = residual(0);
+        else r16 = residual(0);
+        gate = get(gates, 0);
+        post = get(a.n.post, 0), post_bias = get(a.n.post_bias, 0);
+        pre = get(a.n.pre, 0), pre_bias = get(a.n.pre_bias, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[i][e] += w[j] * half_of(y[j], e);
+      }
     }
     if (a.shared) {
-      float v[8];
-      load_halves(a.shared + row + at, n, v);
+      const u4 v = get(a.shared + row, i);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) b[i][e] += v[e];
+      for (int e = 0; e < 8; ++e) b[i][e] += half_of(v, e);
     }
   }
-  // x becomes its norm without the weight
-  auto norm = [&]() {
+  // b becomes its norm without the weight
+  auto norm = [&](float* sums) {
     if (a.n.centred) {
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += b[i][e];
-      const float mean = group_sum(sum, lds) / (float)D;
+        for (int e = 0; e < 8; ++e) sum += has(i, e) ? b[i][e] : 0.f;
+      const float mean = group_sum(sum, sums) / (float)D;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[i][e] = e < left(i) ? b[i][e] - mean : 0.f;
+        for (int e = 0; e < 8; ++e) b[i][e] -= mean;
     }
     float sq = 0.f;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sq += b[i][e] * b[i][e];
-    const float f = 1.f / sqrtf(group_sum(sq, lds) / (float)D + a.n.eps);
+      for (int e = 0; e < 8; ++e) sq += has(i, e) ? b[i][e] * b[i][e] : 0.f;
+    const float f = 1.f / sqrtf(group_sum(sq, sums + 16) / (float)D + a.n.eps);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) b[i][e] *= f;
   };
-  auto scaled = [&](int i, const w4_half* weight, const w4_half* bias) {
-    const int n = left(i), at = 8 * (t + i * step);
-    float v[8];
-    load_halves(weight + at, n, v);
+  auto scaled = [&](int i, u4 weight, u4 bias, bool biased) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[i][e] *= v[e];
-    if (!bias) return;
-    load_halves(bias + at, n, v);
+    for (int e = 0; e < 8; ++e) b[i][e] *= half_of(weight, e);
+    if (!biased) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[i][e] += v[e];
+    for (int e = 0; e < 8; ++e) b[i][e] += half_of(bias, e);
   };
-  if (a.n.post) norm();
+  if (a.n.post) norm(lds[0]);
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int n = left(i), at = 8 * (t + i * step);
-    if (n <= 0) continue;
-    if (a.n.post) scaled(i, a.n.post, a.n.post_bias);
-    float v[8];
-    if (a.n.gate) {
-      load_halves(a.n.gate + tok * a.n.gate_stride + at, n, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[i][e] *= v[e];
+    if constexpr (!AHEAD) {
+      if constexpr (F32) r32 = residual(i);
+      else r16 = residual(i);
+      gate = get(gates, i);
+      post = get(a.n.post, i), post_bias = get(a.n.post_bias, i);
     }
-    if (a.f32) load_floats((const float*)a.residual + row + at, n, v);
-    else load_halves((const w4_half*)a.residual + row + at, n, v);
+    if (a.n.post) scaled(i, post, post_bias, a.n.post_bias);
+    if (gates) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) b[i][e] = v[e] + a.n.residual_scale * b[i][e];
-    if (a.f32) store_floats((float*)a.residual_out + row + at, n, b[i]);
-    else store_halves((w4_half*)a.residual_out + row + at, n, b[i]);
+      for (int e = 0; e < 8; ++e) b[i][e] *= half_of(gate, e);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[i][e] = (F32 ? r32.v[e] : half_of(r16, e)) + a.n.residual_scale * b[i][e];
+    if constexpr (F32) store_floats((float*)a.residual_out + row + at(i), skip(i), end(i), b[i]);
+    else store_halves((w4_half*)a.residual_out + row + at(i), skip(i), end(i), b[i]);
   }
   if (!a.h) return;
-  norm();
+  norm(lds[2]);
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
-    const int n = left(i);
-    if (n <= 0) continue;
-    scaled(i, a.n.pre, a.n.pre_bias);
-    store_halves(a.h + row + 8 * (t + i * step), n, b[i]);
+    if constexpr (!AHEAD) pre = get(a.n.pre, i), pre_bias = get(a.n.pre_bias, i);
+    scaled(i, pre, pre_bias, a.n.pre_bias);
+    store_halves(a.h + row + at(i), skip(i), end(i), b[i]);
   }
+}
+
+template <int PIECES, bool AHEAD, bool WHOLE>
+void go(const NormArgs& a, int threads, hipStream_t s) {
+  if (a.f32) residual_norm_kernel<PIECES, true, AHEAD, WHOLE><<<a.tokens, threads, 0, s>>>(a);
+  else residual_norm_kernel<PIECES, false, AHEAD, WHOLE><<<a.tokens, threads, 0, s>>>(a);
 }
 
 }  // namespace
 
+// A thread has a piece as long as that takes up to 512 threads (777 rows of 4096: 10.0 us, two pieces and 256 threads 10.1;
+// of 4104: 11.3 with two pieces, 12.0 with one and 576 threads, of which a compute unit has fewer rows).
 hipError_t launch_residual_norm(const NormArgs& a, hipStream_t s) {
-  const int pieces = (a.n.dim + 7) / 8, threads = pieces >= RN_MAX_THREADS ? RN_MAX_THREADS : (pieces + 63) / 64 * 64;
-  if (pieces <= RN_MAX_THREADS) residual_norm_kernel<1><<<a.tokens, threads, 0, s>>>(a);
-  else if (pieces <= 2 * RN_MAX_THREADS) residual_norm_kernel<2><<<a.tokens, threads, 0, s>>>(a);
-  else residual_norm_kernel<4><<<a.tokens, threads, 0, s>>>(a);
+  const int pieces = (a.n.dim + 7) / 8;
+  int per = 1;
+  while (per < 4 && pieces > per * 512) per *= 2;
+  const int threads = ((pieces + per - 1) / per + 63) / 64 * 64;
+  if (a.n.dim < 8) go<1, false, false>(a, threads, s);
+  else if (threads <= RN_AHEAD_THREADS && per == 1) go<1, true, true>(a, threads, s);
+  else if (per == 1) go<1, false, true>(a, threads, s);
+  else if (per == 2) go<2, false, true>(a, threads, s);
+  else go<4, false, true>(a, threads, s);
   return hipGetLastError();
 }
 
