@@ -459,11 +459,26 @@ inline void attention_f8_pages(const DeviceF8Pages& p, const DevicePagedBatch& b
 }
 
 // ---- a feed-forward block of experts (additive; no reference counterpart) ------------
-// The structs are w4_abi.h's own: their pointers are device memory.
+// w4_abi.h has the meaning of each member; pointers are device memory.
 using Router = w4_router;
 using DeviceExpertRows = w4_expert_rows;
-using DeviceBlockNorm = w4_block_norm;
+struct DeviceBlockNorm {
+  int dim, centred;
+  float eps, residual_scale;
+  const __half* post;
+  const __half* post_bias;
+  const __half* gate;
+  int gate_stride;
+  const __half* pre;
+  const __half* pre_bias;
+};
 enum class Act { none = 0, silu = 1, gelu = 2 };
+namespace detail {
+inline w4_block_norm abi(const DeviceBlockNorm& n) {
+  return w4_block_norm{n.dim, n.centred, n.eps, n.residual_scale, h(n.post), h(n.post_bias), h(n.gate),
+                       n.gate_stride, h(n.pre), h(n.pre_bias)};
+}
+}  // namespace detail
 
 inline size_t route_experts_workspace(const Router& r, int tokens) {
   size_t bytes = 0;
@@ -499,13 +514,15 @@ inline void gemm_experts(const DevicePackedWm& p, const DeviceExpertRows& rows, 
 inline void residual_norm(const DeviceBlockNorm& n, int tokens, int terms, const __half* y,
                           const float* weights, const __half* shared, const float* residual,
                           float* residual_out, __half* h, hipStream_t stream = 0) {
-  detail::raise(w4_residual_norm(&n, tokens, terms, detail::h(y), weights, detail::h(shared),
+  const auto v = detail::abi(n);
+  detail::raise(w4_residual_norm(&v, tokens, terms, detail::h(y), weights, detail::h(shared),
                                  residual, 1, residual_out, detail::h(h), stream));
 }
 inline void residual_norm(const DeviceBlockNorm& n, int tokens, int terms, const __half* y,
                           const float* weights, const __half* shared, const __half* residual,
                           __half* residual_out, __half* h, hipStream_t stream = 0) {
-  detail::raise(w4_residual_norm(&n, tokens, terms, detail::h(y), weights, detail::h(shared),
+  const auto v = detail::abi(n);
+  detail::raise(w4_residual_norm(&v, tokens, terms, detail::h(y), weights, detail::h(shared),
                                  residual, 0, residual_out, detail::h(h), stream));
 }
 
