@@ -159,10 +159,10 @@ __device__ __forceinline__ double one_over(double d) {
 
 // ---- one token ----------------------------------------------------------------------------------
 
-// Routes token `tok` with the LANES lanes that call it together, lane `l` of them; its k choices are left in ids, in
-// LDS.  KEY: what is compared.
+// Routes token `tok` with the LANES lanes that call it together, lane `l` of them; its k choices are left in ids and
+// their logits in ls, in LDS.  KEY: what is compared.
 template <class KEY, int LANES, int NE>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, bool there, int* ids) {
+__device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, bool there, int* ids, float* ls) {
   constexpr bool EXACT = std::is_same_v<KEY, double>;
   const int E = a.r.experts, k = a.r.top_k;
   // a group has `wide` lanes of its own, of which the last may have fewer than NE
@@ -239,7 +239,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
         b2 = fmax(b2, fmin(b1, c[i]));
         b1 = fmax(b1, c[i]);
       }
-      const int lane = threadIdx.x & 63, of = lane - l;
+      const int of = (threadIdx.x & 63) - l;
       if ((wide & (wide - 1)) == 0) {  // the group's lanes are an aligned power of two
         auto join = [&](KEY d1, KEY d2) {
           b2 = fmax(fmax(b2, d2), fmin(b1, d1));
@@ -283,6 +283,9 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
     const int u = __builtin_bit_cast(int, (float)c[i] + 0.f);  // (-0 is 0)
     f[i] = c[i] > NONE ? u ^ (u >> 31 & 0x7FFFFFFF) : NOTHING;
   }
+  const int lane = threadIdx.x & 63;
+  const unsigned long long lower = ((1ull << lane) - 1) & ~((1ull << (lane - l)) - 1);  // the token's lanes before this one
+  const unsigned long long others = (LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1) << (lane - l)) & ~(1ull << lane);
   for (int j = 0; j < k; ++j) {
     int m = f[0];
 #pragma unroll
@@ -296,10 +299,9 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
       if (EXACT) twice |= f[i] == m && out < NE;
       out = f[i] == m ? i : out;
     }
+    unsigned long long have = __ballot(out < NE);
     if constexpr (EXACT) {
-      const unsigned long long have = __ballot(out < NE && found);
-      const unsigned long long lanes = LANES == 64 ? ~0ull : ((1ull << (LANES & 63)) - 1) << (threadIdx.x & 63 & ~(LANES - 1));
-      if (__any((twice && found) || __popcll(have & lanes) > 1)) {
+      if (__any(found && (twice || __popcll(have & (others | 1ull << lane)) > 1))) {
         KEY d = NONE;
 #pragma unroll
         for (int i = 0; i < NE; ++i) d = f[i] == m ? fmax(d, c[i]) : d;
@@ -307,13 +309,19 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
         out = NE;
 #pragma unroll
         for (int i = NE - 1; i >= 0; --i) out = f[i] == m && c[i] == d ? i : out;
+        have = __ballot(out < NE);
       }
     }
-    const int own = out < NE ? e0 + out : RT_MAX_E, at = lanes_all<LANES>(own, Least());
-    out = own == at ? out : NE;
+    // of the lanes that have it the first: its experts are the lowest
+    const bool won = out < NE && !(have & lower);
+    out = won ? out : NE;
+    float v = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) f[i] = i == out ? NOTHING : f[i];
-    if (l == 0) ids[j] = found ? at : -1;
+    for (int i = 0; i < NE; ++i) {
+      v = i == out ? lg[i] : v;
+      f[i] = i == out ? NOTHING : f[i];
+    }
+    if (won) ids[j] = found ? e0 + out : -1, ls[j] = v;
   }
   __builtin_amdgcn_wave_barrier();  // (a wave's LDS writes are read by the same wave, in order)
   // Weights.  Those that are divided by their sum are taken relative to the largest chosen score: however far below the
@@ -324,8 +332,7 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int tok, int l, 
     const int j = l + n * LANES;
     lj[n] = -INFINITY;
     if (j >= k || ids[j] < 0) continue;
-    const long long at = (long long)tok * a.stride + ids[j];
-    lj[n] = a.f32 ? fminf(((const float*)a.logits)[at], 3.4028234663852886e38f) : fminf((float)((const _Float16*)a.logits)[at], 65504.f);
+    lj[n] = ls[j];
     most = fmaxf(most, lj[n]);
   }
   if (a.r.renorm) most = lanes_all<LANES>(most, Most());
@@ -360,6 +367,7 @@ template <class KEY, int LANES, int NE, bool ONE>
 __global__ __launch_bounds__((ONE ? one_threads<KEY, NE>() : rt_threads(LANES, NE))) void route_kernel(RouteArgs a, int passes, uint16_t* counts, int padded) {
   constexpr int SLOTS = ONE ? RT_ONE : rt_threads(LANES, NE) / LANES;
   __shared__ int ids[SLOTS * RT_MAX_K];
+  __shared__ float ls[(ONE ? one_threads<KEY, NE>() / LANES : SLOTS) * RT_MAX_K];
   __shared__ int chosen[RT_MAX_E];
   __shared__ SortSpace sort[ONE ? 1 : 0 + 1];
   const int t = threadIdx.x, l = t % LANES, E = a.r.experts, k = a.r.top_k;
@@ -374,7 +382,7 @@ __global__ __launch_bounds__((ONE ? one_threads<KEY, NE>() : rt_threads(LANES, N
     const int slot = t / LANES, mine = ONE ? p * at_once + slot : slot, tok = first + p * at_once + slot;
     if (ONE && mine >= RT_ONE) continue;
     int* const my_ids = ids + mine * k;
-    route_token<KEY, LANES, NE>(a, tok, l, tok < there, my_ids);
+    route_token<KEY, LANES, NE>(a, tok, l, tok < there, my_ids, ls + slot * k);
     if (tok < there)
       for (int j = l; j < k; j += LANES)
         if (my_ids[j] >= 0) atomicAdd(&chosen[my_ids[j]], 1);
