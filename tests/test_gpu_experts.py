@@ -162,6 +162,16 @@ def test_larger(T, k, E, width, K, fmt, gs):
     Products(T + 1, T, k, E, width, K, fmt, gs, 0, False, True).call().check()
 
 
+@pytest.mark.parametrize("fmt,gs", [(0, 32), (0, 64), (0, 96), (0, 128), (0, 192), (0, 256), (0, 384), (0, 512), (1, 32), (1, 64),
+                                    (1, 96), (1, 128), (1, 192), (1, 256), (1, 384), (1, 512), (2, 32)])
+@pytest.mark.parametrize("K", [576, 1600, 2112, 3136])
+def test_groups_along_a_long_row(K, fmt, gs):
+    """Every kernel: a row an expert, some, dozens, hundreds; the last group, chunk, stage and window are cut short."""
+    for T in (1, 20, 90, 300):
+        Products(K + T, T, 2 if T > 1 else 1, 4, 40, K, fmt, gs, 1).call().check()
+        Products(K + T + 1, T, 2 if T > 1 else 1, 3, 35 if K % 128 else 36, K, fmt, gs, 0, False, True).call().check()
+
+
 @pytest.mark.parametrize("T", [3, 30, 300])
 def test_rows_that_are_not_finite_stay_in_their_row(T):
     p = Products(T, T, 2, 4, 64, 256, 0, 64, 0, True, True)

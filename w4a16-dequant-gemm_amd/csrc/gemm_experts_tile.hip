@@ -13,7 +13,7 @@
 // A tile of up to 64 places runs a loop of its own: products of rows that are not there would take as long as the others.
 // Two workgroups a compute unit: one's first loads and last stores go beside the other's products (tiles of 256 places,
 // one workgroup: 4096 tokens, 8 of 64 experts, K 2048, width 1024 320 us against 298; 2053 tokens, 2 of 8, K 14336 604
-// against 580).
+// against 580, with parameters stage by stage).
 #include <atomic>
 
 #include "experts.cuh"
@@ -26,12 +26,21 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 
 constexpr int ET_THREADS = 256, ET_WAVES = 4, ET_STAGES = 3;
 constexpr int ET_W_BYTES = 256 * 32;
-constexpr int et_tile(int mj) { return ET_W_BYTES + mj * 32 * 128; }
-constexpr int et_stage(int mj) { return et_tile(mj) + 2 * 256 * 4; }  // + a scale dword and a zero-point word per row of W
+constexpr int et_stage(int mj) { return ET_W_BYTES + mj * 32 * 128; }
 constexpr int ET_PITCH = 128 + 16;                                     // a wave's outputs of one place, padded
-constexpr int ET_PLACES = 128, ET_LDS = ET_STAGES * et_stage(ET_PLACES / 32);
-static_assert(2 * ET_LDS <= 160 * 1024, "two workgroups of a compute unit");
-static_assert(ET_LDS >= ET_WAVES * ET_PLACES * ET_PITCH, "the outputs fit the stage buffers");
+constexpr int ET_PLACES = 128, ET_PARAMS_AT = ET_STAGES * et_stage(ET_PLACES / 32);
+
+// Scales and zero-points come for a window of four stages (gs 32: two), a row's dwords side by side: a load instruction
+// that takes one dword of each of 64 rows goes through as many lines as 4 KB of x (one a stage: MXFP4, 2053 tokens, 2 of 8,
+// K 14336, width 4096 590 us against 528; W4 within 2 % either way).
+// Of a window a row has two dwords of scales, or three where its run may begin at an odd half (MXFP4: byte) of the first:
+// four halves (gs 32, 64), two (gs 128), one (multiples of 256), eight bytes, counted from an even one on.  And a word of
+// zero-points, in which a window lies whole.
+constexpr int ET_SCALES = 3, ET_WINDOW = ET_WAVES * 64 * 4;  // dwords of scales at most; bytes of one dword of every row
+constexpr int et_lds(int scales, int zeros) { return ET_PARAMS_AT + 2 * ET_WINDOW * (scales + zeros); }
+static_assert(2 * et_lds(ET_SCALES, 1) <= 160 * 1024, "two workgroups of a compute unit");
+static_assert(et_lds(2, 0) >= ET_WAVES * ET_PLACES * ET_PITCH, "the outputs fit the stage buffers");
+int et_scales(const WView& v) { return (v.mx ? v.B % 4 : v.gs == 64 && v.G % 2) ? 3 : 2; }
 
 extern __shared__ __attribute__((aligned(16))) uint8_t et_lds_mem[];
 
@@ -55,19 +64,20 @@ __device__ __forceinline__ void et_dma4(const void* base, uint32_t off, uint32_t
 // FMT: 0 W4 symmetric, 1 W4 with zero-points, 2 MXFP4.  GS32: W4 groups of 32 (a lane's 32 k of a stage are one group, the
 // stage two); otherwise gs is a multiple of 64 and a stage lies in one group.  MJ: 32-row tiles of x.
 template <int FMT, bool GS32, bool GATED, int MJ>
-__device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTile& tile) {
+__device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTile& tile, int scales, uint32_t group_mul) {
   constexpr bool ASYM = FMT == 1, MX = FMT == 2;
   constexpr int NI = 2;
   constexpr int WI = 8 / ET_WAVES, XI = 4 * MJ / ET_WAVES;  // 1 KB load instructions of W and of x per wave and stage
-  constexpr int LOADS = WI + XI + 1 + (ASYM ? 1 : 0);
+  constexpr int LOADS = WI + XI;
+  constexpr int WINDOW = GS32 ? 2 : 4;  // stages that parameters come for
   constexpr int CH = NI * MJ / 4;  // chunks of four products per 16-k step
   constexpr int PPC = (LOADS + 4 * CH - 1) / (4 * CH);  // load instructions of a chunk
-  constexpr int TILE = et_tile(MJ), STAGE = et_stage(MJ);
-  static_assert(2 * LOADS < 64, "a stage's requests fit the counter");
+  constexpr int STAGE = et_stage(MJ);
+  static_assert(2 * LOADS + ET_SCALES + 1 < 64, "two stages' requests fit the counter");
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // in an SGPR: LDS addresses go to M0
   const int r = lane & 31, h = lane >> 5;
-  const int K = a.v.K, G = MX ? a.v.B : a.v.G, gs = a.v.gs, wg = words(G), pairs = a.tokens * a.top_k;
+  const int K = a.v.K, G = MX ? a.v.B : a.v.G, wg = words(G), pairs = a.tokens * a.top_k;
   const int R = a.v.N / a.experts, width = GATED ? R / 2 : R;
   const int c0 = tile.column * (GATED ? 128 : 256);  // first output column
   // row of the expert that row n of the tile is; columns past the last repeat it and are not stored
@@ -93,13 +103,37 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
     }
     xo[i] = from * (uint32_t)(K * 2) + (((lane & 7) ^ et_x_key(m)) * 16);
   }
-  // per stage: the dword that holds the scale(s) of row 64 wave + lane, and (ASYM) the word that holds its zero-point
-  const uint32_t row0 = (uint32_t)tile.expert * (uint32_t)R;
-  const uint32_t sn = row0 + row_of(wave * 64 + lane);
-  const uint32_t sc_base = sn * (uint32_t)G, zw_base = sn * (uint32_t)wg;
+  // Parameters of a window: of the wave's 64 rows, entry e of scales is dword e % scales of row e / scales.  Indexes in
+  // dwords from the expert's first on; the last of the array is not passed.
+  const size_t row0 = (size_t)tile.expert * R, left = (size_t)(a.v.N - tile.expert * R);
+  const char* const sb = (const char*)a.v.scales + row0 * G * (MX ? 1 : 2);
+  const uint32_t odd0 = MX ? (uint32_t)(row0 * G) & 3u : (uint32_t)(row0 * G) & 1u;  // (the expert's first scale in its dword)
+  const char* const sd = sb - odd0 * (MX ? 1 : 2);
+  const uint32_t* const zb = a.v.zeros + row0 * wg;
+  const uint32_t sc_last = (uint32_t)min((left * G + odd0) / (MX ? 4 : 2) - 1, (size_t)0x3FFFFFFF);
+  uint32_t se[ET_SCALES];
+#pragma unroll
+  for (int i = 0; i < ET_SCALES; ++i) {
+    const uint32_t e = 64 * i + lane, n = min(scales == 2 ? e >> 1 : e / 3u, 63u);
+    se[i] = (((uint32_t)row_of(wave * 64 + n) * (uint32_t)G + odd0) >> (MX ? 2 : 1)) + (e - n * (uint32_t)scales);
+  }
+  [[maybe_unused]] const uint32_t ze = (uint32_t)row_of(wave * 64 + lane) * (uint32_t)wg;
   const int stages = K >> 6;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)et_lds_mem;
-  auto group_of = [&](uint32_t d) { return GS32 ? 2u * d : (d * 64u) / (uint32_t)gs; };  // of the stage's first k (W4)
+  // group (MXFP4: block) of a stage's first k, and the even one that its window begins with
+  auto group_of = [&](uint32_t d) { return GS32 || MX ? 2u * d : __umulhi(4u * d, group_mul); };
+  auto window_group = [&](uint32_t d) { return group_of(d / WINDOW * WINDOW) & ~1u; };
+  const uint32_t s_at = ET_PARAMS_AT + wave * 256 * scales, z_at = ET_PARAMS_AT + 2 * ET_WINDOW * scales + wave * 256;
+  // of the window that begins with stage d, ahead of that stage's other requests
+  auto request_params = [&](int d) {
+    if (d % WINDOW || d >= stages) return;
+    const uint32_t g = window_group((uint32_t)d), second = d / WINDOW & 1;
+#pragma unroll
+    for (int i = 0; i < ET_SCALES; ++i)
+      if (i < scales)
+        et_dma4(sd, min(se[i] + (g >> (MX ? 2 : 1)), sc_last) * 4u, lds0 + s_at + second * (ET_WINDOW * scales) + i * 256);
+    if constexpr (ASYM) et_dma4(zb, (ze + (g >> 3)) * 4u, lds0 + z_at + second * ET_WINDOW);
+  };
   // Load instruction `part` (0 .. LOADS - 1) of stage d into the buffer at byte offset buf.  A stage past the last is
   // fetched from the last one and never used.
   auto request_part = [&](int d, uint32_t buf, int part) {
@@ -109,21 +143,17 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
       et_dma16(wqb + dd * 32u, wo[part], st + (wave + ET_WAVES * part) * 1024);
     } else if (part < WI + XI) {
       et_dma16(xb + dd * 128u, xo[part - WI], st + ET_W_BYTES + (wave + ET_WAVES * (part - WI)) * 1024);
-    } else if (part == WI + XI) {
-      // MXFP4: the dword around the stage's two E8M0 bytes; gs = 32: the dword of its two scales; else the one around its scale
-      const uint32_t off = MX ? ((sc_base + 2u * dd) & ~3u)
-                              : GS32 ? (sc_base + 2u * dd) * 2u : ((sc_base + group_of(dd)) >> 1) * 4u;
-      et_dma4(a.v.scales, off, st + TILE + wave * 256);
-    } else if (ASYM && part == WI + XI + 1) {
-      et_dma4(a.v.zeros, (zw_base + (group_of(dd) >> 3)) * 4u, st + TILE + 1024 + wave * 256);
     }
   };
 
-  // this lane's rows of the two tiles of its wave, and where their first scale sits in the dword fetched around it
+  // where the window's first scale of this lane's rows of the two tiles of its wave lies
   const int wrow0 = wave * 64 + r;
-  uint32_t par[NI];
+  uint32_t sc_at[NI];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) par[i] = ((row0 + row_of(wrow0 + 32 * i)) * (uint32_t)G) & (MX ? 3u : 1u);
+  for (int i = 0; i < NI; ++i) {
+    const uint32_t in = ((uint32_t)row_of(wrow0 + 32 * i) * (uint32_t)G + odd0) & (MX ? 3u : 1u);
+    sc_at[i] = s_at + (r + 32 * i) * 4 * scales + (MX ? in + h : 2 * (in + (GS32 ? h : 0)));
+  }
   uint32_t mask = 0x00F0000Fu, magic = 0x54006400u;
   asm volatile("" : "+s"(mask));   // opaque: otherwise they come back as literals of two
   asm volatile("" : "+v"(magic));  // separate instructions
@@ -137,33 +167,33 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
   uint32_t xoff[4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) xoff[u] = ET_W_BYTES + et_x_at(r, 4 * h + u);
-  const uint32_t woff = et_w_at(wrow0, h), scoff = TILE + wrow0 * 4;
+  const uint32_t woff = et_w_at(wrow0, h);
   auto read_x = [&](u4* dst, uint32_t buf, int u, int j0, int j1) {
     const uint8_t* p = et_lds_mem + (buf + xoff[u]);
 #pragma unroll
     for (int j = j0; j < j1; ++j) dst[j] = *(const u4*)(p + j * 4096);
   };
-  auto read_w = [&](uint32_t buf) {
+  auto read_w = [&](uint32_t buf, int d) {
     const uint8_t* p = et_lds_mem + (buf + woff);
 #pragma unroll
     for (int i = 0; i < NI; ++i) wv[i] = *(const u4*)(p + i * 1024);
-    p = et_lds_mem + (buf + scoff);
+    const uint32_t second = d / WINDOW & 1, g = group_of((uint32_t)d);
+    p = et_lds_mem + (second * (ET_WINDOW * scales) + (g - window_group((uint32_t)d)) * (MX ? 1 : 2));
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      sc[i] = *(const uint32_t*)(p + i * 128);
-      if (ASYM) zw[i] = *(const uint32_t*)(p + 1024 + i * 128);
+      if (MX) sc[i] = p[sc_at[i]];
+      else sc[i] = *(const uint16_t*)(p + sc_at[i]);
+      if (ASYM) zw[i] = *(const uint32_t*)(et_lds_mem + (z_at + second * ET_WINDOW) + (r + 32 * i) * 4) >> (4 * ((g + (GS32 ? h : 0)) & 7));
     }
   };
-  auto set_group = [&](int d) {
+  auto set_group = [&]() {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      if constexpr (MX) {  // block 2 d + h of the row
-        sf[i] = mx_scale((sc[i] >> (8 * (((par[i] + 2u * d) & 3u) + h))) & 0xFFu);
+      if constexpr (MX) {
+        sf[i] = mx_scale(sc[i]);
       } else {
-        const uint32_t g = group_of((uint32_t)d) + (GS32 ? h : 0);
-        const bool hi = GS32 ? h != 0 : ((par[i] + g) & 1u) != 0;
-        s2v[i] = splat_bits(hi ? (sc[i] >> 16) : (sc[i] & 0xFFFFu));
-        const uint32_t z = ASYM ? ((zw[i] >> (4 * (g & 7))) & 0xFu) : 8u;
+        s2v[i] = splat_bits(sc[i]);
+        const uint32_t z = ASYM ? zw[i] & 0xFu : 8u;
         cneg[i] = as_h2(0xD400E400u | (z << 20) | z);
       }
     }
@@ -206,17 +236,19 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
   // offsets of the buffers of stages d, d + 1, d + 2 (d + 3 takes b0 again).
   uint32_t b0 = 0, b1 = STAGE, b2 = 2 * STAGE;
   constexpr int AHEAD = PPC * CH < LOADS ? PPC * CH : LOADS;
+  request_params(0);
 #pragma unroll
   for (int part = 0; part < LOADS; ++part) request_part(0, b0, part);
 #pragma unroll
   for (int part = 0; part < LOADS; ++part) request_part(1, b1, part);
+  if (GS32) request_params(2);
 #pragma unroll
   for (int part = 0; part < AHEAD; ++part) request_part(2, b2, part);
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS + AHEAD));  // stage 0 has landed
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS + AHEAD));  // stage 0 has landed, its parameters with it
   __syncthreads();
   read_x(xv[0], b0, 0, 0, MJ);
-  read_w(b0);
-  set_group(0);
+  read_w(b0, 0);
+  set_group();
 #pragma unroll
   for (int ph = 0; ph < 4; ++ph) expand_phase(ph, av[0], tmp, 0, 0, 8);
   auto mfma1 = [&](int cur, int c, int k) {  // product 4 c + k of a step
@@ -247,8 +279,11 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
     // Step 3.  Every LDS read of stage d has been issued (the operands of x of this step during step 2, the words at the
     // stage's start): once all waves are here its buffer can take stage d + 3, and stage d + 1 has landed for everyone
     // (outstanding: all of stage d + 2).
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS));
+    // (a window that begins with stage d + 2 has its parameters, two dwords at least, ahead of the stage's other loads)
+    if ((d + 2) % WINDOW == 0 && d + 2 < stages) __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS + 2));
+    else __builtin_amdgcn_s_waitcnt(waitcnt_vm(LOADS));
     __syncthreads();
+    request_params(d + 3);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
 #pragma unroll
@@ -256,11 +291,11 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
         if (PPC * c + p < LOADS) request_part(d + 3, b0, PPC * c + p);
       __builtin_amdgcn_sched_barrier(0);
       if (c == 0) {  // operands of step 0 of stage d + 1: the words, their scales, x
-        read_w(b1);
+        read_w(b1, d + 1 < stages ? d + 1 : d);
         read_x(xv[0], b1, 0, 0, MJ);
       }
       if (c == 1) {
-        set_group(d + 1);
+        set_group();
       }
       // the expansion goes under the last chunks: the words have only just been asked for
       constexpr int FROM = CH >= 2 ? (CH + 1) / 2 : 0;
@@ -273,7 +308,7 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (CH == 1) {
-      set_group(d + 1);
+      set_group();
 #pragma unroll
       for (int ph = 0; ph < 4; ++ph) expand_phase(ph, av[0], tmp, 0, 0, 8);
     }
@@ -324,11 +359,11 @@ __device__ __forceinline__ void experts_tile(const ExpertArgs& a, const ExpertTi
 }
 
 template <int FMT, bool GS32, bool GATED>
-__global__ __launch_bounds__(ET_THREADS, 2) void experts_tile_kernel(ExpertArgs a, int columns) {
+__global__ __launch_bounds__(ET_THREADS, 2) void experts_tile_kernel(ExpertArgs a, int columns, int scales, uint32_t group_mul) {
   const ExpertTile tile = find_expert_tile<ET_PLACES, true, true>(a.offsets, a.experts, a.tokens * a.top_k, columns, blockIdx.x);
   if (tile.rows == 0) return;
-  if (tile.rows > 64) return experts_tile<FMT, GS32, GATED, 4>(a, tile);
-  experts_tile<FMT, GS32, GATED, 2>(a, tile);
+  if (tile.rows > 64) return experts_tile<FMT, GS32, GATED, 4>(a, tile, scales, group_mul);
+  experts_tile<FMT, GS32, GATED, 2>(a, tile, scales, group_mul);
 }
 
 template <int FMT, bool GS32, bool GATED>
@@ -339,14 +374,17 @@ hipError_t go(const ExpertArgs& a, hipStream_t s) {
   if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
   if (dev < 0 || dev >= 64 || !granted[dev]) {
     const hipError_t e = hipFuncSetAttribute((const void*)experts_tile_kernel<FMT, GS32, GATED>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, ET_LDS);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, et_lds(ET_SCALES, 1));
     if (e != hipSuccess) return e;
     if (dev >= 0 && dev < 64) granted[dev] = true;
   }
   const int R = a.v.N / a.experts, columns = GATED ? (R / 2 + 127) / 128 : (R + 255) / 256;
   const long long grid = (most_expert_tiles(a, ET_PLACES) * columns + 15) / 8 * 8;  // (an eighth per XCD, rounded up, of either kind)
   if (grid > 0x7FFFFFFFLL) return hipErrorInvalidConfiguration;
-  experts_tile_kernel<FMT, GS32, GATED><<<dim3((unsigned)grid), dim3(ET_THREADS), ET_LDS, s>>>(a, columns);
+  // the group of slice n of 32 k is (2 n group_mul) >> 32
+  const uint32_t d = a.v.mx ? 1 : a.v.gs / 32, mul = (uint32_t)(((1ull << 31) + d - 1) / d);
+  const int scales = et_scales(a.v);
+  experts_tile_kernel<FMT, GS32, GATED><<<dim3((unsigned)grid), dim3(ET_THREADS), et_lds(scales, FMT == 1), s>>>(a, columns, scales, mul);
   return hipGetLastError();
 }
 
@@ -360,11 +398,11 @@ hipError_t go_act(const ExpertArgs& a, hipStream_t s) {
 bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   const WView& v = a.v;
   const long long G = v.mx ? v.B : v.G, pairs = (long long)a.tokens * a.top_k;
-  if (v.K % 64 || (!v.mx && v.gs != 32 && v.gs % 64)) return false;
+  if (v.K % 64 || (!v.mx && v.gs != 32 && v.gs != 64 && v.gs != 128 && v.gs % 256)) return false;
   // the dword around a scale lies inside the array
   if ((v.mx && v.N * G % 4) || (!v.mx && v.gs != 32 && v.N * G % 2)) return false;
-  // offsets of 32 bits: codes of an expert, scales of all, rows of x (of a tile, or of all tokens)
-  if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32 || v.N * G * 4 >= 1LL << 32) return false;
+  // offsets of 32 bits: codes of an expert, rows of x (of a tile, or of all tokens)
+  if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32) return false;
   if (v.K >= 1 << 23 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
   // K 2048, 64 experts of 2048 rows: 32 places each 71 us against 59 by the kernel for some rows, 64 each 80 against 92.
