@@ -424,6 +424,11 @@ int w4_gemm_experts(const w4_packed_view* p, const w4_expert_rows* rows, int act
                     int from_tokens, w4_half* out, int to_pairs, w4_stream stream);
 int w4_gemm_experts_mx(const w4_packed_mx_view* p, const w4_expert_rows* rows, int act, const w4_half* x,
                        int from_tokens, w4_half* out, int to_pairs, w4_stream stream);
+/* Which kernel they run with arrays aligned to 16 bytes and rows of x that are tokens (plain arithmetic, no GPU needed):
+ * fmt 0 W4 symmetric, 1 W4 with zero-points, 2 MXFP4 (gs ignored); `rows` of an expert.  *plan: 0 the one for any K and group
+ * size, on the vector ALUs; 1 single rows, on the vector ALUs; 2 few experts, shares of K; 3 up to 16 or 32 rows a
+ * workgroup; 4 tiles of up to 128. */
+int w4_gemm_experts_plan_for(int fmt, int experts, int rows, int K, int gs, int tokens, int top_k, int* plan);
 
 /* Per token:  b = sum_j weights[j] * y[j] + shared  (weights NULL: the sum; shared may be NULL)
  *             b = norm(b) * post + post_bias;  r = residual + residual_scale * gate * b;

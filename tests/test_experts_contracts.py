@@ -160,3 +160,29 @@ def test_norms_by_definition():
     want = T(r) + 0.5 * b
     np.testing.assert_allclose(got, want.numpy(), rtol=1e-12)
     np.testing.assert_allclose(h, ln(want, (33,), T(pre), T(bias), 1e-5).numpy(), rtol=1e-10)
+
+
+def test_plan_of_products():
+    """Every kernel has calls, and the rules follow sizes alone."""
+    c = w4amd.capi()
+    plan = c.gemm_experts_plan_for
+    for fmt, gs in ((0, 32), (0, 64), (0, 128), (1, 32), (1, 128), (2, 32)):
+        assert plan(fmt, 64, 2048, 2048, gs, 1, 4) == 1
+        assert plan(fmt, 64, 2048, 2048, gs, 64, 4) == 3
+        assert plan(fmt, 64, 2048, 2048, gs, 512, 4) == 3
+        assert plan(fmt, 64, 2048, 2048, gs, 2048, 4) == 4
+        assert plan(fmt, 8, 1024, 4096, gs, 16, 2) == 2
+        assert plan(fmt, 8, 1024, 2048, gs, 16, 2) == 3
+        assert plan(fmt, 64, 2048, 2049, gs, 64, 4) == 0 and plan(fmt, 64, 2048, 2056, gs, 64, 4) == 0
+        assert plan(fmt, 64, 2048, 2080, gs, 2048, 4) == 3  # tiles take K in stages of 64
+        assert plan(fmt, 3, 35, 1120, gs, 60, 1) == (2 if (3 * 35 * -(-1120 // gs)) % (4 if fmt == 2 else 2) else 3)
+    for gs in (8, 24, 40, 48):
+        assert plan(0, 64, 2048, 2048, gs, 64, 4) == 0
+    for gs in (96, 192, 384):
+        assert plan(0, 64, 2048, 1920, gs, 2048, 4) == 3
+    for gs in (256, 512):
+        assert plan(0, 64, 2048, 2048, gs, 2048, 4) == 4
+    for bad in ((3, 8, 64, 64, 32, 1, 1), (0, 0, 64, 64, 32, 1, 1), (0, 8, 64, 64, 12, 1, 1), (0, 8, 0, 64, 32, 1, 1),
+                (0, 8, 64, 64, 32, 0, 1), (0, 8, 64, 64, 32, 1 << 20, 1 << 10), (0, 1024, 1 << 22, 64, 32, 1, 1)):
+        with pytest.raises(ValueError):
+            plan(*bad)

@@ -121,6 +121,7 @@ SIGNATURES = {
     "w4_route_experts_workspace": ([C.POINTER(Router), C.c_int, C.POINTER(C.c_size_t)], C.c_int),
     "w4_gemm_experts": ([C.POINTER(PackedView), C.POINTER(ExpertRows), C.c_int, vp, C.c_int, vp, C.c_int, vp], C.c_int),
     "w4_gemm_experts_mx": ([C.POINTER(PackedMxView), C.POINTER(ExpertRows), C.c_int, vp, C.c_int, vp, C.c_int, vp], C.c_int),
+    "w4_gemm_experts_plan_for": ([C.c_int] * 7 + [C.POINTER(C.c_int)], C.c_int),
     "w4_residual_norm": ([C.POINTER(BlockNorm), C.c_int, C.c_int, vp, vp, vp, vp, C.c_int, vp, vp, vp], C.c_int),
 }
 
@@ -453,6 +454,13 @@ def gemm_experts_mx(view, rows, act, x, from_tokens, out, to_pairs, stream=0):
     """gemm_experts over MXFP4 matrices"""
     check(load().w4_gemm_experts_mx(C.byref(view), C.byref(rows), act, _n(x), int(from_tokens), _n(out), int(to_pairs),
                                     _n(stream)))
+
+
+def gemm_experts_plan_for(fmt, experts, rows, K, gs, tokens, top_k):
+    """Which kernel gemm_experts runs (include/w4_abi.h)"""
+    plan = C.c_int()
+    check(load().w4_gemm_experts_plan_for(fmt, experts, rows, K, gs, tokens, top_k, C.byref(plan)))
+    return plan.value
 
 
 def residual_norm(norm, tokens, terms, y, weights, shared, residual, residual_f32, residual_out, h, stream=0):

@@ -805,6 +805,20 @@ int w4_gemm_experts_mx(const w4_packed_mx_view* p, const w4_expert_rows* rows, i
   return run_gemm_experts(w4k::view_of(*p), rows, act, x, from_tokens, out, to_pairs, stream);
 }
 
+int w4_gemm_experts_plan_for(int fmt, int experts, int rows, int K, int gs, int tokens, int top_k, int* plan) {
+  REQUIRE(plan && experts >= 1 && experts <= 1024 && rows >= 1 && K >= 1, "gemm experts plan: bad dims");
+  REQUIRE((long long)experts * rows <= INT_MAX && tokens >= 1 && top_k >= 1 && (long long)tokens * top_k < (1LL << 30),
+          "gemm experts plan: bad dims");
+  REQUIRE(fmt >= 0 && fmt <= 2 && (fmt == 2 || (gs >= 8 && gs % 8 == 0)), "gemm experts plan: bad format");
+  w4k::ExpertArgs a{};
+  a.v.mx = fmt == 2, a.v.N = experts * rows, a.v.K = K, a.v.symmetric = fmt != 1;
+  a.v.gs = fmt == 2 ? 32 : gs;
+  a.v.G = a.v.B = (K + a.v.gs - 1) / a.v.gs;
+  a.experts = experts, a.tokens = tokens, a.top_k = top_k, a.from_tokens = 1;
+  *plan = w4k::gemm_experts_plan(a);
+  return W4_OK;
+}
+
 int w4_residual_norm(const w4_block_norm* n, int tokens, int terms, const w4_half* y, const float* weights,
                      const w4_half* shared, const void* residual, int residual_f32, void* residual_out, w4_half* h,
                      w4_stream stream) {

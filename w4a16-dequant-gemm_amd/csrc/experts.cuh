@@ -102,11 +102,15 @@ __device__ __forceinline__ float expert_act(int act, float x) {
   return x / (1.f + __expf(-u));
 }
 
-// gemm_experts_tile.hip: false (nothing launched) when the arguments are not its.
-bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err);
-// gemm_experts_step.hip, gemm_experts_few.hip: the same for few rows per expert, of many experts and of few.
-bool try_experts_token(const ExpertArgs& a, hipStream_t s, hipError_t* err);
-bool try_experts_step(const ExpertArgs& a, hipStream_t s, hipError_t* err);
-bool try_experts_few(const ExpertArgs& a, hipStream_t s, hipError_t* err);
+// Whether a kernel takes the arguments and is ahead of the ones named after it, and its launch.  gemm_experts_tile.hip: many rows per
+// expert; _token: single ones; _step: some rows; _few: some rows of few experts, shares of K.
+bool experts_tile_applies(const ExpertArgs& a);
+bool experts_token_applies(const ExpertArgs& a);
+bool experts_step_applies(const ExpertArgs& a);
+bool experts_few_applies(const ExpertArgs& a);
+hipError_t launch_experts_tile(const ExpertArgs& a, hipStream_t s);
+hipError_t launch_experts_token(const ExpertArgs& a, hipStream_t s);
+hipError_t launch_experts_step(const ExpertArgs& a, hipStream_t s);
+hipError_t launch_experts_few(const ExpertArgs& a, hipStream_t s);
 
 }  // namespace w4k

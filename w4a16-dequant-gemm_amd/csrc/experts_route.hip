@@ -482,6 +482,8 @@ RoutePlan route_plan(const w4_router& r, int tokens) {
   p.blocks = (tokens + block - 1) / block;
   p.padded = (r.experts + 7) / 8 * 8;
   p.sort_tokens = block > 64 ? block : 64;
+  // (each of them reads all blocks' counts: 65536 tokens of 128 experts 41 us with 64 a workgroup, 37 with 256)
+  while (p.sort_tokens < 256 && (tokens + p.sort_tokens - 1) / p.sort_tokens > 256) p.sort_tokens *= 2;
   p.sort_blocks = (tokens + p.sort_tokens - 1) / p.sort_tokens;
   return p;
 }

@@ -89,9 +89,17 @@ hipError_t go_general(const ExpertArgs& a, hipStream_t s) {
 
 }  // namespace
 
+int gemm_experts_plan(const ExpertArgs& a) {
+  return experts_tile_applies(a) ? 4 : experts_token_applies(a) ? 1 : experts_step_applies(a) ? 3 : experts_few_applies(a) ? 2 : 0;
+}
+
 hipError_t launch_gemm_experts(const ExpertArgs& a, hipStream_t s) {
-  hipError_t err = hipSuccess;
-  if (try_experts_tile(a, s, &err) || try_experts_token(a, s, &err) || try_experts_step(a, s, &err) || try_experts_few(a, s, &err)) return err;
+  switch (gemm_experts_plan(a)) {
+    case 4: return launch_experts_tile(a, s);
+    case 3: return launch_experts_step(a, s);
+    case 2: return launch_experts_few(a, s);
+    case 1: return launch_experts_token(a, s);
+  }
   if (a.v.mx) return go_general<2>(a, s);
   return a.v.symmetric ? go_general<0>(a, s) : go_general<1>(a, s);
 }

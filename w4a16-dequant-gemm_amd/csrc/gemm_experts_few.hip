@@ -274,15 +274,18 @@ hipError_t go_groups(const ExpertArgs& a, hipStream_t s) {
 
 }  // namespace
 
-bool try_experts_few(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
+bool experts_few_applies(const ExpertArgs& a) {
   const WView& v = a.v;
   if (v.K % 32 || (!v.mx && v.gs % 32) || v.K >= 1 << 20) return false;
   // offsets of 32 bits: an expert's codes and parameters, rows of x
   const long long R = v.N / a.experts;
   if (R * v.K / 2 >= 0xE0000000LL || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 0xE0000000LL)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 1) || ((uintptr_t)v.zeros & 3)) return false;
-  *err = v.mx ? go_rows<2, 2>(a, s) : v.symmetric ? go_groups<0>(a, s) : go_groups<1>(a, s);
   return true;
+}
+
+hipError_t launch_experts_few(const ExpertArgs& a, hipStream_t s) {
+  return a.v.mx ? go_rows<2, 2>(a, s) : a.v.symmetric ? go_groups<0>(a, s) : go_groups<1>(a, s);
 }
 
 }  // namespace w4k

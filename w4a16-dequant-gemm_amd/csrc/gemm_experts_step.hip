@@ -305,7 +305,7 @@ hipError_t go_groups(const ExpertArgs& a, hipStream_t s) {
 
 }  // namespace
 
-bool try_experts_step(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
+bool experts_step_applies(const ExpertArgs& a) {
   const WView& v = a.v;
   const long long G = v.mx ? v.B : v.G, R = v.N / a.experts, pairs = (long long)a.tokens * a.top_k;
   if (v.K % 32 || (!v.mx && v.gs % 32) || v.K >= 1 << 20) return false;
@@ -316,8 +316,11 @@ bool try_experts_step(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   // A long K over few workgroups is a chain of stages of a microsecond each: the kernel that shares K out is ahead (8 experts
   // of 1024 rows, K 4096, 32 rows: 12.1 us against 20.5; of 2048 rows, K 2048: 12.3 against 11.5).
   if (v.K > 2048 && (pairs < a.experts ? pairs : a.experts) * R < 256 * 128) return false;
-  *err = v.mx ? go_act<2, 2>(a, s) : v.symmetric ? go_groups<0>(a, s) : go_groups<1>(a, s);
   return true;
+}
+
+hipError_t launch_experts_step(const ExpertArgs& a, hipStream_t s) {
+  return a.v.mx ? go_act<2, 2>(a, s) : a.v.symmetric ? go_groups<0>(a, s) : go_groups<1>(a, s);
 }
 
 }  // namespace w4k

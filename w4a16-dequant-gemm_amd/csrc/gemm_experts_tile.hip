@@ -395,7 +395,7 @@ hipError_t go_act(const ExpertArgs& a, hipStream_t s) {
 
 }  // namespace
 
-bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
+bool experts_tile_applies(const ExpertArgs& a) {
   const WView& v = a.v;
   const long long G = v.mx ? v.B : v.G, pairs = (long long)a.tokens * a.top_k;
   if (v.K % 64 || (!v.mx && v.gs != 32 && v.gs != 64 && v.gs != 128 && v.gs % 256)) return false;
@@ -407,10 +407,13 @@ bool try_experts_tile(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
   // K 2048, 64 experts of 2048 rows: 32 places each 71 us against 59 by the kernel for some rows, 64 each 80 against 92.
   if (pairs < 48LL * a.experts) return false;
-  if (v.mx) *err = go_act<2, false>(a, s);
-  else if (v.symmetric) *err = v.gs == 32 ? go_act<0, true>(a, s) : go_act<0, false>(a, s);
-  else *err = v.gs == 32 ? go_act<1, true>(a, s) : go_act<1, false>(a, s);
   return true;
+}
+
+hipError_t launch_experts_tile(const ExpertArgs& a, hipStream_t s) {
+  if (a.v.mx) return go_act<2, false>(a, s);
+  if (a.v.symmetric) return a.v.gs == 32 ? go_act<0, true>(a, s) : go_act<0, false>(a, s);
+  return a.v.gs == 32 ? go_act<1, true>(a, s) : go_act<1, false>(a, s);
 }
 
 }  // namespace w4k

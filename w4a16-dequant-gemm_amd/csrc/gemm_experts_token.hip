@@ -186,7 +186,7 @@ hipError_t go_shape(const ExpertArgs& a, hipStream_t s) {
 
 }  // namespace
 
-bool try_experts_token(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
+bool experts_token_applies(const ExpertArgs& a) {
   const WView& v = a.v;
   const long long R = v.N / a.experts, pairs = (long long)a.tokens * a.top_k;
   if (v.K % 32 || (!v.mx && v.gs % 32) || v.K >= 1 << 20) return false;
@@ -195,8 +195,11 @@ bool try_experts_token(const ExpertArgs& a, hipStream_t s, hipError_t* err) {
   // Experts with a row each, mostly, and so few rows of W that the time is latency.  K 2048, 8 of 128 experts of 2048 rows: 8.2 us
   // against 11.0 by the kernel that shares K out; 16 of 64: 15.4 against 12.3.  K 4096, 8 pairs on 8 experts: 12.8 against 10.8.
   if (2 * pairs > a.experts || pairs * R > 30000) return false;
-  *err = v.mx ? go_shape<2>(a, s) : v.symmetric ? go_shape<0>(a, s) : go_shape<1>(a, s);
   return true;
+}
+
+hipError_t launch_experts_token(const ExpertArgs& a, hipStream_t s) {
+  return a.v.mx ? go_shape<2>(a, s) : a.v.symmetric ? go_shape<0>(a, s) : go_shape<1>(a, s);
 }
 
 }  // namespace w4k

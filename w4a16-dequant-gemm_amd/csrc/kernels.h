@@ -243,6 +243,7 @@ struct ExpertArgs {
   const w4_half* x;
   w4_half* out;
 };
+int gemm_experts_plan(const ExpertArgs& a);  // w4_gemm_experts_plan_for
 hipError_t launch_gemm_experts(const ExpertArgs& a, hipStream_t s);
 
 // residual_norm.hip
