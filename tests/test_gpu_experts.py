@@ -219,3 +219,59 @@ def test_streams_and_repeated_calls_give_the_same_bytes():
             torch.cuda.synchronize()
             p.call(s.cuda_stream)
             assert np.array_equal(p.got().view(np.uint16), first.view(np.uint16))
+
+
+@pytest.mark.parametrize("fmt,gs", [(0, 128), (1, 64), (2, 32)])
+def test_codes_past_four_gigabytes(fmt, gs):
+    """The last of 40 experts of 67 million weights each, by every kernel; some columns and rows are checked."""
+    c = w4amd.capi()
+    E, R, K = 40, 16384, 16384
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(fmt)
+    G = K // (32 if fmt == 2 else gs)
+    q = torch.randint(-2 ** 31, 2 ** 31 - 1, (E * R, K // 8), dtype=torch.int32, device=DEV, generator=gen)
+    zeros = torch.randint(-2 ** 31, 2 ** 31 - 1, (E * R, (G + 7) // 8), dtype=torch.int32, device=DEV, generator=gen)
+    if fmt == 2:
+        scales = torch.randint(119, 124, (E * R, G), dtype=torch.uint8, device=DEV, generator=gen)
+        view, fn = c.packed_mx_view(E * R, K, G, ptr(q), ptr(scales)), c.gemm_experts_mx
+    else:
+        scales = (torch.rand(E * R, G, device=DEV, generator=gen) * 0.004 + 0.001).half()
+        view = c.packed_view(E * R, K, gs, G, fmt == 0, ptr(q), ptr(scales), ptr(zeros) if fmt else 0)
+        fn = c.gemm_experts
+    cols = np.array([0, 1, 777, R // 2 - 1])
+    rows = (E - 1) * R + np.concatenate([cols, R // 2 + cols])
+    words = q[rows].cpu().numpy().view(np.uint32)
+    codes = (words[:, :, None] >> (4 * np.arange(8, dtype=np.uint32)) & 15).reshape(len(rows), K).astype(np.int64)
+    group = np.arange(K) // (K // G)
+    s = scales[rows].cpu().numpy()
+    if fmt == 2:
+        w = experts_ref.E2M1[codes] * np.exp2(s.astype(np.float64) - 127)[:, group]
+    else:
+        z = 8
+        if fmt:
+            zw = zeros[rows].cpu().numpy().view(np.uint32)
+            z = (zw[:, :, None] >> (4 * np.arange(8, dtype=np.uint32)) & 15).reshape(len(rows), -1)[:, group].astype(np.int64)
+        w = (codes - z) * s.astype(np.float64)[:, group]
+    w = w.astype(np.float16).astype(np.float64)
+    seen = set()
+    for T in (1, 9, 30, 1920):
+        seen.add(c.gemm_experts_plan_for(fmt, E, R, K, gs, T, 1))
+        x = torch.randn(T, K, device=DEV, generator=gen).half()
+        order = torch.arange(T, dtype=torch.int32, device=DEV)
+        offsets = torch.zeros(E + 1, dtype=torch.int32, device=DEV)
+        offsets[E] = T
+        out = torch.zeros(T, R // 2, dtype=torch.float16, device=DEV)
+        fn(view, c.expert_rows(E, T, 1, ptr(offsets), ptr(order)), 1, ptr(x), 1, ptr(out), 0)
+        torch.cuda.synchronize()
+        some = np.unique([0, T // 2, T - 1])
+        xs = x[some].cpu().numpy().astype(np.float64)
+        y, off = xs @ w.T, (K + 8) * experts_ref.U * (np.abs(xs) @ np.abs(w).T)
+        a, n = experts_ref.act(1, y[:, :4]), np.abs(y[:, 4:])
+        want = a * y[:, 4:]
+        err = (1.13 * off[:, :4] + np.abs(a) * (12 + np.abs(y[:, :4])) * 2 * experts_ref.U) * (n + off[:, 4:]) + np.abs(a) * off[:, 4:]
+        got = out[some][:, cols].cpu().numpy().astype(np.float64)
+        bound = err + (np.abs(want) + err) * experts_ref.H + experts_ref.SUB
+        assert (np.abs(got - want) <= bound).all(), (T, float(np.abs(got - want).max()))
+        rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+        assert rel <= 1e-3, (T, rel)
+    assert seen == {1, 3, 4}

@@ -403,7 +403,7 @@ bool experts_tile_applies(const ExpertArgs& a) {
   if ((v.mx && v.N * G % 4) || (!v.mx && v.gs != 32 && v.N * G % 2)) return false;
   // offsets of 32 bits: codes of an expert, rows of x (of a tile, or of all tokens)
   if ((long long)(v.N / a.experts) * v.K / 2 >= 1LL << 32) return false;
-  if (v.K >= 1 << 23 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
+  if (v.K >= 1 << 20 || (a.from_tokens && (long long)a.tokens * v.K * 2 >= 1LL << 32)) return false;
   if ((((uintptr_t)v.q | (uintptr_t)a.x) & 15) || ((uintptr_t)v.scales & 3) || ((uintptr_t)v.zeros & 3)) return false;
   // K 2048, 64 experts of 2048 rows: 32 places each 71 us against 59 by the kernel for some rows, 64 each 80 against 92.
   if (pairs < 48LL * a.experts) return false;
